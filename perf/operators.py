@@ -1,0 +1,528 @@
+"""The operators around a block-scaled 8-bit cache: its KV write, the attention that reads it, and
+the step's block tables and slots built on the GPU.
+
+A block-scaled cache holds e4m3 codes and, for every block and key/value head, a key scale and a
+value scale: powers of two 2^e with -40 <= e <= 80, the least that keeps the block's largest finite
+magnitude within 448 codes (0: nothing but zeros). The write encodes a step's rows; a row that needs
+a larger scale than the block has re-encodes the tokens held before it. Attention decodes
+``code * scale``. The tables give every request of a step the blocks it lacks, in request order from
+a list of free ones, and derive each row's position and slot.
+
+``own`` False computes all three in elementary torch operations; True calls the framework.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+_DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+_FP8 = torch.float8_e4m3fn
+_MAX_CODE = 448.0
+_LEAST, _MOST = -40, 80  # exponents of the scales
+
+
+# --- cases ------------------------------------------------------------------------------------------
+
+
+def _step(name, kind, dtype, heads, kv_heads, head_dim, block, requests, shortest, longest, rows_least=1, rows_most=1,
+          *, layout="nhd", padding=0, mix=1):
+    """A store or attend case: ``requests`` contexts of ``shortest`` to ``longest`` positions, each
+    with ``rows_least`` to ``rows_most`` new rows, the last ``padding`` of them empty."""
+    return {"name": name, "kind": kind, "dtype": dtype, "heads": heads, "kv_heads": kv_heads, "head_dim": head_dim,
+            "block": block, "layout": layout, "requests": requests, "shortest": shortest, "longest": longest,
+            "rows_least": rows_least, "rows_most": rows_most, "padding": padding, "mix": mix}
+
+
+def _tables(name, kind, block, requests, shortest, longest, chunks=0, rows_least=1, rows_most=1, *, padding=0,
+            spare=0, lacking=0, mix=1):
+    """A tables case: ``chunks`` of the requests bring ``rows_least`` to ``rows_most`` rows and the
+    others one; the last ``padding`` are empty; ``spare`` rows of the outputs lie behind the step's;
+    the pool has ``lacking`` fewer free blocks than the step asks for (0: enough)."""
+    return {"name": name, "kind": kind, "block": block, "requests": requests, "shortest": shortest,
+            "longest": longest, "chunks": chunks, "rows_least": rows_least, "rows_most": rows_most,
+            "padding": padding, "spare": spare, "lacking": lacking, "mix": mix}
+
+
+def listed():
+    return [
+        # A small model's decode step at a handful of users: one new token each.
+        _step("store_decode_small", "store", "fp16", 9, 3, 64, 16, 4, 128, 1000),
+        # Continuous batching at a full batch: one token each at any offset of its block.
+        _step("store_decode_batch", "store", "bf16", 64, 8, 128, 32, 256, 16, 2048, padding=6, mix=2),
+        # Prompts and prefill chunks of uneven size that start and end inside blocks.
+        _step("store_chunks", "store", "bf16", 32, 8, 128, 16, 8, 600, 3000, 400, 2000, mix=3),
+        # Decode of a small model at a handful of users: every launch counts.
+        _step("attend_decode_small", "attend", "fp16", 9, 3, 64, 16, 4, 128, 1000),
+        # Decode of an 8B model at a full batch of equal contexts.
+        _step("attend_decode_8b", "attend", "bf16", 32, 8, 128, 16, 64, 4096, 4096),
+        # Continuous batching of a large model: contexts from 16 to 16K, some slots of the batch empty.
+        _step("attend_decode_ragged", "attend", "bf16", 64, 8, 128, 32, 128, 16, 16384, padding=3, mix=5),
+        # Speculative decoding: windows of 4 draft tokens over 4K contexts.
+        _step("attend_verify", "attend", "bf16", 32, 8, 128, 16, 32, 4096, 4096, 4, 4),
+        # Chunked prefill of an 8B model: 512-row chunks at the end of 4K contexts.
+        _step("attend_chunks", "attend", "bf16", 32, 8, 128, 16, 4, 4096, 4096, 512, 512),
+        # Uneven chunks of a wide-head model over head-major blocks of an odd size.
+        _step("attend_chunks_wide", "attend", "fp16", 16, 8, 256, 24, 4, 900, 3600, 150, 500, layout="hnd", mix=4),
+        # A decode bucket of a few users moved on by one token.
+        _tables("tables_decode_small", "advance", 16, 8, 128, 1000),
+        # A decode bucket of a full batch moved on by one token, some of its slots empty.
+        _tables("tables_decode_batch", "advance", 32, 256, 16, 16384, padding=9, mix=2),
+        # A step that prefills long prompts in chunks beside many decoding requests, the pool running out
+        # before the last of them.
+        _tables("tables_mixed", "tables", 16, 512, 64, 8192, 12, 300, 4000, padding=5, spare=100, lacking=8, mix=3),
+    ]
+
+
+def _between(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    kind = rng.choice(("store", "attend", "attend", "attend", "tables", "advance"))
+    mix = rng.randrange(1, 1000)
+    if kind in ("tables", "advance"):
+        requests = _between(rng, 1, 512)
+        longest = _between(rng, 32, 16384)
+        case = _tables("", kind, rng.choice((1, 5, 16, 24, 32, 64, 128)), requests, _between(rng, 1, longest), longest,
+                       padding=rng.randrange(0, 1 + requests // 4), lacking=rng.choice((0, 0, 1, 30)), mix=mix)
+        if kind == "tables":
+            most = min(4000, longest)
+            case.update(chunks=rng.randrange(0, 1 + min(8, requests)), rows_most=most,
+                        rows_least=_between(rng, 1, most), spare=rng.randrange(0, 200))
+    else:
+        kv_heads = rng.choice((1, 2, 3, 4, 8))
+        head_dim = rng.choice((64, 128, 256))
+        form = rng.choice(("decode", "verify", "chunks"))
+        most = {"decode": 1, "verify": 8, "chunks": 600}[form]
+        longest = _between(rng, max(32, most), 8192 if form == "decode" else 4096)
+        # at most about what the largest listed case of the kind holds
+        budget = (48 << 20) if form != "chunks" else (6 << 20)
+        requests = max(1, min(_between(rng, 1, 128), budget // (longest * kv_heads * head_dim)))
+        case = _step("", kind, rng.choice(("fp16", "bf16")), kv_heads * rng.choice((1, 2, 3, 4, 5, 8)), kv_heads,
+                     head_dim, rng.choice((1, 7, 16, 24, 32, 64, 128)), requests, _between(rng, most, longest), longest,
+                     min(most, rng.choice((1, 2, 40))), most, layout=rng.choice(("nhd", "hnd")),
+                     padding=rng.randrange(0, 1 + requests // 4), mix=mix)
+    case.pop("name")
+    return case
+
+
+def _generator(seed, device="cpu"):
+    return torch.Generator(device=device).manual_seed(seed)
+
+
+def _log_uniform(count, low, high, g):
+    x = torch.rand(count, generator=g, dtype=torch.float64)
+    x = torch.exp(math.log(low) + x * (math.log(high) - math.log(low)))
+    return x.round().long().clamp(low, high)
+
+
+def _requests(case):
+    """Lengths and row counts of the case's requests (they do not change with the inputs' seed)."""
+    g = _generator(7000 + case["mix"])
+    n, pad = case["requests"], case["padding"]
+    lengths = _log_uniform(n, case["shortest"], case["longest"], g)
+    rows = _log_uniform(n, case["rows_least"], case["rows_most"], g).minimum(lengths)
+    if "chunks" in case:
+        rows[case["chunks"]:] = 1
+    if pad:
+        lengths[n - pad:] = 0
+        rows[n - pad:] = 1
+    return lengths, rows
+
+
+def _blocks(lengths, block):
+    return (lengths + block - 1) // block
+
+
+def work(case):
+    lengths, rows = _requests(case)
+    n, live = int(rows.sum()), lengths > 0
+    if case["kind"] in ("tables", "advance"):
+        had = _blocks((lengths - rows).clamp(min=0), case["block"])
+        new = max(0, int((_blocks(lengths, case["block"]) - had).sum()) - case["lacking"])
+        # lengths and row counts in, lengths out; each new block read and written; each row's three numbers;
+        # the block that a row's slot names where it was there before
+        return {"bytes": 12 * len(lengths) + 8 * new + 16 * (n + case["spare"]) + 4 * n, "flops": 0}
+    width = case["kv_heads"] * case["head_dim"]
+    blocks = int(_blocks(lengths, case["block"]).sum())
+    if case["kind"] == "store":
+        stored = int(rows[live].sum())
+        touched = int((_blocks(lengths, case["block"]) - (lengths - rows).clamp(min=0) // case["block"])[live].sum())
+        return {"bytes": stored * (6 * width + 8) + 16 * touched * case["kv_heads"], "flops": 0}
+    positions = int(lengths.sum())
+    pairs = int((rows * lengths - rows * (rows - 1) // 2)[live].sum())
+    return {"bytes": 2 * positions * width + blocks * (8 * case["kv_heads"] + 4)
+            + 4 * n * case["heads"] * case["head_dim"], "flops": 4 * pairs * case["heads"] * case["head_dim"]}
+
+
+# --- inputs -----------------------------------------------------------------------------------------
+
+
+def _scale_of(amax):
+    """The least power of two 2^e, within the codec's exponents, with amax <= 448 * 2^e; 0 for 0."""
+    mantissa, exponent = torch.frexp(amax)  # 448 = 0.875 * 2^9
+    exponent = (exponent - torch.where(mantissa <= 0.875, 9, 8)).clamp(_LEAST, _MOST)
+    return torch.where(amax > 0, torch.ldexp(torch.ones_like(amax), exponent), torch.zeros_like(amax))
+
+
+def _table(lengths, block, g, width=None):
+    """Every request's blocks, shuffled over a pool whose block 0 is padding; and the pool's size."""
+    counts = _blocks(lengths, block)
+    width = int(width or max(1, int(counts.max())))
+    total = int(counts.sum())
+    ids = 1 + torch.randperm(total, generator=g)
+    table = torch.zeros(len(lengths), width, dtype=torch.int32)
+    mask = torch.arange(width)[None, :] < counts[:, None]
+    table[mask] = ids.int()
+    return table, total + 1
+
+
+def _values(shape, kv_heads, head_dim, g):
+    """Keys or values as layers make them: heads of different size and a few loud channels."""
+    loud = torch.exp(0.8 * torch.randn(kv_heads, 1, generator=g, device="cuda"))
+    channels = torch.where(torch.rand(kv_heads, head_dim, generator=g, device="cuda") < 0.03, 6.0, 1.0)
+    return torch.randn(*shape, kv_heads, head_dim, generator=g, device="cuda") * loud * channels
+
+
+def _rows(lengths, rows, table, block):
+    """Each row's request, position and slot."""
+    request = torch.repeat_interleave(torch.arange(len(rows)), rows)
+    first = torch.cumsum(rows, 0) - rows
+    within = torch.arange(int(rows.sum())) - first[request]
+    position = (lengths - rows)[request] + within
+    live = lengths[request] > 0
+    position = torch.where(live, position, 0)
+    slot = table[request, position // block].long() * block + position % block
+    return request, within, position, torch.where(live, slot, 0)
+
+
+def _prepare_tables(case, seed):
+    g = _generator(seed)
+    lengths, rows = _requests(case)
+    block = case["block"]
+    before = (lengths - rows).clamp(min=0)
+    had = _blocks(before, block)
+    need = int((_blocks(lengths, block) - had).sum())
+    width = int(_blocks(torch.tensor(case["longest"]), block)) + 2
+    table, pool = _table(before, block, g, width)
+    taken = int(torch.randint(1, 50, (1,), generator=g))
+    left = max(0, need - case["lacking"]) if case["lacking"] else need + 20
+    free = (pool + torch.randperm(taken + left, generator=g)).int()
+    count = int(rows.sum()) + case["spare"]
+    state = {
+        "rows": rows.int().cuda(), "lengths": lengths.int().cuda(), "table": table.cuda(), "free": free.cuda(),
+        "taken": torch.tensor([taken], dtype=torch.int32).cuda(), "after": torch.zeros(4, dtype=torch.int32).cuda(),
+        "request_of_row": torch.zeros(count, dtype=torch.int32).cuda(),
+        "positions": torch.zeros(count, dtype=torch.int32).cuda(),
+        "slots": torch.zeros(count, dtype=torch.int64).cuda(),
+        "served": torch.zeros(len(rows), dtype=torch.int32).cuda(),
+    }
+    if own:
+        from ayaka_amd.backend import load_backend
+        from ayaka_amd.enums import DType
+        from ayaka_amd.kvcache import BlockPool, StepTables
+
+        ops = load_backend(["hip"], device="cuda", dtype=DType.BF16)
+        state["ops"] = ops
+        state["pool"] = BlockPool(state["free"], state["taken"], state["after"])
+        if case["kind"] == "advance":
+            meta = ops.attention.graph_metadata(len(rows), width, block, torch.device("cuda", torch.cuda.current_device()))
+            ops.attention.update_graph_metadata(meta, before.int(), table)
+            state["meta"] = meta
+        else:
+            state["tables"] = StepTables(state["request_of_row"], state["positions"], state["slots"], state["served"])
+    return state
+
+
+def prepare(case, seed):
+    if case["kind"] in ("tables", "advance"):
+        return {"case": case, **_prepare_tables(case, seed)}
+    host, g = _generator(seed), _generator(seed, "cuda")
+    lengths, rows = _requests(case)
+    block, kv_heads, head_dim = case["block"], case["kv_heads"], case["head_dim"]
+    table, pool = _table(lengths, block, host)
+    request, within, position, slots = _rows(lengths, rows, table, block)
+    # the cache as its writer leaves it: the held positions encoded with their block's scales, every
+    # other slot (padding block, tails of blocks) a NaN code that nothing may read
+    held = lengths if case["kind"] == "attend" else (lengths - rows).clamp(min=0)
+    in_block = torch.zeros(pool, dtype=torch.int64)
+    start = torch.arange(table.shape[1])[None, :] * block
+    mask = table > 0
+    in_block[table[mask].long()] = (held[:, None] - start)[mask].clamp(0, block)
+    full = (torch.arange(block)[None, :] < in_block[:, None]).cuda()[:, :, None, None]
+    scales, caches = [], []
+    for _ in range(2):
+        x = _values((pool, block), kv_heads, head_dim, g).to(_DTYPES[case["dtype"]]).float()
+        x = torch.where(full, x, 0.0)
+        s = _scale_of(x.abs().amax(dim=(1, 3)))
+        codes = (x / torch.where(s > 0, s, 1.0)[:, None, :, None]).to(_FP8).view(torch.uint8)
+        codes = torch.where(full, codes, 0x7F)
+        if case["layout"] == "hnd":
+            codes = codes.transpose(1, 2)
+        caches.append(codes.contiguous().view(_FP8))
+        scales.append(s)
+        del x, codes
+    state = {"case": case, "k": caches[0], "v": caches[1], "scales": torch.stack(scales, dim=2).contiguous(),
+             "slots": slots.cuda(), "request": request.cuda(), "within": within.cuda(), "position": position.cuda(),
+             "lengths": lengths.int().cuda(), "rows": rows.int().cuda(), "table": table.cuda(),
+             "scale": head_dim ** -0.5}
+    n, dtype = len(slots), _DTYPES[case["dtype"]]
+    if case["kind"] == "attend":
+        state["q"] = torch.randn(n, case["heads"], head_dim, generator=g, device="cuda").to(dtype)
+        state["out"] = torch.empty_like(state["q"])
+    else:
+        # the new rows are now and then louder than what their block holds
+        state["k_new"], state["v_new"] = (
+            (_values((n,), kv_heads, head_dim, g) * torch.exp2(torch.randint(-1, 3, (n, 1, 1), generator=g, device="cuda"))
+             ).to(dtype) for _ in range(2))
+    if own:
+        from ayaka_amd.backend import load_backend
+        from ayaka_amd.enums import DType, ForwardMode, KVLayoutKind
+        from ayaka_amd.kvcache import KVBuffers, fp8_e4m3_block_codec
+
+        ops = load_backend(["hip"], device="cuda", dtype={"fp16": DType.FP16, "bf16": DType.BF16}[case["dtype"]])
+        layout = KVLayoutKind.NHD if case["layout"] == "nhd" else KVLayoutKind.HND
+        decode = bool((rows == 1).all())
+        state["ops"] = ops
+        state["buffers"] = KVBuffers(state["k"], state["v"], layout, fp8_e4m3_block_codec(state["scales"]))
+        state["meta"] = ops.attention.plan(ForwardMode.DECODE if decode else ForwardMode.MIXED, rows.int(),
+                                           lengths.int(), state["table"], block)
+    return state
+
+
+# --- one pass ---------------------------------------------------------------------------------------
+
+
+def run(state):
+    kind = state["case"]["kind"]
+    if kind == "attend":
+        if own:
+            state["ops"].attention.attend(state["q"], state["buffers"], state["meta"], state["out"],
+                                          scale=state["scale"])
+            return state["out"]
+        return _attend(state)
+    if kind == "store":
+        if own:
+            state["ops"].kvcache.store(state["k_new"], state["v_new"], state["buffers"], state["meta"])
+        else:
+            _store(state)
+        return {"k": state["k"], "v": state["v"], "scales": state["scales"]}
+    if own:
+        if kind == "advance":
+            meta = state["meta"]
+            state["ops"].attention.advance_graph_metadata(meta, state["lengths"], state["pool"])
+            return {"table": meta.block_table, "request_of_row": meta.request_of_row, "positions": meta.positions,
+                    "slots": meta.slot_mapping, "lengths": meta.kv_lengths, "after": state["after"][:2]}
+        state["ops"].kvcache.build_tables(state["rows"], state["lengths"], state["table"], state["pool"],
+                                          state["tables"], state["case"]["block"])
+    else:
+        _build_tables(state)
+    return {"table": state["table"], "request_of_row": state["request_of_row"], "positions": state["positions"],
+            "slots": state["slots"], "lengths": state["served"], "after": state["after"][:2]}
+
+
+def _nhd(state, name):
+    """A cache as bytes [blocks, positions, heads, elements], a view whatever its layout."""
+    codes = state[name].view(torch.uint8)
+    return codes.transpose(1, 2) if state["case"]["layout"] == "hnd" else codes
+
+
+def _attend(state):
+    case, q, lengths, table = state["case"], state["q"], state["lengths"].long(), state["table"].long()
+    kv_heads, head_dim, block = case["kv_heads"], case["head_dim"], case["block"]
+    group, requests = case["heads"] // kv_heads, len(lengths)
+    longest, most = case["longest"], max(1, case["rows_most"])
+    longest = min(longest, table.shape[1] * block)
+    position = torch.arange(longest, device=q.device)
+    held = position[None, :] < lengths[:, None]  # [requests, positions]
+
+    def gather(name, which):
+        x = _nhd(state, name)[table].view(_FP8).float()  # [requests, blocks, block, heads, elements]
+        x = x * state["scales"][..., which][table][:, :, None, :, None]
+        x = x.flatten(1, 2)[:, :longest]
+        return torch.where(held[:, :, None, None], x, 0.0).transpose(1, 2).contiguous()
+
+    # rows of a request side by side: [requests, kv heads, rows x group, elements]
+    padded = torch.zeros(requests, most, case["heads"], head_dim, device=q.device)
+    padded[state["request"], state["within"]] = q.float()
+    padded = padded.view(requests, most, kv_heads, group, head_dim).permute(0, 2, 1, 3, 4)
+    sees = torch.full((requests, most), -1, device=q.device, dtype=torch.long)
+    sees[state["request"], state["within"]] = state["position"]
+    visible = held[:, None, :] & (position[None, None, :] <= sees[:, :, None])
+    keys = gather("k", 0).transpose(2, 3).contiguous()
+    scores = torch.matmul(padded.reshape(requests, kv_heads, most * group, head_dim), keys) * state["scale"]
+    del keys
+    scores = scores.view(requests, kv_heads, most, group, longest)
+    scores = torch.where(visible[:, None, :, None, :], scores, -math.inf)
+    largest = scores.amax(-1, keepdim=True)
+    weights = torch.exp(scores - torch.where(largest == -math.inf, 0.0, largest))
+    total = weights.sum(-1, keepdim=True)
+    weights = (weights / torch.where(total > 0, total, 1.0)).view(requests, kv_heads, most * group, longest)
+    out = torch.matmul(weights, gather("v", 1)).view(requests, kv_heads, most, group, head_dim)
+    out = out.permute(0, 2, 1, 3, 4).reshape(requests, most, case["heads"], head_dim)
+    return out[state["request"], state["within"]].to(q.dtype)
+
+
+def _store(state):
+    block, slots, scales = state["case"]["block"], state["slots"], state["scales"]
+    pool = scales.shape[0]
+    live = (slots >= block) & (slots < pool * block)
+    slots = slots[live]
+    block_of, offset = slots // block, slots % block
+    first = torch.full((pool,), block, device=slots.device).scatter_reduce(0, block_of, offset, "amin")
+    touched = (first < block).nonzero()[:, 0]
+    before = torch.arange(block, device=slots.device)[None, :, None] < first[touched][:, None, None]
+    for which, name in enumerate(("k", "v")):
+        x = state[name + "_new"][live].float()
+        codes = _nhd(state, name)
+        finite = torch.isfinite(x)
+        amax = torch.where(finite, x.abs(), 0.0).amax(-1)
+        need = torch.zeros(pool, amax.shape[1], device=x.device).scatter_reduce(
+            0, block_of[:, None].expand_as(amax), amax, "amax")
+        kept = torch.where(first[:, None] > 0, scales[..., which], 0.0)
+        new = torch.maximum(kept, _scale_of(need))
+        grown = (new > kept) & (kept > 0)
+        factor = torch.where(grown, kept / torch.where(new > 0, new, 1.0), 1.0)[touched]
+        old = codes[touched]
+        recoded = (old.view(_FP8).float() * factor[:, None, :, None]).to(_FP8).view(torch.uint8)
+        codes[touched] = torch.where((before & grown[touched][:, None, :])[..., None], recoded, old)
+        x = x / torch.where(new > 0, new, 1.0)[block_of][:, :, None]
+        x = torch.where(finite, x.clamp(-_MAX_CODE, _MAX_CODE), math.nan)
+        codes[block_of, offset] = x.to(_FP8).view(torch.uint8)
+        scales[touched, :, which] = new[touched]
+
+
+def _build_tables(state):
+    block, table, free = state["case"]["block"], state["table"], state["free"].long()
+    rows, lengths = state["rows"].long(), state["lengths"].long()
+    width, count, taken = table.shape[1], state["positions"].shape[0], state["taken"].long()
+    before = (lengths - rows).clamp(min=0)
+    each = rows.clamp(min=0)
+    last = torch.cumsum(each, 0)
+    first = last - each
+    live = (rows >= 0) & (lengths > 0) & (rows <= lengths) & (lengths <= width * block) & (last <= count)
+    had = torch.where(live, (before + block - 1) // block, 0)
+    need = torch.where(live, (lengths + block - 1) // block - had, 0)
+    upto = torch.cumsum(need, 0)
+    served = live & ((need == 0) | (taken + upto <= len(free)))
+    new_before = taken + upto - need
+    # the new blocks' entries of the table
+    column = torch.arange(width, device=table.device)[None, :]
+    fresh = served[:, None] & (column >= had[:, None]) & (column < (had + need)[:, None])
+    ids = free[(new_before[:, None] + column - had[:, None]).clamp(0, len(free) - 1)]
+    table.copy_(torch.where(fresh, ids, table.long()))
+    # the rows
+    row = torch.arange(count, device=table.device)
+    request = torch.searchsorted(last, row, right=True)
+    inside = request < len(rows)
+    request = torch.where(inside, request, 0)
+    shown = inside & served[request]
+    position = torch.where(shown, before[request] + row - first[request], 0)
+    slot = table[request, position // block].long() * block + position % block
+    state["request_of_row"].copy_(request)
+    state["positions"].copy_(position)
+    state["slots"].copy_(torch.where(shown, slot, 0))
+    state["served"].copy_(torch.where(served, lengths, 0))
+    state["after"][:1] = taken + torch.where(served & (need > 0), upto, 0).amax()
+    state["after"][1] = ((lengths != 0) & ~served).sum()
+
+
+# --- the definitions in 64 bits -----------------------------------------------------------------------
+
+
+def _e4m3_values(device):
+    """The value of each of the 256 codes: sign, 4 exponent bits (bias 7), 3 mantissa bits."""
+    code = torch.arange(256, device=device)
+    exponent, mantissa = (code >> 3) & 15, (code & 7).double()
+    value = torch.where(exponent > 0, (1 + mantissa / 8) * torch.exp2(exponent.double() - 7), mantissa * 2.0 ** -9)
+    value = torch.where((code & 127) == 127, math.nan, value)
+    return torch.where(code >= 128, -value, value)
+
+
+def _nearest_code(x):
+    """The finite value of the format nearest to each x (|x| <= 448), a tie to the even code."""
+    grid = _e4m3_values(x.device)[:127]
+    middle = (grid[1:] + grid[:-1]) / 2
+    low = torch.bucketize(x.abs().contiguous(), middle)
+    high = torch.bucketize(x.abs().contiguous(), middle, right=True)
+    return torch.copysign(grid[torch.where(low % 2 == 0, low, high)], x)
+
+
+def _exact_attend(case, state):
+    values = _e4m3_values("cuda")
+    block, kv_heads = case["block"], case["kv_heads"]
+    group = case["heads"] // kv_heads
+    out = torch.zeros(state["q"].shape, dtype=torch.float64, device="cuda")
+    lengths, rows = _requests(case)
+    last = 0
+    for b, (length, count) in enumerate(zip(lengths.tolist(), rows.tolist())):
+        first, last = last, last + count
+        if length == 0:
+            continue
+        ids = state["table"][b, : -(-length // block)].long()
+        k, v = (values[_nhd(state, name)[ids].long()] * state["scales"][ids][..., which].double()[:, None, :, None]
+                for which, name in enumerate(("k", "v")))
+        k, v = (x.flatten(0, 1)[:length] for x in (k, v))  # [positions, heads, elements]
+        hidden = torch.arange(length, device="cuda")[None, :] > (
+            length - count + torch.arange(count, device="cuda"))[:, None]
+        for h in range(kv_heads):
+            q = state["q"][first:last, h * group:(h + 1) * group].double().transpose(0, 1)  # [group, rows, elements]
+            score = (q.reshape(-1, q.shape[2]) @ k[:, h].T.contiguous()).view(group, count, length) * state["scale"]
+            weight = torch.softmax(score.masked_fill(hidden[None], -math.inf), dim=-1)
+            got = (weight.reshape(-1, length) @ v[:, h].contiguous()).view(group, count, -1)
+            out[first:last, h * group:(h + 1) * group] = got.transpose(0, 1)
+    return out
+
+
+def _exact_store(case, state):
+    """Each touched block by its definition: the scale, the earlier tokens, the new ones."""
+    values = _e4m3_values("cuda")
+    block = case["block"]
+    scales = state["scales"].double()
+    lengths, rows = _requests(case)
+    caches = [values[_nhd(state, name).long()] for name in ("k", "v")]  # [blocks, positions, heads, elements]
+    table, last = state["table"].long().cpu(), 0
+    for b, (length, count) in enumerate(zip(lengths.tolist(), rows.tolist())):
+        first, last = last, last + count
+        if length == 0:
+            continue
+        start = length - count
+        head = min(count, -start % block)  # rows of the block that was begun before
+        whole = (count - head) // block
+        ids = table[b, start // block: -(-length // block)].cuda()
+        for which, name in enumerate(("k", "v")):
+            x = state[name + "_new"][first:last].double()
+            pieces = [(ids[:1], start % block, x[None, :head])] if head else []
+            ids_left = ids[1:] if head else ids
+            pieces.append((ids_left[:whole], 0, x[head:head + whole * block].view(whole, block, *x.shape[1:])))
+            if head + whole * block < count:
+                pieces.append((ids_left[whole:], 0, x[None, head + whole * block:]))
+            for at, offset, piece in pieces:
+                if not piece.numel():
+                    continue
+                amax = piece.abs().amax(dim=(1, 3))
+                need = torch.exp2(torch.ceil(torch.log2(amax / _MAX_CODE)).clamp(_LEAST, _MOST))
+                new = torch.where(amax > 0, need, 0.0)
+                if offset:
+                    old = scales[at, :, which]
+                    new = torch.maximum(old, new)
+                    ratio = torch.where((old > 0) & (new > old), old / new, 1.0)
+                    caches[which][at, :offset] = _nearest_code(caches[which][at, :offset] * ratio[:, None, :, None])
+                scales[at, :, which] = new
+                unit = torch.where(new > 0, new, 1.0)[:, None, :, None]
+                caches[which][at, offset:offset + piece.shape[1]] = _nearest_code(
+                    (piece / unit).clamp(-_MAX_CODE, _MAX_CODE))
+    if case["layout"] == "hnd":
+        caches = [x.transpose(1, 2) for x in caches]
+    return {"k": caches[0], "v": caches[1], "scales": scales}
+
+
+def exact(case, seed):
+    if case["kind"] in ("tables", "advance"):
+        return None  # whole numbers
+    state = prepare(case, seed)
+    return _exact_attend(case, state) if case["kind"] == "attend" else _exact_store(case, state)
