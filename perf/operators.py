@@ -289,8 +289,8 @@ def prepare(case, seed):
         decode = bool((rows == 1).all())
         state["ops"] = ops
         state["buffers"] = KVBuffers(state["k"], state["v"], layout, fp8_e4m3_block_codec(state["scales"]))
-        state["meta"] = ops.attention.plan(ForwardMode.DECODE if decode else ForwardMode.MIXED, rows.int(),
-                                           lengths.int(), state["table"], block)
+        state["meta"] = ops.attention.plan(ForwardMode.DECODE if decode else ForwardMode.MIXED, state["rows"],
+                                           state["lengths"], state["table"], block)
     return state
 
 
