@@ -12,6 +12,7 @@
 #include <string>
 
 #include "ayaka_hip.h"
+#include "ayaka_hip_block_scaled.h"
 #include "ayaka_hip_internal.h"
 
 namespace {
@@ -396,6 +397,41 @@ int ayk_reshape_and_cache_e4m3(const void* k, const void* v, void* k_cache, void
                                                      head_dim, num_blocks, block_size, layout == AYK_LAYOUT_HND,
                                                      src_dtype == AYK_DTYPE_BF16, 1.0f / k_scale, 1.0f / v_scale,
                                                      static_cast<hipStream_t>(stream)),
+                  op);
+}
+
+int ayk_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_cache, float* scales,
+                           const int64_t* slot_mapping, int64_t n_rows, int32_t num_kv_heads, int32_t head_dim,
+                           int32_t num_blocks, int32_t block_size, int32_t layout, int32_t src_dtype, void* stream) {
+  const char* op = "ayk_store_block_scaled";
+  if (n_rows < 0) return fail(AYK_ERR_ARGUMENT, "%s: n_rows is negative", op);
+  if (num_kv_heads <= 0 || num_blocks <= 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: num_kv_heads %d, num_blocks %d", op, num_kv_heads, num_blocks);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: head_dim %d is not one of 64, 128, 256", op, head_dim);
+  if (block_size < 1 || block_size > 65536)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: block_size %d is not in [1, 65536]", op, block_size);
+  if (src_dtype != AYK_DTYPE_FP16 && src_dtype != AYK_DTYPE_BF16)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: src_dtype %d is not fp16 (0) or bf16 (1)", op, src_dtype);
+  if (layout != AYK_LAYOUT_NHD && layout != AYK_LAYOUT_HND)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: layout %d is not NHD (0) or HND (1)", op, layout);
+  // the kernel's slots are 31-bit; the attention entry points hold a pool to 2^32 elements
+  if ((uint64_t)num_blocks * (uint64_t)block_size * (uint64_t)num_kv_heads * (uint64_t)head_dim > UINT32_MAX)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: a cache of %d blocks of %d positions exceeds 32-bit element offsets", op,
+                num_blocks, block_size);
+  if (n_rows > INT32_MAX || num_kv_heads > 131070)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %lld rows of %d heads exceed one launch", op, (long long)n_rows,
+                num_kv_heads);
+  if (n_rows == 0) return ok();
+  if (!k || !v || !k_cache || !v_cache || !scales || !slot_mapping)
+    return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  uint32_t magic;
+  int32_t shift;
+  block_divisor(block_size, magic, shift);
+  return launched(ayk::launch_store_block_scaled(k, v, k_cache, v_cache, scales, slot_mapping, n_rows, num_kv_heads,
+                                                 head_dim, num_blocks, block_size, magic, shift,
+                                                 layout == AYK_LAYOUT_HND, src_dtype == AYK_DTYPE_BF16,
+                                                 static_cast<hipStream_t>(stream)),
                   op);
 }
 

@@ -103,6 +103,12 @@ hipError_t launch_reshape_and_cache_e4m3(const void* k, const void* v, void* k_c
                                          int32_t head_dim, int32_t num_blocks, int32_t block_size, bool hnd,
                                          bool bf16, float k_inv, float v_inv, hipStream_t stream);
 
+// KV write into block-scaled fp8 caches (block size divisor as AttnParams' bs_magic / bs_shift).
+hipError_t launch_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_cache, float* scales,
+                                     const int64_t* slot_mapping, int64_t n_rows, int32_t num_kv_heads,
+                                     int32_t head_dim, int32_t num_blocks, int32_t block_size, uint32_t bs_magic,
+                                     int32_t bs_shift, bool hnd, bool bf16, hipStream_t stream);
+
 // mode: 0 = gather (dst index i), 1 = copy (dst ids), 2 = zero (no source)
 hipError_t launch_block_op(int mode, const void* src_k, const void* src_v, void* dst_k, void* dst_v,
                            const void* src_ids, const void* dst_ids, bool ids64, int64_t n,

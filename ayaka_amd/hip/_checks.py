@@ -4,8 +4,8 @@ The messages follow the reference's (``python/ayaka/ops/backends/torch/_checks.p
 ``kvcache.py:39-62``) so that callers and tests read the same refusals. The
 hip backend computes in fp16, bf16 and fp32 (fp32 on kernels of its own: one for decode and for rows
 one by one, one for tiles of rows), on HIP devices, for head widths of 64, 128 and 256 and block sizes of 1 to 65536 positions; it
-stores the ``"raw"`` codec (fp16/bf16/fp32 caches) and ``"fp8_e4m3"`` (``float8_e4m3fn`` caches,
-read by fp16/bf16 models).
+stores the ``"raw"`` codec (fp16/bf16/fp32 caches) and ``"fp8_e4m3"`` and ``"fp8_e4m3_block"``
+(``float8_e4m3fn`` caches, read by fp16/bf16 models).
 """
 
 from __future__ import annotations
@@ -16,13 +16,15 @@ import torch
 
 from ayaka_amd.enums import KVLayoutKind
 from ayaka_amd.errors import BackendError
-from ayaka_amd.kvcache import FP8_E4M3_CODEC, RAW_CODEC, KVBuffers
+from ayaka_amd.kvcache import FP8_E4M3_BLOCK_CODEC, FP8_E4M3_CODEC, RAW_CODEC, BlockScaledFp8Codec, KVBuffers
 
 __all__ = [
     "HEAD_DIMS",
+    "block_scales",
     "capturing",
     "compute_dtype",
     "dtype_name",
+    "require_block_scales",
     "require_buffers",
     "require_device",
     "require_index_tensor",
@@ -43,7 +45,8 @@ _NAMES = {
     torch.float8_e4m3fn: "float8_e4m3fn",
 }
 # The cache element type of each codec this backend stores.
-_CODEC_DTYPES = {RAW_CODEC: _RAW_DTYPES, FP8_E4M3_CODEC: (torch.float8_e4m3fn,)}
+_CODEC_DTYPES = {RAW_CODEC: _RAW_DTYPES, FP8_E4M3_CODEC: (torch.float8_e4m3fn,),
+                 FP8_E4M3_BLOCK_CODEC: (torch.float8_e4m3fn,)}
 
 
 def dtype_name(dtype: torch.dtype) -> str:
@@ -105,11 +108,37 @@ def compute_dtype(op: str, name: str, tensor: torch.Tensor, buffers: KVBuffers) 
         return buffers.k.dtype
     if tensor.dtype not in _DTYPES:
         raise BackendError(
-            f"{op}: {name} is {dtype_name(tensor.dtype)}; over a {buffers.codec!r} cache the hip "
+            f"{op}: {name} is {dtype_name(tensor.dtype)}; over a {str(buffers.codec)!r} cache the hip "
             "backend computes in float16, bfloat16",
             context={"op": op, "argument": name},
         )
     return tensor.dtype
+
+
+def block_scales(buffers: KVBuffers) -> torch.Tensor | None:
+    """The scales of a block-scaled cache, ``None`` for every other codec."""
+    codec = buffers.codec
+    return codec.scales if type(codec) is BlockScaledFp8Codec else None
+
+
+def require_block_scales(op: str, buffers: KVBuffers) -> None:
+    """Refuse a block-scaled cache without scales of its blocks and heads beside it."""
+    scales = block_scales(buffers)
+    if scales is None:
+        raise BackendError(
+            f"{op}: a {FP8_E4M3_BLOCK_CODEC!r} cache needs its scales: make the codec with fp8_e4m3_block_codec",
+            context={"op": op, "argument": "buffers"},
+        )
+    shape = (buffers.num_blocks, buffers.num_kv_heads, 2)
+    require_like(op, "buffers.codec.scales", scales, shape, torch.float32)
+    require_device(op, "buffers.codec.scales", scales, buffers.k.device)
+    if buffers.head_dim not in HEAD_DIMS:
+        raise BackendError(
+            f"{op}: block-scaled caches are built for head widths {sorted(HEAD_DIMS)}, not {buffers.head_dim}",
+            context={"op": op, "argument": "buffers"},
+        )
+    if scales.data_ptr() % 8:
+        raise BackendError(f"{op}: buffers.codec.scales must be 8-byte aligned", context={"op": op})
 
 
 def require_buffers(op: str, buffers: KVBuffers) -> None:
@@ -128,7 +157,7 @@ def require_buffers(op: str, buffers: KVBuffers) -> None:
     k = buffers.k
     if k.dtype not in _CODEC_DTYPES[buffers.codec]:
         allowed = ", ".join(dtype_name(d) for d in _CODEC_DTYPES[buffers.codec])
-        what = "computes in" if buffers.codec == RAW_CODEC else f"stores the {buffers.codec!r} codec as"
+        what = "computes in" if buffers.codec == RAW_CODEC else f"stores the {str(buffers.codec)!r} codec as"
         raise BackendError(
             f"{op}: buffers.k is {dtype_name(k.dtype)}; the hip backend {what} {allowed}",
             context={"op": op, "argument": "buffers.k"},
@@ -155,3 +184,5 @@ def require_buffers(op: str, buffers: KVBuffers) -> None:
             f"and {buffers.v.device}",
             context={"op": op, "argument": "buffers"},
         )
+    if buffers.codec == FP8_E4M3_BLOCK_CODEC:
+        require_block_scales(op, buffers)

@@ -14,7 +14,7 @@ from pathlib import Path
 
 from ayaka_amd.errors import BackendError, CapabilityError
 
-__all__ = ["ABI_VERSION", "EXPORTS", "LIB_PATH", "check", "lib"]
+__all__ = ["ABI_VERSION", "BLOCK_SCALED_EXPORTS", "EXPORTS", "LIB_PATH", "check", "lib"]
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libayaka_hip.so"
 ABI_VERSION = 18
@@ -78,6 +78,14 @@ EXPORTS: dict[str, tuple[object, list[object]]] = {
     "ayk_zero_blocks": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I32, _I64, _P]),
 }
 
+#: The functions of include/ayaka_hip_block_scaled.h.
+BLOCK_SCALED_EXPORTS: dict[str, tuple[object, list[object]]] = {
+    "ayk_store_block_scaled": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+    ),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -102,7 +110,7 @@ def lib() -> ctypes.CDLL:
                 raise CapabilityError(
                     "ops.hip", detail=f"{LIB_PATH} does not load: {exc}", remedy="rebuild it"
                 ) from exc
-            for name, (restype, argtypes) in EXPORTS.items():
+            for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS}.items():
                 fn = getattr(handle, name)
                 fn.restype = restype
                 fn.argtypes = argtypes

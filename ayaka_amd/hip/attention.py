@@ -52,7 +52,7 @@ from ayaka_amd.hip._checks import (
     require_like,
     stream_handle,
 )
-from ayaka_amd.kvcache import FP8_E4M3_CODEC, KVBuffers, codec_scales
+from ayaka_amd.kvcache import FP8_E4M3_BLOCK_CODEC, FP8_E4M3_CODEC, KVBuffers, codec_scales
 
 __all__ = [
     "PARTITION_SIZE",
@@ -1129,6 +1129,8 @@ def attend_with(
     """
     op = "attention.attend"
     require_buffers(op, buffers)
+    if buffers.codec == FP8_E4M3_BLOCK_CODEC:
+        raise BackendError(f"{op}: no kernel reads block-scaled caches", context={"op": op, "argument": "buffers"})
     step = meta.plan
     table = meta.block_table
     if not isinstance(step, (HipAttentionPlan, HipGraphPlan)) or not isinstance(table, torch.Tensor):

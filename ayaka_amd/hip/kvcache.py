@@ -3,8 +3,11 @@
 ``store`` is the KV write (``ayk_reshape_and_cache``): row ``i`` of ``k``/``v``
 lands bit for bit in slot ``meta.slot_mapping[i]`` (reference
 ``python/ayaka/ops/backends/torch/kvcache.py:65-80``); into a ``"fp8_e4m3"``
-cache it lands encoded (``ayk_reshape_and_cache_e4m3``). ``gather``,
-``copy_blocks`` and ``zero_blocks`` move whole blocks (same file, ``:83-115``).
+cache it lands encoded (``ayk_reshape_and_cache_e4m3``), into a
+``"fp8_e4m3_block"`` cache encoded with its block's scales, which the write
+raises where it has to (``ayk_store_block_scaled``). ``gather``,
+``copy_blocks`` and ``zero_blocks`` move whole blocks (same file, ``:83-115``),
+of a block-scaled cache with their scales.
 Both layouts are served; NHD is preferred, as the reference's ``layout()``
 returns (``:30-31``).
 """
@@ -18,6 +21,7 @@ from ayaka_amd.enums import KVLayoutKind
 from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import _fastpath, _lib
 from ayaka_amd.hip._checks import (
+    block_scales,
     compute_dtype,
     require_buffers,
     require_device,
@@ -64,7 +68,9 @@ def store(k: torch.Tensor, v: torch.Tensor, buffers: KVBuffers, meta: AttentionM
     if cache is None:
         _store(k, v, buffers, meta, None)
         return
-    key = ("store", id(buffers), id(meta), _fastpath.signature((k, v, buffers.k, buffers.v)))
+    scales = block_scales(buffers)
+    key = ("store", id(buffers), id(meta), _fastpath.signature((k, v, buffers.k, buffers.v)),
+           0 if scales is None else scales.data_ptr())
     found = _fastpath.lookup(cache, key)
     if found is not None:
         _fastpath.run(found, _stream(found.device))
@@ -97,7 +103,13 @@ def _store(k: torch.Tensor, v: torch.Tensor, buffers: KVBuffers, meta: Attention
         raise BackendError(f"{op}: meta.slot_mapping must be a contiguous int64 tensor")
     if rows == 0:
         return
-    if buffers.codec == FP8_E4M3_CODEC:
+    scales = block_scales(buffers)
+    if scales is not None:
+        fn = _lib.lib().ayk_store_block_scaled
+        args = (k.data_ptr(), v.data_ptr(), buffers.k.data_ptr(), buffers.v.data_ptr(), scales.data_ptr(),
+                slots.data_ptr(), rows, buffers.num_kv_heads, buffers.head_dim, buffers.num_blocks,
+                buffers.block_size, _LAYOUT_CODES[KVLayoutKind(buffers.layout)], _DTYPE_CODES[dtype])
+    elif buffers.codec == FP8_E4M3_CODEC:
         fn = _lib.lib().ayk_reshape_and_cache_e4m3
         args = (k.data_ptr(), v.data_ptr(), buffers.k.data_ptr(), buffers.v.data_ptr(), slots.data_ptr(), rows,
                 buffers.num_kv_heads, buffers.head_dim, buffers.num_blocks, buffers.block_size,
@@ -113,8 +125,11 @@ def _store(k: torch.Tensor, v: torch.Tensor, buffers: KVBuffers, meta: Attention
 
 
 def gather(
-    buffers: KVBuffers, block_ids: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor
+    buffers: KVBuffers, block_ids: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
+    out_scales: torch.Tensor | None = None,
 ) -> None:
+    """Copy whole blocks out (reference ``torch/kvcache.py:83-93``); a block-scaled cache's codes
+    mean nothing without their scales, which go to ``out_scales`` float32 [n, kv_heads, 2]."""
     op = "kvcache.gather"
     require_buffers(op, buffers)
     device = buffers.k.device
@@ -124,6 +139,16 @@ def gather(
     require_like(op, "out_v", out_v, shape, buffers.k.dtype)
     require_device(op, "out_k", out_k, device)
     require_device(op, "out_v", out_v, device)
+    scales = block_scales(buffers)
+    if (scales is None) != (out_scales is None):
+        raise BackendError(
+            f"{op}: out_scales goes with a block-scaled cache: the cache is {str(buffers.codec)!r} and out_scales "
+            f"is {'not given' if out_scales is None else 'given'}",
+            context={"op": op, "argument": "out_scales"},
+        )
+    if scales is not None:
+        require_like(op, "out_scales", out_scales, (block_ids.shape[0], *scales.shape[1:]), scales.dtype)
+        require_device(op, "out_scales", out_scales, device)
     if block_ids.shape[0] == 0:
         return
     _lib.check(
@@ -138,6 +163,26 @@ def gather(
             block_ids.shape[0],
             buffers.num_blocks,
             _block_bytes(buffers),
+            _stream(device),
+        ),
+    )
+    if scales is not None:
+        _move_scales(op, "ayk_gather_blocks", (scales, scales, out_scales, out_scales), (block_ids,), scales, device)
+
+
+def _move_scales(op: str, name: str, tensors: tuple[torch.Tensor, ...], ids: tuple[torch.Tensor, ...],
+                 scales: torch.Tensor, device: torch.device) -> None:
+    """The block op ``name`` on a block-scaled cache's scales, one block of them a row (the op
+    takes two caches of one shape: both are the scales, so each word is written twice alike)."""
+    _lib.check(
+        op,
+        getattr(_lib.lib(), name)(
+            *(t.data_ptr() for t in tensors),
+            *(i.data_ptr() for i in ids),
+            int(ids[0].dtype == torch.int64),
+            ids[0].shape[0],
+            scales.shape[0],
+            scales.shape[1] * 8,
             _stream(device),
         ),
     )
@@ -172,6 +217,9 @@ def copy_blocks(buffers: KVBuffers, src: torch.Tensor, dst: torch.Tensor) -> Non
             _stream(device),
         ),
     )
+    scales = block_scales(buffers)
+    if scales is not None:
+        _move_scales(op, "ayk_copy_blocks", (scales, scales), (src, dst), scales, device)
 
 
 def zero_blocks(buffers: KVBuffers, block_ids: torch.Tensor) -> None:
@@ -194,3 +242,6 @@ def zero_blocks(buffers: KVBuffers, block_ids: torch.Tensor) -> None:
             _stream(device),
         ),
     )
+    scales = block_scales(buffers)
+    if scales is not None:
+        _move_scales(op, "ayk_zero_blocks", (scales, scales), (block_ids,), scales, device)

@@ -16,7 +16,11 @@ Restates the reference's layout definition (``python/ayaka/ops/kvcache.py:1-38``
   torch's cast to that type gives (round to nearest even; a magnitude that
   rounds above 448 becomes NaN); readers decode it exactly to the compute dtype.
   A layer may carry a key and a value scale (:func:`fp8_e4m3_codec`): the codes
-  are then those of ``x / scale`` and readers multiply by the scale.
+  are then those of ``x / scale`` and readers multiply by the scale. It also adds
+  ``"fp8_e4m3_block"`` (:func:`fp8_e4m3_block_codec`): the same codes under a key
+  scale and a value scale for every block and key/value head, which the KV write
+  settles from the values themselves, so nothing is calibrated and no finite value
+  becomes NaN.
 
 Importing this module does not import torch.
 """
@@ -32,11 +36,24 @@ if TYPE_CHECKING:
 
     from ayaka_amd.attention import AttentionMetadata
 
-__all__ = ["FP8_E4M3_CODEC", "RAW_CODEC", "KVBuffers", "KVCacheOps", "ScaledFp8Codec", "codec_scales", "fp8_e4m3_codec"]
+__all__ = [
+    "FP8_E4M3_BLOCK_CODEC",
+    "FP8_E4M3_CODEC",
+    "RAW_CODEC",
+    "BlockScaledFp8Codec",
+    "KVBuffers",
+    "KVCacheOps",
+    "ScaledFp8Codec",
+    "codec_scales",
+    "fp8_e4m3_block_codec",
+    "fp8_e4m3_codec",
+]
 
 RAW_CODEC = "raw"
 #: Keys and values as OCP fp8 e4m3 codes (``torch.float8_e4m3fn``), no scale.
 FP8_E4M3_CODEC = "fp8_e4m3"
+#: The same codes with a key and a value scale for every block and key/value head.
+FP8_E4M3_BLOCK_CODEC = "fp8_e4m3_block"
 
 
 class ScaledFp8Codec(str):
@@ -79,8 +96,58 @@ def fp8_e4m3_codec(k_scale: float = 1.0, v_scale: float = 1.0) -> ScaledFp8Codec
     return ScaledFp8Codec(k_scale, v_scale)
 
 
+class BlockScaledFp8Codec(str):
+    """The ``"fp8_e4m3_block"`` codec of one layer, carrying the scales of its cache.
+
+    It is the string ``"fp8_e4m3_block"`` (equal to :data:`FP8_E4M3_BLOCK_CODEC`) with
+    ``scales``, a contiguous float32 ``[num_blocks, kv_heads, 2]`` tensor on the cache's device:
+    the key scale and the value scale of every block and key/value head. An element is worth
+    ``code * scale``. Scales are powers of two 2^e with -40 <= e <= 80, the least that keeps the
+    largest finite magnitude a block holds within 448 codes, or 0 for a block of nothing but
+    zeros; a fresh cache starts with zeros. ``store`` settles them as it writes: the first token
+    of a block starts its scale afresh, and a later one that needs a larger scale re-encodes the
+    block's tokens (a power of two apart, so exactly, down to the codes' subnormals).
+
+    Storing infinities and NaN gives the NaN code and leaves the scale to the finite values.
+    A layer's copy, swap and clear move the scales with the blocks (``copy_blocks``,
+    ``gather(..., out_scales=)``, ``zero_blocks``).
+    """
+
+    __slots__ = ("_scales",)
+
+    def __new__(cls, scales: "Tensor") -> "BlockScaledFp8Codec":
+        import torch
+
+        if scales.dtype != torch.float32 or scales.ndim != 3 or scales.shape[2] != 2 or not scales.is_contiguous():
+            raise ValueError(
+                "scales must be a contiguous float32 [num_blocks, kv_heads, 2] tensor, got "
+                f"{str(scales.dtype).removeprefix('torch.')} {list(scales.shape)}"
+            )
+        codec = super().__new__(cls, FP8_E4M3_BLOCK_CODEC)
+        codec._scales = scales
+        return codec
+
+    @property
+    def scales(self) -> "Tensor":
+        return self._scales
+
+    def __repr__(self) -> str:
+        return f"fp8_e4m3_block_codec(scales={list(self._scales.shape)} on {self._scales.device})"
+
+    def __reduce__(self):
+        return (BlockScaledFp8Codec, (self._scales,))
+
+
+def fp8_e4m3_block_codec(scales: "Tensor") -> BlockScaledFp8Codec:
+    """The ``"fp8_e4m3_block"`` codec of a layer whose blocks have these scales (see
+    :class:`BlockScaledFp8Codec`); ``torch.zeros(num_blocks, kv_heads, 2)`` on the cache's device
+    for a fresh cache."""
+    return BlockScaledFp8Codec(scales)
+
+
 def codec_scales(codec: str) -> tuple[float, float]:
-    """``(k_scale, v_scale)`` of a codec: its own for a :class:`ScaledFp8Codec`, else (1, 1)."""
+    """``(k_scale, v_scale)`` of a codec: its own for a :class:`ScaledFp8Codec`, else (1, 1) (a
+    :class:`BlockScaledFp8Codec` has none for the whole layer)."""
     return (getattr(codec, "k_scale", 1.0), getattr(codec, "v_scale", 1.0))
 
 
