@@ -73,6 +73,8 @@ struct AttnCall {
       dtype, kv_dtype;
   float scale;
   float k_scale, v_scale;  // the cache holds keys / k_scale and values / v_scale (1, 1: as they are)
+  bool scaled = false;     // a block-scaled cache (kv_dtype fp8 e4m3, both scales 1), with
+  const float* block_scales = nullptr;  // these scales
 };
 
 // Check a call and fill the launch record; returns AYK_OK or an error code.
@@ -104,6 +106,9 @@ int prepare(const char* op, const AttnCall& c, ayk::AttnParams& p, int& heads_pe
   if (c.n_rows > 0 && (!c.out || !c.q || !c.k_cache || !c.v_cache || !c.block_table ||
                        !c.kv_lengths))
     return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  if (c.scaled && c.n_rows > 0 && (!c.block_scales || reinterpret_cast<uintptr_t>(c.block_scales) % 8 != 0))
+    return fail(AYK_ERR_ARGUMENT, "%s: block_scales at %p is null or not 8-byte aligned", op,
+                (const void*)c.block_scales);
   const int group = c.num_heads / c.num_kv_heads;
   const int chunks = head_chunks_for(group);
   heads_per_chunk = group / chunks;
@@ -157,6 +162,7 @@ int prepare(const char* op, const AttnCall& c, ayk::AttnParams& p, int& heads_pe
   // (exact at k_scale 1), and a value's scale multiplies each normalised output.
   p.scale_log2 = c.scale * c.k_scale * 1.4426950408889634f;
   p.v_scale = c.v_scale;
+  p.block_scales = c.block_scales;
   p.partition_size = INT32_MAX;
   p.max_partitions = 1;
   p.wave_split = 1;
@@ -288,8 +294,9 @@ int launch(const char* op, const ayk::AttnParams& p, int head_dim, int gc, bool 
     return ok();
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t err = mfma ? ayk::launch_attention_mfma(q, head_dim, gc, bf16, split, kv8, waves, s)
-                        : ayk::launch_attention_dpp(q, head_dim, gc, bf16, split, waves, s);
+  hipError_t err = q.block_scales ? ayk::launch_attention_block_scaled(q, head_dim, gc, bf16, split, s)
+                   : mfma         ? ayk::launch_attention_mfma(q, head_dim, gc, bf16, split, kv8, waves, s)
+                                  : ayk::launch_attention_dpp(q, head_dim, gc, bf16, split, waves, s);
   if (err == hipSuccess && split && !q.arrivals && !(flags & AYK_FLAG_PARTIALS_ONLY))
     err = ayk::launch_partition_reduce(q, head_dim, bf16, compute_units(), s);
   return launched(err, op);
@@ -340,6 +347,230 @@ void* static_scratch(const char* op, void* stream) {
   }
   g_scratch_ptr[dev].store(ptr, std::memory_order_release);  // two threads may race here: same address
   return ptr;
+}
+
+// The body of ayk_paged_attention_v1 and its block-scaled form.
+int attend_v1(const char* op, const AttnCall& c, int32_t flags, void* stream) {
+  ayk::AttnParams p;
+  int gc = 0;
+  const int rc = prepare(op, c, p, gc);
+  if (rc != AYK_OK) return rc;
+  if (c.n_rows == 0) return ok();
+  if (c.dtype == AYK_DTYPE_FP32) return launch_f32(op, p, c.head_dim, gc, false, flags, stream);
+  return launch(op, p, c.head_dim, gc, c.dtype == AYK_DTYPE_BF16, c.kv_dtype == AYK_DTYPE_FP8_E4M3, false, flags,
+                stream);
+}
+
+// The body of ayk_paged_attention_v2 and its block-scaled form.
+int attend_v2(const char* op, const AttnCall& c, int32_t partition_size, int32_t max_partitions,
+              const int32_t* work_items, int32_t n_work_items, const int32_t* staged, void* workspace,
+              size_t workspace_bytes, uint32_t* arrivals, int32_t flags, void* stream) {
+  ayk::AttnParams p;
+  int gc = 0;
+  const int rc = prepare(op, c, p, gc);
+  if (rc != AYK_OK) return rc;
+  if (partition_size <= 0 || partition_size % 64 != 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: partition_size %d is not a positive multiple of 64", op,
+                partition_size);
+  if (max_partitions <= 0 || max_partitions > 65535)
+    return fail(AYK_ERR_ARGUMENT, "%s: max_partitions %d is not in [1, 65535]", op, max_partitions);
+  if (n_work_items < 0 || (n_work_items > 0 && !work_items))
+    return fail(AYK_ERR_ARGUMENT, "%s: %d work items at %p", op, n_work_items, (const void*)work_items);
+  if (staged && n_work_items == 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: staged parameters need a work list (the grid's capacity)", op);
+  if (c.n_rows == 0) return ok();
+  // Staged parameters pack the rows' partials: at most one slot per work item.
+  const int32_t slot_rows = staged ? n_work_items : c.n_rows;
+  const int32_t slots_per_row = staged ? 1 : max_partitions;
+  const size_t need = ayk_paged_attention_v2_workspace_bytes(slot_rows, c.num_heads, c.head_dim, slots_per_row);
+  if (!workspace || workspace_bytes < need)
+    return fail(AYK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes,
+                need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: workspace is not 16-byte aligned", op);
+  const size_t parts = (size_t)slot_rows * c.num_heads * slots_per_row;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + parts * c.head_dim;
+  p.partition_size = partition_size;
+  p.max_partitions = max_partitions;
+  p.work = n_work_items > 0 ? work_items : nullptr;
+  p.n_work = n_work_items;
+  p.staged = staged;
+  // The single launch merges in the partition kernel; without counters, or when
+  // asked, a reduce kernel does (and PARTIALS_ONLY runs neither merge).
+  p.arrivals = (flags & (AYK_FLAG_SEPARATE_REDUCE | AYK_FLAG_PARTIALS_ONLY)) ? nullptr : arrivals;
+  p.max_len = (int32_t)std::min<int64_t>(p.max_len, (int64_t)partition_size * max_partitions);
+  if (c.dtype == AYK_DTYPE_FP32) return launch_f32(op, p, c.head_dim, gc, true, flags, stream);
+  return launch(op, p, c.head_dim, gc, c.dtype == AYK_DTYPE_BF16, c.kv_dtype == AYK_DTYPE_FP8_E4M3, true, flags,
+                stream);
+}
+
+// The body of ayk_paged_prefill and its block-scaled form.
+int attend_prefill(const char* op, const AttnCall& c, const int32_t* tiles, int32_t n_tiles, int32_t tile_pairs,
+                   int32_t partition_size, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!c.request_of_row || !c.positions)
+    return fail(AYK_ERR_ARGUMENT, "%s: request_of_row and positions are required", op);
+  ayk::AttnParams p;
+  int gc = 0;
+  const int rc = prepare(op, c, p, gc);
+  if (rc != AYK_OK) return rc;
+  if (c.dtype == AYK_DTYPE_FP32)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: fp32 runs on the decode entry points (multi-row steps too)", op);
+  // Tiles of the full capacity, or of a half or a quarter (2 or 4 waves then share
+  // each group of pairs and split its chunks), or at head_dim 128 and 256 of twice it (an
+  // 8-wave workgroup; waves_per_group 0 below).
+  const int full_pairs = ayk::prefill_tile_pairs_for(c.head_dim);
+  const bool twice = c.head_dim != 64 && tile_pairs == 2 * full_pairs;
+  const int waves_per_group = twice ? 0 : tile_pairs > 0 && full_pairs % tile_pairs == 0 ? full_pairs / tile_pairs : -1;
+  if (waves_per_group != 0 && waves_per_group != 1 && waves_per_group != 2 && waves_per_group != 4)
+    return fail(AYK_ERR_ARGUMENT, "%s: tile_pairs %d is not %d, %d or %d%s", op, tile_pairs, full_pairs,
+                full_pairs / 2, full_pairs / 4, c.head_dim != 64 ? " (or twice the first)" : "");
+  if (p.group > tile_pairs)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %d query heads per key/value head exceed a tile of %d", op, p.group,
+                tile_pairs);
+  if (n_tiles < 0 || (n_tiles > 0 && !tiles))
+    return fail(AYK_ERR_ARGUMENT, "%s: %d tiles at %p", op, n_tiles, (const void*)tiles);
+  if ((int64_t)n_tiles * c.num_kv_heads > INT32_MAX)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %d tiles x %d key/value heads exceed one launch", op, n_tiles,
+                c.num_kv_heads);
+  if (partition_size < 0 || partition_size % 64 != 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: partition_size %d is not 0 or a positive multiple of 64", op,
+                partition_size);
+  if (n_tiles == 0 || c.n_rows == 0) return ok();
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool walk = ayk::walking();  // the host address walk: the launch's loads, no launch
+  // bf16 models over bf16 caches: a workspace with room for one int32 per workgroup (after the
+  // partials, 16-byte aligned) lets the kernel run P.V in fp16 where the values allow and hand
+  // the other workgroups to a bf16 pass (the slots need no initial contents)
+  size_t partial_bytes = 0;
+  if (partition_size > 0) {
+    const int64_t parts = ((int64_t)p.max_len + partition_size - 1) / partition_size;
+    if (parts >= 1 && parts <= 65535)
+      partial_bytes = (ayk_paged_attention_v2_workspace_bytes(c.n_rows, c.num_heads, c.head_dim, (int32_t)parts) + 15) & ~size_t(15);
+  }
+  const size_t flag_bytes = (size_t)n_tiles * c.num_kv_heads * sizeof(uint32_t);
+  if (c.dtype == AYK_DTYPE_BF16 && c.kv_dtype == AYK_DTYPE_BF16 && workspace && workspace_bytes >= partial_bytes + flag_bytes &&
+      reinterpret_cast<uintptr_t>(workspace) % 16 == 0)
+    p.arrivals = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + partial_bytes);
+  if (partition_size == 0 && walk) {
+    ayk::walk_prefill(p, tiles, n_tiles, c.head_dim, c.kv_dtype == AYK_DTYPE_FP8_E4M3, waves_per_group);
+    return ok();
+  }
+  const bool bf16 = c.dtype == AYK_DTYPE_BF16;
+  auto launch_tiles = [&] {
+    return p.block_scales
+               ? ayk::launch_prefill_block_scaled(p, tiles, n_tiles, c.head_dim, bf16, waves_per_group, s)
+               : ayk::launch_prefill(p, tiles, n_tiles, c.head_dim, bf16, c.kv_dtype == AYK_DTYPE_FP8_E4M3,
+                                     waves_per_group, s);
+  };
+  if (partition_size == 0) return launched(launch_tiles(), op);
+  const int64_t max_partitions = ((int64_t)p.max_len + partition_size - 1) / partition_size;
+  if (max_partitions < 1 || max_partitions > 65535)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %lld partitions of %d positions per row are not in [1, 65535]", op,
+                (long long)max_partitions, partition_size);
+  const size_t need = ayk_paged_attention_v2_workspace_bytes(c.n_rows, c.num_heads, c.head_dim, (int32_t)max_partitions);
+  if (!workspace || workspace_bytes < need)
+    return fail(AYK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: workspace is not 16-byte aligned", op);
+  const size_t parts = (size_t)c.n_rows * c.num_heads * max_partitions;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + parts * c.head_dim;
+  p.partition_size = partition_size;
+  p.max_partitions = (int32_t)max_partitions;
+  if (walk) {
+    ayk::walk_prefill(p, tiles, n_tiles, c.head_dim, c.kv_dtype == AYK_DTYPE_FP8_E4M3, waves_per_group);
+    return ok();
+  }
+  hipError_t err = launch_tiles();
+  if (err == hipSuccess) err = ayk::launch_row_reduce(p, c.head_dim, bf16, s);
+  return launched(err, op);
+}
+
+// The body of ayk_paged_attention_windows and its block-scaled form.
+int attend_windows(const char* op, const AttnCall& c, const int32_t* tiles, int32_t n_tiles, int32_t partition_size,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (!c.request_of_row || !c.positions)
+    return fail(AYK_ERR_ARGUMENT, "%s: request_of_row and positions are required", op);
+  ayk::AttnParams p;
+  int gc = 0;
+  const int rc = prepare(op, c, p, gc);
+  if (rc != AYK_OK) return rc;
+  if (c.dtype == AYK_DTYPE_FP32)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: fp32 runs on the decode entry points (multi-row steps too)", op);
+  if (p.group > 16)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %d query heads per key/value head exceed a window's 16 columns", op,
+                p.group);
+  if (n_tiles < 0 || (n_tiles > 0 && !tiles))
+    return fail(AYK_ERR_ARGUMENT, "%s: %d tiles at %p", op, n_tiles, (const void*)tiles);
+  if ((int64_t)n_tiles * c.num_kv_heads > INT32_MAX)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %d tiles x %d key/value heads exceed one launch", op, n_tiles,
+                c.num_kv_heads);
+  if (partition_size < 0 || partition_size % 64 != 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: partition_size %d is not 0 or a positive multiple of 64", op,
+                partition_size);
+  if (n_tiles == 0 || c.n_rows == 0) return ok();
+  // one wave per key/value head, its 16 columns the tile's (row, query head) pairs
+  p.head_chunks = 1;
+  p.num_virtual_heads = c.num_kv_heads;
+  p.work = tiles;
+  p.n_work = n_tiles;
+  p.arrivals = nullptr;
+  // Few tiles leave compute units idle: each key/value head of a tile then gets up to 8
+  // waves, which take every n-th chunk and merge in LDS (as v1 does for decode rows),
+  // the most that keep the launch within one round of 8-wave workgroups. Measured
+  // (µs, one wave -> the chosen split, library partitions): 16 x 4-row windows over 1K
+  // 33.8 -> 20.2, 32 x 4 over 4K 97.9 -> 89.7, 64 x 2 over 2K 89.2 -> 82.1.
+  p.wave_split = 1;
+  {
+    const int64_t slots = (int64_t)compute_units() * ayk::kMaxWavesPerGroup;
+    while (p.wave_split < ayk::kMaxWavesPerGroup && (int64_t)n_tiles * c.num_kv_heads * p.wave_split * 2 <= slots)
+      p.wave_split *= 2;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool bf16 = c.dtype == AYK_DTYPE_BF16, kv8 = c.kv_dtype == AYK_DTYPE_FP8_E4M3;
+  const bool walk = ayk::walking();  // the host address walk: the launch's loads, no launch
+  if (partition_size == 0 && walk) {
+    ayk::walk_decode(p, c.head_dim, true, kv8, false, true);
+    return ok();
+  }
+  auto launch_windows = [&](bool split) {
+    return p.block_scales ? ayk::launch_window_block_scaled(p, c.head_dim, bf16, split, s)
+                          : ayk::launch_window_mfma(p, c.head_dim, bf16, split, kv8, s);
+  };
+  if (partition_size == 0) return launched(launch_windows(false), op);
+  const int64_t max_partitions = ((int64_t)p.max_len + partition_size - 1) / partition_size;
+  if (max_partitions < 1 || max_partitions > 65535)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %lld partitions of %d positions per row are not in [1, 65535]", op,
+                (long long)max_partitions, partition_size);
+  const size_t need = ayk_paged_attention_v2_workspace_bytes(c.n_rows, c.num_heads, c.head_dim, (int32_t)max_partitions);
+  if (!workspace || workspace_bytes < need)
+    return fail(AYK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: workspace is not 16-byte aligned", op);
+  const size_t parts = (size_t)c.n_rows * c.num_heads * max_partitions;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + parts * c.head_dim;
+  p.partition_size = partition_size;
+  p.max_partitions = (int32_t)max_partitions;
+  if (walk) {
+    ayk::walk_decode(p, c.head_dim, true, kv8, true, true);
+    return ok();
+  }
+  hipError_t err = launch_windows(true);
+  if (err == hipSuccess) err = ayk::launch_row_reduce(p, c.head_dim, bf16, s);
+  return launched(err, op);
+}
+
+// A call of a block-scaled entry point: fp8 codes, the layer's scales 1, every block's own beside them.
+AttnCall block_scaled_call(void* out, const void* q, const void* k_cache, const void* v_cache, const float* scales,
+                           const int32_t* block_table, int64_t table_stride, const int32_t* kv_lengths,
+                           const int32_t* request_of_row, const int32_t* positions, int32_t n_rows, int32_t num_heads,
+                           int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+                           int32_t max_blocks, int32_t layout, int32_t dtype, float scale) {
+  return AttnCall{out, q, k_cache, v_cache, block_table, table_stride, kv_lengths, request_of_row, positions,
+                  n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, layout,
+                  dtype, AYK_DTYPE_FP8_E4M3, scale, 1.f, 1.f, true, scales};
 }
 
 }  // namespace
@@ -442,18 +673,11 @@ int ayk_paged_attention_v1(void* out, const void* q, const void* k_cache, const 
                            int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks,
                            int32_t block_size, int32_t max_blocks, int32_t layout, int32_t dtype,
                            int32_t kv_dtype, float scale, float k_scale, float v_scale, int32_t flags, void* stream) {
-  const char* op = "ayk_paged_attention_v1";
-  AttnCall c{out,       q,          k_cache,  v_cache,      block_table, table_stride,
-             kv_lengths, request_of_row, positions, n_rows, num_heads, num_kv_heads,
-             head_dim,  num_blocks, block_size, max_blocks, layout, dtype, kv_dtype, scale, k_scale, v_scale};
-  ayk::AttnParams p;
-  int gc = 0;
-  const int rc = prepare(op, c, p, gc);
-  if (rc != AYK_OK) return rc;
-  if (n_rows == 0) return ok();
-  if (dtype == AYK_DTYPE_FP32) return launch_f32(op, p, head_dim, gc, false, flags, stream);
-  return launch(op, p, head_dim, gc, dtype == AYK_DTYPE_BF16, kv_dtype == AYK_DTYPE_FP8_E4M3, false, flags,
-                stream);
+  return attend_v1("ayk_paged_attention_v1",
+                   AttnCall{out, q, k_cache, v_cache, block_table, table_stride, kv_lengths, request_of_row, positions,
+                            n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, layout,
+                            dtype, kv_dtype, scale, k_scale, v_scale},
+                   flags, stream);
 }
 
 size_t ayk_paged_attention_v2_workspace_bytes(int32_t n_rows, int32_t num_heads, int32_t head_dim,
@@ -474,48 +698,12 @@ int ayk_paged_attention_v2(void* out, const void* q, const void* k_cache, const 
                            const int32_t* work_items, int32_t n_work_items, const int32_t* staged,
                            void* workspace, size_t workspace_bytes, uint32_t* arrivals, int32_t flags,
                            void* stream) {
-  const char* op = "ayk_paged_attention_v2";
-  AttnCall c{out,       q,          k_cache,  v_cache,      block_table, table_stride,
-             kv_lengths, request_of_row, positions, n_rows, num_heads, num_kv_heads,
-             head_dim,  num_blocks, block_size, max_blocks, layout, dtype, kv_dtype, scale, k_scale, v_scale};
-  ayk::AttnParams p;
-  int gc = 0;
-  const int rc = prepare(op, c, p, gc);
-  if (rc != AYK_OK) return rc;
-  if (partition_size <= 0 || partition_size % 64 != 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: partition_size %d is not a positive multiple of 64", op,
-                partition_size);
-  if (max_partitions <= 0 || max_partitions > 65535)
-    return fail(AYK_ERR_ARGUMENT, "%s: max_partitions %d is not in [1, 65535]", op, max_partitions);
-  if (n_work_items < 0 || (n_work_items > 0 && !work_items))
-    return fail(AYK_ERR_ARGUMENT, "%s: %d work items at %p", op, n_work_items, (const void*)work_items);
-  if (staged && n_work_items == 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: staged parameters need a work list (the grid's capacity)", op);
-  if (n_rows == 0) return ok();
-  // Staged parameters pack the rows' partials: at most one slot per work item.
-  const int32_t slot_rows = staged ? n_work_items : n_rows;
-  const int32_t slots_per_row = staged ? 1 : max_partitions;
-  const size_t need = ayk_paged_attention_v2_workspace_bytes(slot_rows, num_heads, head_dim, slots_per_row);
-  if (!workspace || workspace_bytes < need)
-    return fail(AYK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes,
-                need);
-  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: workspace is not 16-byte aligned", op);
-  const size_t parts = (size_t)slot_rows * num_heads * slots_per_row;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + parts * head_dim;
-  p.partition_size = partition_size;
-  p.max_partitions = max_partitions;
-  p.work = n_work_items > 0 ? work_items : nullptr;
-  p.n_work = n_work_items;
-  p.staged = staged;
-  // The single launch merges in the partition kernel; without counters, or when
-  // asked, a reduce kernel does (and PARTIALS_ONLY runs neither merge).
-  p.arrivals = (flags & (AYK_FLAG_SEPARATE_REDUCE | AYK_FLAG_PARTIALS_ONLY)) ? nullptr : arrivals;
-  p.max_len = (int32_t)std::min<int64_t>(p.max_len, (int64_t)partition_size * max_partitions);
-  if (dtype == AYK_DTYPE_FP32) return launch_f32(op, p, head_dim, gc, true, flags, stream);
-  return launch(op, p, head_dim, gc, dtype == AYK_DTYPE_BF16, kv_dtype == AYK_DTYPE_FP8_E4M3, true, flags,
-                stream);
+  return attend_v2("ayk_paged_attention_v2",
+                   AttnCall{out, q, k_cache, v_cache, block_table, table_stride, kv_lengths, request_of_row, positions,
+                            n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, layout,
+                            dtype, kv_dtype, scale, k_scale, v_scale},
+                   partition_size, max_partitions, work_items, n_work_items, staged, workspace, workspace_bytes,
+                   arrivals, flags, stream);
 }
 
 int ayk_paged_attention_v2_static(void* out, const void* q, const void* k_cache, const void* v_cache,
@@ -570,84 +758,11 @@ int ayk_paged_prefill(void* out, const void* q, const void* k_cache, const void*
                       int32_t num_blocks, int32_t block_size, int32_t max_blocks, int32_t layout, int32_t dtype,
                       int32_t kv_dtype, float scale, float k_scale, float v_scale, int32_t partition_size, void* workspace,
                       size_t workspace_bytes, void* stream) {
-  const char* op = "ayk_paged_prefill";
-  if (!request_of_row || !positions)
-    return fail(AYK_ERR_ARGUMENT, "%s: request_of_row and positions are required", op);
-  AttnCall c{out,       q,          k_cache,  v_cache,      block_table, table_stride,
-             kv_lengths, request_of_row, positions, n_rows, num_heads, num_kv_heads,
-             head_dim,  num_blocks, block_size, max_blocks, layout,      dtype,       kv_dtype, scale, k_scale, v_scale};
-  ayk::AttnParams p;
-  int gc = 0;
-  const int rc = prepare(op, c, p, gc);
-  if (rc != AYK_OK) return rc;
-  if (dtype == AYK_DTYPE_FP32)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: fp32 runs on the decode entry points (multi-row steps too)", op);
-  // Tiles of the full capacity, or of a half or a quarter (2 or 4 waves then share
-  // each group of pairs and split its chunks), or at head_dim 128 and 256 of twice it (an
-  // 8-wave workgroup; waves_per_group 0 below).
-  const int full_pairs = ayk::prefill_tile_pairs_for(head_dim);
-  const bool twice = head_dim != 64 && tile_pairs == 2 * full_pairs;
-  const int waves_per_group = twice ? 0 : tile_pairs > 0 && full_pairs % tile_pairs == 0 ? full_pairs / tile_pairs : -1;
-  if (waves_per_group != 0 && waves_per_group != 1 && waves_per_group != 2 && waves_per_group != 4)
-    return fail(AYK_ERR_ARGUMENT, "%s: tile_pairs %d is not %d, %d or %d%s", op, tile_pairs, full_pairs,
-                full_pairs / 2, full_pairs / 4, head_dim != 64 ? " (or twice the first)" : "");
-  if (p.group > tile_pairs)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: %d query heads per key/value head exceed a tile of %d", op, p.group,
-                tile_pairs);
-  if (n_tiles < 0 || (n_tiles > 0 && !tiles))
-    return fail(AYK_ERR_ARGUMENT, "%s: %d tiles at %p", op, n_tiles, (const void*)tiles);
-  if ((int64_t)n_tiles * num_kv_heads > INT32_MAX)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: %d tiles x %d key/value heads exceed one launch", op, n_tiles,
-                num_kv_heads);
-  if (partition_size < 0 || partition_size % 64 != 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: partition_size %d is not 0 or a positive multiple of 64", op,
-                partition_size);
-  if (n_tiles == 0 || n_rows == 0) return ok();
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool walk = ayk::walking();  // the host address walk: the launch's loads, no launch
-  // bf16 models over bf16 caches: a workspace with room for one int32 per workgroup (after the
-  // partials, 16-byte aligned) lets the kernel run P.V in fp16 where the values allow and hand
-  // the other workgroups to a bf16 pass (the slots need no initial contents)
-  size_t partial_bytes = 0;
-  if (partition_size > 0) {
-    const int64_t parts = ((int64_t)p.max_len + partition_size - 1) / partition_size;
-    if (parts >= 1 && parts <= 65535)
-      partial_bytes = (ayk_paged_attention_v2_workspace_bytes(n_rows, num_heads, head_dim, (int32_t)parts) + 15) & ~size_t(15);
-  }
-  const size_t flag_bytes = (size_t)n_tiles * num_kv_heads * sizeof(uint32_t);
-  if (dtype == AYK_DTYPE_BF16 && kv_dtype == AYK_DTYPE_BF16 && workspace && workspace_bytes >= partial_bytes + flag_bytes &&
-      reinterpret_cast<uintptr_t>(workspace) % 16 == 0)
-    p.arrivals = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + partial_bytes);
-  if (partition_size == 0 && walk) {
-    ayk::walk_prefill(p, tiles, n_tiles, head_dim, kv_dtype == AYK_DTYPE_FP8_E4M3, waves_per_group);
-    return ok();
-  }
-  if (partition_size == 0)
-    return launched(ayk::launch_prefill(p, tiles, n_tiles, head_dim, dtype == AYK_DTYPE_BF16,
-                                        kv_dtype == AYK_DTYPE_FP8_E4M3, waves_per_group, s),
-                    op);
-  const int64_t max_partitions = ((int64_t)p.max_len + partition_size - 1) / partition_size;
-  if (max_partitions < 1 || max_partitions > 65535)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: %lld partitions of %d positions per row are not in [1, 65535]", op,
-                (long long)max_partitions, partition_size);
-  const size_t need = ayk_paged_attention_v2_workspace_bytes(n_rows, num_heads, head_dim, (int32_t)max_partitions);
-  if (!workspace || workspace_bytes < need)
-    return fail(AYK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
-  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: workspace is not 16-byte aligned", op);
-  const size_t parts = (size_t)n_rows * num_heads * max_partitions;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + parts * head_dim;
-  p.partition_size = partition_size;
-  p.max_partitions = (int32_t)max_partitions;
-  if (walk) {
-    ayk::walk_prefill(p, tiles, n_tiles, head_dim, kv_dtype == AYK_DTYPE_FP8_E4M3, waves_per_group);
-    return ok();
-  }
-  hipError_t err = ayk::launch_prefill(p, tiles, n_tiles, head_dim, dtype == AYK_DTYPE_BF16,
-                                       kv_dtype == AYK_DTYPE_FP8_E4M3, waves_per_group, s);
-  if (err == hipSuccess) err = ayk::launch_row_reduce(p, head_dim, dtype == AYK_DTYPE_BF16, s);
-  return launched(err, op);
+  return attend_prefill("ayk_paged_prefill",
+                        AttnCall{out, q, k_cache, v_cache, block_table, table_stride, kv_lengths, request_of_row, positions,
+                                 n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, layout,
+                                 dtype, kv_dtype, scale, k_scale, v_scale},
+                        tiles, n_tiles, tile_pairs, partition_size, workspace, workspace_bytes, stream);
 }
 
 int ayk_paged_attention_windows(void* out, const void* q, const void* k_cache, const void* v_cache,
@@ -657,76 +772,73 @@ int ayk_paged_attention_windows(void* out, const void* q, const void* k_cache, c
                                 int32_t head_dim, int32_t num_blocks, int32_t block_size, int32_t max_blocks,
                                 int32_t layout, int32_t dtype, int32_t kv_dtype, float scale, float k_scale, float v_scale, int32_t partition_size,
                                 void* workspace, size_t workspace_bytes, void* stream) {
-  const char* op = "ayk_paged_attention_windows";
-  if (!request_of_row || !positions)
-    return fail(AYK_ERR_ARGUMENT, "%s: request_of_row and positions are required", op);
-  AttnCall c{out,       q,          k_cache,  v_cache,      block_table, table_stride,
-             kv_lengths, request_of_row, positions, n_rows, num_heads, num_kv_heads,
-             head_dim,  num_blocks, block_size, max_blocks, layout,      dtype,       kv_dtype, scale, k_scale, v_scale};
-  ayk::AttnParams p;
-  int gc = 0;
-  const int rc = prepare(op, c, p, gc);
-  if (rc != AYK_OK) return rc;
-  if (dtype == AYK_DTYPE_FP32)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: fp32 runs on the decode entry points (multi-row steps too)", op);
-  if (p.group > 16)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: %d query heads per key/value head exceed a window's 16 columns", op,
-                p.group);
-  if (n_tiles < 0 || (n_tiles > 0 && !tiles))
-    return fail(AYK_ERR_ARGUMENT, "%s: %d tiles at %p", op, n_tiles, (const void*)tiles);
-  if ((int64_t)n_tiles * num_kv_heads > INT32_MAX)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: %d tiles x %d key/value heads exceed one launch", op, n_tiles,
-                num_kv_heads);
-  if (partition_size < 0 || partition_size % 64 != 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: partition_size %d is not 0 or a positive multiple of 64", op,
-                partition_size);
-  if (n_tiles == 0 || n_rows == 0) return ok();
-  // one wave per key/value head, its 16 columns the tile's (row, query head) pairs
-  p.head_chunks = 1;
-  p.num_virtual_heads = num_kv_heads;
-  p.work = tiles;
-  p.n_work = n_tiles;
-  p.arrivals = nullptr;
-  // Few tiles leave compute units idle: each key/value head of a tile then gets up to 8
-  // waves, which take every n-th chunk and merge in LDS (as v1 does for decode rows),
-  // the most that keep the launch within one round of 8-wave workgroups. Measured
-  // (µs, one wave -> the chosen split, library partitions): 16 x 4-row windows over 1K
-  // 33.8 -> 20.2, 32 x 4 over 4K 97.9 -> 89.7, 64 x 2 over 2K 89.2 -> 82.1.
-  p.wave_split = 1;
-  {
-    const int64_t slots = (int64_t)compute_units() * ayk::kMaxWavesPerGroup;
-    while (p.wave_split < ayk::kMaxWavesPerGroup && (int64_t)n_tiles * num_kv_heads * p.wave_split * 2 <= slots)
-      p.wave_split *= 2;
-  }
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool bf16 = dtype == AYK_DTYPE_BF16, kv8 = kv_dtype == AYK_DTYPE_FP8_E4M3;
-  const bool walk = ayk::walking();  // the host address walk: the launch's loads, no launch
-  if (partition_size == 0 && walk) {
-    ayk::walk_decode(p, head_dim, true, kv8, false, true);
-    return ok();
-  }
-  if (partition_size == 0) return launched(ayk::launch_window_mfma(p, head_dim, bf16, false, kv8, s), op);
-  const int64_t max_partitions = ((int64_t)p.max_len + partition_size - 1) / partition_size;
-  if (max_partitions < 1 || max_partitions > 65535)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: %lld partitions of %d positions per row are not in [1, 65535]", op,
-                (long long)max_partitions, partition_size);
-  const size_t need = ayk_paged_attention_v2_workspace_bytes(n_rows, num_heads, head_dim, (int32_t)max_partitions);
-  if (!workspace || workspace_bytes < need)
-    return fail(AYK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);
-  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
-    return fail(AYK_ERR_ARGUMENT, "%s: workspace is not 16-byte aligned", op);
-  const size_t parts = (size_t)n_rows * num_heads * max_partitions;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + parts * head_dim;
-  p.partition_size = partition_size;
-  p.max_partitions = (int32_t)max_partitions;
-  if (walk) {
-    ayk::walk_decode(p, head_dim, true, kv8, true, true);
-    return ok();
-  }
-  hipError_t err = ayk::launch_window_mfma(p, head_dim, bf16, true, kv8, s);
-  if (err == hipSuccess) err = ayk::launch_row_reduce(p, head_dim, bf16, s);
-  return launched(err, op);
+  return attend_windows("ayk_paged_attention_windows",
+                        AttnCall{out, q, k_cache, v_cache, block_table, table_stride, kv_lengths, request_of_row, positions,
+                                 n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks, layout,
+                                 dtype, kv_dtype, scale, k_scale, v_scale},
+                        tiles, n_tiles, partition_size, workspace, workspace_bytes, stream);
+}
+
+int ayk_paged_attention_v1_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                        const float* scales, const int32_t* block_table, int64_t table_stride,
+                                        const int32_t* kv_lengths, const int32_t* request_of_row,
+                                        const int32_t* positions, int32_t n_rows, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+                                        int32_t max_blocks, int32_t layout, int32_t dtype, float scale, int32_t flags,
+                                        void* stream) {
+  const AttnCall c =
+      block_scaled_call(out, q, k_cache, v_cache, scales, block_table, table_stride, kv_lengths, request_of_row,
+                        positions, n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks,
+                        layout, dtype, scale);
+  return attend_v1("ayk_paged_attention_v1_block_scaled", c, flags, stream);
+}
+
+int ayk_paged_attention_v2_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                        const float* scales, const int32_t* block_table, int64_t table_stride,
+                                        const int32_t* kv_lengths, const int32_t* request_of_row,
+                                        const int32_t* positions, int32_t n_rows, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+                                        int32_t max_blocks, int32_t layout, int32_t dtype, float scale,
+                                        int32_t partition_size, int32_t max_partitions, const int32_t* work_items,
+                                        int32_t n_work_items, const int32_t* staged, void* workspace,
+                                        size_t workspace_bytes, uint32_t* arrivals, int32_t flags, void* stream) {
+  const AttnCall c =
+      block_scaled_call(out, q, k_cache, v_cache, scales, block_table, table_stride, kv_lengths, request_of_row,
+                        positions, n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks,
+                        layout, dtype, scale);
+  return attend_v2("ayk_paged_attention_v2_block_scaled", c, partition_size, max_partitions, work_items, n_work_items,
+                   staged, workspace, workspace_bytes, arrivals, flags, stream);
+}
+
+int ayk_paged_prefill_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                   const float* scales, const int32_t* block_table, int64_t table_stride,
+                                   const int32_t* kv_lengths, const int32_t* request_of_row, const int32_t* positions,
+                                   const int32_t* tiles, int32_t n_tiles, int32_t tile_pairs, int32_t n_rows,
+                                   int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks,
+                                   int32_t block_size, int32_t max_blocks, int32_t layout, int32_t dtype, float scale,
+                                   int32_t partition_size, void* workspace, size_t workspace_bytes, void* stream) {
+  const AttnCall c =
+      block_scaled_call(out, q, k_cache, v_cache, scales, block_table, table_stride, kv_lengths, request_of_row,
+                        positions, n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks,
+                        layout, dtype, scale);
+  return attend_prefill("ayk_paged_prefill_block_scaled", c, tiles, n_tiles, tile_pairs, partition_size, workspace,
+                        workspace_bytes, stream);
+}
+
+int ayk_paged_attention_windows_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                             const float* scales, const int32_t* block_table, int64_t table_stride,
+                                             const int32_t* kv_lengths, const int32_t* request_of_row,
+                                             const int32_t* positions, const int32_t* tiles, int32_t n_tiles,
+                                             int32_t n_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t num_blocks, int32_t block_size, int32_t max_blocks, int32_t layout,
+                                             int32_t dtype, float scale, int32_t partition_size, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+  const AttnCall c =
+      block_scaled_call(out, q, k_cache, v_cache, scales, block_table, table_stride, kv_lengths, request_of_row,
+                        positions, n_rows, num_heads, num_kv_heads, head_dim, num_blocks, block_size, max_blocks,
+                        layout, dtype, scale);
+  return attend_windows("ayk_paged_attention_windows_block_scaled", c, tiles, n_tiles, partition_size, workspace, workspace_bytes,
+                        stream);
 }
 
 static int block_op_checks(const char* op, int64_t n, int32_t num_blocks, int64_t block_bytes) {

@@ -7,6 +7,7 @@
 #include <cstdint>
 
 #include "ayaka_hip_internal.h"
+#include "block_scale.h"
 #include "kv_address.h"
 
 namespace ayk {
@@ -145,6 +146,64 @@ __device__ __forceinline__ typename KvRaw<KV8>::T load_kv_raw(const uint16_t* ba
   typedef typename KvRaw<KV8>::T T;
   if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p8));
   else return *reinterpret_cast<const T*>(p8);
+}
+
+// ---------------------------------------------------------------------------
+// Block-scaled fp8 caches (codec "fp8_e4m3_block", scales in block_scale.h).
+//
+// The codes go through the same products as an unscaled cache's, and the scales join the scores,
+// where there is one value per position rather than head_dim: with a key scale 2^k and a value
+// scale 2^e, position t's score (log2 domain) is 2^k scale (q . code), and
+//   out = sum_t 2^(score_t - M) 2^e_t code_t / sum_t 2^(score_t - M)
+//       = sum_t u_t code_t / sum_t u_t 2^-e_t,     u_t = 2^(score_t + e_t - m).
+// So a kernel keeps its running maximum m over score_t + e_t (one fma makes it), its weights u_t
+// stay at most 2^kRescaleSlack whatever the scales -- an fp16 P loses nothing -- and only the weight sum
+// multiplies by 2^-e_t. m and the sum describe each other as before, so merges do not change.
+// The sum cannot underflow: scales span 2^120, so a position that carries the sum has a weight of
+// 2^-120 at least.
+//
+// Per position the kernels stage {2^k scale, e, 2^-e}.
+struct PositionScale {
+  float key;    // what a raw q.k is multiplied by
+  float shift;  // e
+  float unit;   // 2^-e
+};
+
+__device__ __forceinline__ PositionScale position_scale(f32x2 s, float scale_log2) {
+  const int e = scale_exponent(s.y);
+  return PositionScale{scale_log2 * power_of_two(scale_exponent(s.x)), (float)e, power_of_two(-e)};
+}
+
+// The key and value scale of block `id` and key/value head `kvh`.
+__device__ __forceinline__ f32x2 load_block_scale(const AttnParams& p, uint32_t id, int kv_heads, int kvh) {
+  return *reinterpret_cast<const f32x2*>(p.block_scales + 2 * ((int64_t)id * kv_heads + kvh));
+}
+
+// The NaN codes (0x7f, 0xff) among 8 loaded codes, one bit each; they are replaced by zeros.
+// A masked position's weight is 0, and 0 * NaN would reach every row of its tile: where a chunk is
+// masked for some rows, the rows that do attend to such a value get their NaN from these bits.
+__device__ __forceinline__ uint32_t take_nan_codes(u32x2& w) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t n = (((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in each such byte
+    w[i] &= ~(n * 0xffu);
+    bits |= ((n | n >> 7 | n >> 14 | n >> 21) & 0xfu) << (4 * i);
+  }
+  return bits;
+}
+
+// Set the elements of o (slice t: elements 16t + 4mq + i) whose bit is set in a position's NaN
+// bits, one byte per 8 elements.
+template <int DT>
+__device__ __forceinline__ void put_nan(f32x4 (&o)[DT], const uint8_t* bits, int mq) {
+#pragma unroll
+  for (int t = 0; t < DT; ++t) {
+    const uint32_t b = (uint32_t)bits[2 * t + (mq >> 1)] >> (4 * (mq & 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((b >> i) & 1u) o[t][i] = __uint_as_float(0x7fc00000u);
+  }
 }
 
 // Loaded elements as 8 packed compute-type values (4 pairs).
@@ -445,13 +504,18 @@ __device__ __forceinline__ void store_zero_rows(const AttnParams& p, int row, in
 // Stage the block-table entries of positions [s0, s1) in LDS as element offsets
 // of their blocks (block id x block stride; ids outside the pool become the
 // padding block 0); returns the first staged block index. The host checks that
-// every offset in the pool fits 32 bits.
+// every offset in the pool fits 32 bits. IDS: the block ids too, into s_ids (the
+// scales of a block-scaled cache lie by id).
+template <bool IDS = false>
 __device__ __forceinline__ int stage_table(const AttnParams& p, const int32_t* tbl, uint32_t* s_tbl, int s0, int s1,
-                                           int tid, int threads) {
+                                           int tid, int threads, uint32_t* s_ids = nullptr) {
   const int b0 = block_of(p, s0);
   const int nb = block_of(p, s1 - 1) - b0 + 1;
   __syncthreads();  // the previous segment is done with s_tbl
-  for (int i = tid; i < nb; i += threads) s_tbl[i] = table_entry(p, tbl[b0 + i]);
+  for (int i = tid; i < nb; i += threads) {
+    s_tbl[i] = table_entry(p, tbl[b0 + i]);
+    if constexpr (IDS) s_ids[i] = block_id(p, tbl[b0 + i]);
+  }
   __syncthreads();
   return b0;
 }
@@ -484,16 +548,23 @@ __device__ __forceinline__ void table_ahead(const AttnParams& p, const int32_t* 
 
 // Stage the prefetched first segment [s0, s1) (s0 the prefetch's t_begin, s1 within its span)
 // in LDS, as stage_table does; returns its first block index.
-template <int PF>
+template <int PF, bool IDS = false>
 __device__ __forceinline__ int commit_table(const AttnParams& p, const int32_t* tbl, uint32_t* s_tbl,
-                                            const TableAhead<PF>& a, int s1, int tid, int threads) {
+                                            const TableAhead<PF>& a, int s1, int tid, int threads,
+                                            uint32_t* s_ids = nullptr) {
   const int nb = block_of(p, s1 - 1) - a.b0 + 1;
 #pragma unroll
   for (int k = 0; k < PF; ++k) {
     const int i = tid + k * threads;
-    if (i < nb) s_tbl[i] = table_entry(p, a.e[k]);
+    if (i < nb) {
+      s_tbl[i] = table_entry(p, a.e[k]);
+      if constexpr (IDS) s_ids[i] = block_id(p, a.e[k]);
+    }
   }
-  for (int i = tid + PF * threads; i < nb; i += threads) s_tbl[i] = table_entry(p, tbl[a.b0 + i]);
+  for (int i = tid + PF * threads; i < nb; i += threads) {
+    s_tbl[i] = table_entry(p, tbl[a.b0 + i]);
+    if constexpr (IDS) s_ids[i] = block_id(p, tbl[a.b0 + i]);
+  }
   __syncthreads();
   return a.b0;
 }

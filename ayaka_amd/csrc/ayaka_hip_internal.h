@@ -54,6 +54,8 @@ struct AttnParams {
                         // (1, 2, 4 or 8; a workgroup holds 8 / wave_split virtual heads)
   float scale_log2;     // scale * k_scale * log2(e): scores live in the log2 domain
   float v_scale;        // each normalised output (and partial) is multiplied by it
+  const float* block_scales;  // block-scaled fp8 caches: [num_blocks, num_kv_heads, 2] key and value
+                              // scales (k_scale and v_scale are then 1); nullptr: no such cache
 };
 
 // The per-(row, head[, partition]) attention kernels; `waves` is the workgroup size in waves.
@@ -70,6 +72,12 @@ hipError_t launch_prefill(const AttnParams& p, const int32_t* tiles, int n_tiles
 // Window launch of the decode kernel: p.work holds p.n_work tiles of the multi-row tile list
 // (first row, rows, request, partition) of at most 16 / group rows; p.head_chunks 1.
 hipError_t launch_window_mfma(const AttnParams& p, int head_dim, bool bf16, bool split, bool kv8, hipStream_t stream);
+// The same three over block-scaled fp8 caches (p.block_scales set).
+hipError_t launch_attention_block_scaled(const AttnParams& p, int head_dim, int heads_per_chunk, bool bf16, bool split,
+                                         hipStream_t stream);
+hipError_t launch_window_block_scaled(const AttnParams& p, int head_dim, bool bf16, bool split, hipStream_t stream);
+hipError_t launch_prefill_block_scaled(const AttnParams& p, const int32_t* tiles, int n_tiles, int head_dim, bool bf16,
+                                       int waves_per_group, hipStream_t stream);
 // fp32 models: the VALU decode kernel (v1, or v2 partitions) and its partition merge.
 hipError_t launch_attention_f32(const AttnParams& p, int head_dim, int heads_per_chunk, bool split,
                                 hipStream_t stream);

@@ -56,6 +56,11 @@ AYK_HD uint32_t table_entry(const AttnParams& p, int b) {
   return ((unsigned)b < (unsigned)p.num_blocks) ? (uint32_t)b * (uint32_t)p.block_stride : 0u;
 }
 
+// The block id a table entry stands for: itself, or the padding block 0 for one outside the pool.
+AYK_HD uint32_t block_id(const AttnParams& p, int b) {
+  return ((unsigned)b < (unsigned)p.num_blocks) ? (uint32_t)b : 0u;
+}
+
 // Element offset of position t in the cache, from the staged table segment that starts at
 // block b0: its block's offset plus (t mod block size) x token stride, the products on the
 // 24-bit multiplier (the block index is below the table width and the token stride below

@@ -84,6 +84,27 @@ BLOCK_SCALED_EXPORTS: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _P],
     ),
+    "ayk_paged_attention_v1_block_scaled": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P,
+         _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P],
+    ),
+    "ayk_paged_attention_v2_block_scaled": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P,
+         _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32,
+         _I32, _I32, _P, _I32, _P, _P, _SZ, _P, _I32, _P],
+    ),
+    "ayk_paged_prefill_block_scaled": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I32, _I32, _I32,
+         _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P, _SZ, _P],
+    ),
+    "ayk_paged_attention_windows_block_scaled": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P,
+         _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P, _SZ, _P],
+    ),
 }
 
 _lock = threading.Lock()

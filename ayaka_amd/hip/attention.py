@@ -19,6 +19,9 @@ steps of several rows per request (prefill chunks, verify windows) use the multi
 kernel (``ayk_paged_prefill``), where row ``j`` attends to positions
 ``0 .. position_j`` (the reference's causal rule, ``attention.py:209-234``).
 
+Block-scaled caches (codec ``"fp8_e4m3_block"``) take the same launches through the entry
+points of ``include/ayaka_hip_block_scaled.h``.
+
 ``graph_metadata`` / ``update_graph_metadata`` follow the reference's
 fixed-address record (``attention.py:274-374``): device tensors allocated once,
 host staging pinned, asynchronous copies on the current stream. Each update also
@@ -43,6 +46,7 @@ from ayaka_amd.attention import AttentionMetadata
 from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import _fastpath, _lib
 from ayaka_amd.hip._checks import (
+    block_scales,
     compute_dtype,
     HEAD_DIMS,
     capturing,
@@ -127,7 +131,29 @@ _KV_FP8_E4M3 = 2
 
 def _kv_code(buffers: KVBuffers, dtype: torch.dtype) -> int:
     """The C ABI's cache element type: the compute dtype, or fp8 e4m3 codes."""
-    return _KV_FP8_E4M3 if buffers.codec == FP8_E4M3_CODEC else _DTYPE_CODES[dtype]
+    return _KV_FP8_E4M3 if buffers.codec in (FP8_E4M3_CODEC, FP8_E4M3_BLOCK_CODEC) else _DTYPE_CODES[dtype]
+
+
+def _library_call(name: str, buffers: KVBuffers) -> ctypes._CFuncPtr:
+    """The library's attention entry point ``name`` for this cache's codec."""
+    return getattr(_lib.lib(), name if block_scales(buffers) is None else name + "_block_scaled")
+
+
+def _cache_args(buffers: KVBuffers) -> tuple[int, ...]:
+    """The entry points' cache pointers: keys, values and, of a block-scaled cache, its scales."""
+    scales = block_scales(buffers)
+    caches = (buffers.k.data_ptr(), buffers.v.data_ptr())
+    return caches if scales is None else (*caches, scales.data_ptr())
+
+
+def _scale_args(buffers: KVBuffers, dtype: torch.dtype, scale: float) -> tuple[float, ...]:
+    """The entry points' cache element type and scales (a block-scaled cache implies all but the
+    softmax scale)."""
+    if block_scales(buffers) is not None:
+        return (float(scale),)
+    return (_kv_code(buffers, dtype), float(scale), *codec_scales(buffers.codec))
+
+
 _QK_FLAGS = {None: 0, "dpp": 1, "mfma": 2}
 #: v2 flag: launch the partition kernel only (benchmarks time the dominant kernel with it).
 PARTIALS_ONLY = 4
@@ -1074,7 +1100,9 @@ def attend(
     if cache is None:
         attend_with(q, buffers, meta, out, scale=scale, partitions=None)
         return
-    key = ("attend", id(buffers), id(meta), scale, _fastpath.signature((q, out, buffers.k, buffers.v)))
+    scales = block_scales(buffers)
+    key = ("attend", id(buffers), id(meta), scale, _fastpath.signature((q, out, buffers.k, buffers.v)),
+           0 if scales is None else scales.data_ptr())
     found = _fastpath.lookup(cache, key)
     if found is not None:
         stream = stream_handle(found.device)
@@ -1129,8 +1157,6 @@ def attend_with(
     """
     op = "attention.attend"
     require_buffers(op, buffers)
-    if buffers.codec == FP8_E4M3_BLOCK_CODEC:
-        raise BackendError(f"{op}: no kernel reads block-scaled caches", context={"op": op, "argument": "buffers"})
     step = meta.plan
     table = meta.block_table
     if not isinstance(step, (HipAttentionPlan, HipGraphPlan)) or not isinstance(table, torch.Tensor):
@@ -1236,13 +1262,13 @@ def attend_with(
             nbytes = -(-nbytes // 16) * 16 + 4 * (tiles.numel() // 4) * kv_heads
         if nbytes:
             scratch = _workspace(op, device, nbytes, capturing(q), stream)
-        _call(op, lib.ayk_paged_prefill, (
-            out.data_ptr(), q.data_ptr(), buffers.k.data_ptr(), buffers.v.data_ptr(), table.data_ptr(),
+        _call(op, _library_call("ayk_paged_prefill", buffers), (
+            out.data_ptr(), q.data_ptr(), *_cache_args(buffers), table.data_ptr(),
             table.stride(0), meta.kv_lengths.data_ptr(), meta.request_of_row.data_ptr(),
             meta.positions.data_ptr(), tiles.data_ptr(), tiles.numel() // 4, pairs, n_rows, heads, kv_heads,
             buffers.head_dim, buffers.num_blocks, block_size, table.shape[1],
-            _LAYOUT_CODES[KVLayoutKind(buffers.layout)], _DTYPE_CODES[q.dtype], _kv_code(buffers, q.dtype),
-            float(scale), *codec_scales(buffers.codec), size, scratch.data_ptr() if scratch is not None else 0,
+            _LAYOUT_CODES[KVLayoutKind(buffers.layout)], _DTYPE_CODES[q.dtype],
+            *_scale_args(buffers, q.dtype, scale), size, scratch.data_ptr() if scratch is not None else 0,
             scratch.numel() if scratch is not None else 0,
         ), stream, device, scratch is not None, _record)
         return
@@ -1253,8 +1279,7 @@ def attend_with(
     common = (
         out.data_ptr(),
         q.data_ptr(),
-        buffers.k.data_ptr(),
-        buffers.v.data_ptr(),
+        *_cache_args(buffers),
         table.data_ptr(),
         table.stride(0),
         meta.kv_lengths.data_ptr(),
@@ -1269,9 +1294,7 @@ def attend_with(
         table.shape[1],
         _LAYOUT_CODES[KVLayoutKind(buffers.layout)],
         _DTYPE_CODES[q.dtype],
-        _kv_code(buffers, q.dtype),
-        float(scale),
-        *codec_scales(buffers.codec),
+        *_scale_args(buffers, q.dtype, scale),
     )
     if row_tiles:
         _call(op, lib.ayk_paged_attention_v1, (*common, ROW_TILES), stream, device, False, _record)
@@ -1305,8 +1328,8 @@ def attend_with(
         )
     flags = _QK_FLAGS[qk] | (PARTIALS_ONLY if partials_only else 0) | _MERGE_FLAGS[merge]
     if partitions == 0:
-        _call(op, lib.ayk_paged_attention_v1, (*common, flags | _WAVE_FLAGS[waves]), stream, device, False,
-              _record)
+        _call(op, _library_call("ayk_paged_attention_v1", buffers), (*common, flags | _WAVE_FLAGS[waves]), stream,
+              device, False, _record)
         return
     if staged is not None:  # the rows' partials packed into one slot per work item
         nbytes = lib.ayk_paged_attention_v2_workspace_bytes(step.capacity, heads, buffers.head_dim, 1)
@@ -1324,7 +1347,7 @@ def attend_with(
     elif isinstance(step, HipAttentionPlan) and not capturing(q):
         items = step.work_items(partition_size, device)
         work, n_work = items.data_ptr(), items.numel() // 2
-    _call(op, lib.ayk_paged_attention_v2, (
+    _call(op, _library_call("ayk_paged_attention_v2", buffers), (
         *common, partition_size, partitions, work, n_work, staged.data_ptr() if staged is not None else 0,
         scratch.data_ptr(), scratch.numel(), arrivals.data_ptr(), flags | _WAVE_FLAGS[waves],
     ), stream, device, True, _record)
@@ -1361,12 +1384,12 @@ def _attend_windows(op: str, q: torch.Tensor, buffers: KVBuffers, meta: Attentio
         max_partitions = -(-table.shape[1] * buffers.block_size // size)
         nbytes = lib.ayk_paged_attention_v2_workspace_bytes(n_rows, heads, buffers.head_dim, max_partitions)
         scratch = _workspace(op, device, nbytes, capturing(q), stream)
-    _call(op, lib.ayk_paged_attention_windows, (
-        out.data_ptr(), q.data_ptr(), buffers.k.data_ptr(), buffers.v.data_ptr(), table.data_ptr(),
+    _call(op, _library_call("ayk_paged_attention_windows", buffers), (
+        out.data_ptr(), q.data_ptr(), *_cache_args(buffers), table.data_ptr(),
         table.stride(0), meta.kv_lengths.data_ptr(), meta.request_of_row.data_ptr(), meta.positions.data_ptr(),
         tiles.data_ptr(), tiles.numel() // 4, n_rows, heads, kv_heads, buffers.head_dim, buffers.num_blocks,
         buffers.block_size, table.shape[1], _LAYOUT_CODES[KVLayoutKind(buffers.layout)], _DTYPE_CODES[q.dtype],
-        _kv_code(buffers, q.dtype), float(scale), *codec_scales(buffers.codec), size,
+        *_scale_args(buffers, q.dtype, scale), size,
         scratch.data_ptr() if scratch is not None else 0,
         scratch.numel() if scratch is not None else 0,
     ), stream, device, scratch is not None, record)

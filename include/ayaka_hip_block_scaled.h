@@ -44,6 +44,51 @@ int ayk_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_
                            const int64_t* slot_mapping, int64_t n_rows, int32_t num_kv_heads, int32_t head_dim,
                            int32_t num_blocks, int32_t block_size, int32_t layout, int32_t src_dtype, void* stream);
 
+/*
+ * Attention over a block-scaled cache: the entry points of ayaka_hip.h with the cache's scales in
+ * the place of kv_dtype, k_scale and v_scale, and otherwise their arguments, semantics, work lists,
+ * workspaces and flags (AYK_FLAG_QK_DPP is refused, as over every fp8 cache; dtype is fp16 or bf16):
+ *   ayk_paged_attention_v1_block_scaled       ayk_paged_attention_v1
+ *   ayk_paged_attention_v2_block_scaled       ayk_paged_attention_v2
+ *   ayk_paged_prefill_block_scaled            ayk_paged_prefill
+ *   ayk_paged_attention_windows_block_scaled  ayk_paged_attention_windows
+ * Position t of a request counts with the scales of its block: its score is
+ * scale * key scale * q.code and its value code * value scale. A NaN code at a position a row does
+ * not attend to does not reach the row; one at a position it attends to makes the elements it
+ * belongs to NaN (a value's) or the row's head (a key's).
+ */
+int ayk_paged_attention_v1_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                        const float* scales, const int32_t* block_table, int64_t table_stride,
+                                        const int32_t* kv_lengths, const int32_t* request_of_row,
+                                        const int32_t* positions, int32_t n_rows, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+                                        int32_t max_blocks, int32_t layout, int32_t dtype, float scale, int32_t flags,
+                                        void* stream);
+int ayk_paged_attention_v2_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                        const float* scales, const int32_t* block_table, int64_t table_stride,
+                                        const int32_t* kv_lengths, const int32_t* request_of_row,
+                                        const int32_t* positions, int32_t n_rows, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size,
+                                        int32_t max_blocks, int32_t layout, int32_t dtype, float scale,
+                                        int32_t partition_size, int32_t max_partitions, const int32_t* work_items,
+                                        int32_t n_work_items, const int32_t* staged, void* workspace,
+                                        size_t workspace_bytes, uint32_t* arrivals, int32_t flags, void* stream);
+int ayk_paged_prefill_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                   const float* scales, const int32_t* block_table, int64_t table_stride,
+                                   const int32_t* kv_lengths, const int32_t* request_of_row, const int32_t* positions,
+                                   const int32_t* tiles, int32_t n_tiles, int32_t tile_pairs, int32_t n_rows,
+                                   int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_blocks,
+                                   int32_t block_size, int32_t max_blocks, int32_t layout, int32_t dtype, float scale,
+                                   int32_t partition_size, void* workspace, size_t workspace_bytes, void* stream);
+int ayk_paged_attention_windows_block_scaled(void* out, const void* q, const void* k_cache, const void* v_cache,
+                                             const float* scales, const int32_t* block_table, int64_t table_stride,
+                                             const int32_t* kv_lengths, const int32_t* request_of_row,
+                                             const int32_t* positions, const int32_t* tiles, int32_t n_tiles,
+                                             int32_t n_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t num_blocks, int32_t block_size, int32_t max_blocks, int32_t layout,
+                                             int32_t dtype, float scale, int32_t partition_size, void* workspace,
+                                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ from ayaka_amd.kvcache import (
 )
 from oracle import block_scaled
 from oracle.numerics import e4m3_to_f32
+from tests import test_kv_reach as kv_reach
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "ayaka_hip_block_scaled.h"
 
@@ -175,3 +176,81 @@ def test_the_library_refuses_bad_stores(changes: dict, code: int, message: bytes
 
 def test_no_rows_is_no_launch() -> None:
     assert _store(n_rows=0, k=None, scales=None) == 0
+
+
+# --- the library's attention entry points ---------------------------------------------------------------
+
+
+def _v1(**kw: object) -> int:
+    args = dict(out=1, q=1, k=1, v=1, scales=8, table=1, stride=4, lengths=1, ror=None, pos=None, n_rows=1, heads=8,
+                kv_heads=2, head_dim=128, num_blocks=10, block_size=16, max_blocks=4, layout=0, dtype=1, scale=1.0,
+                flags=0, stream=None)
+    args.update(kw)
+    return _lib.lib().ayk_paged_attention_v1_block_scaled(*args.values())
+
+
+@pytest.mark.parametrize("changes,code,message", [
+    ({"scales": None}, 1, b"block_scales"),
+    ({"scales": 12}, 1, b"not 8-byte aligned"),
+    ({"dtype": 3}, 2, b"under fp16/bf16"),
+    ({"flags": 1}, 2, b"16-bit caches only"),
+    ({"head_dim": 96}, 2, b"head_dim 96"),
+    ({"heads": 7}, 1, b"not a positive multiple"),
+    ({"q": None}, 1, b"null"),
+])
+def test_the_library_refuses_bad_attention(changes: dict, code: int, message: bytes) -> None:
+    assert _v1(**changes) == code
+    assert message in _lib.lib().ayk_last_error()
+
+
+def test_multi_row_and_split_refusals() -> None:
+    lib = _lib.lib()
+    base = (1, 1, 1, 1, 8, 1, 4, 1)
+    shape = (1, 8, 2, 128, 10, 16, 4, 0, 1, 1.0)
+    assert lib.ayk_paged_attention_v2_block_scaled(*base, None, None, *shape, 100, 4, None, 0, None, 1, 1 << 20, None,
+                                                   0, None) == 1
+    assert b"ayk_paged_attention_v2_block_scaled: partition_size 100" in lib.ayk_last_error()
+    assert lib.ayk_paged_attention_v2_block_scaled(*base, None, None, *shape, 64, 4, None, 0, None, 16, 16, None, 0,
+                                                   None) == 4
+    assert lib.ayk_paged_prefill_block_scaled(*base, None, None, 1, 1, 128, *shape, 0, None, 0, None) == 1
+    assert b"request_of_row and positions are required" in lib.ayk_last_error()
+    assert lib.ayk_paged_prefill_block_scaled(*base, 1, 1, 1, 1, 100, *shape, 0, None, 0, None) == 1
+    assert b"tile_pairs 100" in lib.ayk_last_error()
+    wide = (1, 34, 2, 128, 10, 16, 4, 0, 1, 1.0)
+    assert lib.ayk_paged_attention_windows_block_scaled(*base, 1, 1, 1, 1, *wide, 0, None, 0, None) == 2
+    assert b"17 query heads" in lib.ayk_last_error()
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_loads_stay_in_the_cache(head_dim: int) -> None:
+    # the block-scaled launches form the fp8 launches' addresses: the host walk of each entry point
+    rng = np.random.default_rng(head_dim)
+    for case in range(12):
+        block = kv_reach.BLOCK_SIZES[case % len(kv_reach.BLOCK_SIZES)]
+        kv_heads, group = [(2, 4), (3, 1), (1, 8), (4, 2)][case % 4]
+        lengths = kv_reach._lengths(rng, block, int(rng.integers(1, 5)))
+        step = kv_reach.Step(rng, lengths, block, kv_heads, head_dim, True, case % 2)
+        heads = kv_heads * group
+
+        def common(rows, req, pos):
+            args = kv_reach._common(step, heads, rows, req, pos)
+            return (*args[:4], 8, *args[4:-4], args[-3])  # scales in, kv_dtype and the layer's scales out
+
+        def check(call, label):
+            kv_reach._check(step, kv_reach._walk(step, call), f"case {case} block {block} {label}")
+
+        rows = len(lengths)
+        check(lambda lib: lib.ayk_paged_attention_v1_block_scaled(*common(rows, None, None), 0, None), "v1")
+        parts = -(-step.width * block // 64)
+        nbytes = _lib.lib().ayk_paged_attention_v2_workspace_bytes(rows, heads, head_dim, parts)
+        check(lambda lib: lib.ayk_paged_attention_v2_block_scaled(
+            *common(rows, None, None), 64, parts, None, 0, None, kv_reach.FAKE, nbytes, None, 0, None), "v2")
+        counts = [min(n, 16 // group) or 1 for n in lengths]
+        req, pos = kv_reach._rows(step, counts)
+        tiles = kv_reach._tiles(counts, max(counts), 1)
+        args = common(len(req), req, pos)
+        check(lambda lib: lib.ayk_paged_attention_windows_block_scaled(
+            *args[:10], kv_reach._ptr(tiles), tiles.size // 4, *args[10:], 0, None, 0, None), "windows")
+        pairs = _lib.lib().ayk_paged_prefill_tile_pairs(head_dim)
+        check(lambda lib: lib.ayk_paged_prefill_block_scaled(
+            *args[:10], kv_reach._ptr(tiles), tiles.size // 4, pairs, *args[10:], 0, None, 0, None), "multi-row")
