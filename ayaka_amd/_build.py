@@ -19,7 +19,8 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_DIR = PACKAGE_DIR.parent
 SOURCES = ("api.hip", "paged_attention.hip", "paged_attention_mfma.hip", "paged_prefill.hip", "kv_cache.hip",
            "paged_attention_f32.hip", "paged_rows_f32.hip", "split_model.cpp", "kv_reach.hip",
-           "store_block_scaled.hip", "paged_attention_block_scaled.hip", "paged_prefill_block_scaled.hip")
+           "store_block_scaled.hip", "paged_attention_block_scaled.hip", "paged_prefill_block_scaled.hip",
+           "step_tables.hip")
 LIB_PATH = PACKAGE_DIR / "lib" / "libayaka_hip.so"
 ARCH = "gfx950"
 

@@ -22,7 +22,7 @@ if TYPE_CHECKING:
     from torch import Tensor, device
 
     from ayaka_amd.enums import ForwardMode
-    from ayaka_amd.kvcache import KVBuffers
+    from ayaka_amd.kvcache import BlockPool, KVBuffers
 
 __all__ = ["AttentionMetadata", "AttentionOps"]
 
@@ -79,3 +79,5 @@ class AttentionOps(Protocol):
     def update_graph_metadata(
         self, meta: AttentionMetadata, kv_lengths: Tensor, block_rows: Tensor
     ) -> None: ...
+
+    def advance_graph_metadata(self, meta: AttentionMetadata, kv_lengths: Tensor, pool: BlockPool) -> None: ...

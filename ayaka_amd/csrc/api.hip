@@ -14,6 +14,7 @@
 #include "ayaka_hip.h"
 #include "ayaka_hip_block_scaled.h"
 #include "ayaka_hip_internal.h"
+#include "ayaka_hip_tables.h"
 
 namespace {
 
@@ -562,6 +563,45 @@ int attend_windows(const char* op, const AttnCall& c, const int32_t* tiles, int3
   return launched(err, op);
 }
 
+// Check a step-tables call and fill its record.
+int prepare_tables(const char* op, const int32_t* lengths, int32_t n_requests, int32_t* block_table,
+                   int64_t table_stride, int32_t max_blocks, const int32_t* free_blocks, int32_t n_free,
+                   const int32_t* taken, int32_t* after, int32_t block_size, int32_t* positions,
+                   int64_t* slot_mapping, int32_t n_rows, int32_t* kv_lengths, ayk::TablesParams& p) {
+  if (n_requests < 0 || n_rows < 0 || n_free < 0)
+    return fail(AYK_ERR_ARGUMENT, "%s: %d requests, %d rows, %d free blocks", op, n_requests, n_rows, n_free);
+  if (n_requests > AYK_TABLES_MAX_REQUESTS)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %d requests exceed %d", op, n_requests, AYK_TABLES_MAX_REQUESTS);
+  if (block_size < 1 || block_size > 65536)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: block_size %d is not in [1, 65536]", op, block_size);
+  if (max_blocks < 0 || table_stride < max_blocks)
+    return fail(AYK_ERR_ARGUMENT, "%s: max_blocks %d, table_stride %lld", op, max_blocks, (long long)table_stride);
+  // positions, and sums of one with a block or a partition, are 32-bit
+  if ((int64_t)max_blocks * block_size > INT32_MAX - 65536)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: a table of %d blocks of %d positions exceeds %d positions per row", op,
+                max_blocks, block_size, INT32_MAX - 65536);
+  if (!taken || !after || (n_requests > 0 && (!lengths || !kv_lengths || (max_blocks > 0 && !block_table))) ||
+      (n_rows > 0 && (!positions || !slot_mapping)) || (n_free > 0 && !free_blocks))
+    return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  p = ayk::TablesParams{};
+  p.lengths = lengths;
+  p.block_table = block_table;
+  p.free_blocks = free_blocks;
+  p.taken = taken;
+  p.after = after;
+  p.positions = positions;
+  p.slot_mapping = slot_mapping;
+  p.kv_lengths = kv_lengths;
+  p.table_stride = table_stride;
+  p.n_requests = n_requests;
+  p.max_blocks = max_blocks;
+  p.n_free = n_free;
+  p.n_rows = n_rows;
+  p.block_size = block_size;
+  block_divisor(block_size, p.bs_magic, p.bs_shift);
+  return AYK_OK;
+}
+
 // A call of a block-scaled entry point: fp8 codes, the layer's scales 1, every block's own beside them.
 AttnCall block_scaled_call(void* out, const void* q, const void* k_cache, const void* v_cache, const float* scales,
                            const int32_t* block_table, int64_t table_stride, const int32_t* kv_lengths,
@@ -839,6 +879,53 @@ int ayk_paged_attention_windows_block_scaled(void* out, const void* q, const voi
                         layout, dtype, scale);
   return attend_windows("ayk_paged_attention_windows_block_scaled", c, tiles, n_tiles, partition_size, workspace, workspace_bytes,
                         stream);
+}
+
+int ayk_build_tables(const int32_t* rows, const int32_t* lengths, int32_t n_requests, int32_t* block_table,
+                     int64_t table_stride, int32_t max_blocks, const int32_t* free_blocks, int32_t n_free,
+                     const int32_t* taken, int32_t* after, int32_t block_size, int32_t* request_of_row,
+                     int32_t* positions, int64_t* slot_mapping, int32_t n_rows, int32_t* kv_lengths, void* stream) {
+  const char* op = "ayk_build_tables";
+  ayk::TablesParams p;
+  const int rc = prepare_tables(op, lengths, n_requests, block_table, table_stride, max_blocks, free_blocks, n_free,
+                                taken, after, block_size, positions, slot_mapping, n_rows, kv_lengths, p);
+  if (rc != AYK_OK) return rc;
+  if ((n_requests > 0 && !rows) || (n_rows > 0 && !request_of_row))
+    return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  p.rows = rows;
+  p.request_of_row = request_of_row;
+  return launched(ayk::launch_step_tables(p, static_cast<hipStream_t>(stream)), op);
+}
+
+int ayk_advance_decode_tables(const int32_t* lengths, int32_t n_requests, int32_t* block_table, int64_t table_stride,
+                              int32_t max_blocks, const int32_t* free_blocks, int32_t n_free, const int32_t* taken,
+                              int32_t* after, int32_t block_size, int32_t* positions, int64_t* slot_mapping,
+                              int32_t* kv_lengths, int32_t* staged, int32_t capacity, const int32_t* sizes,
+                              int32_t n_sizes, int32_t groups, int32_t cost, int32_t compute_units, void* stream) {
+  const char* op = "ayk_advance_decode_tables";
+  ayk::TablesParams p;
+  const int rc = prepare_tables(op, lengths, n_requests, block_table, table_stride, max_blocks, free_blocks, n_free,
+                                taken, after, block_size, positions, slot_mapping, n_requests, kv_lengths, p);
+  if (rc != AYK_OK) return rc;
+  if (!staged) return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  if (capacity < n_requests)
+    return fail(AYK_ERR_ARGUMENT, "%s: a work list of %d items holds no partition of each of %d rows", op, capacity,
+                n_requests);
+  if (!sizes || n_sizes < 1 || n_sizes > AYK_TABLES_MAX_SIZES || groups < 1 || cost < 0 || compute_units < 1)
+    return fail(AYK_ERR_ARGUMENT, "%s: %d sizes at %p, %d groups, cost %d, %d compute units", op, n_sizes,
+                (const void*)sizes, groups, cost, compute_units);
+  for (int32_t i = 0; i < n_sizes; ++i) {
+    if (sizes[i] <= 0 || sizes[i] % 64 != 0 || (i > 0 && sizes[i] <= sizes[i - 1]))
+      return fail(AYK_ERR_ARGUMENT, "%s: size %d, %d, is not a multiple of 64 above the one before it", op, i, sizes[i]);
+    p.sizes[i] = sizes[i];
+  }
+  p.staged = staged;
+  p.capacity = capacity;
+  p.n_sizes = n_sizes;
+  p.groups = groups;
+  p.cost = cost;
+  p.compute_units = compute_units;
+  return launched(ayk::launch_step_tables(p, static_cast<hipStream_t>(stream)), op);
 }
 
 static int block_op_checks(const char* op, int64_t n, int32_t num_blocks, int64_t block_bytes) {

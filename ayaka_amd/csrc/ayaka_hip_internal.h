@@ -117,6 +117,29 @@ hipError_t launch_store_block_scaled(const void* k, const void* v, void* k_cache
                                      int32_t head_dim, int32_t num_blocks, int32_t block_size, uint32_t bs_magic,
                                      int32_t bs_shift, bool hnd, bool bf16, hipStream_t stream);
 
+// Step tables on the device (ayaka_hip_tables.h); `staged` set: a decode bucket's, with its v2 split.
+#define AYK_TABLES_SIZES 32
+struct TablesParams {
+  const int32_t* rows;  // nullptr with `staged`: one each
+  const int32_t* lengths;
+  int32_t* block_table;
+  const int32_t* free_blocks;
+  const int32_t* taken;
+  int32_t* after;
+  int32_t* request_of_row;
+  int32_t* positions;
+  int64_t* slot_mapping;
+  int32_t* kv_lengths;
+  int32_t* staged;
+  int64_t table_stride;
+  int32_t n_requests, max_blocks, n_free, n_rows, block_size;
+  uint32_t bs_magic;
+  int32_t bs_shift;
+  int32_t capacity, n_sizes, groups, cost, compute_units;
+  int32_t sizes[AYK_TABLES_SIZES];
+};
+hipError_t launch_step_tables(const TablesParams& p, hipStream_t stream);
+
 // mode: 0 = gather (dst index i), 1 = copy (dst ids), 2 = zero (no source)
 hipError_t launch_block_op(int mode, const void* src_k, const void* src_v, void* dst_k, void* dst_v,
                            const void* src_ids, const void* dst_ids, bool ids64, int64_t n,

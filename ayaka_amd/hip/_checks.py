@@ -16,7 +16,14 @@ import torch
 
 from ayaka_amd.enums import KVLayoutKind
 from ayaka_amd.errors import BackendError
-from ayaka_amd.kvcache import FP8_E4M3_BLOCK_CODEC, FP8_E4M3_CODEC, RAW_CODEC, BlockScaledFp8Codec, KVBuffers
+from ayaka_amd.kvcache import (
+    FP8_E4M3_BLOCK_CODEC,
+    FP8_E4M3_CODEC,
+    RAW_CODEC,
+    BlockPool,
+    BlockScaledFp8Codec,
+    KVBuffers,
+)
 
 __all__ = [
     "HEAD_DIMS",
@@ -29,6 +36,7 @@ __all__ = [
     "require_device",
     "require_index_tensor",
     "require_like",
+    "require_pool",
     "stream_handle",
 ]
 
@@ -139,6 +147,16 @@ def require_block_scales(op: str, buffers: KVBuffers) -> None:
         )
     if scales.data_ptr() % 8:
         raise BackendError(f"{op}: buffers.codec.scales must be 8-byte aligned", context={"op": op})
+
+
+def require_pool(op: str, pool: BlockPool, device: torch.device) -> None:
+    """Refuse a pool of free blocks that the step tables' kernel cannot draw from."""
+    for name, tensor, shape in (("free", pool.free, (pool.free.numel(),)), ("taken", pool.taken, (1,)),
+                                ("after", pool.after, (4,))):
+        require_like(op, f"pool.{name}", tensor, shape, torch.int32)
+        if tensor.device != device:
+            raise BackendError(f"{op}: pool.{name} is on {tensor.device}, the table is on {device}",
+                               context={"op": op, "argument": f"pool.{name}"})
 
 
 def require_buffers(op: str, buffers: KVBuffers) -> None:

@@ -14,7 +14,7 @@ from pathlib import Path
 
 from ayaka_amd.errors import BackendError, CapabilityError
 
-__all__ = ["ABI_VERSION", "BLOCK_SCALED_EXPORTS", "EXPORTS", "LIB_PATH", "check", "lib"]
+__all__ = ["ABI_VERSION", "BLOCK_SCALED_EXPORTS", "EXPORTS", "LIB_PATH", "TABLES_EXPORTS", "check", "lib"]
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libayaka_hip.so"
 ABI_VERSION = 18
@@ -107,6 +107,18 @@ BLOCK_SCALED_EXPORTS: dict[str, tuple[object, list[object]]] = {
     ),
 }
 
+#: The functions of include/ayaka_hip_tables.h.
+TABLES_EXPORTS: dict[str, tuple[object, list[object]]] = {
+    "ayk_build_tables": (
+        ctypes.c_int,
+        [_P, _P, _I32, _P, _I64, _I32, _P, _I32, _P, _P, _I32, _P, _P, _P, _I32, _P, _P],
+    ),
+    "ayk_advance_decode_tables": (
+        ctypes.c_int,
+        [_P, _I32, _P, _I64, _I32, _P, _I32, _P, _P, _I32, _P, _P, _P, _P, _I32, _P, _I32, _I32, _I32, _I32, _P],
+    ),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -131,7 +143,7 @@ def lib() -> ctypes.CDLL:
                 raise CapabilityError(
                     "ops.hip", detail=f"{LIB_PATH} does not load: {exc}", remedy="rebuild it"
                 ) from exc
-            for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS}.items():
+            for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS, **TABLES_EXPORTS}.items():
                 fn = getattr(handle, name)
                 fn.restype = restype
                 fn.argtypes = argtypes

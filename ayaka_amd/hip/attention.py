@@ -28,6 +28,7 @@ host staging pinned, asynchronous copies on the current stream. Each update also
 stages the step's v2 partition size and work list on the device, so ``attend`` on
 graph metadata reads nothing on the host that changes between replays: its
 captured launch covers the bucket's capacity and the kernels read the step's split.
+``advance_graph_metadata`` is the update made on the device, from lengths the host need not know.
 """
 
 from __future__ import annotations
@@ -54,14 +55,16 @@ from ayaka_amd.hip._checks import (
     require_device,
     require_index_tensor,
     require_like,
+    require_pool,
     stream_handle,
 )
-from ayaka_amd.kvcache import FP8_E4M3_BLOCK_CODEC, FP8_E4M3_CODEC, KVBuffers, codec_scales
+from ayaka_amd.kvcache import FP8_E4M3_BLOCK_CODEC, FP8_E4M3_CODEC, BlockPool, KVBuffers, codec_scales
 
 __all__ = [
     "PARTITION_SIZE",
     "HipAttentionPlan",
     "HipGraphPlan",
+    "advance_graph_metadata",
     "attend",
     "attend_with",
     "choose_partitions",
@@ -1518,6 +1521,73 @@ def update_graph_metadata(
     used = _stage_split(staging, lens, block_size)
     end = staging.staged_offset + 4 * used
     staging.device_all[:end].copy_(staging.host_all[:end], non_blocking=True)
+
+
+@functools.cache
+def _advance_sizes(kv_bytes: int, min_size: int) -> ctypes.Array:
+    """The partition sizes a device-side update chooses from, as the library reads them."""
+    offered = FP8_PARTITION_CANDIDATES if kv_bytes == 1 else PARTITION_CANDIDATES
+    sizes = [size for size in offered if size >= min_size] or [min_size]
+    return (ctypes.c_int32 * len(sizes))(*sizes)
+
+
+def advance_graph_metadata(meta: AttentionMetadata, kv_lengths: torch.Tensor, pool: BlockPool) -> None:
+    """Write the next decode step into ``meta`` on the device.
+
+    What :func:`update_graph_metadata` computes on the host -- every request's newest position and
+    its slot, the lengths, the step's v2 split -- from ``kv_lengths``, an int32 [B] tensor in device
+    memory, and the bucket's own block table: a request whose newest token starts a block is given
+    one from ``pool``, in request order, entered into ``meta.block_table``. A length of 0 is
+    padding. A request longer than the table, of negative length, with the padding block 0 where its
+    last held block should be, or in need of a block when the pool has run out becomes padding too
+    (its output is zeros and nothing is stored for it) and counts into ``pool.after[1]``, for the
+    host to look at when it next reads the device.
+
+    One kernel on the current stream, which the host does not wait for and a graph may capture: a
+    captured step can advance itself (``kv_lengths`` may be ``meta.kv_lengths``, which the graph
+    raises by one where it is not 0 before the call). The split is sized for
+    the head shape of the bucket's first ``attend``; its choice of partition size follows a simpler
+    model than the host's, so results may differ from a host-updated step's by rounding.
+    :func:`update_graph_metadata` rewrites everything, the table included: read it back first when
+    blocks were handed out since.
+    """
+    op = "attention.advance_graph_metadata"
+    staging = meta.plan
+    table = meta.block_table
+    if not isinstance(staging, HipGraphPlan) or not isinstance(table, torch.Tensor):
+        raise BackendError(
+            f"{op}: meta was not made by this backend's graph_metadata",
+            context={"op": op, "argument": "meta"},
+        )
+    # the staged split no longer is the host's: attend must not stage that one again
+    staging.staged_shape.clear()
+    shape = tuple(staging.head_shape)
+    key = ("advance", id(meta), shape, _fastpath.signature((kv_lengths, pool.free, pool.taken, pool.after)))
+    found = _fastpath.lookup(staging.launches, key)
+    if found is not None:
+        _fastpath.run(found, stream_handle(found.device))
+        return
+    device = table.device
+    if not table.is_cuda:
+        raise BackendError(f"{op}: the hip backend runs on a HIP device; meta is on {device}",
+                           context={"op": op, "argument": "meta"})
+    requests, width = table.shape
+    require_like(op, "kv_lengths", kv_lengths, (requests,), torch.int32)
+    if kv_lengths.device != device:
+        raise BackendError(f"{op}: kv_lengths is on {kv_lengths.device}, meta is on {device}",
+                           context={"op": op, "argument": "kv_lengths"})
+    require_pool(op, pool, device)
+    kv_heads, group, kv_bytes = shape or (8, 1, 2)
+    sizes = _advance_sizes(kv_bytes, staging.min_size)
+    record = _fastpath.Recorder()
+    _call(op, _lib.lib().ayk_advance_decode_tables, (
+        kv_lengths.data_ptr(), requests, table.data_ptr(), width, width, pool.free.data_ptr(), pool.free.shape[0],
+        pool.taken.data_ptr(), pool.after.data_ptr(), meta.block_size, meta.positions.data_ptr(),
+        meta.slot_mapping.data_ptr(), meta.kv_lengths.data_ptr(), staging.staged.data_ptr(), staging.capacity,
+        ctypes.addressof(sizes), len(sizes), -(-kv_heads * head_chunks(group) // 8), WORKGROUP_COSTS[kv_bytes],
+        COMPUTE_UNITS,
+    ), stream_handle(device), device, False, record)
+    _fastpath.remember(staging.launches, key, (meta,), record)
 
 
 def _stage_split(staging: HipGraphPlan, lengths: np.ndarray, block_size: int) -> int:

@@ -7,7 +7,9 @@ cache it lands encoded (``ayk_reshape_and_cache_e4m3``), into a
 ``"fp8_e4m3_block"`` cache encoded with its block's scales, which the write
 raises where it has to (``ayk_store_block_scaled``). ``gather``,
 ``copy_blocks`` and ``zero_blocks`` move whole blocks (same file, ``:83-115``),
-of a block-scaled cache with their scales.
+of a block-scaled cache with their scales. ``build_tables`` gives a step's
+requests the blocks they lack and derives its slots on the device
+(``ayk_build_tables``).
 Both layouts are served; NHD is preferred, as the reference's ``layout()``
 returns (``:30-31``).
 """
@@ -27,11 +29,12 @@ from ayaka_amd.hip._checks import (
     require_device,
     require_index_tensor,
     require_like,
+    require_pool,
     stream_handle,
 )
-from ayaka_amd.kvcache import FP8_E4M3_CODEC, KVBuffers, codec_scales
+from ayaka_amd.kvcache import FP8_E4M3_CODEC, BlockPool, KVBuffers, StepTables, codec_scales
 
-__all__ = ["copy_blocks", "gather", "layout", "store", "zero_blocks"]
+__all__ = ["build_tables", "copy_blocks", "gather", "layout", "store", "zero_blocks"]
 
 _LAYOUT_CODES = {KVLayoutKind.NHD: 0, KVLayoutKind.HND: 1}
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
@@ -245,3 +248,55 @@ def zero_blocks(buffers: KVBuffers, block_ids: torch.Tensor) -> None:
     scales = block_scales(buffers)
     if scales is not None:
         _move_scales(op, "ayk_zero_blocks", (scales, scales), (block_ids,), scales, device)
+
+
+def build_tables(
+    rows_per_request: torch.Tensor,
+    kv_lengths: torch.Tensor,
+    block_table: torch.Tensor,
+    pool: BlockPool,
+    tables: StepTables,
+    block_size: int,
+) -> None:
+    """Give every request of a step the blocks it lacks, and derive its rows' positions and slots.
+
+    All on the device, from int32 device tensors: request ``b`` brings ``rows_per_request[b]`` rows,
+    the last of the ``kv_lengths[b]`` tokens it has after the step, and its row of ``block_table``
+    [B, W] already holds the blocks of the tokens before them. The blocks it lacks come from
+    ``pool`` in request order and are written into ``block_table``; ``tables`` receives what
+    ``attention.plan`` derives on the host (reference ``torch/attention.py:64-164``).
+
+    A request that cannot be served -- negative rows, more rows than tokens, more blocks than W,
+    rows past the tables' N, the padding block 0 where its last held block should be, or a pool that
+    runs out at it or before it while it needs a block -- gets no block, slots and positions of 0 and a length of 0 in ``tables.kv_lengths``, and counts
+    into ``pool.after[1]``; a request of length 0 is padding and does not. Rows of the tables behind
+    the last request's get request, position and slot 0. ``tables.kv_lengths`` may be
+    ``kv_lengths`` itself. Nothing waits for the device, and the call can be captured.
+    """
+    op = "kvcache.build_tables"
+    device = block_table.device
+    if not block_table.is_cuda:
+        raise BackendError(f"{op}: the hip backend runs on a HIP device; block_table is on {device}",
+                           context={"op": op, "argument": "block_table"})
+    requests, rows = kv_lengths.shape[0] if kv_lengths.ndim == 1 else -1, tables.positions.numel()
+    width = block_table.shape[1] if block_table.ndim == 2 else -1
+    require_pool(op, pool, device)
+    for name, tensor, shape, dtype in (
+        ("rows_per_request", rows_per_request, (requests,), torch.int32),
+        ("kv_lengths", kv_lengths, (requests,), torch.int32),
+        ("block_table", block_table, (requests, width), torch.int32),
+        ("tables.request_of_row", tables.request_of_row, (rows,), torch.int32),
+        ("tables.positions", tables.positions, (rows,), torch.int32),
+        ("tables.slot_mapping", tables.slot_mapping, (rows,), torch.int64),
+        ("tables.kv_lengths", tables.kv_lengths, (requests,), torch.int32),
+    ):
+        require_like(op, name, tensor, shape, dtype)
+        if tensor.device != device:
+            raise BackendError(f"{op}: {name} is on {tensor.device}, the table is on {device}",
+                               context={"op": op, "argument": name})
+    _lib.check(op, _lib.lib().ayk_build_tables(
+        rows_per_request.data_ptr(), kv_lengths.data_ptr(), requests, block_table.data_ptr(), width, width,
+        pool.free.data_ptr(), pool.free.shape[0], pool.taken.data_ptr(), pool.after.data_ptr(), block_size,
+        tables.request_of_row.data_ptr(), tables.positions.data_ptr(), tables.slot_mapping.data_ptr(), rows,
+        tables.kv_lengths.data_ptr(), _stream(device),
+    ))

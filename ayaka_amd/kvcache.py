@@ -40,10 +40,12 @@ __all__ = [
     "FP8_E4M3_BLOCK_CODEC",
     "FP8_E4M3_CODEC",
     "RAW_CODEC",
+    "BlockPool",
     "BlockScaledFp8Codec",
     "KVBuffers",
     "KVCacheOps",
     "ScaledFp8Codec",
+    "StepTables",
     "codec_scales",
     "fp8_e4m3_block_codec",
     "fp8_e4m3_codec",
@@ -182,6 +184,40 @@ except ImportError:
     KVBuffers = _KVBuffers  # type: ignore[misc]
 
 
+class BlockPool(NamedTuple):
+    """The free blocks a step's requests draw from, in device memory.
+
+    ``free`` int32 [F] lists block ids in the order they are handed out, ``taken`` int32 [1] how
+    many of them are. A step that draws blocks writes ``after`` int32 [4]: how many are taken after
+    it, and how many requests it could not serve; the other two words are the ops' own. ``after`` is
+    zeros before its first use. :meth:`in_place` makes a pool that advances itself (``taken`` is
+    ``after``'s first word), as a decode loop on the device needs; with a ``taken`` of its own the
+    caller moves the count on. The host returns blocks by rewriting ``free`` and ``taken`` between
+    steps. Steps that overlap in time need an ``after`` each.
+    """
+
+    free: Tensor
+    taken: Tensor
+    after: Tensor
+
+    @classmethod
+    def in_place(cls, free: Tensor) -> "BlockPool":
+        """A pool of which nothing is taken yet and whose count advances with every step."""
+        after = free.new_zeros(4)
+        return cls(free, after[:1], after)
+
+
+class StepTables(NamedTuple):
+    """What a step's cache writes and attention read of its requests, at fixed addresses in device
+    memory: ``request_of_row``, ``positions`` (int32) and ``slot_mapping`` (int64), each [N], and
+    ``kv_lengths`` int32 [B] (see :class:`~ayaka_amd.attention.AttentionMetadata`)."""
+
+    request_of_row: Tensor
+    positions: Tensor
+    slot_mapping: Tensor
+    kv_lengths: Tensor
+
+
 class KVCacheOps(Protocol):
     """Writing, reading and clearing the paged cache (reference ``ops/kvcache.py:94-144``)."""
 
@@ -196,3 +232,8 @@ class KVCacheOps(Protocol):
     def copy_blocks(self, buffers: KVBuffers, src: Tensor, dst: Tensor) -> None: ...
 
     def zero_blocks(self, buffers: KVBuffers, block_ids: Tensor) -> None: ...
+
+    def build_tables(
+        self, rows_per_request: Tensor, kv_lengths: Tensor, block_table: Tensor, pool: BlockPool,
+        tables: StepTables, block_size: int,
+    ) -> None: ...
