@@ -908,6 +908,8 @@ int ayk_advance_decode_tables(const int32_t* lengths, int32_t n_requests, int32_
                                 taken, after, block_size, positions, slot_mapping, n_requests, kv_lengths, p);
   if (rc != AYK_OK) return rc;
   if (!staged) return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  if (capacity > AYK_TABLES_MAX_ITEMS)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: a work list of %d items exceeds %d", op, capacity, AYK_TABLES_MAX_ITEMS);
   if (capacity < n_requests)
     return fail(AYK_ERR_ARGUMENT, "%s: a work list of %d items holds no partition of each of %d rows", op, capacity,
                 n_requests);
@@ -915,9 +917,10 @@ int ayk_advance_decode_tables(const int32_t* lengths, int32_t n_requests, int32_
     return fail(AYK_ERR_ARGUMENT, "%s: %d sizes at %p, %d groups, cost %d, %d compute units", op, n_sizes,
                 (const void*)sizes, groups, cost, compute_units);
   for (int32_t i = 0; i < n_sizes; ++i) {
-    if (sizes[i] <= 0 || sizes[i] % 64 != 0 || (i > 0 && sizes[i] <= sizes[i - 1]))
-      return fail(AYK_ERR_ARGUMENT, "%s: size %d, %d, is not a multiple of 64 above the one before it", op, i, sizes[i]);
+    if (sizes[i] <= 0 || sizes[i] > (1 << 30) || sizes[i] % 64 != 0 || (i > 0 && sizes[i] <= sizes[i - 1]))
+      return fail(AYK_ERR_ARGUMENT, "%s: size %d, %d, is not a multiple of 64, up to 2^30, above the one before it", op, i, sizes[i]);
     p.sizes[i] = sizes[i];
+    block_divisor(sizes[i], p.size_magic[i], p.size_shift[i]);
   }
   p.staged = staged;
   p.capacity = capacity;

@@ -8,6 +8,14 @@
 // reads the run's slice of the rows, takes the largest magnitude over the wave, settles the scale,
 // re-encodes the tokens held before the run if the scale grew, and encodes the rows. Nothing is
 // shared between waves, so there is no atomic and no order to depend on.
+//
+// A wave looks for the runs that begin among `range` rows: one row each while the step's rows are
+// few (decode: every wave's chain of loads runs beside the others'), 16 once they would fill the
+// GPU several times over (a wave per row, most of them to find that the row begins no run, took
+// 35.4 us for 9.1K rows of 8 heads of 128; see launch_store_block_scaled). The rows of a run of up
+// to 16 positions stay in registers between the maximum and the encoding, one v_cvt_scalef32_pk_fp8
+// per two elements: it divides by the scale, rounds to nearest even and gives NaN for what is not
+// finite, exactly as the codec says.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -22,31 +30,51 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// fp32 of magnitude 448 at most, or NaN, to an e4m3 code, to nearest even.
-__device__ __forceinline__ uint32_t code_of(float f) {
-  const uint32_t u = __float_as_uint(f);
-  const uint32_t sign = (u >> 24) & 0x80u;
-  const uint32_t mag = u & 0x7fffffffu;
-  uint32_t code;
-  if (mag > 0x7f800000u) code = 0x7fu;
-  else if (mag < 0x3c800000u) code = (uint32_t)__builtin_rintf(__uint_as_float(mag) * 512.0f);  // below 2^-6
-  else code = ((mag + 0x7ffffu + ((mag >> 20) & 1u)) >> 20) - (120u << 3);
-  return code | sign;
+// Two elements, divided by the scale, to e4m3 codes in the low (HIGH: high) half of `to`.
+template <bool BF16, bool HIGH>
+__device__ __forceinline__ i16x2 encode_pair(i16x2 to, uint32_t w, float scale) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(to, __builtin_bit_cast(bf16x2, w), scale, HIGH);
+  else
+    return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(to, __builtin_bit_cast(f16x2, w), scale, HIGH);
 }
 
+// Four codes times a power of two below 1, to nearest even (NaN stays NaN).
+__device__ __forceinline__ uint32_t lower_codes(uint32_t codes, float ratio) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  int out = __builtin_amdgcn_cvt_pk_fp8_f32(a.x * ratio, a.y * ratio, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b.x * ratio, b.y * ratio, out, true);
+}
+
+// A 16-bit magnitude's value.
 template <bool BF16>
 __device__ __forceinline__ float widen(uint32_t h) {
   if constexpr (BF16) return __uint_as_float(h << 16);
   else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
 
-// x / scale for the encoder: magnitudes above 448 saturate, what is not finite is NaN.
-template <bool BF16>
-__device__ __forceinline__ float scaled(uint32_t h, float inv) {
-  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-  const float x = fminf(fmaxf(widen<BF16>(h) * inv, -448.f), 448.f);
-  return (h & 0x7fffu) >= kInf ? __uint_as_float(0x7fc00000u) : x;
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);
+}
+
+// The largest x of the wave, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, lane_dpp<0xB1>(x));   // quad_perm [1,0,3,2]: lane ^ 1
+  x = max(x, lane_dpp<0x4E>(x));   // quad_perm [2,3,0,1]: lane ^ 2
+  x = max(x, lane_dpp<0x141>(x));  // row_half_mirror: the other quad of the 8
+  x = max(x, lane_dpp<0x140>(x));  // row_mirror: the other 8 of the 16
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(r[0], r[1]);
+  const auto t = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(t[0], t[1]);
 }
 
 struct StoreParams {
@@ -73,88 +101,134 @@ __device__ __forceinline__ int slot_block(const StoreParams& p, int64_t i, int& 
 }
 
 template <int D, bool BF16>
-__global__ __launch_bounds__(256) void store_block_scaled_kernel(const StoreParams p) {
+__global__ __launch_bounds__(256) void store_block_scaled_kernel(const StoreParams p, int range) {
   constexpr int LPR = D / 8;     // lanes per row: 8 elements each
-  constexpr int RPP = 64 / LPR;  // rows per pass of the wave
+  constexpr int RPP = 64 / LPR;  // rows per load of the wave
+  constexpr int U = 16 / RPP;    // loads of 16 rows
+  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
   const int lane = threadIdx.x & 63;
-  const int unit = blockIdx.y * 4 + (threadIdx.x >> 6);  // (head, tensor)
+  // four heads of one tensor side by side where there are as many: their rows are contiguous
+  const int unit = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (unit >= 2 * p.num_kv_heads) return;
-  const int head = unit >> 1, which = unit & 1;
-  const int64_t row0 = blockIdx.x;
+  const int which = unit >= p.num_kv_heads ? 1 : 0, head = unit - which * p.num_kv_heads;
+  // lane l looks at row row0 - 1 + l: the row before the range, the range, and what its last run may need
+  const int64_t row0 = (int64_t)blockIdx.x * range;
+  const int64_t mine = row0 - 1 + lane;
   int offset = 0;
-  const int block = slot_block(p, row0, offset);
-  if (block == 0) return;
-  int other = 0;
-  if (row0 > 0 && slot_block(p, row0 - 1, other) == block) return;  // not the first row of its run
-  // the run's length and its first offset
-  int64_t count = 0;
-  int first = p.block_size;
-  for (bool more = true; more;) {
-    const int64_t i = row0 + count + lane;
-    int at = 0;
-    const bool same = i < p.n_rows && slot_block(p, i, at) == block;
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(same);
-    const int n = mask == ~0ull ? 64 : __builtin_ctzll(~mask);
-    first = min(first, lane < n ? at : first);
-    count += n;
-    more = n == 64;
-  }
-#pragma unroll
-  for (int st = 1; st < 64; st <<= 1) first = min(first, __shfl_xor(first, st));
+  const int block = mine >= 0 && mine < p.n_rows ? slot_block(p, mine, offset) : 0;
+  const int before = __shfl_up(block, 1);
+  uint64_t runs = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= range && block != 0 && block != before);
 
   const int r = lane / LPR, c = lane % LPR;
   const int64_t row_elems = (int64_t)p.num_kv_heads * D;
-  const uint16_t* src = p.rows[which] + row0 * row_elems + head * D + c * 8;
-  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-  uint32_t top = 0;
-  for (int64_t i = r; i < count; i += RPP) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * row_elems);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
-      top = max(top, lo < kInf ? lo : 0u);
-      top = max(top, hi < kInf ? hi : 0u);
+  for (; runs; runs &= runs - 1) {
+    const int at = __builtin_ctzll(runs);
+    const int blk = __builtin_amdgcn_readlane(block, at);
+    const uint64_t same = __builtin_amdgcn_ballot_w64(block == blk) >> at;  // bits past lane 63 read as 0
+    int64_t count = same == ~0ull ? 64 : __builtin_ctzll(~same);
+    uint32_t first = ~wave_max(lane >= at && lane < at + (int)count ? ~(uint32_t)offset : 0u);  // the least
+    for (bool more = at + count == 64; more;) {  // a run longer than the wave sees
+      const int64_t i = row0 - 1 + at + count + lane;
+      int o = 0;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(i < p.n_rows && slot_block(p, i, o) == blk);
+      const int n = mask == ~0ull ? 64 : __builtin_ctzll(~mask);
+      first = min(first, ~wave_max(lane < n ? ~(uint32_t)o : 0u));
+      count += n;
+      more = n == 64;
     }
-  }
-#pragma unroll
-  for (int st = 1; st < 64; st <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, st));
+    float* scale_at = p.scales + ((int64_t)blk * p.num_kv_heads + head) * 2 + which;
+    const float stored = *scale_at;  // read beside the rows
+    const uint16_t* src = p.rows[which] + (row0 - 1 + at) * row_elems + head * D + c * 8;
+    uint8_t* dst = p.cache[which] + (int64_t)blk * p.block_stride + head * p.head_stride + c * 8;
 
-  float* scale_at = p.scales + ((int64_t)block * p.num_kv_heads + head) * 2 + which;
-  const float need = scale_for(widen<BF16>(top));
-  const float old = first > 0 ? canonical_scale(*scale_at) : 0.f;
-  const float now = fmaxf(old, need);
-  uint8_t* dst = p.cache[which] + (int64_t)block * p.block_stride + head * p.head_stride + c * 8;
-  if (now > old && old > 0.f) {
-    const float ratio = old / now;  // a power of two: exact
-    for (int t = r; t < first; t += RPP) {
-      u32x2* at = reinterpret_cast<u32x2*>(dst + (int64_t)t * p.token_stride);
-      u32x2 w = *at;
+    u32x4 w[U];
+    auto load = [&](int64_t base) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint32_t out = 0;
-        out |= code_of(__builtin_amdgcn_cvt_f32_fp8((int)w[e], 0) * ratio);
-        out |= code_of(__builtin_amdgcn_cvt_f32_fp8((int)w[e], 1) * ratio) << 8;
-        out |= code_of(__builtin_amdgcn_cvt_f32_fp8((int)w[e], 2) * ratio) << 16;
-        out |= code_of(__builtin_amdgcn_cvt_f32_fp8((int)w[e], 3) * ratio) << 24;
-        w[e] = out;
+      for (int u = 0; u < U; ++u) {  // past the run's end its last row again
+        const int64_t i = base + u * RPP + r;
+        w[u] = *reinterpret_cast<const u32x4*>(src + (i < count ? i : count - 1) * row_elems);
       }
-      *at = w;
-    }
-  }
-  const float inv = now > 0.f ? 1.0f / now : 1.0f;
-  for (int64_t i = r; i < count; i += RPP) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * row_elems);
-    int at = 0;
-    slot_block(p, row0 + i, at);
-    u32x2 out = {0u, 0u};
+    };
+    auto largest = [&](bool finite) {
+      u16x2 top = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t pair = code_of(scaled<BF16>(w[e] & 0xffffu, inv)) | code_of(scaled<BF16>(w[e] >> 16, inv)) << 8;
-      out[e >> 1] |= pair << (16 * (e & 1));
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u16x2 m = __builtin_bit_cast(u16x2, w[u][e] & 0x7fff7fffu);
+          if (finite) {
+            m.x = m.x < kInf ? m.x : 0;
+            m.y = m.y < kInf ? m.y : 0;
+          }
+          top = __builtin_elementwise_max(top, m);
+        }
+      return (uint32_t)max(top.x, top.y);
+    };
+    load(0);
+    uint32_t top = largest(false);
+    for (int64_t base = 16; base < count; base += 16) {
+      load(base);
+      top = max(top, largest(false));
     }
-    *reinterpret_cast<u32x2*>(dst + (int64_t)at * p.token_stride) = out;
+    top = wave_max(top);
+    if (top >= kInf) {  // something is not finite: the finite values alone settle the scale
+      top = 0;
+      for (int64_t base = 0; base < count; base += 16) {
+        load(base);
+        top = max(top, largest(true));
+      }
+      top = wave_max(top);
+    }
+    const float old = first > 0 ? canonical_scale(stored) : 0.f;
+    const float now = fmaxf(old, scale_for(widen<BF16>(top)));
+    if (now > old && old > 0.f) {
+      const float ratio = old / now;  // a power of two: exact
+      for (int t = r; t < (int)first; t += RPP) {
+        u32x2* cell = reinterpret_cast<u32x2*>(dst + (int64_t)t * p.token_stride);
+        const u32x2 codes = *cell;
+        *cell = u32x2{lower_codes(codes.x, ratio), lower_codes(codes.y, ratio)};
+      }
+    }
+    const float by = now > 0.f ? now : 1.f;
+    // the largest scale: magnitudes past 448 of it saturate (bf16 values above 2^88 alone)
+    const bool saturate = BF16 && now == power_of_two(kScaleMost);
+    auto encode = [&](int64_t base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = base + u * RPP + r;
+        int o = __shfl(offset, (at + (int)i) & 63);  // its lane's, where the wave saw the row
+        if (i >= count) continue;
+        if (at + i > 63) slot_block(p, row0 - 1 + at + i, o);
+        u32x4 x = w[u];
+        if (saturate) {
+          constexpr uint32_t kMost = (uint32_t)(127 + 8 + kScaleMost) << 7 | 0x60u;  // 448 * 2^80 in bf16
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
+            lo = lo > kMost && lo < kInf ? kMost : lo;
+            hi = hi > kMost && hi < kInf ? kMost : hi;
+            x[e] = (x[e] & 0x80008000u) | lo | hi << 16;
+          }
+        }
+        i16x2 lo = {0, 0}, hi = {0, 0};
+        lo = encode_pair<BF16, false>(lo, x.x, by);
+        lo = encode_pair<BF16, true>(lo, x.y, by);
+        hi = encode_pair<BF16, false>(hi, x.z, by);
+        hi = encode_pair<BF16, true>(hi, x.w, by);
+        *reinterpret_cast<u32x2*>(dst + (int64_t)o * p.token_stride) =
+            u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+      }
+    };
+    if (count <= 16) {
+      encode(0);
+    } else {
+      for (int64_t base = 0; base < count; base += 16) {
+        load(base);
+        encode(base);
+      }
+    }
+    if (lane == 0) *scale_at = now;
   }
-  if (lane == 0) *scale_at = now;
 }
 
 }  // namespace
@@ -180,11 +254,14 @@ hipError_t launch_store_block_scaled(const void* k, const void* v, void* k_cache
   p.block_stride = B * H * D;
   p.token_stride = hnd ? D : H * D;
   p.head_stride = hnd ? B * D : D;
-  const dim3 grid((unsigned)n_rows, (unsigned)((2 * num_kv_heads + 3) / 4)), block(256);
+  // Rows a wave looks for runs among (see above): 16 from as many rows on as give every compute unit
+  // 16 waves of one.
+  const int range = n_rows * 2 * num_kv_heads < 16 * 256 ? 1 : 16;
+  const dim3 grid((unsigned)((n_rows + range - 1) / range), (unsigned)((2 * num_kv_heads + 3) / 4)), block(256);
 #define AYK_STORE(W)                                                                                   \
   do {                                                                                                 \
-    if (bf16) hipLaunchKernelGGL((store_block_scaled_kernel<W, true>), grid, block, 0, stream, p);     \
-    else hipLaunchKernelGGL((store_block_scaled_kernel<W, false>), grid, block, 0, stream, p);         \
+    if (bf16) hipLaunchKernelGGL((store_block_scaled_kernel<W, true>), grid, block, 0, stream, p, range);     \
+    else hipLaunchKernelGGL((store_block_scaled_kernel<W, false>), grid, block, 0, stream, p, range);         \
   } while (0)
   switch (head_dim) {
     case 64: AYK_STORE(64); break;

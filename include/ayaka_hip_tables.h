@@ -19,6 +19,8 @@ extern "C" {
 
 /* Most requests of one step. */
 #define AYK_TABLES_MAX_REQUESTS 4096
+/* Most work items of one step. */
+#define AYK_TABLES_MAX_ITEMS (1 << 18)
 /* Most partition sizes ayk_advance_decode_tables chooses from. */
 #define AYK_TABLES_MAX_SIZES 32
 
@@ -55,7 +57,7 @@ int ayk_build_tables(const int32_t* rows, const int32_t* lengths, int32_t n_requ
  * written), and with it the step's v2 split staged for ayk_paged_attention_v2: `staged` receives
  * {partition size, item count, each row's first partial slot, (row, partition) pairs}, as that
  * call's `staged` and `work_items` (staged + 2 + n_requests) read them, of at most `capacity`
- * items. The size is the one of sizes[0 .. n_sizes) (HOST memory; rising multiples of 64) whose
+ * items. The size is the one of sizes[0 .. n_sizes) (HOST memory; rising multiples of 64 up to 2^30) whose
  * work, dealt to compute_units workgroups of one item and head group (`groups` per item) each
  * costing its positions plus `cost`, is modelled to end first, or one partition per row where no
  * size's items fit; partitions are listed full ones first, then falling by 1/256 of the size.

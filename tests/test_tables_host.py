@@ -123,8 +123,10 @@ def _advance(sizes=(64, 128), **kw: object) -> int:
 @pytest.mark.parametrize("changes,code,message", [
     ({"staged": None}, 1, b"null"),
     ({"capacity": 1}, 1, b"1 items holds no partition of each of 2 rows"),
+    ({"capacity": (1 << 18) + 1}, 2, b"262145 items exceeds 262144"),
     ({"sizes": (64, 64)}, 1, b"size 1, 64"),
     ({"sizes": (100,)}, 1, b"size 0, 100"),
+    ({"sizes": (64, (1 << 30) + 64)}, 1, b"up to 2^30"),
     ({"sizes": tuple(range(64, 64 * 34, 64))}, 1, b"33 sizes"),
     ({"groups": 0}, 1, b"0 groups"),
     ({"cost": -1}, 1, b"cost -1"),
