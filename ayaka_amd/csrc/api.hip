@@ -690,7 +690,7 @@ int ayk_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_
   if ((uint64_t)num_blocks * (uint64_t)block_size * (uint64_t)num_kv_heads * (uint64_t)head_dim > UINT32_MAX)
     return fail(AYK_ERR_UNSUPPORTED, "%s: a cache of %d blocks of %d positions exceeds 32-bit element offsets", op,
                 num_blocks, block_size);
-  if (n_rows > INT32_MAX || num_kv_heads > 131070)
+  if (n_rows > INT32_MAX || num_kv_heads > 32767)
     return fail(AYK_ERR_UNSUPPORTED, "%s: %lld rows of %d heads exceed one launch", op, (long long)n_rows,
                 num_kv_heads);
   if (n_rows == 0) return ok();

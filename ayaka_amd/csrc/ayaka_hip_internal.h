@@ -136,6 +136,7 @@ struct TablesParams {
   uint32_t bs_magic;
   int32_t bs_shift;
   int32_t capacity, n_sizes, groups, cost, compute_units;
+  int32_t workgroups;  // of the launch (set by it)
   int32_t sizes[AYK_TABLES_SIZES];       // partition sizes, and their divisors as bs_magic and bs_shift
   uint32_t size_magic[AYK_TABLES_SIZES];
   int32_t size_shift[AYK_TABLES_SIZES];

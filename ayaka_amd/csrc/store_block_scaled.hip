@@ -9,13 +9,15 @@
 // re-encodes the tokens held before the run if the scale grew, and encodes the rows. Nothing is
 // shared between waves, so there is no atomic and no order to depend on.
 //
-// A wave looks for the runs that begin among `range` rows: one row each while the step's rows are
-// few (decode: every wave's chain of loads runs beside the others'), 16 once they would fill the
-// GPU several times over (a wave per row, most of them to find that the row begins no run, took
-// 35.4 us for 9.1K rows of 8 heads of 128; see launch_store_block_scaled). The rows of a run of up
-// to 16 positions stay in registers between the maximum and the encoding, one v_cvt_scalef32_pk_fp8
-// per two elements: it divides by the scale, rounds to nearest even and gives NaN for what is not
-// finite, exactly as the codec says.
+// Rows of a run of up to 16 positions stay in registers between the maximum and the encoding, one
+// v_cvt_scalef32_pk_fp8 per two elements: it divides by the scale, rounds to nearest even and gives
+// NaN for what is not finite, exactly as the codec says. A wave looks for the runs that begin among
+// `range` rows. Blocks of up to 16 positions: a workgroup's waves are four heads, each on its own.
+// Larger blocks (COOP): its waves are of one head and tensor; they share the runs of up to 16 rows
+// out and take longer ones together, 16 rows each at a time, their maxima meeting in LDS.
+//
+// Bound by memory once a step is large: 16.4K rows of 8 heads of 128 move 101 MB in 21 us (4.8
+// TB/s; a large copy makes 5.0). Small ones are one chain of loads: 4 us from 4 to 256 rows.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -100,15 +102,15 @@ __device__ __forceinline__ int slot_block(const StoreParams& p, int64_t i, int& 
   return block;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool COOP>
 __global__ __launch_bounds__(256) void store_block_scaled_kernel(const StoreParams p, int range) {
   constexpr int LPR = D / 8;     // lanes per row: 8 elements each
   constexpr int RPP = 64 / LPR;  // rows per load of the wave
   constexpr int U = 16 / RPP;    // loads of 16 rows
   constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-  const int lane = threadIdx.x & 63;
-  // four heads of one tensor side by side where there are as many: their rows are contiguous
-  const int unit = blockIdx.y * 4 + (threadIdx.x >> 6);
+  __shared__ uint32_t s_top[2][4];  // COOP: the waves' maxima of a long run
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int unit = COOP ? blockIdx.y : blockIdx.y * 4 + wave;
   if (unit >= 2 * p.num_kv_heads) return;
   const int which = unit >= p.num_kv_heads ? 1 : 0, head = unit - which * p.num_kv_heads;
   // lane l looks at row row0 - 1 + l: the row before the range, the range, and what its last run may need
@@ -121,11 +123,12 @@ __global__ __launch_bounds__(256) void store_block_scaled_kernel(const StorePara
 
   const int r = lane / LPR, c = lane % LPR;
   const int64_t row_elems = (int64_t)p.num_kv_heads * D;
+  int shared_out = 0, together = 0;  // COOP: runs of either kind so far (the same in every wave)
   for (; runs; runs &= runs - 1) {
     const int at = __builtin_ctzll(runs);
     const int blk = __builtin_amdgcn_readlane(block, at);
     const uint64_t same = __builtin_amdgcn_ballot_w64(block == blk) >> at;  // bits past lane 63 read as 0
-    int64_t count = same == ~0ull ? 64 : __builtin_ctzll(~same);
+    int64_t count = __builtin_ctzll(~same);
     uint32_t first = ~wave_max(lane >= at && lane < at + (int)count ? ~(uint32_t)offset : 0u);  // the least
     for (bool more = at + count == 64; more;) {  // a run longer than the wave sees
       const int64_t i = row0 - 1 + at + count + lane;
@@ -136,6 +139,10 @@ __global__ __launch_bounds__(256) void store_block_scaled_kernel(const StorePara
       count += n;
       more = n == 64;
     }
+    // this wave's rows of the run: 16 from `begin` on, and `step` further on the next 16
+    const bool split = COOP && count > 16;
+    if (COOP && !split && (shared_out++ & 3) != wave) continue;
+    const int64_t begin = split ? 16 * wave : 0, step = split ? 64 : 16;
     float* scale_at = p.scales + ((int64_t)blk * p.num_kv_heads + head) * 2 + which;
     const float stored = *scale_at;  // read beside the rows
     const uint16_t* src = p.rows[which] + (row0 - 1 + at) * row_elems + head * D + c * 8;
@@ -164,26 +171,38 @@ __global__ __launch_bounds__(256) void store_block_scaled_kernel(const StorePara
         }
       return (uint32_t)max(top.x, top.y);
     };
-    load(0);
+    // of the whole run, in every wave that has a part in it
+    auto run_max = [&](uint32_t top) {
+      top = wave_max(top);
+      if (split) {
+        uint32_t* all = s_top[together++ & 1];
+        if (lane == 0) all[wave] = top;
+        __syncthreads();
+        top = max(max(all[0], all[1]), max(all[2], all[3]));
+      }
+      return top;
+    };
+    load(begin);
     uint32_t top = largest(false);
-    for (int64_t base = 16; base < count; base += 16) {
+    for (int64_t base = begin + step; base < count; base += step) {
       load(base);
       top = max(top, largest(false));
     }
-    top = wave_max(top);
-    if (top >= kInf) {  // something is not finite: the finite values alone settle the scale
+    top = run_max(top);
+    const bool odd = top >= kInf;
+    if (odd) {  // something is not finite: the finite values alone settle the scale
       top = 0;
-      for (int64_t base = 0; base < count; base += 16) {
+      for (int64_t base = begin; base < count; base += step) {
         load(base);
         top = max(top, largest(true));
       }
-      top = wave_max(top);
+      top = run_max(top);
     }
     const float old = first > 0 ? canonical_scale(stored) : 0.f;
     const float now = fmaxf(old, scale_for(widen<BF16>(top)));
     if (now > old && old > 0.f) {
       const float ratio = old / now;  // a power of two: exact
-      for (int t = r; t < (int)first; t += RPP) {
+      for (int t = r + (split ? wave * RPP : 0); t < (int)first; t += split ? 4 * RPP : RPP) {
         u32x2* cell = reinterpret_cast<u32x2*>(dst + (int64_t)t * p.token_stride);
         const u32x2 codes = *cell;
         *cell = u32x2{lower_codes(codes.x, ratio), lower_codes(codes.y, ratio)};
@@ -219,15 +238,15 @@ __global__ __launch_bounds__(256) void store_block_scaled_kernel(const StorePara
             u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
       }
     };
-    if (count <= 16) {
-      encode(0);
+    if (begin + step >= count && !odd) {  // the rows are still in registers
+      encode(begin);
     } else {
-      for (int64_t base = 0; base < count; base += 16) {
+      for (int64_t base = begin; base < count; base += step) {
         load(base);
         encode(base);
       }
     }
-    if (lane == 0) *scale_at = now;
+    if (lane == 0 && (!split || wave == 0)) *scale_at = now;
   }
 }
 
@@ -254,21 +273,36 @@ hipError_t launch_store_block_scaled(const void* k, const void* v, void* k_cache
   p.block_stride = B * H * D;
   p.token_stride = hnd ? D : H * D;
   p.head_stride = hnd ? B * D : D;
-  // Rows a wave looks for runs among (see above): 16 from as many rows on as give every compute unit
-  // 16 waves of one.
-  const int range = n_rows * 2 * num_kv_heads < 16 * 256 ? 1 : 16;
-  const dim3 grid((unsigned)((n_rows + range - 1) / range), (unsigned)((2 * num_kv_heads + 3) / 4)), block(256);
-#define AYK_STORE(W)                                                                                   \
-  do {                                                                                                 \
-    if (bf16) hipLaunchKernelGGL((store_block_scaled_kernel<W, true>), grid, block, 0, stream, p, range);     \
-    else hipLaunchKernelGGL((store_block_scaled_kernel<W, false>), grid, block, 0, stream, p, range);         \
+  // Rows to a range. Few rows (a decode step): every run on a wave of its own, beside the others.
+  // Many: as many as keep the waves that find no run to do few, for starting them is what such a step
+  // then costs (16.4K rows of 8 heads of 128 that follow each other, us: blocks of 16, a wave to each
+  // row 127, 4 rows 49, 16 rows 21; blocks of 64 and ranges of 16 47, of 32 27). Where each row
+  // begins a run a long range does them one after the other (1024 such rows: 9.4, 8.7, 16.8), so
+  // between the two a middle one. By the waves that one row each would take:
+  const int64_t waves = n_rows * 2 * num_kv_heads;
+  const bool coop = block_size > 16;
+  const int range = coop ? (waves <= 8192 ? 4 : waves <= 32768 ? 16 : block_size <= 32 ? 32 : 63)
+                         : (waves <= 8192 ? 1 : waves <= 32768 ? 4 : 16);
+  const dim3 grid((unsigned)((n_rows + range - 1) / range),
+                  (unsigned)(coop ? 2 * num_kv_heads : (2 * num_kv_heads + 3) / 4));
+  const dim3 block(256);
+#define AYK_STORE(W, C)                                                                                    \
+  do {                                                                                                     \
+    if (bf16) hipLaunchKernelGGL((store_block_scaled_kernel<W, true, C>), grid, block, 0, stream, p, range); \
+    else hipLaunchKernelGGL((store_block_scaled_kernel<W, false, C>), grid, block, 0, stream, p, range);     \
+  } while (0)
+#define AYK_STORE_WIDTH(W)             \
+  do {                                 \
+    if (coop) AYK_STORE(W, true);      \
+    else AYK_STORE(W, false);          \
   } while (0)
   switch (head_dim) {
-    case 64: AYK_STORE(64); break;
-    case 128: AYK_STORE(128); break;
-    case 256: AYK_STORE(256); break;
+    case 64: AYK_STORE_WIDTH(64); break;
+    case 128: AYK_STORE_WIDTH(128); break;
+    case 256: AYK_STORE_WIDTH(256); break;
     default: return hipErrorInvalidValue;
   }
+#undef AYK_STORE_WIDTH
 #undef AYK_STORE
   return hipGetLastError();
 }
