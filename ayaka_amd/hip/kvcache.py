@@ -38,6 +38,7 @@ __all__ = ["build_tables", "copy_blocks", "gather", "layout", "store", "zero_blo
 
 _LAYOUT_CODES = {KVLayoutKind.NHD: 0, KVLayoutKind.HND: 1}
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
+_I32 = torch.int32
 
 
 def layout() -> KVLayoutKind:
@@ -274,12 +275,40 @@ def build_tables(
     ``kv_lengths`` itself. Nothing waits for the device, and the call can be captured.
     """
     op = "kvcache.build_tables"
+    free, taken, after = pool
+    request_of_row, positions, slots, lengths = tables
+    requests, rows, width = kv_lengths.numel(), positions.numel(), block_table.shape[-1] if block_table.ndim else 0
+    index = block_table.get_device()
+    if not (index >= 0 and block_table.ndim == 2 and block_table.shape[0] == requests and block_table.dtype is _I32
+            and block_table.is_contiguous() and _vector(rows_per_request, requests, _I32, index)
+            and _vector(kv_lengths, requests, _I32, index) and _vector(lengths, requests, _I32, index)
+            and _vector(request_of_row, rows, _I32, index) and _vector(positions, rows, _I32, index)
+            and _vector(slots, rows, torch.int64, index) and _vector(free, free.numel(), _I32, index)
+            and _vector(taken, 1, _I32, index) and _vector(after, 4, _I32, index)):
+        _refuse_tables(op, rows_per_request, kv_lengths, block_table, pool, tables)
+    _lib.check(op, _lib.lib().ayk_build_tables(
+        rows_per_request.data_ptr(), kv_lengths.data_ptr(), requests, block_table.data_ptr(), width, width,
+        free.data_ptr(), free.numel(), taken.data_ptr(), after.data_ptr(), block_size, request_of_row.data_ptr(),
+        positions.data_ptr(), slots.data_ptr(), rows, lengths.data_ptr(), _stream(block_table.device),
+    ))
+
+
+def _vector(tensor: torch.Tensor, count: int, dtype: torch.dtype, index: int) -> bool:
+    """Whether ``tensor`` is a contiguous vector of ``count`` elements on device ``index`` (the quick
+    form of the checks below: ten tensors a call, on a kernel of a few microseconds)."""
+    return (tensor.numel() == count and tensor.ndim == 1 and tensor.dtype is dtype and tensor.is_contiguous()
+            and tensor.get_device() == index)
+
+
+def _refuse_tables(op: str, rows_per_request: torch.Tensor, kv_lengths: torch.Tensor, block_table: torch.Tensor,
+                   pool: BlockPool, tables: StepTables) -> None:
+    """Say what is wrong with a call of :func:`build_tables`."""
     device = block_table.device
     if not block_table.is_cuda:
         raise BackendError(f"{op}: the hip backend runs on a HIP device; block_table is on {device}",
                            context={"op": op, "argument": "block_table"})
-    requests, rows = kv_lengths.shape[0] if kv_lengths.ndim == 1 else -1, tables.positions.numel()
-    width = block_table.shape[1] if block_table.ndim == 2 else -1
+    requests, rows = kv_lengths.numel(), tables.positions.numel()
+    width = block_table.shape[1] if block_table.ndim == 2 else 0
     require_pool(op, pool, device)
     for name, tensor, shape, dtype in (
         ("rows_per_request", rows_per_request, (requests,), torch.int32),
@@ -294,9 +323,3 @@ def build_tables(
         if tensor.device != device:
             raise BackendError(f"{op}: {name} is on {tensor.device}, the table is on {device}",
                                context={"op": op, "argument": name})
-    _lib.check(op, _lib.lib().ayk_build_tables(
-        rows_per_request.data_ptr(), kv_lengths.data_ptr(), requests, block_table.data_ptr(), width, width,
-        pool.free.data_ptr(), pool.free.shape[0], pool.taken.data_ptr(), pool.after.data_ptr(), block_size,
-        tables.request_of_row.data_ptr(), tables.positions.data_ptr(), tables.slot_mapping.data_ptr(), rows,
-        tables.kv_lengths.data_ptr(), _stream(device),
-    ))
