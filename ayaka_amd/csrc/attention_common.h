@@ -179,30 +179,39 @@ __device__ __forceinline__ f32x2 load_block_scale(const AttnParams& p, uint32_t 
   return *reinterpret_cast<const f32x2*>(p.block_scales + 2 * ((int64_t)id * kv_heads + kvh));
 }
 
-// The NaN codes (0x7f, 0xff) among 8 loaded codes, one bit each; they are replaced by zeros.
-// A masked position's weight is 0, and 0 * NaN would reach every row of its tile: where a chunk is
-// masked for some rows, the rows that do attend to such a value get their NaN from these bits.
-__device__ __forceinline__ uint32_t take_nan_codes(u32x2& w) {
-  uint32_t bits = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t n = (((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in each such byte
-    w[i] &= ~(n * 0xffu);
-    bits |= ((n | n >> 7 | n >> 14 | n >> 21) & 0xfu) << (4 * i);
-  }
-  return bits;
+// One bit (the lowest of its byte) for each NaN code, 0x7f or 0xff, of a word.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
 }
 
-// Set the elements of o (slice t: elements 16t + 4mq + i) whose bit is set in a position's NaN
-// bits, one byte per 8 elements.
-template <int DT>
-__device__ __forceinline__ void put_nan(f32x4 (&o)[DT], const uint8_t* bits, int mq) {
+// Replace the NaN codes among 8 loaded codes by zeros; whether there were any. A masked position's
+// weight is 0, and 0 * NaN would reach every row of its tile: where a chunk is masked for some rows its
+// NaN values are taken out, and put back at the end into the rows that do attend to them.
+__device__ __forceinline__ bool take_nan_codes(u32x2& w) {
+  const uint32_t a = nan_codes(w.x), b = nan_codes(w.y);
+  w.x &= ~(a * 0xffu);
+  w.y &= ~(b * 0xffu);
+  return (a | b) != 0;
+}
+
+// NaN into the elements of o (slice t: elements 16t + 4mq + i of a pair's output) at which a value of
+// positions [from, to), up to and with position `limit`, is NaN. `values` is the head's in the cache.
+template <int D>
+__device__ __forceinline__ void put_nan_values(const AttnParams& p, const int32_t* tbl, const uint16_t* values,
+                                               int from, int to, int limit, int mq, f32x4 (&o)[D / 16]) {
+  const uint8_t* codes = reinterpret_cast<const uint8_t*>(values) + 4 * mq;
+#pragma unroll 1
+  for (int t = max(from, 0); t < to; ++t) {
+    const int b = block_of(p, t);
+    const int64_t at = (int64_t)table_entry(p, tbl[b]) + (int64_t)(t - b * p.block_size) * p.token_stride;
+    if (t > limit) continue;
 #pragma unroll
-  for (int t = 0; t < DT; ++t) {
-    const uint32_t b = (uint32_t)bits[2 * t + (mq >> 1)] >> (4 * (mq & 1));
+    for (int k = 0; k < D / 16; ++k) {
+      const uint32_t n = nan_codes(*reinterpret_cast<const uint32_t*>(codes + at + 16 * k));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if ((b >> i) & 1u) o[t][i] = __uint_as_float(0x7fc00000u);
+      for (int i = 0; i < 4; ++i)
+        if ((n >> (8 * i)) & 1u) o[k][i] = __uint_as_float(0x7fc00000u);
+    }
   }
 }
 

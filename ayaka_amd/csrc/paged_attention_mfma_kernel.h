@@ -92,7 +92,6 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
   static_assert(!BS || (KV8 && CH <= kWave), "a chunk's scales, one position per lane");
   __shared__ uint32_t s_ids[BS ? kTableCap : 1];                                      // block ids, beside s_tbl
   __shared__ __attribute__((aligned(16))) float s_sc[BS ? kMaxWaves : 1][3][CH];      // a chunk's scales
-  __shared__ __attribute__((aligned(8))) uint8_t s_nan[BS && WIN ? kMaxWaves : 1][MT * CPT];  // take_nan_codes
   __shared__ int s_last;
   // v1 with a row's context split among waves: each slice's running max and weight sum
   __shared__ float s_slice_m[kMaxWaves][16], s_slice_l[kMaxWaves][16];
@@ -217,6 +216,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
   const uint16_t* kbase = kv_at<KV8>(p.k_cache, (int64_t)kvh * p.head_stride + c * 8);
   const uint16_t* vbase = kv_at<KV8>(p.v_cache, (int64_t)kvh * p.head_stride + c * 8);
 
+  [[maybe_unused]] bool nan_taken = false;  // BS windows: NaN values of chunks that some rows do not see
   for (int s0 = t_begin; s0 < t_end; s0 += seg_len) {
     const int s1 = min(t_end, s0 + seg_len);
     const int b0 = (!WIN && s0 == t_begin) ? commit_table<2, BS>(p, tbl, s_tbl, ahead, s1, tid, threads, s_ids)
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
     auto consume = [&](int ci, const Raw(&kc)[NL], const Raw(&vc)[NL], auto&& keys_used, auto&& values_used) {
       const int tc = s0 + ci * CH;
       const bool tail = tc + CH > s1;
-      // BS windows: some row of the tile does not see all of the chunk, so its NaN values are kept apart
+      // BS windows: some row of the tile does not see all of the chunk, so its NaN values are taken out
       const bool apart = BS && WIN && tc + CH - 1 > win_least;
       if constexpr (BS) {
         const PositionScale ps = position_scale(sc, scale_log2);
@@ -330,25 +330,17 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
         // The tile's values to LDS (token-major, read back transposed) only now: their
         // loads were issued with this chunk's, and the wait for them overlaps q.k and
         // the softmax (C2 24.7 -> 24.0 us, fp8 C3 87.7 -> 86.2 us).
-        uint64_t nan_lanes = 0;  // BS windows: lanes that hold NaN values of a chunk kept apart
-        if constexpr (BS && WIN) {
-          if (apart) {
-            uint32_t any = 0;
 #pragma unroll
-            for (int j = 0; j < NL1; ++j) {
+        for (int j = 0; j < NL1; ++j) {
+          if constexpr (BS && WIN) {
+            if (apart) {
               Raw raw = vc[sub * NL1 + j];
-              const uint32_t bits = take_nan_codes(raw);
-              any |= bits;
-              s_nan[wave][(j * TPL + r) * CPT + c] = (uint8_t)bits;
+              nan_taken |= take_nan_codes(raw);
               *reinterpret_cast<u32x4*>(&s_v[wave][(j * TPL + r) * VP + c * 8]) = kv_pairs<KV8, PB>(raw);
+              continue;
             }
-            nan_lanes = __builtin_amdgcn_ballot_w64(any != 0);
           }
-        }
-        if (!apart) {
-#pragma unroll
-          for (int j = 0; j < NL1; ++j)
-            *reinterpret_cast<u32x4*>(&s_v[wave][(j * TPL + r) * VP + c * 8]) = kv_pairs<KV8, PB>(vc[sub * NL1 + j]);
+          *reinterpret_cast<u32x4*>(&s_v[wave][(j * TPL + r) * VP + c * 8]) = kv_pairs<KV8, PB>(vc[sub * NL1 + j]);
         }
         wave_lds_sync();
         if (sub == SUB - 1) values_used();
@@ -357,16 +349,6 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
           const u32x2 va = lds_read_transposed(&s_v[wave][(4 * mq + (mt >> 2)) * VP + t * 16 + 4 * (mt & 3)]);
           o[t] = mfma_pv<PB>(va, phi, o[t]);
           if constexpr (split_p(PB)) o[t] = mfma_pv<PB>(va, plo, o[t]);
-        }
-        if constexpr (BS && WIN) {
-          if (nan_lanes != 0) {
-#pragma unroll 1
-            for (int k = 0; k < MT; ++k) {
-              const int t = tc + sub * MT + k;
-              if (win_col && t <= win_lim && t < s1) put_nan(o, &s_nan[wave][k * CPT], mq);
-            }
-            wave_lds_sync();  // the next tile's bits go to the same place
-          }
         }
       }
     };
@@ -439,6 +421,12 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
         ci += ws;
       }
     }
+  }
+  if constexpr (BS && WIN) {
+    // (such a chunk begins at most CH - 1 positions before the first one that some row does not see)
+    if (__builtin_amdgcn_ballot_w64(nan_taken))
+      put_nan_values<D>(p, tbl, kv_at<KV8>(p.v_cache, (int64_t)kvh * p.head_stride), max(t_begin, win_least - CH + 2),
+                        t_end, win_col ? win_lim : -1, mq, o);
   }
   // Head mt's weight sum over the wave's 4 token groups (its lanes share m_h).
   l_h += __shfl_xor(l_h, 16);

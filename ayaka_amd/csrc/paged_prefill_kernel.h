@@ -94,12 +94,22 @@ __host__ __device__ constexpr int prefill_workgroups_per_cu(int head_dim, int wa
 // same grid, runs only the marked workgroups, with the split bf16 P. fp8 caches decode
 // straight to fp16 (every e4m3 value is one), so bf16 models over them always take one MFMA.
 //
-// BS: a block-scaled fp8 cache (KV8). Each chunk's key and value scales are staged beside it, one
-// position per thread, and join the scores (see PositionScale).
-template <int D, bool BF16, bool KV8, int PS, int W = kPrefillWaves, int MODE = 0, bool BS = false>
+// SCALES: a block-scaled fp8 cache (KV8), by how many positions are sure to share a scale: 16 (block
+// sizes that are multiples of it), 4 or 1; 0: no such cache. The scales join the scores (see
+// PositionScale). A table segment's are staged with it, {key, shift} per block, so the chunk loop
+// loads and converts nothing for them. A lane's 4 scores of a tile are of consecutive positions: a
+// scale they share enters with the maximum, the exponent's fma and the tile's weight sum, a few
+// instructions per tile where a scale per position takes one more per score.
+// 4 x 512 rows over 4K of 32/8 heads of 128, blocks of 16: 136 us (0.94 PFLOP/s) against 125 over
+// unscaled codes, 138 with a chunk's scales staged by position; 4 chunks of 150-500 rows over
+// 900-3600, 16/8 heads of 256, blocks of 24: 97 us against 90, 113 so. Of the first's 11 us the
+// maximum takes 4, the sum 2, the reads of the scales 3.
+template <int D, bool BF16, bool KV8, int PS, int W = kPrefillWaves, int MODE = 0, int SCALES = 0>
 __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D, PS)) void paged_prefill_kernel(
     const AttnParams p, const int32_t* tiles) {
   static_assert(W == kPrefillWaves || (W == 8 && PS == 1 && D != 64), "the double tile: 8 waves, one per pair group");
+  constexpr bool BS = SCALES != 0;
+  constexpr bool QUADS = SCALES >= 4;  // a lane's 4 positions of a tile share a scale
   static_assert(!BS || (KV8 && MODE == 0), "block scales: fp8 caches");
   static_assert(MODE == 0 || (BF16 && !KV8), "the fp16 values pass: bf16 models over bf16 caches");
   constexpr bool V16_ALWAYS = KV8 && BF16;  // fp8 codes decode to fp16 values
@@ -148,11 +158,8 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   __shared__ Lds lds;
   __shared__ float s_ml[MERGE_WAVES][PT][2][16];
   __shared__ int s_vbad[2][W];  // V16_FAST: per buffer, each wave's vote (a value that does not convert)
-  __shared__ uint32_t s_ids[BS ? kTableCap : 1];                              // block ids, beside s_tbl
-  __shared__ __attribute__((aligned(16))) float s_sc[BS ? 2 : 1][3][CH];      // a chunk's scales
-  __shared__ uint8_t s_nan[BS ? 2 : 1][BS ? PIECES : 1];                      // take_nan_codes
-  __shared__ int s_nan_any[BS ? 2 : 1][W];  // each wave's vote: it staged NaN values (chunks kept apart)
-  static_assert(!BS || CH <= THREADS, "a chunk's scales, one position per thread");
+  __shared__ f32x2 s_sc[BS ? kTableCap : 1];  // the segment's blocks' scales, beside s_tbl
+  __shared__ int s_nan;                       // BS: a NaN value was taken out of a staged chunk
   auto& s_k = lds.st.k;
   auto& s_v = lds.st.v;
 
@@ -269,16 +276,30 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   // stored, and the fallback pass computes the workgroup (the rest of the chunks still run:
   // leaving the loop early costs the common case registers)
   bool stop = false;
+  if constexpr (BS) {
+    if (tid == 0) s_nan = 0;  // (staging a table begins with a barrier)
+  }
   for (int s0 = t_begin; s0 < t_end; s0 += seg_len) {
     const int s1 = min(t_end, s0 + seg_len);
-    const int b0 = stage_table<BS>(p, tbl, s_tbl, s0, s1, tid, THREADS, s_ids);
+    const int b0 = stage_table(p, tbl, s_tbl, s0, s1, tid, THREADS);
+    // BS: the scales of the segment's blocks, in flight beside the first chunk
+    constexpr int SEG_LOADS = BS ? (kTableCap + THREADS - 1) / THREADS : 1;
+    [[maybe_unused]] f32x2 seg_scale[SEG_LOADS];
+    [[maybe_unused]] const int seg_blocks = block_of(p, s1 - 1) - b0 + 1;
+    if constexpr (BS) {
+#pragma unroll
+      for (int k = 0; k < SEG_LOADS; ++k) {
+        const int i = tid + k * THREADS;
+        seg_scale[k] = f32x2{1.f, 1.f};
+        if (i < seg_blocks) seg_scale[k] = load_block_scale(p, block_id(p, tbl[b0 + i]), kv_heads, kvh);
+      }
+    }
     const int nch = (s1 - s0 + CH - 1) / CH;
-    // BS: some row of the tile does not see all of chunk ci, so its NaN values are kept apart
+    // BS: some row of the tile does not see all of chunk ci, so its NaN values are taken out
     auto apart = [&](int ci) { return BS && s0 + ci * CH + CH - 1 > tile_least; };
 
     typedef typename KvRaw<KV8>::T Raw;
     Raw kr[PER_THREAD], vr[PER_THREAD];
-    f32x2 scr = {1.f, 1.f};  // BS: the scales of position tid of the chunk
     // Chunk ci into registers kr and vr (K and V pieces of a position share its offset).
     // Positions past the segment's last one are read as that one (weight 0, finite
     // values). Block sizes that are a multiple of PER_THREAD (uniform across the launch)
@@ -292,35 +313,18 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
         kr[u] = load_kv_raw<KV8, false>(kbase, off[u]);
         vr[u] = load_kv_raw<KV8, false>(vbase, off[u]);
       }
-      if constexpr (BS) {
-        const int t = min(s0 + ci * CH + tid % CH, s1 - 1);
-        scr = load_block_scale(p, s_ids[block_of(p, t) - b0], kv_heads, kvh);
-      }
     };
     auto stage_keys = [&](int buf) {
-      if constexpr (BS) {
-        if (tid < CH) {
-          const PositionScale sc = position_scale(scr, scale_log2);
-          s_sc[buf][0][tid] = sc.key;
-          s_sc[buf][1][tid] = sc.shift;
-          s_sc[buf][2][tid] = sc.unit;
-        }
-      }
 #pragma unroll
       for (int u = 0; u < PER_THREAD; ++u) s_k[buf][key_slot(first_pos + u, piece_c)] = kv_pairs<KV8, BF16>(kr[u]);
     };
     auto stage_values = [&](int ci, int buf) {
       if constexpr (BS) {
         if (apart(ci)) {
-          uint32_t any = 0;
+          bool any = false;
 #pragma unroll
-          for (int u = 0; u < PER_THREAD; ++u) {
-            const uint32_t bits = take_nan_codes(vr[u]);
-            any |= bits;
-            s_nan[buf][(first_pos + u) * CPT + piece_c] = (uint8_t)bits;
-          }
-          const uint64_t lanes = __builtin_amdgcn_ballot_w64(any != 0);
-          if (lane == 0) s_nan_any[buf][wave] = lanes != 0;
+          for (int u = 0; u < PER_THREAD; ++u) any |= take_nan_codes(vr[u]);
+          if (any) s_nan = 1;
         }
       }
       typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -371,35 +375,53 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
     // state; mid() runs between the rescale and the weights.
     // P.V's operand type: fp16 when the values in LDS are fp16 values, else the model's
     constexpr bool PB = V16 ? false : BF16;
-    auto fold = [&](int ci, int vb, Scores& acc, auto&& mid) {
+    // BS: {key, shift} of position t's block; and of each tile's 4 positions of this lane
+    [[maybe_unused]] auto scale_at = [&](int t) { return s_sc[block_of(p, min(t, s1 - 1)) - b0]; };
+    struct TileScales {
+      f32x2 v[BS ? PTL_W : 1];
+    };
+    [[maybe_unused]] const int uniform_ps = PS == 1 ? 0 : __builtin_amdgcn_readfirstlane(ps);
+    [[maybe_unused]] auto read_scales = [&](int ci, TileScales& ts) {
+#pragma unroll
+      for (int w = 0; w < PTL_W; ++w) {
+        // (a whole tile's block is uniform, and so found without the vector units)
+        const int t = s0 + ci * CH + (uniform_ps * PTL_W + w) * 16;
+        ts.v[w] = SCALES == 16 ? scale_at(t) : SCALES == 4 ? scale_at(t + 4 * mq) : f32x2{1.f, 0.f};
+      }
+    };
+    auto fold = [&](int ci, int vb, Scores& acc, [[maybe_unused]] const TileScales& ts, auto&& mid) {
       const int buf = vb;
       const int tb = s0 + ci * CH;
-      // BS: a score times its key scale, plus its value scale's exponent
-      if constexpr (BS) {
+      // BS, blocks of other sizes: every score takes its own scale first, and the tile's is {1, 0}
+      if constexpr (BS && !QUADS) {
 #pragma unroll
-        for (int w = 0; w < PTL_W; ++w) {
-          const int at = (ps * PTL_W + w) * 16 + 4 * mq;
-          const f32x4 key = *reinterpret_cast<const f32x4*>(&s_sc[buf][0][at]);
-          const f32x4 shift = *reinterpret_cast<const f32x4*>(&s_sc[buf][1][at]);
+        for (int w = 0; w < PTL_W; ++w)
 #pragma unroll
-          for (int j = 0; j < PT; ++j)
+          for (int i = 0; i < 4; ++i) {
+            const f32x2 sc = scale_at(tb + (ps * PTL_W + w) * 16 + 4 * mq + i);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[w][j][i] = __builtin_fmaf(acc[w][j][i], key[i], shift[i]);
-        }
+            for (int j = 0; j < PT; ++j) acc[w][j][i] = __builtin_fmaf(acc[w][j][i], sc.x, sc.y);
+          }
       }
       // uniform: no position masked (and, for folding the scale into the exponent,
       // a scale >= 0, under which the largest raw score gives the largest scaled one)
-      const bool whole = tb + CH <= s1 && tb + CH - 1 <= wave_min_pos && (BS || scale_log2 >= 0.f);
+      const bool whole = tb + CH <= s1 && tb + CH - 1 <= wave_min_pos && scale_log2 >= 0.f;
       // the scale applied to a score in the exponent below (1 once the scores are scaled)
-      const float sc = whole && !BS ? scale_log2 : 1.f;
+      const float sc = whole ? scale_log2 : 1.f;
 #pragma unroll
       for (int j = 0; j < PT; ++j) {
         float mx = -INFINITY;
         if (whole) {
 #pragma unroll
-          for (int w = 0; w < PTL_W; ++w)
+          for (int w = 0; w < PTL_W; ++w) {
+            if constexpr (BS) {
+              const float top = fmaxf(fmaxf(acc[w][j][0], acc[w][j][1]), fmaxf(acc[w][j][2], acc[w][j][3]));
+              mx = fmaxf(mx, __builtin_fmaf(top, ts.v[w].x, ts.v[w].y));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, acc[w][j][i]);
+              for (int i = 0; i < 4; ++i) mx = fmaxf(mx, acc[w][j][i]);
+            }
+          }
           if constexpr (!BS) mx *= scale_log2;
         } else {
           // position tb + pt*16 + 4*mq + i is visible iff pt*16 + i <= lim
@@ -409,7 +431,8 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int pt = ps * PTL_W + w;
-              acc[w][j][i] = pt * 16 + i <= lim ? (BS ? acc[w][j][i] : acc[w][j][i] * scale_log2) : -INFINITY;
+              const float scaled = BS ? __builtin_fmaf(acc[w][j][i], ts.v[w].x, ts.v[w].y) : acc[w][j][i] * scale_log2;
+              acc[w][j][i] = pt * 16 + i <= lim ? scaled : -INFINITY;
               mx = fmaxf(mx, acc[w][j][i]);
             }
         }
@@ -433,21 +456,33 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
 #pragma unroll
       for (int j = 0; j < PT; ++j)
 #pragma unroll
-        for (int w = 0; w < PTL_W; ++w)
+        for (int w = 0; w < PTL_W; ++w) {
+          const float by = BS ? (whole ? ts.v[w].x : 1.f) : sc;
+          const float from = BS ? (whole ? ts.v[w].y - m[j] : -m[j]) : -m[j];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = fast_exp2(__builtin_fmaf(acc[w][j][i], sc, -m[j]));
+            const float e = fast_exp2(__builtin_fmaf(acc[w][j][i], by, from));
             acc[w][j][i] = e;
             if constexpr (!LSUM_MFMA && !BS) l[j] += e;
           }
+        }
       if constexpr (BS) {
+        // a weight enters the sum by 2^-shift
 #pragma unroll
         for (int w = 0; w < PTL_W; ++w) {
-          const f32x4 unit = *reinterpret_cast<const f32x4*>(&s_sc[buf][2][(ps * PTL_W + w) * 16 + 4 * mq]);
+          if constexpr (QUADS) {
+            const float unit = fast_exp2(-ts.v[w].y);
 #pragma unroll
-          for (int j = 0; j < PT; ++j)
+            for (int j = 0; j < PT; ++j)
+              l[j] = __builtin_fmaf((acc[w][j][0] + acc[w][j][1]) + (acc[w][j][2] + acc[w][j][3]), unit, l[j]);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) l[j] = __builtin_fmaf(acc[w][j][i], unit[i], l[j]);
+            for (int i = 0; i < 4; ++i) {
+              const float unit = fast_exp2(-scale_at(tb + (ps * PTL_W + w) * 16 + 4 * mq + i).y);
+#pragma unroll
+              for (int j = 0; j < PT; ++j) l[j] = __builtin_fmaf(acc[w][j][i], unit, l[j]);
+            }
+          }
         }
       }
       if constexpr (PTL_W >= 2) {
@@ -507,26 +542,19 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
           }
         }
       }
-      if constexpr (BS) {
-        if (apart(ci)) {
-          int any = 0;
-#pragma unroll
-          for (int v = 0; v < W; ++v) any |= s_nan_any[buf][v];
-          if (any) {
-#pragma unroll 1
-            for (int k = ps * PTL_W * 16; k < (ps + 1) * PTL_W * 16; ++k) {
-#pragma unroll
-              for (int j = 0; j < PT; ++j)
-                if (tb + k <= my_pos[j] && tb + k < s1) put_nan(o[j], &s_nan[buf][k * CPT], mq);
-            }
-          }
-        }
-      }
     };
 
     load_chunk(0);
     stage_keys(0);
     stage_values(0, 0);
+    if constexpr (BS) {
+#pragma unroll
+      for (int k = 0; k < SEG_LOADS; ++k) {
+        const int i = tid + k * THREADS;
+        const PositionScale sc = position_scale(seg_scale[k], scale_log2);
+        if (i < seg_blocks) s_sc[i] = f32x2{sc.key, sc.shift};
+      }
+    }
     lds_barrier();
     // Two chunks per iteration, so that each body's LDS buffer is a constant (immediate
     // address offsets instead of per-access arithmetic).
@@ -547,10 +575,12 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
       // that its matrix instructions issue ahead of the other wave's max and rescale
       // VALU work, which fills the issue slots between them (5-6% on prefill chunks).
       Scores acc;
+      TileScales ts;
+      if constexpr (BS) read_scales(ci, ts);
       __builtin_amdgcn_s_setprio(1);
       scores(buf, acc);
       __builtin_amdgcn_s_setprio(0);
-      fold(ci, buf, acc, [] { __builtin_amdgcn_s_setprio(1); });
+      fold(ci, buf, acc, ts, [] { __builtin_amdgcn_s_setprio(1); });
       __builtin_amdgcn_s_setprio(0);
       if (ci + 1 < nch) {
         stage_keys(buf ^ 1);
@@ -571,6 +601,15 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   if (stop) {
     if (tid == 0) p.arrivals[blockIdx.x] = 1;
     return;
+  }
+  if constexpr (BS) {
+    if (s_nan) {  // uniform: the last chunk ended on a barrier
+      // the chunks that lost NaN values begin at most CH - 1 positions before the first one that some
+      // row does not see
+#pragma unroll
+      for (int j = 0; j < PT; ++j)
+        put_nan_values<D>(p, tbl, vbase, max(t_begin, tile_least - CH + 2), t_end, my_pos[j], mq, o[j]);
+    }
   }
   // Each pair's weight sum over the 4 position groups; lane (mq, mt) holds
   // elements 16*t + 4*mq + i of pair mt of each group.
@@ -637,15 +676,21 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   }
 }
 
-// Over block-scaled fp8 caches.
+// Over block-scaled fp8 caches; SCALES as the kernel's.
 template <int D, int PS, int W = kPrefillWaves>
 static hipError_t launch_prefill_ps_block_scaled(const AttnParams& p, const int32_t* tiles, dim3 grid, bool bf16,
                                                  hipStream_t stream) {
   const dim3 block(W * kWave);
-  if (bf16)
-    hipLaunchKernelGGL((paged_prefill_kernel<D, true, true, PS, W, 0, true>), grid, block, 0, stream, p, tiles);
-  else
-    hipLaunchKernelGGL((paged_prefill_kernel<D, false, true, PS, W, 0, true>), grid, block, 0, stream, p, tiles);
+  if (p.block_size % 16 == 0) {
+    if (bf16) hipLaunchKernelGGL((paged_prefill_kernel<D, true, true, PS, W, 0, 16>), grid, block, 0, stream, p, tiles);
+    else hipLaunchKernelGGL((paged_prefill_kernel<D, false, true, PS, W, 0, 16>), grid, block, 0, stream, p, tiles);
+  } else if (p.block_size % 4 == 0) {
+    if (bf16) hipLaunchKernelGGL((paged_prefill_kernel<D, true, true, PS, W, 0, 4>), grid, block, 0, stream, p, tiles);
+    else hipLaunchKernelGGL((paged_prefill_kernel<D, false, true, PS, W, 0, 4>), grid, block, 0, stream, p, tiles);
+  } else {
+    if (bf16) hipLaunchKernelGGL((paged_prefill_kernel<D, true, true, PS, W, 0, 1>), grid, block, 0, stream, p, tiles);
+    else hipLaunchKernelGGL((paged_prefill_kernel<D, false, true, PS, W, 0, 1>), grid, block, 0, stream, p, tiles);
+  }
   return hipGetLastError();
 }
 
