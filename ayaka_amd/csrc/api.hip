@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <string>
 
 #include "ayaka_hip.h"
@@ -51,6 +52,13 @@ void block_divisor(int32_t bs, uint32_t& magic, int32_t& shift) {
   while ((1 << s) < bs) ++s;
   shift = s;
   magic = (uint32_t)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - (uint64_t)bs) / (uint64_t)bs + 1);
+}
+
+// Whether any of these addresses is not a multiple of `to`.
+bool misaligned(uintptr_t to, std::initializer_list<const void*> addresses) {
+  for (const void* at : addresses)
+    if (reinterpret_cast<uintptr_t>(at) % to != 0) return true;
+  return false;
 }
 
 // Split a group of query heads into equal chunks of at most 8 heads (one workgroup each).
@@ -107,9 +115,14 @@ int prepare(const char* op, const AttnCall& c, ayk::AttnParams& p, int& heads_pe
   if (c.n_rows > 0 && (!c.out || !c.q || !c.k_cache || !c.v_cache || !c.block_table ||
                        !c.kv_lengths))
     return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
-  if (c.scaled && c.n_rows > 0 && (!c.block_scales || reinterpret_cast<uintptr_t>(c.block_scales) % 8 != 0))
-    return fail(AYK_ERR_ARGUMENT, "%s: block_scales at %p is null or not 8-byte aligned", op,
-                (const void*)c.block_scales);
+  if (c.scaled && c.n_rows > 0) {
+    if (!c.block_scales || misaligned(8, {c.block_scales}))
+      return fail(AYK_ERR_ARGUMENT, "%s: block_scales at %p is null or not 8-byte aligned", op,
+                  (const void*)c.block_scales);
+    if (misaligned(16, {c.q, c.out}) || misaligned(8, {c.k_cache, c.v_cache}))
+      return fail(AYK_ERR_ARGUMENT, "%s: q at %p and out at %p are not 16-byte aligned, or caches at %p and %p 8-byte",
+                  op, c.q, c.out, c.k_cache, c.v_cache);
+  }
   const int group = c.num_heads / c.num_kv_heads;
   const int chunks = head_chunks_for(group);
   heads_per_chunk = group / chunks;
@@ -696,6 +709,9 @@ int ayk_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_
   if (n_rows == 0) return ok();
   if (!k || !v || !k_cache || !v_cache || !scales || !slot_mapping)
     return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  if (misaligned(16, {k, v}) || misaligned(8, {k_cache, v_cache}) || misaligned(4, {scales}))
+    return fail(AYK_ERR_ARGUMENT, "%s: rows at %p and %p are not 16-byte aligned, or caches at %p and %p 8-byte", op, k,
+                v, k_cache, v_cache);
   uint32_t magic;
   int32_t shift;
   block_divisor(block_size, magic, shift);

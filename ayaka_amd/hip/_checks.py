@@ -69,6 +69,7 @@ def capturing(tensor: torch.Tensor) -> bool:
 # torch's raw handle of the current stream, without building a Stream object per call
 # (about 3 us of host time each): the ops launch once per layer and per call.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def stream_handle(device: torch.device) -> int:
@@ -76,7 +77,15 @@ def stream_handle(device: torch.device) -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index if device.index is not None else torch.cuda.current_device()
-    return _raw_stream(index)
+    handle = _raw_stream(index)
+    if handle == 0 and _current_device() != index:
+        # handle 0 is the current device's default stream, whichever device that is
+        raise BackendError(
+            f"the tensors are on device {index} and its default stream is current, but device {_current_device()} "
+            "is: run the call under torch.cuda.device(...)",
+            context={"device": index},
+        )
+    return handle
 
 
 def require_like(

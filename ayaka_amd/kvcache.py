@@ -226,7 +226,8 @@ class KVCacheOps(Protocol):
     def store(self, k: Tensor, v: Tensor, buffers: KVBuffers, meta: AttentionMetadata) -> None: ...
 
     def gather(
-        self, buffers: KVBuffers, block_ids: Tensor, out_k: Tensor, out_v: Tensor
+        self, buffers: KVBuffers, block_ids: Tensor, out_k: Tensor, out_v: Tensor,
+        out_scales: Tensor | None = None,
     ) -> None: ...
 
     def copy_blocks(self, buffers: KVBuffers, src: Tensor, dst: Tensor) -> None: ...

@@ -151,7 +151,7 @@ def test_block_scaled_caches_hold_fp8_codes() -> None:
 
 
 def _store(**kw: object) -> int:
-    args = dict(k=1, v=1, k_cache=1, v_cache=1, scales=8, slots=1, n_rows=1, kv_heads=2, head_dim=64, num_blocks=4,
+    args = dict(k=16, v=16, k_cache=8, v_cache=8, scales=8, slots=8, n_rows=1, kv_heads=2, head_dim=64, num_blocks=4,
                 block_size=16, layout=0, dtype=1, stream=None)
     args.update(kw)
     return _lib.lib().ayk_store_block_scaled(*args.values())
@@ -168,6 +168,9 @@ def _store(**kw: object) -> int:
     ({"num_blocks": 1 << 21, "block_size": 16}, 2, b"32-bit element offsets"),
     ({"n_rows": 1 << 32}, 2, b"exceed one launch"),
     ({"scales": None}, 1, b"null"),
+    ({"k": 24}, 1, b"not 16-byte aligned"),
+    ({"v": 18}, 1, b"not 16-byte aligned"),
+    ({"v_cache": 12}, 1, b"not 16-byte aligned"),
 ])
 def test_the_library_refuses_bad_stores(changes: dict, code: int, message: bytes) -> None:
     assert _store(**changes) == code
@@ -182,7 +185,7 @@ def test_no_rows_is_no_launch() -> None:
 
 
 def _v1(**kw: object) -> int:
-    args = dict(out=1, q=1, k=1, v=1, scales=8, table=1, stride=4, lengths=1, ror=None, pos=None, n_rows=1, heads=8,
+    args = dict(out=16, q=16, k=8, v=8, scales=8, table=1, stride=4, lengths=1, ror=None, pos=None, n_rows=1, heads=8,
                 kv_heads=2, head_dim=128, num_blocks=10, block_size=16, max_blocks=4, layout=0, dtype=1, scale=1.0,
                 flags=0, stream=None)
     args.update(kw)
@@ -197,6 +200,9 @@ def _v1(**kw: object) -> int:
     ({"head_dim": 96}, 2, b"head_dim 96"),
     ({"heads": 7}, 1, b"not a positive multiple"),
     ({"q": None}, 1, b"null"),
+    ({"q": 8}, 1, b"not 16-byte aligned"),
+    ({"out": 24}, 1, b"not 16-byte aligned"),
+    ({"k": 4}, 1, b"not 16-byte aligned"),
 ])
 def test_the_library_refuses_bad_attention(changes: dict, code: int, message: bytes) -> None:
     assert _v1(**changes) == code
@@ -205,7 +211,7 @@ def test_the_library_refuses_bad_attention(changes: dict, code: int, message: by
 
 def test_multi_row_and_split_refusals() -> None:
     lib = _lib.lib()
-    base = (1, 1, 1, 1, 8, 1, 4, 1)
+    base = (16, 16, 8, 8, 8, 1, 4, 1)
     shape = (1, 8, 2, 128, 10, 16, 4, 0, 1, 1.0)
     assert lib.ayk_paged_attention_v2_block_scaled(*base, None, None, *shape, 100, 4, None, 0, None, 1, 1 << 20, None,
                                                    0, None) == 1
@@ -254,3 +260,14 @@ def test_loads_stay_in_the_cache(head_dim: int) -> None:
         pairs = _lib.lib().ayk_paged_prefill_tile_pairs(head_dim)
         check(lambda lib: lib.ayk_paged_prefill_block_scaled(
             *args[:10], kv_reach._ptr(tiles), tiles.size // 4, pairs, *args[10:], 0, None, 0, None), "multi-row")
+
+
+def test_a_default_stream_of_another_device_is_refused(monkeypatch: pytest.MonkeyPatch) -> None:
+    # the raw handle 0 names the current device's default stream, whichever device the tensors are on
+    monkeypatch.setattr(_checks, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(_checks, "_current_device", lambda: 0)
+    assert _checks.stream_handle(torch.device("cuda", 0)) == 0
+    with pytest.raises(BackendError, match="tensors are on device 1 .* under torch.cuda.device"):
+        _checks.stream_handle(torch.device("cuda", 1))
+    monkeypatch.setattr(_checks, "_raw_stream", lambda index: 77)  # a stream of its own names its device
+    assert _checks.stream_handle(torch.device("cuda", 1)) == 77

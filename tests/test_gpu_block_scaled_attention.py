@@ -112,7 +112,7 @@ class Step:
                         s = self.scale * (kk @ q[at + j, h])
                         w = np.exp(s - s.max())
                         w /= w.sum()
-                        size = self.scale * (np.abs(kk) @ np.abs(q[at + j, h])).max()
+                        size = abs(self.scale) * (np.abs(kk) @ np.abs(q[at + j, h])).max()
                         d = ((dim + 8) * size + 2 * (size + 128) + end + 16) * 2.0 ** -24
                         y[at + j, h] = w @ vv
                         vs = self.scales[ids, h // group, 1].repeat(self.block)[:end]
@@ -377,6 +377,60 @@ def test_a_captured_decode_bucket(ops) -> None:
             size = y.float().abs().max()
             assert (x.float() - y.float()).abs().max() <= 2 * size * (2.0 ** -8 + 2.0 ** -10), at
             assert not x[lengths == 0].any()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+@pytest.mark.parametrize("mode,steps", [("decode", [(1, 300), (1, 0)]), ("mixed", [(4, 300)]), ("mixed", [(50, 300)])])
+def test_softmax_scales_of_zero_and_below(ops, mode, steps, scale) -> None:
+    for block in (16, 12, 7):
+        step = Step(steps, heads=8, head_dim=128, mode=mode, block=block, seed=4)
+        step.scale = scale
+        # (S is of the scores' magnitudes; a scale of 0 averages the values)
+        run(ops, step)
+
+
+def test_queries_and_outputs_inside_other_tensors(ops) -> None:
+    # rows that begin 16 bytes into their storage, caches 8 bytes; a step's first rows of larger outputs,
+    # whose other rows stay as they were
+    step = Step([(1, 40), (1, 77)], heads=4, mode="decode", head_dim=64)
+    q, buffers, meta, out = step.device(ops)
+
+    def moved(t, bytes_in, rows=None):
+        flat = torch.full((t.numel() * t.element_size() + bytes_in + 512,), 0x55, dtype=torch.uint8, device=DEV)
+        view = flat[bytes_in:bytes_in + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+        view.view(torch.uint8).copy_(t.view(torch.uint8))
+        return view, flat
+
+    q2, _ = moved(q, 16)
+    out2, whole = moved(out, 16)
+    k2, _ = moved(buffers.k, 8)
+    v2, _ = moved(buffers.v, 8)
+    ops.attention.attend(q2, buffers._replace(k=k2, v=v2), meta, out2, scale=step.scale)
+    step.check(out2)
+    size = out.numel() * out.element_size()
+    assert (whole[:16] == 0x55).all() and (whole[16 + size:] == 0x55).all()
+    odd, _ = moved(q, 2)
+    with pytest.raises(BackendError, match="not 16-byte aligned"):
+        ops.attention.attend(odd, buffers, meta, out, scale=step.scale)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_a_captured_multi_row_step(ops, rows) -> None:
+    step = Step([(rows, 900), (2, 60)], heads=8, head_dim=128, block=16, seed=6)
+    q, buffers, meta, out = step.device(ops)
+    ops.attention.attend(q, buffers, meta, out, scale=step.scale)  # its tiles and scratch
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.attention.attend(q, buffers, meta, out, scale=step.scale)
+    for _ in range(3):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        ops.attention.attend(q, buffers, meta, torch.empty_like(out), scale=step.scale)
+    step.check(out)
 
 
 def test_repeated_calls_follow_scales_that_moved(ops) -> None:

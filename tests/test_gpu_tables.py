@@ -312,6 +312,26 @@ def test_a_request_left_without_its_block_stays_out(ops) -> None:
     Built(ops, [1, 1, 1], [6, 6, 9], np.array([[3, 0, 0], [3, 4, 0], [5, 6, 0]]), [30, 31], 0, 4, 3).check()
 
 
+def test_a_bucket_of_one_partition_per_row(ops) -> None:
+    # a table of one partition runs the single-pass kernel: the staged split is written and not read
+    heads, kv_heads, dim, block = 4, 2, 64, 16
+    buffers = bucket_caches("block", 20, block, kv_heads, dim)
+    meta = ops.attention.graph_metadata(3, 3, block, DEV)
+    assert meta.plan.partitions == 1
+    table = np.array([[1, 2, 0], [3, 0, 0], [0, 0, 0]])
+    ops.attention.update_graph_metadata(meta, torch.tensor([20, 16, 0], dtype=torch.int32),
+                                        torch.from_numpy(table.astype(np.int32)))
+    lengths = np.array([21, 17, 1])
+    ops.attention.advance_graph_metadata(meta, dev(lengths), BlockPool.in_place(dev([9, 10])))
+    check_split(meta, lengths)
+    q = torch.randn(3, heads, dim, device=DEV).to(torch.bfloat16)
+    out, eager = torch.empty_like(q), torch.empty_like(q)
+    ops.attention.attend(q, buffers, meta, out, scale=0.125)
+    planned = ops.attention.plan(ForwardMode.DECODE, dev([1, 1, 1]), dev(lengths), meta.block_table, block)
+    hip_attention.attend_with(q, buffers, planned, eager, scale=0.125, partitions=0)
+    assert torch.equal(out, eager)
+
+
 def test_attend_keeps_the_device_split(ops) -> None:
     # a first attend whose head shape the host had not guessed stages the host's split again, but
     # not over one that the device has made since
