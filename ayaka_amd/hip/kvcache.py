@@ -269,10 +269,11 @@ def build_tables(
 
     A request that cannot be served -- negative rows, more rows than tokens, more blocks than W,
     rows past the tables' N, the padding block 0 where its last held block should be, or a pool that
-    runs out at it or before it while it needs a block -- gets no block, slots and positions of 0 and a length of 0 in ``tables.kv_lengths``, and counts
-    into ``pool.after[1]``; a request of length 0 is padding and does not. Rows of the tables behind
-    the last request's get request, position and slot 0. ``tables.kv_lengths`` may be
-    ``kv_lengths`` itself. Nothing waits for the device, and the call can be captured.
+    runs out at it or before it while it needs a block -- gets no block, slots and positions of 0 and
+    a length of 0 in ``tables.kv_lengths``, and counts into ``pool.after[1]``; a request of length 0
+    is padding and does not. Rows of the tables behind the last request's get request, position and
+    slot 0. ``tables.kv_lengths`` may be ``kv_lengths`` itself. Nothing waits for the device, and the
+    call can be captured.
     """
     op = "kvcache.build_tables"
     free, taken, after = pool

@@ -10,8 +10,8 @@
  * value scale for every block and key/value head. An element is worth code * scale. A scale is a
  * power of two 2^e, -40 <= e <= 80, or 0 for a block of nothing but zeros; a fresh cache's scales
  * are zeros. Head widths are 64, 128 and 256; caches are written from and read by fp16 and bf16
- * models. Rows (k, v, q, out) are 16-byte aligned, caches 8-byte. The reference defines the codec field and only the "raw" codec
- * (python/ayaka/ops/kvcache.py:35-36, :54-55).
+ * models. Rows (k, v, q, out) are 16-byte aligned, caches 8-byte. The reference defines the codec
+ * field and only the "raw" codec (python/ayaka/ops/kvcache.py:35-36, :54-55).
  */
 #ifndef AYAKA_HIP_BLOCK_SCALED_H
 #define AYAKA_HIP_BLOCK_SCALED_H

@@ -33,8 +33,9 @@ extern "C" {
  *
  * A request is not served if it asks for what cannot be: negative rows, more rows than tokens, more
  * blocks than max_blocks, a row past n_rows; if the last entry it should hold is the padding block 0
- * (a step before this one did not serve it, and its length was raised all the same); or if the free blocks run out at it (from there on, in
- * request order, only requests that need no block are served). Nothing of its table row is written,
+ * (a step before this one did not serve it, and its length was raised all the same); or if the free
+ * blocks run out at it (from there on, in request order, only requests that need no block are
+ * served). Nothing of its table row is written,
  * its rows get position 0 and slot 0 (which the KV write drops or keeps to the padding block), and
  * it counts into after[1] unless its length is 0 (padding: not an error). Rows behind the last
  * request's get request 0, position 0, slot 0. A negative rows[b] numbers no rows.
