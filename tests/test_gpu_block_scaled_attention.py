@@ -446,6 +446,42 @@ def test_repeated_calls_follow_scales_that_moved(ops) -> None:
     step.check(out)
 
 
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+def test_a_pool_just_under_the_largest(ops, layout) -> None:
+    # blocks whose byte offsets pass 2^31, up to the pool's last, beside its first: the write, the moves and
+    # every kind of step give bit for bit what they give over a small pool
+    block, kv_heads, dim = 16, 8, 128
+    blocks = 2 ** 32 // (block * kv_heads * dim) - 1
+    shape = (blocks, block, kv_heads, dim) if layout == "nhd" else (blocks, kv_heads, block, dim)
+    big = KVBuffers(*(torch.empty(shape, dtype=torch.float8_e4m3fn, device=DEV) for _ in range(2)), LAYOUTS[layout],
+                    fp8_e4m3_block_codec(torch.zeros(blocks, kv_heads, 2, device=DEV)))
+    codes = lambda t: t.view(torch.uint8)
+    for mode, steps in (("decode", [(1, 700), (1, 33)]), ("mixed", [(3, 500), (2, 40)]), ("mixed", [(50, 300), (70, 90)])):
+        step = Step(steps, layout=layout, heads=16, kv_heads=kv_heads, head_dim=dim, block=block, mode=mode, seed=8)
+        q, small, meta, out = step.device(ops)
+        n = small.k.shape[0]
+        ids = torch.arange(n, device=DEV)
+        ids[n // 2:] += blocks - n  # the upper half at the pool's end
+        assert int(ids[-1]) == blocks - 1
+        for a, b in ((big.k, small.k), (big.v, small.v)):
+            codes(a)[ids] = codes(b)
+        big.codec.scales[ids] = small.codec.scales
+        table = ids[torch.from_numpy(step.table).to(DEV)]
+        far = ops.attention.plan(step.mode, torch.tensor(step.rows, device=DEV), torch.tensor(step.lengths, device=DEV),
+                                 table, block)
+        rows = [torch.randn(len(q), kv_heads, dim, device=DEV).to(q.dtype) for _ in range(2)]
+        again = torch.full_like(out, float("nan"))
+        for buffers, metadata, to in ((small, meta, out), (big, far, again)):
+            ops.kvcache.store(*rows, buffers, metadata)
+            ops.attention.attend(q, buffers, metadata, to, scale=step.scale)
+        assert torch.equal(out, again)
+        got = [torch.empty_like(small.k), torch.empty_like(small.v)]
+        scales = torch.empty_like(small.codec.scales)
+        ops.kvcache.gather(big, ids, *got, out_scales=scales)
+        assert torch.equal(codes(got[0]), codes(small.k)) and torch.equal(codes(got[1]), codes(small.v))
+        assert torch.equal(scales.nan_to_num(-1.0), small.codec.scales.nan_to_num(-1.0))
+
+
 def test_another_stream(ops) -> None:
     step = Step([(1, 900), (1, 2000), (1, 50)], heads=8, head_dim=128, mode="decode")
     q, buffers, meta, out = step.device(ops)
