@@ -146,7 +146,7 @@ int prepare(const char* op, const AttnCall& c, ayk::AttnParams& p, int& heads_pe
     p.token_stride = D;
     p.head_stride = B * D;
   }
-  if ((uint64_t)c.num_blocks * (uint64_t)p.block_stride > UINT32_MAX)
+  if ((uint64_t)c.num_blocks > UINT32_MAX / (uint64_t)p.block_stride)  // (their product could wrap)
     return fail(AYK_ERR_UNSUPPORTED, "%s: a cache of %d blocks of %lld elements exceeds 32-bit element offsets",
                 op, c.num_blocks, (long long)p.block_stride);
   if (p.token_stride >= (1 << 24))
@@ -700,7 +700,7 @@ int ayk_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_
   if (layout != AYK_LAYOUT_NHD && layout != AYK_LAYOUT_HND)
     return fail(AYK_ERR_UNSUPPORTED, "%s: layout %d is not NHD (0) or HND (1)", op, layout);
   // the kernel's slots are 31-bit; the attention entry points hold a pool to 2^32 elements
-  if ((uint64_t)num_blocks * (uint64_t)block_size * (uint64_t)num_kv_heads * (uint64_t)head_dim > UINT32_MAX)
+  if ((uint64_t)num_blocks * (uint64_t)block_size > UINT32_MAX / ((uint64_t)num_kv_heads * (uint64_t)head_dim))
     return fail(AYK_ERR_UNSUPPORTED, "%s: a cache of %d blocks of %d positions exceeds 32-bit element offsets", op,
                 num_blocks, block_size);
   if (n_rows > INT32_MAX || num_kv_heads > 32767)

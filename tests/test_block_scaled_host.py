@@ -166,6 +166,7 @@ def _store(**kw: object) -> int:
     ({"dtype": 3}, 2, b"src_dtype 3"),
     ({"layout": 2}, 2, b"layout 2"),
     ({"num_blocks": 1 << 21, "block_size": 16}, 2, b"32-bit element offsets"),
+    ({"num_blocks": 1 << 30, "block_size": 1 << 16, "kv_heads": 1 << 12, "head_dim": 256}, 2, b"32-bit element offsets"),
     ({"n_rows": 1 << 32}, 2, b"exceed one launch"),
     ({"scales": None}, 1, b"null"),
     ({"k": 24}, 1, b"not 16-byte aligned"),
@@ -198,6 +199,8 @@ def _v1(**kw: object) -> int:
     ({"dtype": 3}, 2, b"under fp16/bf16"),
     ({"flags": 1}, 2, b"16-bit caches only"),
     ({"head_dim": 96}, 2, b"head_dim 96"),
+    ({"num_blocks": 1 << 30, "block_size": 1 << 16, "heads": 1 << 12, "kv_heads": 1 << 12, "head_dim": 256}, 2,
+     b"32-bit element offsets"),
     ({"heads": 7}, 1, b"not a positive multiple"),
     ({"q": None}, 1, b"null"),
     ({"q": 8}, 1, b"not 16-byte aligned"),
