@@ -157,11 +157,24 @@ __device__ __forceinline__ typename KvRaw<KV8>::T load_kv_raw(const uint16_t* ba
 //   out = sum_t 2^(score_t - M) 2^e_t code_t / sum_t 2^(score_t - M)
 //       = sum_t u_t code_t / sum_t u_t 2^-e_t,     u_t = 2^(score_t + e_t - m).
 // So a kernel keeps its running maximum m over score_t + e_t (one fma makes it), its weights u_t
-// stay at most 2^kRescaleSlack whatever the scales -- an fp16 P loses nothing -- and only the weight sum
-// multiplies by 2^-e_t. m and the sum describe each other as before, so merges do not change.
-// The sum cannot underflow: scales span 2^120, so a position that carries the sum has a weight of
-// 2^-120 at least.
+// stay at most 2^kRescaleSlack whatever the scales, and only the weight sum multiplies by 2^-e_t.
 //
+// The sum's terms are 2^(score_t - m), between 2^-80 and 2^40 of the largest weight's, and u_t may be
+// 2^-120 for a position that carries the sum and less for many that carry it together, where
+// v_exp_f32 gives zeros below 2^-126. While no value scale above 2^kLoudShift has been met, scales
+// span 2^80 and a term is lost only 46 bits below the largest: even 2^26 of them change the sum by
+// 2^-20. From the first louder block on a kernel takes the terms from exponentials of their own,
+// 2^(v_t - m - e_t) (v_t the shifted score). Where m moves on, by up to 120 bits more than the
+// scores did, sums are scaled in two steps (times_exp2), in partitions and merges alike.
+//
+constexpr float kLoudShift = 40.f;
+
+// x * 2^d for d <= 0, where 2^d alone may be below the smallest normal number.
+__device__ __forceinline__ float times_exp2(float x, float d) {
+  const float half = fast_exp2(0.5f * d);
+  return x * half * half;
+}
+
 // Per position the kernels stage {2^k scale, e, 2^-e}.
 struct PositionScale {
   float key;    // what a raw q.k is multiplied by
@@ -401,7 +414,8 @@ __device__ __forceinline__ void store_head_t(const AttnParams& p, int row, int p
 // Thread t owns items t, t + threads, ... (an item = one head's 4 elements), at
 // most IPT of them, and loads partition i of all its items before folding them,
 // two partitions at a time, so the loads of one thread overlap.
-template <int D, int IPT, bool BF16>
+// BS: partitions of a block-scaled cache, whose sums may lie far apart (see PositionScale).
+template <int D, int IPT, bool BF16, bool BS = false>
 __device__ __forceinline__ void merge_partitions(const AttnParams& p, int row, int np, int head_lo, int head_hi,
                                                  int tid, int threads) {
   using E = Elem<BF16>;
@@ -425,7 +439,8 @@ __device__ __forceinline__ void merge_partitions(const AttnParams& p, int row, i
     const float mn = fmaxf(m[k], mi);
     const float a = fast_exp2(m[k] - mn);
     const float b = wi * fast_exp2(mi - mn);
-    l[k] = l[k] * a + b;
+    if constexpr (BS) l[k] = times_exp2(l[k], m[k] - mn) + times_exp2(wi, mi - mn);
+    else l[k] = l[k] * a + b;
     acc[k] = acc[k] * a + v * b;
     m[k] = mn;
   };
@@ -477,7 +492,7 @@ __device__ __forceinline__ void merge_partitions(const AttnParams& p, int row, i
 // workgroup's acquire fence follows the add that read every other one. One
 // release (an L2 write-back) per workgroup and one acquire (an L2 invalidate)
 // per merge: per-thread device fences would cost far more than the merge saves.
-template <int D, int GC, bool BF16>
+template <int D, int GC, bool BF16, bool BS = false>
 __device__ __forceinline__ void arrive_and_merge(const AttnParams& p, int row, int group, int groups, int np,
                                                  int head_lo, int head_hi, int tid, int threads, int* s_flag) {
   __syncthreads();
@@ -495,7 +510,7 @@ __device__ __forceinline__ void arrive_and_merge(const AttnParams& p, int row, i
   __syncthreads();
   if (!*s_flag) return;
   // A workgroup holds at most GC heads per wave, so GC * D / 4 items per 64 threads.
-  merge_partitions<D, (GC * D / 4 + kWave - 1) / kWave, BF16>(p, row, np, head_lo, head_hi, tid, threads);
+  merge_partitions<D, (GC * D / 4 + kWave - 1) / kWave, BF16, BS>(p, row, np, head_lo, head_hi, tid, threads);
 }
 
 // Zero the output rows of GC heads of a padding row (v1): nothing of the cache is read.

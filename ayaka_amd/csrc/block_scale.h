@@ -6,8 +6,9 @@
 // Powers of two, because e4m3 is a floating format: its relative precision does not depend on
 // the scale, so a finer scale would gain nothing, while a block whose scale grows by 2^k
 // re-encodes its tokens by lowering their exponents: exact for every code that stays normal.
-// The range of e keeps every ratio of two scales (2^120) inside fp32, which the attention
-// kernels' sums rely on: weights in units of the largest scale never underflow a whole sum.
+// The range of e keeps every ratio of two scales (2^120), and every sum of weights in units of one,
+// inside fp32; what a weight in units of the largest scale loses, the attention kernels' sums take
+// from exponentials of their own (PositionScale).
 #pragma once
 
 #include <hip/hip_runtime.h>

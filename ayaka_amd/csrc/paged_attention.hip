@@ -305,7 +305,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_kernel(cons
 constexpr int kReduceThreads = 256;
 
 // F32: an fp32 model's merge, its output written in fp32 (BF16 then unused).
-template <int D, bool BF16, int S, bool F32 = false>
+// BS: partitions of a block-scaled cache, whose sums may lie far apart (see PositionScale).
+template <int D, bool BF16, int S, bool F32 = false, bool BS = false>
 __global__ __launch_bounds__(kReduceThreads) void partition_reduce_kernel(const AttnParams p) {
   using E = Elem<BF16>;
   constexpr int QUADS = D / 4;                // float4 groups of a row
@@ -343,7 +344,8 @@ __global__ __launch_bounds__(kReduceThreads) void partition_reduce_kernel(const 
     const float mn = real ? fmaxf(m, mi) : m;
     const float a = fast_exp2(m - mn);
     const float b = real ? wi * fast_exp2(mi - mn) : 0.f;
-    l = l * a + b;
+    if constexpr (BS) l = times_exp2(l, m - mn) + (real ? times_exp2(wi, mi - mn) : 0.f);
+    else l = l * a + b;
     acc = acc * a + v * b;
     m = mn;
   };
@@ -392,7 +394,8 @@ __global__ __launch_bounds__(kReduceThreads) void partition_reduce_kernel(const 
 #pragma unroll
     for (int k = 0; k < S; ++k) {
       const float w = fast_exp2(s_m[hl][k] - mn);
-      L += s_l[hl][k] * w;
+      if constexpr (BS) L += times_exp2(s_l[hl][k], s_m[hl][k] - mn);
+      else L += s_l[hl][k] * w;
       total += s_acc[hl][k][quad] * w;
     }
   }
@@ -460,7 +463,7 @@ hipError_t launch_attention_dpp(const AttnParams& p, int head_dim, int gc, bool 
 // of many rows launches one workgroup per row rather than per (row, head). Rows
 // with one partition were written by the partition kernel and rows of padding
 // requests were zeroed by it; both return at once.
-template <int D, bool BF16>
+template <int D, bool BF16, bool BS>
 __global__ __launch_bounds__(kReduceThreads) void row_reduce_kernel(const AttnParams p) {
   constexpr int IPT = 4;
   constexpr int HEADS_PER_PASS = kReduceThreads * IPT / (D / 4);
@@ -470,31 +473,33 @@ __global__ __launch_bounds__(kReduceThreads) void row_reduce_kernel(const AttnPa
   const int np = len > 0 ? (len - 1) / p.partition_size + 1 : 0;
   if (np <= 1) return;
   for (int h0 = 0; h0 < p.num_heads; h0 += HEADS_PER_PASS)
-    merge_partitions<D, IPT, BF16>(p, row, np, h0, min(p.num_heads, h0 + HEADS_PER_PASS), threadIdx.x,
+    merge_partitions<D, IPT, BF16, BS>(p, row, np, h0, min(p.num_heads, h0 + HEADS_PER_PASS), threadIdx.x,
                                    kReduceThreads);
 }
 
-hipError_t launch_row_reduce(const AttnParams& p, int head_dim, bool bf16, hipStream_t stream) {
+template <int D>
+static void launch_row_reduce_d(const AttnParams& p, bool bf16, hipStream_t stream) {
   const dim3 grid((unsigned)p.n_rows), block(kReduceThreads);
+  if (p.block_scales) {
+    if (bf16) hipLaunchKernelGGL((row_reduce_kernel<D, true, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((row_reduce_kernel<D, false, true>), grid, block, 0, stream, p);
+  } else {
+    if (bf16) hipLaunchKernelGGL((row_reduce_kernel<D, true, false>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((row_reduce_kernel<D, false, false>), grid, block, 0, stream, p);
+  }
+}
+
+hipError_t launch_row_reduce(const AttnParams& p, int head_dim, bool bf16, hipStream_t stream) {
   switch (head_dim) {
-    case 64:
-      if (bf16) hipLaunchKernelGGL((row_reduce_kernel<64, true>), grid, block, 0, stream, p);
-      else hipLaunchKernelGGL((row_reduce_kernel<64, false>), grid, block, 0, stream, p);
-      break;
-    case 128:
-      if (bf16) hipLaunchKernelGGL((row_reduce_kernel<128, true>), grid, block, 0, stream, p);
-      else hipLaunchKernelGGL((row_reduce_kernel<128, false>), grid, block, 0, stream, p);
-      break;
-    case 256:
-      if (bf16) hipLaunchKernelGGL((row_reduce_kernel<256, true>), grid, block, 0, stream, p);
-      else hipLaunchKernelGGL((row_reduce_kernel<256, false>), grid, block, 0, stream, p);
-      break;
+    case 64: launch_row_reduce_d<64>(p, bf16, stream); break;
+    case 128: launch_row_reduce_d<128>(p, bf16, stream); break;
+    case 256: launch_row_reduce_d<256>(p, bf16, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
 
-template <int D, bool BF16, bool F32 = false>
+template <int D, bool BF16, bool F32 = false, bool BS = false>
 static hipError_t launch_reduce_typed(const AttnParams& p, int compute_units, hipStream_t stream) {
   // Partition slots per (row, head): one for up to 4 partitions per row, and up to 16 when
   // one slot still gives every compute unit a workgroup (many pairs, most of whose rows often
@@ -514,10 +519,10 @@ static hipError_t launch_reduce_typed(const AttnParams& p, int compute_units, hi
   const int s = one_slot ? 1 : (p.max_partitions <= 16 || groups4 >= compute_units) ? S4 : S_MAX;
   const dim3 block(kReduceThreads);
   auto grid = [&](int heads) { return dim3((unsigned)((pairs + heads - 1) / heads)); };
-  if (s == 1) hipLaunchKernelGGL((partition_reduce_kernel<D, BF16, 1, F32>), grid(S_MAX), block, 0, stream, p);
+  if (s == 1) hipLaunchKernelGGL((partition_reduce_kernel<D, BF16, 1, F32, BS>), grid(S_MAX), block, 0, stream, p);
   else if (s == S4)
-    hipLaunchKernelGGL((partition_reduce_kernel<D, BF16, S4, F32>), grid(S_MAX / S4), block, 0, stream, p);
-  else hipLaunchKernelGGL((partition_reduce_kernel<D, BF16, S_MAX, F32>), grid(1), block, 0, stream, p);
+    hipLaunchKernelGGL((partition_reduce_kernel<D, BF16, S4, F32, BS>), grid(S_MAX / S4), block, 0, stream, p);
+  else hipLaunchKernelGGL((partition_reduce_kernel<D, BF16, S_MAX, F32, BS>), grid(1), block, 0, stream, p);
   return hipGetLastError();
 }
 
@@ -530,15 +535,20 @@ hipError_t launch_partition_reduce_f32(const AttnParams& p, int head_dim, int co
   }
 }
 
+template <int D>
+static hipError_t launch_reduce_d(const AttnParams& p, bool bf16, int cu, hipStream_t stream) {
+  if (p.block_scales)
+    return bf16 ? launch_reduce_typed<D, true, false, true>(p, cu, stream)
+                : launch_reduce_typed<D, false, false, true>(p, cu, stream);
+  return bf16 ? launch_reduce_typed<D, true>(p, cu, stream) : launch_reduce_typed<D, false>(p, cu, stream);
+}
+
 hipError_t launch_partition_reduce(const AttnParams& p, int head_dim, bool bf16, int compute_units,
                                    hipStream_t stream) {
-  const int cu = compute_units;
   switch (head_dim) {
-    case 64: return bf16 ? launch_reduce_typed<64, true>(p, cu, stream) : launch_reduce_typed<64, false>(p, cu, stream);
-    case 128:
-      return bf16 ? launch_reduce_typed<128, true>(p, cu, stream) : launch_reduce_typed<128, false>(p, cu, stream);
-    case 256:
-      return bf16 ? launch_reduce_typed<256, true>(p, cu, stream) : launch_reduce_typed<256, false>(p, cu, stream);
+    case 64: return launch_reduce_d<64>(p, bf16, compute_units, stream);
+    case 128: return launch_reduce_d<128>(p, bf16, compute_units, stream);
+    case 256: return launch_reduce_d<256>(p, bf16, compute_units, stream);
     default: return hipErrorInvalidValue;
   }
 }

@@ -217,6 +217,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
   const uint16_t* vbase = kv_at<KV8>(p.v_cache, (int64_t)kvh * p.head_stride + c * 8);
 
   [[maybe_unused]] bool nan_taken = false;  // BS windows: NaN values of chunks that some rows do not see
+  [[maybe_unused]] bool loud = false;       // BS: a value scale above 2^kLoudShift has been met (uniform)
   for (int s0 = t_begin; s0 < t_end; s0 += seg_len) {
     const int s1 = min(t_end, s0 + seg_len);
     const int b0 = (!WIN && s0 == t_begin) ? commit_table<2, BS>(p, tbl, s_tbl, ahead, s1, tid, threads, s_ids)
@@ -261,6 +262,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
       const bool apart = BS && WIN && tc + CH - 1 > win_least;
       if constexpr (BS) {
         const PositionScale ps = position_scale(sc, scale_log2);
+        loud |= __builtin_amdgcn_ballot_w64(ps.shift > kLoudShift) != 0;
         if (lane < CH) {
           s_sc[wave][0][lane] = ps.key;
           s_sc[wave][1][lane] = ps.shift;
@@ -303,7 +305,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
       if (__builtin_amdgcn_ballot_w64(mx > m_h + kRescaleSlack)) {
         const float mn = fmaxf(m_h, column_max(mx));
         const float alpha = fast_exp2(m_h - mn);  // head mt's, and o[] holds head mt
-        l_h *= alpha;
+        if constexpr (BS) l_h = times_exp2(l_h, m_h - mn);
+        else l_h *= alpha;
         m_h = mn;
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[t] *= alpha;
@@ -317,9 +320,15 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
           if constexpr (!BS) l_h += w[i];
         }
         if constexpr (BS) {
-          const f32x4 unit = *reinterpret_cast<const f32x4*>(&s_sc[wave][2][sub * MT + 4 * mq]);
+          if (loud) {
+            const f32x4 shift = *reinterpret_cast<const f32x4*>(&s_sc[wave][1][sub * MT + 4 * mq]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) l_h = __builtin_fmaf(w[i], unit[i], l_h);
+            for (int i = 0; i < 4; ++i) l_h += fast_exp2(acc[sub][i] - m_h - shift[i]);
+          } else {
+            const f32x4 unit = *reinterpret_cast<const f32x4*>(&s_sc[wave][2][sub * MT + 4 * mq]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l_h = __builtin_fmaf(w[i], unit[i], l_h);
+          }
         }
         // O^T += V^T P^T: P^T is the lane's own weights (tokens 4*mq + i of head mt, the
         // B operand layout); V^T comes transposed from the token-major tile (lane mt of
@@ -457,7 +466,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
         const float mj = s_slice_m[src][mt], lj = s_slice_l[src][mt];
         const float mn = fmaxf(m_h, mj);
         const float a = fast_exp2(m_h - mn), b = fast_exp2(mj - mn);
-        l_h = l_h * a + lj * b;
+        if constexpr (BS) l_h = times_exp2(l_h, m_h - mn) + times_exp2(lj, mj - mn);
+        else l_h = l_h * a + lj * b;
         m_h = mn;
         const u32x4* vs = reinterpret_cast<const u32x4*>(&s_v[src][0]);
 #pragma unroll
@@ -483,7 +493,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void paged_attention_mfma_kernel
     if (np > 1 && p.arrivals) {
       const int vh_lo = wg.group * heads_per_wg;
       const int vh_hi = min(p.num_virtual_heads, vh_lo + heads_per_wg);
-      arrive_and_merge<D, GC, BF16>(p, row, wg.group, groups, np, vh_lo * GC, vh_hi * GC, tid, threads, &s_last);
+      arrive_and_merge<D, GC, BF16, BS>(p, row, wg.group, groups, np, vh_lo * GC, vh_hi * GC, tid, threads, &s_last);
     }
   }
 }

@@ -160,6 +160,7 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   __shared__ int s_vbad[2][W];  // V16_FAST: per buffer, each wave's vote (a value that does not convert)
   __shared__ f32x2 s_sc[BS ? kTableCap : 1];  // the segment's blocks' scales, beside s_tbl
   __shared__ int s_nan;                       // BS: a NaN value was taken out of a staged chunk
+  __shared__ int s_loud;                      // BS: a value scale above 2^kLoudShift has been staged
   auto& s_k = lds.st.k;
   auto& s_v = lds.st.v;
 
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   // leaving the loop early costs the common case registers)
   bool stop = false;
   if constexpr (BS) {
-    if (tid == 0) s_nan = 0;  // (staging a table begins with a barrier)
+    if (tid == 0) s_nan = s_loud = 0;  // (staging a table begins with a barrier)
   }
   for (int s0 = t_begin; s0 < t_end; s0 += seg_len) {
     const int s1 = min(t_end, s0 + seg_len);
@@ -389,6 +390,7 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
         ts.v[w] = SCALES == 16 ? scale_at(t) : SCALES == 4 ? scale_at(t + 4 * mq) : f32x2{1.f, 0.f};
       }
     };
+    [[maybe_unused]] bool loud = false;  // BS: s_loud, once the segment's scales are staged
     auto fold = [&](int ci, int vb, Scores& acc, [[maybe_unused]] const TileScales& ts, auto&& mid) {
       const int buf = vb;
       const int tb = s0 + ci * CH;
@@ -442,13 +444,32 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
         if (__builtin_amdgcn_ballot_w64(mx > m[j] + kRescaleSlack)) {
           const float mn = fmaxf(m[j], column_max(mx));
           const float alpha = fast_exp2(m[j] - mn);
-          l[j] *= alpha;
+          if constexpr (BS) l[j] = times_exp2(l[j], m[j] - mn);
+          else l[j] *= alpha;
           if constexpr (LSUM_MFMA) lo1[j] *= alpha;
 #pragma unroll
           for (int t = 0; t < DT; ++t) o[j][t] *= alpha;
           m[j] = mn;
         }
       }
+      // BS, behind a loud block: the sum's terms from exponentials of their own, and none (0 of each
+      // weight) from the weights below
+      if constexpr (BS) {
+        if (loud) {
+#pragma unroll
+          for (int w = 0; w < PTL_W; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float shift = QUADS ? ts.v[w].y : scale_at(tb + (ps * PTL_W + w) * 16 + 4 * mq + i).y;
+#pragma unroll
+              for (int j = 0; j < PT; ++j) {
+                const float scaled = whole ? __builtin_fmaf(acc[w][j][i], ts.v[w].x, ts.v[w].y) : acc[w][j][i];
+                l[j] += fast_exp2(scaled - m[j] - shift);
+              }
+            }
+        }
+      }
+      [[maybe_unused]] const float sum_from = loud ? -INFINITY : 0.f;
       mid();
       // Weights after every group's max and rescale: from here to the end of the chunk
       // the code has no branch, so the scheduler can overlap one group's exponentials
@@ -471,14 +492,14 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
 #pragma unroll
         for (int w = 0; w < PTL_W; ++w) {
           if constexpr (QUADS) {
-            const float unit = fast_exp2(-ts.v[w].y);
+            const float unit = fast_exp2(sum_from - ts.v[w].y);
 #pragma unroll
             for (int j = 0; j < PT; ++j)
               l[j] = __builtin_fmaf((acc[w][j][0] + acc[w][j][1]) + (acc[w][j][2] + acc[w][j][3]), unit, l[j]);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float unit = fast_exp2(-scale_at(tb + (ps * PTL_W + w) * 16 + 4 * mq + i).y);
+              const float unit = fast_exp2(sum_from - scale_at(tb + (ps * PTL_W + w) * 16 + 4 * mq + i).y);
 #pragma unroll
               for (int j = 0; j < PT; ++j) l[j] = __builtin_fmaf(acc[w][j][i], unit, l[j]);
             }
@@ -552,10 +573,14 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
       for (int k = 0; k < SEG_LOADS; ++k) {
         const int i = tid + k * THREADS;
         const PositionScale sc = position_scale(seg_scale[k], scale_log2);
-        if (i < seg_blocks) s_sc[i] = f32x2{sc.key, sc.shift};
+        if (i < seg_blocks) {
+          s_sc[i] = f32x2{sc.key, sc.shift};
+          if (sc.shift > kLoudShift) s_loud = 1;
+        }
       }
     }
     lds_barrier();
+    if constexpr (BS) loud = __builtin_amdgcn_readfirstlane(s_loud) != 0;
     // Two chunks per iteration, so that each body's LDS buffer is a constant (immediate
     // address offsets instead of per-access arithmetic).
     // V16_FAST: whether a chunk's values all converted (every wave's vote, uniform)
@@ -648,14 +673,16 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
 #pragma unroll
       for (int w = 1; w < PS; ++w) mn = fmaxf(mn, s_ml[pg * (PS - 1) + w - 1][j][0][mt]);
       const float a0 = fast_exp2(m[j] - mn);
-      lsum[j] *= a0;
+      if constexpr (BS) lsum[j] = times_exp2(lsum[j], m[j] - mn);
+      else lsum[j] *= a0;
 #pragma unroll
       for (int t = 0; t < DT; ++t) o[j][t] *= a0;
 #pragma unroll
       for (int w = 1; w < PS; ++w) {
         const int slot = pg * (PS - 1) + w - 1;
         const float a = fast_exp2(s_ml[slot][j][0][mt] - mn);
-        lsum[j] += s_ml[slot][j][1][mt] * a;
+        if constexpr (BS) lsum[j] += times_exp2(s_ml[slot][j][1][mt], s_ml[slot][j][0][mt] - mn);
+        else lsum[j] += s_ml[slot][j][1][mt] * a;
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[j][t] += lds.o[slot][j][t][lane] * a;
       }
