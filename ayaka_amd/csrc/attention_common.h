@@ -182,9 +182,11 @@ struct PositionScale {
   float unit;   // 2^-e
 };
 
+// Scales count as the write counts them (canonical_scale): a key block without one scores 0; a value
+// block without one has codes of zero and takes the least e.
 __device__ __forceinline__ PositionScale position_scale(f32x2 s, float scale_log2) {
-  const int e = scale_exponent(s.y);
-  return PositionScale{scale_log2 * power_of_two(scale_exponent(s.x)), (float)e, power_of_two(-e)};
+  const int e = scale_exponent(canonical_scale(s.y));
+  return PositionScale{scale_log2 * canonical_scale(s.x), (float)e, power_of_two(-e)};
 }
 
 // The key and value scale of block `id` and key/value head `kvh`.

@@ -9,7 +9,9 @@
  * `scales`, float32 [num_blocks, num_kv_heads, 2], contiguous, 8-byte aligned: a key scale and a
  * value scale for every block and key/value head. An element is worth code * scale. A scale is a
  * power of two 2^e, -40 <= e <= 80, or 0 for a block of nothing but zeros; a fresh cache's scales
- * are zeros. Head widths are 64, 128 and 256; caches are written from and read by fp16 and bf16
+ * are zeros. Both the write and attention read a scale that is not one of these as the nearest below
+ * it: 2^-40 or 2^80 beyond the range, and 0 for anything not above 0. A block's value scale of 0 says
+ * that its codes are zeros: attention takes whatever they are as at most 448 * 2^-40. Head widths are 64, 128 and 256; caches are written from and read by fp16 and bf16
  * models. Rows (k, v, q, out) are 16-byte aligned, caches 8-byte. The reference defines the codec
  * field and only the "raw" codec (python/ayaka/ops/kvcache.py:35-36, :54-55).
  */

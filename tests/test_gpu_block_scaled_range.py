@@ -133,3 +133,44 @@ def test_many_table_segments(ops) -> None:
             run(ops, step, label=at)
             run(ops, step, label=at, **(dict(partitions=0) if rows == 1 else
                                         dict(prefill=True, window=rows == 3, partitions=0)))
+
+
+# --- scales that the write does not make ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("mode,rows", [("decode", 1), ("mixed", 3), ("mixed", 40)])
+def test_a_scale_that_is_not_above_zero_counts_as_zero(ops, mode, rows) -> None:
+    # as the write counts it: keys of such a block score 0 whatever their codes, values are codes of zero
+    for block in (16, 12, 7):
+        step = Step([(rows, 300)], heads=8, head_dim=128, block=block, mode=mode, seed=5)
+        ids = step.table[0, 1:4]
+        step.codes[1][ids] = 0
+        step.scales[ids, :, 0] = 0.0
+        # (a value scale of 0 is read as 2^-40: the oracle's tolerance divides by it)
+        step.scales[ids, :, 1] = 2.0 ** -40
+        q, buffers, meta, out = step.device(ops)
+        outs = []
+        for key, value in ((0.0, 2.0 ** -40), (0.0, 0.0), (-4.0, -2.0 ** 30), (-0.0, -0.0), (-np.inf, -np.nan)):
+            buffers.codec.scales[torch.from_numpy(ids).to(buffers.k.device)] = torch.tensor(
+                np.array([key, value], np.float32), device=buffers.k.device)
+            out.fill_(float("nan"))
+            ops.attention.attend(q, buffers, meta, out, scale=step.scale)
+            step.check(out, f"scales {key} and {value}")
+            outs.append(out.clone())
+        assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_scales_between_and_beyond_the_powers_count_as_the_one_below(ops) -> None:
+    step = Step([(1, 100)], heads=4, head_dim=64, mode="decode", seed=6)
+    q, buffers, meta, out = step.device(ops)
+    ids = torch.from_numpy(step.table[0, :7]).to(buffers.k.device)
+    outs = []
+    for pair in ((0.25, 2.0 ** -40), (0.3, 2.0 ** -45), (0.49999, 1e-38)):
+        buffers.codec.scales[ids] = torch.tensor(pair, device=buffers.k.device)
+        ops.attention.attend(q, buffers, meta, out, scale=step.scale)
+        outs.append(out.clone())
+    for pair in ((0.25, 2.0 ** 80), (0.25, 2.0 ** 90), (0.25, float("inf")), (0.25, float("nan"))):
+        buffers.codec.scales[ids] = torch.tensor(pair, device=buffers.k.device)
+        ops.attention.attend(q, buffers, meta, out, scale=step.scale)
+        outs.append(out.clone())
+    assert all(torch.equal(o, outs[0]) for o in outs[1:3]) and all(torch.equal(o, outs[3]) for o in outs[4:])
