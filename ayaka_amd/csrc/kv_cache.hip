@@ -260,7 +260,11 @@ hipError_t launch_block_op(int mode, const void* src_k, const void* src_v, void*
                            const void* src_ids, const void* dst_ids, bool ids64, int64_t n,
                            int32_t num_blocks, int64_t block_bytes, hipStream_t stream) {
   if (n == 0 || block_bytes == 0) return hipSuccess;
-  const int vec = (block_bytes % 16 == 0) ? 16 : (block_bytes % 4 == 0) ? 4 : 2;
+  // vectors that the block's size and every address are a multiple of: a cache, an output or a
+  // block-scaled cache's scales may begin anywhere their elements may
+  const uint64_t low = (uint64_t)block_bytes | reinterpret_cast<uintptr_t>(src_k) | reinterpret_cast<uintptr_t>(src_v) |
+                       reinterpret_cast<uintptr_t>(dst_k) | reinterpret_cast<uintptr_t>(dst_v);
+  const int vec = (low % 16 == 0) ? 16 : (low % 4 == 0) ? 4 : (low % 2 == 0) ? 2 : 1;
   const int64_t nvec = block_bytes / vec;
   const unsigned gy = (unsigned)std::min<int64_t>((nvec + 255) / 256, 64);
   const dim3 grid((unsigned)n, gy), block(256);
@@ -277,8 +281,12 @@ hipError_t launch_block_op(int mode, const void* src_k, const void* src_v, void*
       hipLaunchKernelGGL(block_op_kernel<4>, grid, block, 0, stream, mode, sk, sv, dk, dv, src_ids,
                          dst_ids, (int32_t)ids64, num_blocks, block_bytes);
       break;
-    default:
+    case 2:
       hipLaunchKernelGGL(block_op_kernel<2>, grid, block, 0, stream, mode, sk, sv, dk, dv, src_ids,
+                         dst_ids, (int32_t)ids64, num_blocks, block_bytes);
+      break;
+    default:
+      hipLaunchKernelGGL(block_op_kernel<1>, grid, block, 0, stream, mode, sk, sv, dk, dv, src_ids,
                          dst_ids, (int32_t)ids64, num_blocks, block_bytes);
       break;
   }
