@@ -630,7 +630,7 @@ AttnCall block_scaled_call(void* out, const void* q, const void* k_cache, const 
 
 extern "C" {
 
-int ayk_abi_version(void) { return 18; }
+int ayk_abi_version(void) { return 19; }
 
 int ayk_paged_prefill_tile_pairs(int32_t head_dim) { return ayk::prefill_tile_pairs_for(head_dim); }
 

@@ -17,7 +17,7 @@ from ayaka_amd.errors import BackendError, CapabilityError
 __all__ = ["ABI_VERSION", "BLOCK_SCALED_EXPORTS", "EXPORTS", "LIB_PATH", "TABLES_EXPORTS", "check", "lib"]
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libayaka_hip.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -143,17 +143,23 @@ def lib() -> ctypes.CDLL:
                 raise CapabilityError(
                     "ops.hip", detail=f"{LIB_PATH} does not load: {exc}", remedy="rebuild it"
                 ) from exc
-            for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS, **TABLES_EXPORTS}.items():
-                fn = getattr(handle, name)
-                fn.restype = restype
-                fn.argtypes = argtypes
-            version = handle.ayk_abi_version()
-            if version != ABI_VERSION:
+            # the version first: a library of another one may lack exports of this one
+            try:
+                version = handle.ayk_abi_version()
+                if version != ABI_VERSION:
+                    raise CapabilityError(
+                        "ops.hip",
+                        detail=f"{LIB_PATH} has ABI {version}, this package expects {ABI_VERSION}",
+                        remedy="rebuild it",
+                    )
+                for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS, **TABLES_EXPORTS}.items():
+                    fn = getattr(handle, name)
+                    fn.restype = restype
+                    fn.argtypes = argtypes
+            except AttributeError as exc:
                 raise CapabilityError(
-                    "ops.hip",
-                    detail=f"{LIB_PATH} has ABI {version}, this package expects {ABI_VERSION}",
-                    remedy="rebuild it",
-                )
+                    "ops.hip", detail=f"{LIB_PATH} lacks an export: {exc}", remedy="rebuild it"
+                ) from exc
             _lib = handle
     return _lib
 
