@@ -178,7 +178,7 @@ def require_buffers(op: str, buffers: KVBuffers) -> None:
     if buffers.codec not in _CODEC_DTYPES:
         raise BackendError(
             f"{op}: the hip backend stores the {RAW_CODEC!r} and {FP8_E4M3_CODEC!r} codecs, "
-            f"not {buffers.codec!r}",
+            f"not {str(buffers.codec)!r} (and {FP8_E4M3_BLOCK_CODEC!r}, made with fp8_e4m3_block_codec)",
             context={"op": op, "argument": "buffers"},
         )
     k = buffers.k

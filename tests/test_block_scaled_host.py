@@ -274,3 +274,8 @@ def test_a_default_stream_of_another_device_is_refused(monkeypatch: pytest.Monke
         _checks.stream_handle(torch.device("cuda", 1))
     monkeypatch.setattr(_checks, "_raw_stream", lambda index: 77)  # a stream of its own names its device
     assert _checks.stream_handle(torch.device("cuda", 1)) == 77
+
+
+def test_the_refusal_of_other_codecs_names_this_one() -> None:
+    with pytest.raises(BackendError, match="not 'int8' .*'fp8_e4m3_block', made with fp8_e4m3_block_codec"):
+        _checks.require_buffers("op", _buffers("int8"))
