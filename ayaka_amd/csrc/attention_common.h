@@ -439,10 +439,17 @@ __device__ __forceinline__ void merge_partitions(const AttnParams& p, int row, i
   }
   auto fold = [&](int k, float mi, float wi, f32x4 v) {
     const float mn = fmaxf(m[k], mi);
-    const float a = fast_exp2(m[k] - mn);
-    const float b = wi * fast_exp2(mi - mn);
-    if constexpr (BS) l[k] = times_exp2(l[k], m[k] - mn) + times_exp2(wi, mi - mn);
-    else l[k] = l[k] * a + b;
+    float a, b;
+    if constexpr (BS) {  // as times_exp2
+      const float ha = fast_exp2(0.5f * (m[k] - mn)), hb = fast_exp2(0.5f * (mi - mn));
+      a = ha * ha;
+      b = wi * hb * hb;
+      l[k] = l[k] * ha * ha + b;
+    } else {
+      a = fast_exp2(m[k] - mn);
+      b = wi * fast_exp2(mi - mn);
+      l[k] = l[k] * a + b;
+    }
     acc[k] = acc[k] * a + v * b;
     m[k] = mn;
   };

@@ -342,10 +342,17 @@ __global__ __launch_bounds__(kReduceThreads) void partition_reduce_kernel(const 
   const int nfold = np > 1 ? np : 0;  // rows of one partition (or none) fold nothing
   auto fold = [&](float mi, float wi, f32x4 v, bool real) {
     const float mn = real ? fmaxf(m, mi) : m;
-    const float a = fast_exp2(m - mn);
-    const float b = real ? wi * fast_exp2(mi - mn) : 0.f;
-    if constexpr (BS) l = times_exp2(l, m - mn) + (real ? times_exp2(wi, mi - mn) : 0.f);
-    else l = l * a + b;
+    float a, b;
+    if constexpr (BS) {  // as times_exp2
+      const float ha = fast_exp2(0.5f * (m - mn)), hb = fast_exp2(0.5f * (mi - mn));
+      a = ha * ha;
+      b = real ? wi * hb * hb : 0.f;
+      l = l * ha * ha + b;
+    } else {
+      a = fast_exp2(m - mn);
+      b = real ? wi * fast_exp2(mi - mn) : 0.f;
+      l = l * a + b;
+    }
     acc = acc * a + v * b;
     m = mn;
   };
