@@ -274,6 +274,10 @@ def build_tables(
     is padding and does not. Rows of the tables behind the last request's get request, position and
     slot 0. ``tables.kv_lengths`` may be ``kv_lengths`` itself. Nothing waits for the device, and the
     call can be captured.
+
+    The slots serve ``store`` at once. To attend to the step, plan it from ``tables.kv_lengths`` and
+    ``block_table`` (``attention.plan``, which reads them on the host); only a decode bucket is served
+    without the host (``attention.advance_graph_metadata``).
     """
     op = "kvcache.build_tables"
     free, taken, after = pool

@@ -210,7 +210,10 @@ class BlockPool(NamedTuple):
 class StepTables(NamedTuple):
     """What a step's cache writes and attention read of its requests, at fixed addresses in device
     memory: ``request_of_row``, ``positions`` (int32) and ``slot_mapping`` (int64), each [N], and
-    ``kv_lengths`` int32 [B] (see :class:`~ayaka_amd.attention.AttentionMetadata`)."""
+    ``kv_lengths`` int32 [B] (see :class:`~ayaka_amd.attention.AttentionMetadata`).
+
+    ``store`` writes by the slots as they are. ``attend`` takes its launch and tile lists from a plan:
+    ``attention.plan`` on ``kv_lengths`` and the block table, which reads both on the host."""
 
     request_of_row: Tensor
     positions: Tensor

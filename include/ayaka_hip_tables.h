@@ -3,8 +3,10 @@
  * lack, and every row's position and slot, from the requests' lengths in device memory.
  *
  * Conventions and error codes are those of ayaka_hip.h. All pointers are device pointers unless
- * said otherwise; nothing is read on the host, so a step can be planned, and captured into a
- * graph, without the host knowing its lengths. The rules are those the reference applies on the
+ * said otherwise; nothing is read on the host, so the calls can be captured into a graph and need
+ * no lengths there. A decode bucket is then ready for attention (ayk_paged_attention_v2 reads the
+ * staged split); a step of any rows is ready for the KV write, while its attention still takes a
+ * tile or work list made from lengths the host knows. The rules are those the reference applies on the
  * host: positions and slots as python/ayaka/ops/backends/torch/attention.py:64-164, a decode
  * bucket's as :308-374 (SLOT = table[position / block_size] * block_size + position % block_size).
  */
