@@ -104,11 +104,16 @@ class BlockScaledFp8Codec(str):
     It is the string ``"fp8_e4m3_block"`` (equal to :data:`FP8_E4M3_BLOCK_CODEC`) with
     ``scales``, a contiguous float32 ``[num_blocks, kv_heads, 2]`` tensor on the cache's device:
     the key scale and the value scale of every block and key/value head. An element is worth
-    ``code * scale``. Scales are powers of two 2^e with -40 <= e <= 80, the least that keeps the
-    largest finite magnitude a block holds within 448 codes, or 0 for a block of nothing but
-    zeros; a fresh cache starts with zeros. ``store`` settles them as it writes: the first token
-    of a block starts its scale afresh, and a later one that needs a larger scale re-encodes the
-    block's tokens (a power of two apart, so exactly, down to the codes' subnormals).
+    ``code * scale``. Scales are powers of two 2^e with -40 <= e <= 80, or 0 for a block of nothing
+    but zeros; a fresh cache starts with zeros. ``store`` settles them as it writes: the first call
+    that writes a block from its first token on takes the least scale that keeps its largest finite
+    magnitude there within 448 codes, and a later call the larger of what it needs in the same way
+    and the block's scale. Growth re-encodes the block's tokens (a power of two apart, so exactly,
+    down to the codes' subnormals). A scale never falls while tokens are added, also where the loud
+    one was a rejected draft that the next call overwrites.
+
+    Attention resolves what blocks far quieter than the loudest add to an output element to 2^-25 of
+    the largest scaled weight (the C header has the rule).
 
     Storing infinities and NaN gives the NaN code and leaves the scale to the finite values.
     A layer's copy, swap and clear move the scales with the blocks (``copy_blocks``,
