@@ -159,6 +159,14 @@ __device__ __forceinline__ typename KvRaw<KV8>::T load_kv_raw(const uint16_t* ba
 // So a kernel keeps its running maximum m over score_t + e_t (one fma makes it), its weights u_t
 // stay at most 2^kRescaleSlack whatever the scales, and only the weight sum multiplies by 2^-e_t.
 //
+// u_t enters P.V as one fp16 value, as over every fp8 cache: half a step, 2^-11 of itself, down to
+// 2^-14, and below that an absolute 2^-25. Here u_t carries the value scale too, so positions whose
+// value scale is 2^s below the loudest seen are resolved to 2^-25 of the largest scaled weight,
+// 2^(s - 25) in their own unit: nothing beside a bf16 output up to s of 12, and always small next to
+// the row's largest element, but an element that the loud blocks leave at 0 loses its relative
+// accuracy from s of 16 on (2e-3 of it at 16, 5% at 20, half at 24). Weights in two parts would cost the
+// multi-row kernel a second P.V product, for scales that one head's values do not reach.
+//
 // The sum's terms are 2^(score_t - m), between 2^-80 and 2^40 of the largest weight's, and u_t may be
 // 2^-120 for a position that carries the sum and less for many that carry it together, where
 // v_exp_f32 gives zeros below 2^-126. While no value scale above 2^kLoudShift has been met, scales
@@ -621,7 +629,7 @@ __device__ __forceinline__ f32x4 mfma_pv(u32x2 v, u32x2 w, f32x4 acc) {
 // bits) is off by up to 2^-9 of itself, the size of the accuracy bar, so bf16 P
 // takes two MFMAs: packed high parts and packed parts of the remainder, both by
 // truncation, |w - h - l| < 2^-14 w. An fp16 weight rounded to nearest (11 bits)
-// is within 2^-12 w, and one MFMA suffices: then only `hi` is set.
+// is within 2^-11 w (2^-25 below 2^-14), and one MFMA suffices: then only `hi` is set.
 constexpr bool split_p(bool bf16) { return bf16; }
 
 // Split 4 fp32 weights w (finite, >= 0) as above.

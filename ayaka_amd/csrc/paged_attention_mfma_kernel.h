@@ -20,7 +20,7 @@
 //    a token-major LDS tile through ds_read_b64_tr_b16. A bf16 P is split into
 //    a truncated high part and the remainder (two MFMAs, fp32-level accuracy;
 //    one bf16 P would cost ~2e-3 relative); an fp16 P rounded to nearest is
-//    within 2^-12 and takes one.
+//    within 2^-11 and takes one.
 //  * fp8 caches (KV8) are decoded at their use; a chunk then holds two 16-token
 //    tiles (one at head_dim 256), so a wave keeps as many bytes in flight as
 //    with 16-bit caches.

@@ -29,7 +29,7 @@
 //    ds_read_b64_tr_b16 (two 4-position reads per operand). A bf16 P is
 //    split by truncation into a 16-bit high part and the 16-bit remainder, two
 //    MFMAs, which keeps the product at fp32-level accuracy (one bf16 P would cost
-//    ~2e-3 relative); an fp16 P rounded to nearest is within 2^-12 and takes one.
+//    ~2e-3 relative); an fp16 P rounded to nearest is within 2^-11 and takes one.
 //  * Keys and values are staged with 16-byte LDS stores, values token-major in
 //    rows D + 16 elements apart, which keeps the transposing reads of a 16-lane
 //    group spread over the banks.

@@ -55,7 +55,10 @@ int ayk_store_block_scaled(const void* k, const void* v, void* k_cache, void* v_
  *   ayk_paged_prefill_block_scaled            ayk_paged_prefill
  *   ayk_paged_attention_windows_block_scaled  ayk_paged_attention_windows
  * Position t of a request counts with the scales of its block: its score is
- * scale * key scale * q.code and its value code * value scale. A NaN code at a position a row does
+ * scale * key scale * q.code and its value code * value scale. Weights times their value scales are
+ * rounded to 16 bits in units of the largest: half a step, 2^-11, down to 2^-14 of it and an absolute
+ * 2^-25 of it below, so what blocks far quieter than the loudest add to an element is resolved to
+ * that. A NaN code at a position a row does
  * not attend to does not reach the row; one at a position it attends to makes the elements it
  * belongs to NaN (a value's) or the row's head (a key's).
  */
