@@ -100,10 +100,11 @@ __host__ __device__ constexpr int prefill_workgroups_per_cu(int head_dim, int wa
 // loads and converts nothing for them. A lane's 4 scores of a tile are of consecutive positions: a
 // scale they share enters with the maximum, the exponent's fma and the tile's weight sum, a few
 // instructions per tile where a scale per position takes one more per score.
-// 4 x 512 rows over 4K of 32/8 heads of 128, blocks of 16: 136 us (0.94 PFLOP/s) against 125 over
-// unscaled codes, 138 with a chunk's scales staged by position; 4 chunks of 150-500 rows over
-// 900-3600, 16/8 heads of 256, blocks of 24: 97 us against 90, 113 so. Of the first's 11 us the
-// maximum takes 4, the sum 2, the reads of the scales 3.
+// 4 x 512 rows over 4K of 32/8 heads of 128, blocks of 16: 136 us (0.95 PFLOP/s) against 121 over
+// layer-scaled codes; 4 chunks of 150-500 rows over 900-3600, 16/8 heads of 256, blocks of 24: 97 us
+// against 89. Of the first's, the maximum takes 4, the sum 2, the reads of the scales 3, the exact
+// sum's branch and half steps 3. (Before that branch, 133 and 95 us; 138 and 113 with a chunk's
+// scales staged by position.)
 template <int D, bool BF16, bool KV8, int PS, int W = kPrefillWaves, int MODE = 0, int SCALES = 0>
 __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D, PS)) void paged_prefill_kernel(
     const AttnParams p, const int32_t* tiles) {
