@@ -1559,13 +1559,13 @@ def advance_graph_metadata(meta: AttentionMetadata, kv_lengths: torch.Tensor, po
             f"{op}: meta was not made by this backend's graph_metadata",
             context={"op": op, "argument": "meta"},
         )
-    # the staged split no longer is the host's: attend must not stage that one again
-    staging.staged_shape.clear()
     shape = tuple(staging.head_shape)
     key = ("advance", id(meta), shape, _fastpath.signature((kv_lengths, pool.free, pool.taken, pool.after)))
     found = _fastpath.lookup(staging.launches, key)
     if found is not None:
         _fastpath.run(found, stream_handle(found.device))
+        # the staged split no longer is the host's: attend must not stage that one again
+        staging.staged_shape.clear()
         return
     device = table.device
     if not table.is_cuda:
@@ -1587,6 +1587,7 @@ def advance_graph_metadata(meta: AttentionMetadata, kv_lengths: torch.Tensor, po
         ctypes.addressof(sizes), len(sizes), -(-kv_heads * head_chunks(group) // 8), WORKGROUP_COSTS[kv_bytes],
         COMPUTE_UNITS,
     ), stream_handle(device), device, False, record)
+    staging.staged_shape.clear()
     _fastpath.remember(staging.launches, key, (meta,), record)
 
 

@@ -136,3 +136,16 @@ def _advance(sizes=(64, 128), **kw: object) -> int:
 def test_the_library_refuses_bad_advances(changes: dict, code: int, message: bytes) -> None:
     assert _advance(**changes) == code
     assert message in _lib.lib().ayk_last_error()
+
+
+def test_a_refused_advance_leaves_the_hosts_split() -> None:
+    # the split that the last update staged is still the bucket's: a first attend of another head shape
+    # stages it again for that shape
+    meta = hip_attention.graph_metadata(2, 64, 16, torch.device("cpu"))
+    hip_attention.update_graph_metadata(meta, torch.tensor([900, 40], dtype=torch.int32),
+                                        torch.arange(1, 129, dtype=torch.int32).view(2, 64))
+    staged = list(meta.plan.staged_shape)
+    assert staged
+    with pytest.raises(BackendError):
+        hip_attention.advance_graph_metadata(meta, torch.zeros(2, dtype=torch.int32), _pool())
+    assert meta.plan.staged_shape == staged
