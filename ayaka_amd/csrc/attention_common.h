@@ -340,9 +340,9 @@ __device__ __forceinline__ void row_context(const AttnParams& p, int row, int& r
   len = max(0, min(len, p.max_len));
 }
 
-// Running-max sentinel: below any real score yet finite, so exp2(sentinel - m) is 0
+// Running-max sentinel: below any finite score yet finite itself, so exp2(sentinel - m) is 0
 // for a real m and 1 when nothing has been seen, and no -inf - -inf NaN can arise.
-constexpr float kNoScore = -1.0e30f;
+constexpr float kNoScore = -__FLT_MAX__;
 // How far (log2 units) the running max may trail a chunk's max before the
 // accumulators are rescaled: weights stay below 2^8, far inside fp32.
 constexpr float kRescaleSlack = 8.0f;

@@ -73,9 +73,10 @@ __device__ __forceinline__ void split_weights(const float (&w)[8], u32x4& hi, u3
 }
 
 // Workgroups per CU the register budget is set for: two, except quarter tiles at head_dim 256,
-// whose 64-position stage (133 KB of LDS) leaves room for one.
-__host__ __device__ constexpr int prefill_workgroups_per_cu(int head_dim, int waves_per_group) {
-  return head_dim == 256 && waves_per_group == 4 ? 1 : 2;
+// whose 64-position stage (133 KB of LDS) leaves room for one, and block scales shared by 4 or
+// 16 positions at head_dim 64, which fit three (without the bound some take 2 registers too many).
+__host__ __device__ constexpr int prefill_workgroups_per_cu(int head_dim, int waves_per_group, int scales) {
+  return head_dim == 256 && waves_per_group == 4 ? 1 : head_dim == 64 && scales >= 4 ? 3 : 2;
 }
 
 // W: waves per workgroup, kPrefillWaves, or 8 for the double tile (head_dim 128 and 256, one
@@ -106,7 +107,7 @@ __host__ __device__ constexpr int prefill_workgroups_per_cu(int head_dim, int wa
 // sum's branch and half steps 3. (Before that branch, 133 and 95 us; 138 and 113 with a chunk's
 // scales staged by position.)
 template <int D, bool BF16, bool KV8, int PS, int W = kPrefillWaves, int MODE = 0, int SCALES = 0>
-__global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D, PS)) void paged_prefill_kernel(
+__global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D, PS, SCALES)) void paged_prefill_kernel(
     const AttnParams p, const int32_t* tiles) {
   static_assert(W == kPrefillWaves || (W == 8 && PS == 1 && D != 64), "the double tile: 8 waves, one per pair group");
   constexpr bool BS = SCALES != 0;
@@ -274,6 +275,10 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
   // BS: the position up to which every row of the tile sees the context
   int tile_least = 0;
   if constexpr (BS) tile_least = min(p.positions[first_row], kv_len - 1);
+  // A running maximum above 2^24 in magnitude: there a product's rounding, which a fused multiply-add
+  // against the rounded maximum keeps, is a unit and more of an exponent (inf weights from 2^31 on),
+  // so the scores are scaled, and rounded, before the maximum is taken off them. Uniform in the wave.
+  bool far = false;
   // V16_FAST: a chunk whose values did not all convert (uniform); its results are then not
   // stored, and the fallback pass computes the workgroup (the rest of the chunks still run:
   // leaving the loop early costs the common case registers)
@@ -408,12 +413,13 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
       }
       // uniform: no position masked (and, for folding the scale into the exponent,
       // a scale >= 0, under which the largest raw score gives the largest scaled one)
-      const bool whole = tb + CH <= s1 && tb + CH - 1 <= wave_min_pos && scale_log2 >= 0.f;
-      // the scale applied to a score in the exponent below (1 once the scores are scaled)
-      const float sc = whole ? scale_log2 : 1.f;
+      const bool whole = tb + CH <= s1 && tb + CH - 1 <= wave_min_pos && scale_log2 >= 0.f && !far;
+      // a group's scores are yet to be scaled, in the exponent below
+      bool raw[PT];
 #pragma unroll
       for (int j = 0; j < PT; ++j) {
         float mx = -INFINITY;
+        raw[j] = whole;
         if (whole) {
 #pragma unroll
           for (int w = 0; w < PTL_W; ++w) {
@@ -451,6 +457,20 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
 #pragma unroll
           for (int t = 0; t < DT; ++t) o[j][t] *= alpha;
           m[j] = mn;
+          if (__builtin_amdgcn_ballot_w64(fabsf(mn) > 16777216.f && mn != kNoScore)) {
+            far = true;
+            if (whole) {
+#pragma clang fp contract(off)
+              raw[j] = false;
+#pragma unroll
+              for (int w = 0; w < PTL_W; ++w)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if constexpr (BS) acc[w][j][i] = __builtin_fmaf(acc[w][j][i], ts.v[w].x, ts.v[w].y);
+                  else acc[w][j][i] *= scale_log2;
+                }
+            }
+          }
         }
       }
       // BS, behind a loud block: the sum's terms from exponentials of their own, and none (0 of each
@@ -464,7 +484,7 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
               const float shift = QUADS ? ts.v[w].y : scale_at(tb + (ps * PTL_W + w) * 16 + 4 * mq + i).y;
 #pragma unroll
               for (int j = 0; j < PT; ++j) {
-                const float scaled = whole ? __builtin_fmaf(acc[w][j][i], ts.v[w].x, ts.v[w].y) : acc[w][j][i];
+                const float scaled = raw[j] ? __builtin_fmaf(acc[w][j][i], ts.v[w].x, ts.v[w].y) : acc[w][j][i];
                 l[j] += fast_exp2(scaled - m[j] - shift);
               }
             }
@@ -479,8 +499,8 @@ __global__ __launch_bounds__(W * kWave, W == 8 ? 1 : prefill_workgroups_per_cu(D
       for (int j = 0; j < PT; ++j)
 #pragma unroll
         for (int w = 0; w < PTL_W; ++w) {
-          const float by = BS ? (whole ? ts.v[w].x : 1.f) : sc;
-          const float from = BS ? (whole ? ts.v[w].y - m[j] : -m[j]) : -m[j];
+          const float by = raw[j] ? (BS ? ts.v[w].x : scale_log2) : 1.f;
+          const float from = BS ? (raw[j] ? ts.v[w].y - m[j] : -m[j]) : -m[j];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float e = fast_exp2(__builtin_fmaf(acc[w][j][i], by, from));
