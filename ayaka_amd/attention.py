@@ -22,7 +22,7 @@ if TYPE_CHECKING:
     from torch import Tensor, device
 
     from ayaka_amd.enums import ForwardMode
-    from ayaka_amd.kvcache import BlockPool, KVBuffers
+    from ayaka_amd.kvcache import BlockPool, KVBuffers, LatentBuffers, LatentWeights
 
 __all__ = ["AttentionMetadata", "AttentionOps"]
 
@@ -70,6 +70,15 @@ class AttentionOps(Protocol):
 
     def attend(
         self, q: Tensor, buffers: KVBuffers, meta: AttentionMetadata, out: Tensor, *, scale: float
+    ) -> None: ...
+
+    def attend_latent(
+        self, q: Tensor, buffers: LatentBuffers, meta: AttentionMetadata, out: Tensor, *, scale: float
+    ) -> None: ...
+
+    def attend_latent_chunks(
+        self, q: Tensor, weights: LatentWeights, buffers: LatentBuffers, meta: AttentionMetadata,
+        out: Tensor, *, scale: float,
     ) -> None: ...
 
     def graph_metadata(

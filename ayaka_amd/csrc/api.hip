@@ -9,19 +9,19 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
-#include <initializer_list>
 #include <string>
 
+#include "api_common.h"
 #include "ayaka_hip.h"
 #include "ayaka_hip_block_scaled.h"
 #include "ayaka_hip_internal.h"
 #include "ayaka_hip_tables.h"
 
 namespace {
-
 thread_local std::string g_last_error;
+}
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+namespace ayk_api {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -43,6 +43,34 @@ int launched(hipError_t err, const char* what) {
   return ok();
 }
 
+bool misaligned(uintptr_t to, std::initializer_list<const void*> addresses) {
+  for (const void* at : addresses)
+    if (reinterpret_cast<uintptr_t>(at) % to != 0) return true;
+  return false;
+}
+
+int compute_units() {
+  static int cached[64] = {0};  // queried once per device
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cached[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
+}  // namespace ayk_api
+
+namespace {
+
+using ayk_api::compute_units;
+using ayk_api::fail;
+using ayk_api::launched;
+using ayk_api::misaligned;
+using ayk_api::ok;
+
 // The kernels' division of a position by the block size (block_of in attention_common.h):
 // shift l = ceil(log2 bs) and magic m = floor(2^32 (2^l - bs) / bs) + 1, exact for every
 // position below 2^31 (Granlund and Montgomery's round-up method; checked exhaustively on
@@ -54,12 +82,15 @@ void block_divisor(int32_t bs, uint32_t& magic, int32_t& shift) {
   magic = (uint32_t)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - (uint64_t)bs) / (uint64_t)bs + 1);
 }
 
-// Whether any of these addresses is not a multiple of `to`.
-bool misaligned(uintptr_t to, std::initializer_list<const void*> addresses) {
-  for (const void* at : addresses)
-    if (reinterpret_cast<uintptr_t>(at) % to != 0) return true;
-  return false;
+}  // namespace
+
+ayk::Divisor ayk::divisor_of(int32_t d) {
+  Divisor by;
+  block_divisor(d, by.magic, by.shift);
+  return by;
 }
+
+namespace {
 
 // Split a group of query heads into equal chunks of at most 8 heads (one workgroup each).
 int head_chunks_for(int group) {
@@ -181,19 +212,6 @@ int prepare(const char* op, const AttnCall& c, ayk::AttnParams& p, int& heads_pe
   p.max_partitions = 1;
   p.wave_split = 1;
   return AYK_OK;
-}
-
-// Compute units of the current device (queried once per device).
-int compute_units() {
-  static int cached[64] = {0};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cached[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cached[dev] = n;
-  }
-  return cached[dev];
 }
 
 // Whether v2 merges its partitions inside the partition kernel (rather than in
@@ -630,7 +648,7 @@ AttnCall block_scaled_call(void* out, const void* q, const void* k_cache, const 
 
 extern "C" {
 
-int ayk_abi_version(void) { return 19; }
+int ayk_abi_version(void) { return 20; }
 
 int ayk_paged_prefill_tile_pairs(int32_t head_dim) { return ayk::prefill_tile_pairs_for(head_dim); }
 

@@ -143,6 +143,66 @@ struct TablesParams {
 };
 hipError_t launch_step_tables(const TablesParams& p, hipStream_t stream);
 
+// Division of 0 <= n < 2^31 by d as (umulhi(n, magic) + n) >> shift (see block_divisor in api.hip).
+struct Divisor {
+  uint32_t magic;
+  int32_t shift;
+};
+Divisor divisor_of(int32_t d);
+
+// Rows rotated by their positions and written (rotate_store.hip). Strides in elements.
+struct RotateStream {
+  const void* from;
+  void* to;
+  int64_t from_row, from_head;
+  int64_t to_row, to_head;  // by_slot: to_row is the stride of a block's positions
+  int64_t to_block;
+  int32_t heads, width;     // no heads: no such stream
+  int32_t rotated;          // elements of a head that rotate (even; 0: all pass through)
+  int32_t by_slot;
+  int32_t tasks_per_head;   // set by the launch, with by_tasks
+  Divisor by_tasks;
+};
+struct RotateParams {
+  RotateStream stream[3];
+  const int32_t* positions;
+  const int64_t* slots;
+  const double* turns;  // [pairs], turns per position
+  float magnitude;
+  int32_t pairs, n_rows, block_size;
+  int32_t num_slots;
+  Divisor by_block;
+  int32_t begin[3];  // of each stream's tasks; this and the rest set by the launch
+  int32_t tasks_per_row, rows_per_workgroup;
+  Divisor by_tasks;
+};
+int rotate_most_pairs();
+// type: AYK_DTYPE_* of every stream's elements
+hipError_t launch_rotate_store(RotateParams p, int type, bool side_by_side, int compute_units, hipStream_t stream);
+
+// Attention over a latent cache (latent_attention.hip). Strides in elements.
+struct LatentParams {
+  void* out;
+  const uint16_t* q;
+  const uint16_t* cache;
+  const int32_t* block_table;
+  const int32_t* kv_lengths;
+  const int32_t* rows;  // rows of each request
+  int64_t table_stride;
+  int32_t n_requests, n_rows, heads, num_blocks, block_size;
+  Divisor by_block;
+  int32_t max_len;
+  float scale_log2;
+  int32_t* places;  // where each workgroup begins, partials' (m, l) and partial outputs: the workspace
+  float* part_ml;
+  float* part_o;
+};
+// (row, head) pairs of one tile for rows of `heads` heads, `rows` of them to a request on average
+int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads);
+size_t latent_workspace_bytes(int32_t latent_dim, int pairs, int compute_units);
+hipError_t launch_latent_attention(const LatentParams& p, int32_t latent_dim, bool bf16, int pairs, int compute_units,
+                                   hipStream_t stream);
+
 // mode: 0 = gather (dst index i), 1 = copy (dst ids), 2 = zero (no source)
 hipError_t launch_block_op(int mode, const void* src_k, const void* src_v, void* dst_k, void* dst_v,
                            const void* src_ids, const void* dst_ids, bool ids64, int64_t n,

@@ -217,12 +217,12 @@ __device__ __forceinline__ int64_t read_id(const void* ids, bool ids64, int64_t 
   return ids64 ? static_cast<const int64_t*>(ids)[i] : (int64_t) static_cast<const int32_t*>(ids)[i];
 }
 
-// grid.x = block pair i; grid.y * 256 lanes stride over the block's vectors.
+// grid.x = block pair i; grid.y * 256 lanes stride over the block's vectors. One cache given as both
+// (a latent cache, or the scales of a block-scaled one) is moved once.
 template <int VEC>
 __global__ __launch_bounds__(256) void block_op_kernel(int mode, const uint8_t* __restrict__ src_k,
                                                        const uint8_t* __restrict__ src_v,
-                                                       uint8_t* __restrict__ dst_k,
-                                                       uint8_t* __restrict__ dst_v,
+                                                       uint8_t* dst_k, uint8_t* dst_v,
                                                        const void* src_ids, const void* dst_ids,
                                                        int32_t ids64, int32_t num_blocks,
                                                        int64_t block_bytes) {
@@ -238,6 +238,7 @@ __global__ __launch_bounds__(256) void block_op_kernel(int mode, const uint8_t* 
     if (dst_blk < 0 || dst_blk >= num_blocks) return;
   }
   const int64_t nvec = block_bytes / VEC;
+  const bool two = dst_k != dst_v;
   for (int64_t j = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; j < nvec;
        j += (int64_t)gridDim.y * blockDim.x) {
     V* dk = reinterpret_cast<V*>(dst_k + dst_blk * block_bytes) + j;
@@ -246,12 +247,13 @@ __global__ __launch_bounds__(256) void block_op_kernel(int mode, const uint8_t* 
     // copy 4.8 -> 6.2 TB/s of bytes read plus written; a plain device copy runs 5.4).
     if (mode == 2) {
       __builtin_nontemporal_store(V{}, dk);
-      __builtin_nontemporal_store(V{}, dv);
+      if (two) __builtin_nontemporal_store(V{}, dv);
     } else {
       const V a = __builtin_nontemporal_load(reinterpret_cast<const V*>(src_k + src_blk * block_bytes) + j);
-      const V b = __builtin_nontemporal_load(reinterpret_cast<const V*>(src_v + src_blk * block_bytes) + j);
+      V b{};
+      if (two) b = __builtin_nontemporal_load(reinterpret_cast<const V*>(src_v + src_blk * block_bytes) + j);
       __builtin_nontemporal_store(a, dk);
-      __builtin_nontemporal_store(b, dv);
+      if (two) __builtin_nontemporal_store(b, dv);
     }
   }
 }

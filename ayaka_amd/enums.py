@@ -17,7 +17,7 @@ class KVLayoutKind(str, enum.Enum):
 
     NHD = "nhd"  # [block_size, num_kv_heads, head_dim]
     HND = "hnd"  # [num_kv_heads, block_size, head_dim]
-    NLD = "NLD"  # latent planes; no backend here serves it
+    NLD = "NLD"  # latent planes: [block_size, latent_dim + rope_dim] (LatentBuffers)
 
     def __str__(self) -> str:
         return self.value

@@ -23,7 +23,9 @@ from ayaka_amd.kvcache import (
     BlockPool,
     BlockScaledFp8Codec,
     KVBuffers,
+    LatentBuffers,
 )
+from ayaka_amd.rotary import Rotary
 
 __all__ = [
     "HEAD_DIMS",
@@ -35,8 +37,11 @@ __all__ = [
     "require_buffers",
     "require_device",
     "require_index_tensor",
+    "require_latent_buffers",
     "require_like",
     "require_pool",
+    "require_rotary",
+    "require_rows",
     "stream_handle",
 ]
 
@@ -213,3 +218,66 @@ def require_buffers(op: str, buffers: KVBuffers) -> None:
         )
     if buffers.codec == FP8_E4M3_BLOCK_CODEC:
         require_block_scales(op, buffers)
+
+
+def require_latent_buffers(op: str, buffers: LatentBuffers) -> None:
+    """Refuse a latent cache that is not one: kind, dtype, shape, strides, device."""
+    argument = {"op": op, "argument": "buffers"}
+    if not isinstance(buffers, LatentBuffers):
+        raise BackendError(f"{op}: buffers must be LatentBuffers, got {type(buffers).__name__}", context=argument)
+    cache, latent_dim = buffers.cache, buffers.latent_dim
+    if cache.dtype not in _RAW_DTYPES:
+        allowed = ", ".join(dtype_name(d) for d in _RAW_DTYPES)
+        raise BackendError(f"{op}: buffers.cache is {dtype_name(cache.dtype)}; the hip backend stores latents as {allowed}",
+                           context=argument)
+    if cache.ndim != 3 or not 0 < latent_dim < cache.shape[2]:
+        raise BackendError(
+            f"{op}: buffers.cache must be [num_blocks, block_size, latent_dim + rope_dim] with a latent_dim of "
+            f"{latent_dim} and a rope_dim above 0, got {list(cache.shape)}",
+            context=argument,
+        )
+    if not cache.is_contiguous():
+        raise BackendError(f"{op}: buffers.cache must be contiguous", context=argument)
+    if not cache.is_cuda:
+        raise BackendError(f"{op}: the hip backend runs on a HIP device; buffers are on {cache.device}", context=argument)
+
+
+def require_rotary(op: str, rotary: Rotary, device: torch.device) -> int:
+    """The pairs of a rotation these kernels can apply."""
+    turns = rotary.turns
+    if turns.dtype != torch.float64 or turns.ndim != 1 or not turns.is_contiguous() or turns.numel() == 0:
+        raise BackendError(
+            f"{op}: rotary.turns must be a contiguous float64 vector, got {dtype_name(turns.dtype)} {list(turns.shape)}",
+            context={"op": op, "argument": "rotary"},
+        )
+    if turns.device != device:
+        raise BackendError(f"{op}: rotary.turns is on {turns.device}, the rows are on {device}",
+                           context={"op": op, "argument": "rotary"})
+    return turns.numel()
+
+
+def require_rows(op: str, name: str, tensor: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
+                 device: torch.device, *, written: bool = False) -> None:
+    """Refuse rows [N, (heads,) width] whose elements are not next to each other, and rows to write
+    into that may share memory."""
+    if tuple(tensor.shape) != shape or tensor.dtype != dtype:
+        raise BackendError(
+            f"{op}: {name} must be {dtype_name(dtype)} {list(shape)}, got {dtype_name(tensor.dtype)} {list(tensor.shape)}",
+            context={"op": op, "argument": name},
+        )
+    if tensor.device != device:
+        raise BackendError(f"{op}: {name} is on {tensor.device}, the other rows are on {device}",
+                           context={"op": op, "argument": name})
+    if tensor.numel() and tensor.stride(-1) != 1:
+        raise BackendError(f"{op}: the elements of a row of {name} must be next to each other, got strides "
+                           f"{list(tensor.stride())}", context={"op": op, "argument": name})
+    if written and tensor.numel():
+        # the dimensions by stride: each must step over what the smaller ones cover
+        covered = shape[-1]
+        for stride, size in sorted(zip(tensor.stride()[:-1], shape[:-1])):
+            if size == 1:
+                continue
+            if stride < covered:
+                raise BackendError(f"{op}: rows of {name} share memory, got strides {list(tensor.stride())}",
+                                   context={"op": op, "argument": name})
+            covered = stride * (size - 1) + covered

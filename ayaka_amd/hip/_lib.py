@@ -14,10 +14,10 @@ from pathlib import Path
 
 from ayaka_amd.errors import BackendError, CapabilityError
 
-__all__ = ["ABI_VERSION", "BLOCK_SCALED_EXPORTS", "EXPORTS", "LIB_PATH", "TABLES_EXPORTS", "check", "lib"]
+__all__ = ["ABI_VERSION", "BLOCK_SCALED_EXPORTS", "EXPORTS", "LATENT_EXPORTS", "LIB_PATH", "TABLES_EXPORTS", "check", "lib"]
 
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libayaka_hip.so"
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -119,6 +119,25 @@ TABLES_EXPORTS: dict[str, tuple[object, list[object]]] = {
     ),
 }
 
+#: The functions of include/ayaka_hip_latent.h.
+LATENT_EXPORTS: dict[str, tuple[object, list[object]]] = {
+    "ayk_rotate_and_cache": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P,
+         _I32, _I32, _F32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+    ),
+    "ayk_store_latent": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P,
+         _I32, _I32, _F32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+    ),
+    "ayk_latent_attention_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
+    "ayk_latent_attention": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P, _SZ, _P],
+    ),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -152,7 +171,8 @@ def lib() -> ctypes.CDLL:
                         detail=f"{LIB_PATH} has ABI {version}, this package expects {ABI_VERSION}",
                         remedy="rebuild it",
                     )
-                for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS, **TABLES_EXPORTS}.items():
+                for name, (restype, argtypes) in {**EXPORTS, **BLOCK_SCALED_EXPORTS, **TABLES_EXPORTS,
+                                                   **LATENT_EXPORTS}.items():
                     fn = getattr(handle, name)
                     fn.restype = restype
                     fn.argtypes = argtypes

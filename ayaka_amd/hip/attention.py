@@ -66,6 +66,7 @@ __all__ = [
     "HipGraphPlan",
     "advance_graph_metadata",
     "attend",
+    "attend_latent",
     "attend_with",
     "choose_partitions",
     "choose_split",
@@ -1618,3 +1619,7 @@ def _stage_split(staging: HipGraphPlan, lengths: np.ndarray, block_size: int) ->
     return work + items.size
 
 
+
+
+# the family's ops over latent caches, which share this module's plans and scratch
+from ayaka_amd.hip.latent import attend_latent  # noqa: E402

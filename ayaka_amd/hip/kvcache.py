@@ -9,7 +9,9 @@ raises where it has to (``ayk_store_block_scaled``). ``gather``,
 ``copy_blocks`` and ``zero_blocks`` move whole blocks (same file, ``:83-115``),
 of a block-scaled cache with their scales. ``build_tables`` gives a step's
 requests the blocks they lack and derives its slots on the device
-(``ayk_build_tables``).
+(``ayk_build_tables``). ``rotate``, ``store_rotated`` and ``store_latent`` apply a step's
+rotary positions, the last two together with the cache write
+(``include/ayaka_hip_latent.h``).
 Both layouts are served; NHD is preferred, as the reference's ``layout()``
 returns (``:30-31``).
 """
@@ -28,16 +30,22 @@ from ayaka_amd.hip._checks import (
     require_buffers,
     require_device,
     require_index_tensor,
+    require_latent_buffers,
     require_like,
     require_pool,
+    require_rotary,
+    require_rows,
     stream_handle,
 )
-from ayaka_amd.kvcache import FP8_E4M3_CODEC, BlockPool, KVBuffers, StepTables, codec_scales
+from ayaka_amd.kvcache import FP8_E4M3_CODEC, RAW_CODEC, BlockPool, KVBuffers, LatentBuffers, StepTables, codec_scales
+from ayaka_amd.rotary import Rotary
 
-__all__ = ["build_tables", "copy_blocks", "gather", "layout", "store", "zero_blocks"]
+__all__ = ["build_tables", "copy_blocks", "gather", "layout", "rotate", "store", "store_latent", "store_rotated",
+           "zero_blocks"]
 
 _LAYOUT_CODES = {KVLayoutKind.NHD: 0, KVLayoutKind.HND: 1}
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
+_ROW_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 3}
 _I32 = torch.int32
 
 
@@ -128,14 +136,227 @@ def _store(k: torch.Tensor, v: torch.Tensor, buffers: KVBuffers, meta: Attention
     _lib.check(op, fn(*args, _stream(device)))
 
 
+def _rotation(op: str, meta: AttentionMetadata, rotary: Rotary | None, device: torch.device,
+              width: int) -> tuple:
+    """The entry points' positions, and turns, pairs, order and magnitude of a rotation of rows of
+    ``width`` elements (``None``: nothing turns)."""
+    if rotary is None:
+        return 0, (0, 0, 0, 1.0)
+    pairs = require_rotary(op, rotary, device)
+    if 2 * pairs > width:
+        raise BackendError(f"{op}: the rotation turns {2 * pairs} elements of heads of {width}",
+                           context={"op": op, "argument": "rotary"})
+    positions = meta.positions
+    if positions.dtype != _I32 or not positions.is_contiguous():
+        raise BackendError(f"{op}: meta.positions must be a contiguous int32 tensor", context={"op": op})
+    require_device(op, "meta.positions", positions, device)
+    return positions.data_ptr(), (rotary.turns.data_ptr(), pairs, int(rotary.interleaved), float(rotary.magnitude))
+
+
+def _slots(op: str, meta: AttentionMetadata, buffers: "KVBuffers | LatentBuffers") -> torch.Tensor:
+    if meta.block_size != buffers.block_size:
+        raise BackendError(
+            f"{op}: the step was planned for blocks of {meta.block_size} positions "
+            f"but the cache has blocks of {buffers.block_size}",
+            context={"op": op, "argument": "meta"},
+        )
+    slots = meta.slot_mapping
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        raise BackendError(f"{op}: meta.slot_mapping must be a contiguous int64 tensor")
+    require_device(op, "meta.slot_mapping", slots, buffers.k.device)
+    return slots
+
+
+def _turned(op: str, name: str, rows: torch.Tensor, out: torch.Tensor | None, n_rows: int, width: int,
+            dtype: torch.dtype, device: torch.device) -> tuple[int, tuple]:
+    """Rows [N, heads, width] to rotate, into ``out`` or in place: the heads, and the entry points'
+    addresses and strides."""
+    out = rows if out is None else out
+    heads = rows.shape[1] if rows.ndim == 3 else 0
+    shape = (n_rows, heads, width)
+    require_rows(op, name, rows, shape, dtype, device, written=out is rows)
+    if out is not rows:
+        require_rows(op, f"{name}_out", out, shape, dtype, device, written=True)
+        if out.data_ptr() == rows.data_ptr() and out.stride() != rows.stride() and rows.numel():
+            raise BackendError(f"{op}: {name}_out shares memory with {name} at other strides",
+                               context={"op": op, "argument": f"{name}_out"})
+    return heads, (rows.data_ptr(), *rows.stride()[:2], out.data_ptr(), *out.stride()[:2])
+
+
+_NO_ROWS = (0, 0, 0, 0, 0, 0)
+
+
+def _replayed(meta: AttentionMetadata, key: tuple, keep: tuple, call) -> None:
+    """``call(record)``, or the launch it recorded in the step's plan when it ran with this ``key``."""
+    cache = getattr(meta.plan, "launches", None)
+    if cache is None:
+        call(None)
+        return
+    found = _fastpath.lookup(cache, key)
+    if found is not None:
+        _fastpath.run(found, _stream(found.device))
+        return
+    record = _fastpath.Recorder()
+    call(record)
+    _fastpath.remember(cache, key, keep, record)
+
+
+def rotate(q: torch.Tensor | None, k: torch.Tensor | None, meta: AttentionMetadata, rotary: Rotary,
+           q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """Rotate a step's queries and keys by their positions, in place or into ``q_out`` and ``k_out``.
+
+    ``q`` [N, heads, head_dim] and ``k`` [N, kv_heads, head_dim] may be views of a larger tensor (the
+    parts of one projection's output) whose heads are contiguous; either may be ``None``. Row i turns by
+    ``meta.positions[i]``; of each head the first ``2 * len(rotary.turns)`` elements turn and the others
+    are copied. Angles are reduced in 64 bits, products are fp32, each result is rounded once. An
+    output is its input or overlaps neither input. For caches that ``store_rotated`` does not
+    write: ``store`` takes the rotated keys.
+    """
+    op = "kvcache.rotate"
+    given = [t for t in (q, k) if t is not None]
+    if not given:
+        raise BackendError(f"{op}: neither q nor k is given", context={"op": op})
+    tensors = (*given, q if q_out is None else q_out, k if k_out is None else k_out, rotary.turns)
+    key = ("rotate", id(meta), id(rotary), q is None, k is None,
+           _fastpath.signature(tuple(t for t in tensors if t is not None)))
+    _replayed(meta, key, (meta, rotary), lambda record: _rotate(op, q, k, meta, rotary, q_out, k_out, record))
+
+
+def _rotate(op: str, q, k, meta: AttentionMetadata, rotary: Rotary, q_out, k_out, record) -> None:
+    first = q if q is not None else k
+    if first.ndim != 3 or first.dtype not in _ROW_DTYPE_CODES or not first.is_cuda:
+        raise BackendError(
+            f"{op}: rows must be float16, bfloat16 or float32 [N, heads, head_dim] on a HIP device, got "
+            f"{first.dtype} {list(first.shape)} on {first.device}", context={"op": op})
+    n_rows, width, dtype, device = meta.positions.shape[0], first.shape[2], first.dtype, first.device
+    heads, q_args = _turned(op, "q", q, q_out, n_rows, width, dtype, device) if q is not None else (0, _NO_ROWS)
+    kv_heads, k_args = _turned(op, "k", k, k_out, n_rows, width, dtype, device) if k is not None else (0, _NO_ROWS)
+    positions, turn = _rotation(op, meta, rotary, device, width)
+    if n_rows == 0:
+        return
+    _launch(op, _lib.lib().ayk_rotate_and_cache, (
+        *q_args, *k_args, 0, 0, 0, 0, 0, positions, 0, *turn, n_rows, heads, kv_heads, width, 0, 0, 0,
+        _ROW_DTYPE_CODES[dtype]), device, record)
+
+
+def _launch(op: str, fn, args: tuple, device: torch.device, record: "_fastpath.Recorder | None") -> None:
+    if record is not None:
+        record(op, fn, args, device, False)
+    _lib.check(op, fn(*args, _stream(device)))
+
+
+def store_rotated(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, buffers: KVBuffers,
+                  meta: AttentionMetadata, rotary: Rotary, q_out: torch.Tensor | None = None) -> None:
+    """Rotate a step's queries and keys by their positions and write the keys and values into the cache.
+
+    What ``rotate`` and then ``store`` would do, in one launch: ``q`` is rotated in place or into
+    ``q_out`` (see :func:`rotate`), the rotated ``k`` and ``v`` go to the slots of ``meta`` and are left
+    as they are themselves. Both may be views, as ``q``. The cache is of the ``"raw"`` codec in the dtype
+    of the rows. Rows of padding requests are not stored.
+    """
+    op = "kvcache.store_rotated"
+    tensors = (k, v, buffers.k, buffers.v, rotary.turns)
+    if q is not None:
+        tensors += (q, q if q_out is None else q_out)
+    key = ("store_rotated", id(buffers), id(meta), id(rotary), _fastpath.signature(tensors))
+    _replayed(meta, key, (buffers, meta, rotary),
+              lambda record: _store_rotated(op, q, k, v, buffers, meta, rotary, q_out, record))
+
+
+def _store_rotated(op: str, q, k, v, buffers: KVBuffers, meta: AttentionMetadata, rotary: Rotary, q_out, record) -> None:
+    require_buffers(op, buffers)
+    if buffers.codec != RAW_CODEC:
+        raise BackendError(
+            f"{op}: writes the {RAW_CODEC!r} codec, not {str(buffers.codec)!r}: kvcache.rotate and kvcache.store do",
+            context={"op": op, "argument": "buffers"},
+        )
+    device, dtype, width, kv_heads = buffers.k.device, buffers.k.dtype, buffers.head_dim, buffers.num_kv_heads
+    slots = _slots(op, meta, buffers)
+    n_rows = slots.shape[0]
+    for name, rows in (("k", k), ("v", v)):
+        require_rows(op, name, rows, (n_rows, kv_heads, width), dtype, device)
+    heads, q_args = _turned(op, "q", q, q_out, n_rows, width, dtype, device) if q is not None else (0, _NO_ROWS)
+    positions, turn = _rotation(op, meta, rotary, device, width)
+    if n_rows == 0:
+        return
+    _launch(op, _lib.lib().ayk_rotate_and_cache, (
+        *q_args, k.data_ptr(), *k.stride()[:2], 0, 0, 0, v.data_ptr(), *v.stride()[:2], buffers.k.data_ptr(),
+        buffers.v.data_ptr(), positions, slots.data_ptr(), *turn, n_rows, heads, kv_heads, width, buffers.num_blocks,
+        buffers.block_size, _LAYOUT_CODES[KVLayoutKind(buffers.layout)], _ROW_DTYPE_CODES[dtype]), device, record)
+
+
+def store_latent(latent: torch.Tensor, k_rope: torch.Tensor, buffers: LatentBuffers, meta: AttentionMetadata,
+                 rotary: Rotary | None = None, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> None:
+    """Write a step's latents and key parts into a latent cache, rotating the key parts and the queries'.
+
+    Row i of ``latent`` [N, latent_dim] and, rotated by ``meta.positions[i]``, of ``k_rope`` [N, rope_dim]
+    goes to its slot; ``q`` [N, heads, rope_dim], the queries' rotary parts, is rotated in place or
+    into ``q_out`` (the tail of the absorbed queries, say) in the same launch. All may be views whose
+    rows are contiguous. Without ``rotary`` the key parts are stored as they are, and there is no ``q``.
+    Rows of padding requests are not stored.
+    """
+    op = "kvcache.store_latent"
+    tensors = (latent, k_rope, buffers.k)
+    if rotary is not None:
+        tensors += (rotary.turns,)
+    if q is not None:
+        tensors += (q, q if q_out is None else q_out)
+    key = ("store_latent", id(buffers), id(meta), id(rotary), _fastpath.signature(tensors))
+    _replayed(meta, key, (buffers, meta, rotary),
+              lambda record: _store_latent(op, latent, k_rope, buffers, meta, rotary, q, q_out, record))
+
+
+def _store_latent(op: str, latent, k_rope, buffers: LatentBuffers, meta: AttentionMetadata, rotary, q, q_out,
+                  record) -> None:
+    require_latent_buffers(op, buffers)
+    cache, latent_dim, rope_dim = buffers.cache, buffers.latent_dim, buffers.rope_dim
+    device, dtype = cache.device, cache.dtype
+    slots = _slots(op, meta, buffers)
+    n_rows = slots.shape[0]
+    require_rows(op, "latent", latent, (n_rows, latent_dim), dtype, device)
+    require_rows(op, "k_rope", k_rope, (n_rows, rope_dim), dtype, device)
+    if rotary is not None and 2 * rotary.turns.numel() != rope_dim:
+        raise BackendError(f"{op}: the rotation turns {2 * rotary.turns.numel()} elements, key parts have {rope_dim}",
+                           context={"op": op, "argument": "rotary"})
+    if rotary is None and q is not None:
+        raise BackendError(f"{op}: q is given and nothing to rotate it by", context={"op": op, "argument": "q"})
+    heads, q_args = _turned(op, "q", q, q_out, n_rows, rope_dim, dtype, device) if q is not None else (0, _NO_ROWS)
+    positions, turn = _rotation(op, meta, rotary, device, rope_dim)
+    if n_rows == 0:
+        return
+    _launch(op, _lib.lib().ayk_store_latent, (
+        latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0), *q_args, cache.data_ptr(), positions,
+        slots.data_ptr(), *turn, n_rows, heads, latent_dim, rope_dim, buffers.num_blocks, buffers.block_size,
+        _ROW_DTYPE_CODES[dtype]), device, record)
+
+
+def _require_any(op: str, buffers: "KVBuffers | LatentBuffers") -> None:
+    if isinstance(buffers, LatentBuffers):
+        require_latent_buffers(op, buffers)
+    else:
+        require_buffers(op, buffers)
+
+
+def _planes(buffers: "KVBuffers | LatentBuffers") -> tuple[torch.Tensor, torch.Tensor]:
+    """The two caches a block op moves; a latent cache is one, given twice (and moved once)."""
+    return (buffers.cache, buffers.cache) if isinstance(buffers, LatentBuffers) else (buffers.k, buffers.v)
+
+
 def gather(
-    buffers: KVBuffers, block_ids: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
+    buffers: KVBuffers | LatentBuffers, block_ids: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor | None = None,
     out_scales: torch.Tensor | None = None,
 ) -> None:
     """Copy whole blocks out (reference ``torch/kvcache.py:83-93``); a block-scaled cache's codes
-    mean nothing without their scales, which go to ``out_scales`` float32 [n, kv_heads, 2]."""
+    mean nothing without their scales, which go to ``out_scales`` float32 [n, kv_heads, 2]. A latent
+    cache's blocks go to ``out_k``; it has no ``out_v``."""
     op = "kvcache.gather"
-    require_buffers(op, buffers)
+    _require_any(op, buffers)
+    one = isinstance(buffers, LatentBuffers)
+    if one != (out_v is None):
+        raise BackendError(f"{op}: out_v goes with a cache of keys and values, and a latent cache has none",
+                           context={"op": op, "argument": "out_v"})
+    if one:
+        out_v = out_k
     device = buffers.k.device
     _ids(op, "block_ids", block_ids, device)
     shape = (block_ids.shape[0], *buffers.k.shape[1:])
@@ -158,8 +379,7 @@ def gather(
     _lib.check(
         op,
         _lib.lib().ayk_gather_blocks(
-            buffers.k.data_ptr(),
-            buffers.v.data_ptr(),
+            *(t.data_ptr() for t in _planes(buffers)),
             out_k.data_ptr(),
             out_v.data_ptr(),
             block_ids.data_ptr(),
@@ -192,9 +412,9 @@ def _move_scales(op: str, name: str, tensors: tuple[torch.Tensor, ...], ids: tup
     )
 
 
-def copy_blocks(buffers: KVBuffers, src: torch.Tensor, dst: torch.Tensor) -> None:
+def copy_blocks(buffers: KVBuffers | LatentBuffers, src: torch.Tensor, dst: torch.Tensor) -> None:
     op = "kvcache.copy_blocks"
-    require_buffers(op, buffers)
+    _require_any(op, buffers)
     device = buffers.k.device
     _ids(op, "src", src, device)
     _ids(op, "dst", dst, device)
@@ -210,8 +430,7 @@ def copy_blocks(buffers: KVBuffers, src: torch.Tensor, dst: torch.Tensor) -> Non
     _lib.check(
         op,
         _lib.lib().ayk_copy_blocks(
-            buffers.k.data_ptr(),
-            buffers.v.data_ptr(),
+            *(t.data_ptr() for t in _planes(buffers)),
             src.data_ptr(),
             dst.data_ptr(),
             int(src.dtype == torch.int64),
@@ -226,9 +445,9 @@ def copy_blocks(buffers: KVBuffers, src: torch.Tensor, dst: torch.Tensor) -> Non
         _move_scales(op, "ayk_copy_blocks", (scales, scales), (src, dst), scales, device)
 
 
-def zero_blocks(buffers: KVBuffers, block_ids: torch.Tensor) -> None:
+def zero_blocks(buffers: KVBuffers | LatentBuffers, block_ids: torch.Tensor) -> None:
     op = "kvcache.zero_blocks"
-    require_buffers(op, buffers)
+    _require_any(op, buffers)
     device = buffers.k.device
     _ids(op, "block_ids", block_ids, device)
     if block_ids.shape[0] == 0:
@@ -236,8 +455,7 @@ def zero_blocks(buffers: KVBuffers, block_ids: torch.Tensor) -> None:
     _lib.check(
         op,
         _lib.lib().ayk_zero_blocks(
-            buffers.k.data_ptr(),
-            buffers.v.data_ptr(),
+            *(t.data_ptr() for t in _planes(buffers)),
             block_ids.data_ptr(),
             int(block_ids.dtype == torch.int64),
             block_ids.shape[0],

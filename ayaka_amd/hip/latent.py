@@ -1,0 +1,118 @@
+"""Attention over latent caches: the host side of ``attention.attend_latent``.
+
+The launch (``include/ayaka_hip_latent.h``) reads lengths, rows and tables on the device and splits the
+step's contexts there, so an eagerly planned step, a verify window and a captured bucket are the same
+call; the workspace is the one the device's split launches share.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ayaka_amd.attention import AttentionMetadata
+from ayaka_amd.errors import BackendError
+from ayaka_amd.hip import _fastpath, _lib
+from ayaka_amd.hip import attention as _attention
+from ayaka_amd.hip._checks import capturing, dtype_name, require_device, require_latent_buffers, require_like, stream_handle
+from ayaka_amd.kvcache import LatentBuffers
+
+__all__ = ["LATENT_DIMS", "ROPE_DIM", "attend_latent"]
+
+#: Widths of the latent, and of the rotary part, the kernels are built for.
+LATENT_DIMS = frozenset({256, 512})
+ROPE_DIM = 64
+_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _require_latent_step(op: str, q: torch.Tensor, buffers: LatentBuffers, meta: AttentionMetadata, out: torch.Tensor,
+                         width: int, out_width: int) -> int:
+    """The heads of a call of this backend's kernels: cache, step, q [N, heads, width] and out
+    [N, heads, out_width] checked."""
+    require_latent_buffers(op, buffers)
+    cache, table = buffers.cache, meta.block_table
+    if buffers.latent_dim not in LATENT_DIMS or buffers.rope_dim != ROPE_DIM:
+        raise BackendError(
+            f"{op}: the hip kernels are built for latents of {sorted(LATENT_DIMS)} elements and rotary parts of "
+            f"{ROPE_DIM}, not {buffers.latent_dim} and {buffers.rope_dim}",
+            context={"op": op, "argument": "buffers"},
+        )
+    if cache.dtype not in _DTYPE_CODES:
+        raise BackendError(f"{op}: buffers.cache is {dtype_name(cache.dtype)}; over a latent cache the hip backend "
+                           "computes in float16, bfloat16", context={"op": op, "argument": "buffers"})
+    if not isinstance(meta.plan, (_attention.HipAttentionPlan, _attention.HipGraphPlan)) or not isinstance(table, torch.Tensor):
+        raise BackendError(
+            f"{op}: this step was planned by another backend; plan it with the same ops",
+            context={"op": op, "argument": "meta"},
+        )
+    if meta.block_size != buffers.block_size:
+        raise BackendError(
+            f"{op}: the step was planned for blocks of {meta.block_size} positions "
+            f"but the cache has blocks of {buffers.block_size}",
+            context={"op": op, "argument": "meta"},
+        )
+    heads = q.shape[1] if q.ndim == 3 else 0
+    if heads == 0:
+        raise BackendError(f"{op}: q must be [N, heads, {width}], got {list(q.shape)}", context={"op": op, "argument": "q"})
+    n_rows = meta.request_of_row.shape[0]
+    require_like(op, "q", q, (n_rows, heads, width), cache.dtype)
+    require_like(op, "out", out, (n_rows, heads, out_width), cache.dtype)
+    for name, tensor in (("q", q), ("out", out), ("meta.kv_lengths", meta.kv_lengths), ("meta.block_table", table),
+                         ("meta.rows_per_request", meta.rows_per_request)):
+        require_device(op, name, tensor, cache.device)
+    if table.dtype != torch.int32 or not table.is_contiguous() or table.ndim != 2:
+        raise BackendError(f"{op}: meta.block_table must be a contiguous int32 [B, max_blocks] tensor")
+    for name, tensor in (("meta.kv_lengths", meta.kv_lengths), ("meta.rows_per_request", meta.rows_per_request)):
+        require_like(op, name, tensor, (table.shape[0],), torch.int32)
+    return heads
+
+
+def _replayed(meta: AttentionMetadata, key: tuple, keep: tuple, q: torch.Tensor, call) -> None:
+    cache = getattr(meta.plan, "launches", None)
+    if cache is None:
+        call(None)
+        return
+    found = _fastpath.lookup(cache, key)
+    if found is not None:
+        stream = stream_handle(found.device)
+        if found.scratch:
+            _attention._order_scratch(found.device, stream, capturing(q))
+        _fastpath.run(found, stream)
+        return
+    record = _fastpath.Recorder()
+    call(record)
+    _fastpath.remember(cache, key, keep, record)
+
+
+def attend_latent(q: torch.Tensor, buffers: LatentBuffers, meta: AttentionMetadata, out: torch.Tensor, *,
+                  scale: float) -> None:
+    """Attention of every row over its request's latent context, keys and values absorbed.
+
+    ``q`` [N, heads, latent_dim + 64] holds each head's query taken through the keys' matrix, and behind
+    it its rotated part (what ``store_latent`` rotates); the score of a cached row is their product
+    times ``scale``, and ``out`` [N, heads, latent_dim] receives the weighted sum of the latents, for the
+    values' matrix to be applied to. Rows see positions up to their own; padding rows get zeros.
+    Any step serves: decode, verify windows, chunks (``attend_latent_chunks`` does those of many rows
+    with a third of the work per score), graph metadata. Captured after one eager call.
+    """
+    op = "attention.attend_latent"
+    key = ("attend_latent", id(buffers), id(meta), scale, _fastpath.signature((q, out, buffers.k)))
+    _replayed(meta, key, (buffers, meta), q, lambda record: _attend_latent(op, q, buffers, meta, out, scale, record))
+
+
+def _attend_latent(op: str, q: torch.Tensor, buffers: LatentBuffers, meta: AttentionMetadata, out: torch.Tensor,
+                   scale: float, record: "_fastpath.Recorder | None") -> None:
+    require_latent_buffers(op, buffers)
+    heads = _require_latent_step(op, q, buffers, meta, out, buffers.latent_dim + buffers.rope_dim, buffers.latent_dim)
+    cache, table, n_rows = buffers.cache, meta.block_table, q.shape[0]
+    if n_rows == 0:
+        return
+    device, lib = cache.device, _lib.lib()
+    stream, requests = stream_handle(device), table.shape[0]
+    nbytes = lib.ayk_latent_attention_workspace_bytes(n_rows, requests, heads, buffers.latent_dim)
+    scratch = _attention._workspace(op, device, nbytes, capturing(q), stream)
+    _attention._call(op, lib.ayk_latent_attention, (
+        out.data_ptr(), q.data_ptr(), cache.data_ptr(), table.data_ptr(), table.stride(0), meta.kv_lengths.data_ptr(),
+        meta.rows_per_request.data_ptr(), requests, n_rows, heads, buffers.latent_dim, buffers.rope_dim,
+        buffers.num_blocks, buffers.block_size, table.shape[1], _DTYPE_CODES[cache.dtype], float(scale),
+        scratch.data_ptr(), scratch.numel(),
+    ), stream, device, True, record)

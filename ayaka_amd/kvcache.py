@@ -21,6 +21,9 @@ Restates the reference's layout definition (``python/ayaka/ops/kvcache.py:1-38``
   scale and a value scale for every block and key/value head, which the KV write
   settles from the values themselves, so nothing is calibrated and no finite value
   becomes NaN.
+* A latent cache (:class:`LatentBuffers`, layout ``NLD``) is one tensor ``[num_blocks, block_size,
+  latent_dim + rope_dim]`` in the compute dtype: a token's latent vector and, behind it, its rotated
+  key part, shared by all heads. Slots, tables and the padding block are the same.
 
 Importing this module does not import torch.
 """
@@ -35,6 +38,7 @@ if TYPE_CHECKING:
     from torch import Tensor
 
     from ayaka_amd.attention import AttentionMetadata
+    from ayaka_amd.rotary import Rotary
 
 __all__ = [
     "FP8_E4M3_BLOCK_CODEC",
@@ -44,6 +48,8 @@ __all__ = [
     "BlockScaledFp8Codec",
     "KVBuffers",
     "KVCacheOps",
+    "LatentBuffers",
+    "LatentWeights",
     "ScaledFp8Codec",
     "StepTables",
     "codec_scales",
@@ -189,6 +195,53 @@ except ImportError:
     KVBuffers = _KVBuffers  # type: ignore[misc]
 
 
+class LatentBuffers(NamedTuple):
+    """The latent cache of one layer: ``cache`` contiguous ``[num_blocks, block_size, latent_dim +
+    rope_dim]`` in the compute dtype, the latent first."""
+
+    cache: Tensor
+    latent_dim: int
+
+    @property
+    def k(self) -> Tensor:
+        """What scores are taken with: the whole rows."""
+        return self.cache
+
+    @property
+    def v(self) -> Tensor:
+        """What outputs are sums of: the latents, a view."""
+        return self.cache[..., : self.latent_dim]
+
+    @property
+    def layout(self) -> KVLayoutKind:
+        return KVLayoutKind.NLD
+
+    @property
+    def codec(self) -> str:
+        return RAW_CODEC
+
+    @property
+    def num_blocks(self) -> int:
+        return int(self.cache.shape[0])
+
+    @property
+    def block_size(self) -> int:
+        return int(self.cache.shape[1])
+
+    @property
+    def rope_dim(self) -> int:
+        return int(self.cache.shape[2]) - self.latent_dim
+
+
+class LatentWeights(NamedTuple):
+    """What expands a layer's latents into keys and values: head ``h``'s key (without its rotary part)
+    is ``keys[h] @ latent``, its value ``values[h] @ latent``; ``keys`` contiguous ``[heads, nope_dim,
+    latent_dim]``, ``values`` ``[heads, value_dim, latent_dim]``, in the compute dtype."""
+
+    keys: Tensor
+    values: Tensor
+
+
 class BlockPool(NamedTuple):
     """The free blocks a step's requests draw from, in device memory.
 
@@ -233,14 +286,29 @@ class KVCacheOps(Protocol):
 
     def store(self, k: Tensor, v: Tensor, buffers: KVBuffers, meta: AttentionMetadata) -> None: ...
 
+    def rotate(
+        self, q: Tensor | None, k: Tensor | None, meta: AttentionMetadata, rotary: Rotary,
+        q_out: Tensor | None = None, k_out: Tensor | None = None,
+    ) -> None: ...
+
+    def store_rotated(
+        self, q: Tensor | None, k: Tensor, v: Tensor, buffers: KVBuffers, meta: AttentionMetadata,
+        rotary: Rotary, q_out: Tensor | None = None,
+    ) -> None: ...
+
+    def store_latent(
+        self, latent: Tensor, k_rope: Tensor, buffers: LatentBuffers, meta: AttentionMetadata,
+        rotary: Rotary | None = None, q: Tensor | None = None, q_out: Tensor | None = None,
+    ) -> None: ...
+
     def gather(
-        self, buffers: KVBuffers, block_ids: Tensor, out_k: Tensor, out_v: Tensor,
+        self, buffers: KVBuffers | LatentBuffers, block_ids: Tensor, out_k: Tensor, out_v: Tensor | None = None,
         out_scales: Tensor | None = None,
     ) -> None: ...
 
-    def copy_blocks(self, buffers: KVBuffers, src: Tensor, dst: Tensor) -> None: ...
+    def copy_blocks(self, buffers: KVBuffers | LatentBuffers, src: Tensor, dst: Tensor) -> None: ...
 
-    def zero_blocks(self, buffers: KVBuffers, block_ids: Tensor) -> None: ...
+    def zero_blocks(self, buffers: KVBuffers | LatentBuffers, block_ids: Tensor) -> None: ...
 
     def build_tables(
         self, rows_per_request: Tensor, kv_lengths: Tensor, block_table: Tensor, pool: BlockPool,
