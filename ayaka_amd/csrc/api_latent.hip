@@ -207,7 +207,7 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
   const int pairs = ayk::latent_tile_pairs(n_rows, n_requests, num_heads);
   const int64_t positions = (int64_t)max_blocks * block_size;
   const int64_t tiles = (int64_t)n_rows * num_heads / pairs + n_requests;
-  if ((int64_t)n_rows * num_heads > INT32_MAX || positions > INT32_MAX - 64 || tiles * (positions / 32 + 1) > INT32_MAX)
+  if ((int64_t)n_rows * num_heads > INT32_MAX || positions > INT32_MAX - 64 || tiles * (positions / 32 + 8) > INT32_MAX)
     return fail(AYK_ERR_UNSUPPORTED, "%s: %d rows of %d heads over tables of %lld positions exceed one launch", op, n_rows,
                 num_heads, (long long)positions);
   ayk::LatentParams p{};

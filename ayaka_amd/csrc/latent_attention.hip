@@ -8,34 +8,41 @@
 // The rows of a request's queries, [rows x heads, DC + 64], are one contiguous matrix, so any number
 // of rows and heads is cut into tiles of NC consecutive (row, head) pairs; every pair of a tile reads
 // the same context, which a workgroup streams once for all of them. With NC pairs a position of
-// 2 (DC + 64) bytes takes 2 NC (2 DC + 64) operations: at NC 64, DC 512 the matrix cores need a
-// quarter of the time that memory does, so what counts is that loads never pause.
+// 2 (DC + 64) bytes takes 2 NC (2 DC + 64) operations: at DC 512 memory and matrix cores take the
+// same time at about 190 pairs (255 with P.V's two products for bf16 counted once).
 //
-//  * A workgroup (4 waves, one per compute unit) holds 4 chunks of 32 positions in LDS (147 KB):
-//    one being worked on, three on their way, fetched straight into LDS (global_load_lds_dwordx4,
-//    no registers). 110 KB in flight per compute unit cover the latency at the full rate.
+//  * A workgroup (4 waves, one workgroup per compute unit) holds 4 chunks of 32 positions in LDS
+//    (147 KB), fetched straight into it (global_load_lds_dwordx4, no registers), up to three on their
+//    way while one is worked on: 110 KB in flight per compute unit cover the latency at the full rate.
 //  * 16-byte pieces of a row are stored in an order that depends on the position (swizzle), which
 //    keeps both the row-wise reads (q.k) and the transposing ones (P.V) spread over the banks.
-//  * q.k: S^T = K Q^T, v_mfma_f32_16x16x32, keys from LDS, q in registers for the whole tile: a wave
-//    takes 16 of the chunk's positions and half of the pairs.
-//  * P.V: O^T += V^T P^T; the values are the latents already in LDS, read transposed
-//    (ds_read_b64_tr_b16); each wave takes a quarter of DC for all pairs. P goes through LDS, bf16 in
-//    two parts (high and remainder by truncation: one bf16 would lose 2^-9 of each weight, as much as
-//    the output's own rounding), fp16 rounded to nearest (2^-12).
+//  * S^T = K Q^T, then O^T += V^T P^T, v_mfma_f32_16x16x32 with q and O in registers; the values are the
+//    latents already in LDS, read transposed (ds_read_b64_tr_b16). A bf16 P is taken in two parts (high
+//    and remainder by truncation: one bf16 would lose 2^-9 of each weight, as much as the output's own
+//    rounding), an fp16 P rounded to nearest (2^-12).
 //  * The running maximum moves only when a score passes it by kRescaleSlack; until then weights up to
-//    2^kRescaleSlack keep their accuracy, and the waves need no word from each other. When one does,
-//    a flag read after the barrier sends all of them through the exchange of maxima.
+//    2^kRescaleSlack keep their accuracy and nothing is rescaled.
 //
-// Work is split without the host: positions, cut into chunks, of all tiles form one line, and of G
-// workgroups the g-th takes [g T / G, (g + 1) T / G). The lengths are read on the device, so eager
-// steps and replays of a captured one run the same code. A workgroup that begins or ends inside a
-// tile leaves a partial (m, l, O), at most two of them, and latent_merge_kernel joins each cut tile.
+// Two kernels, by what bounds them. Few pairs (16 or 32), latent_shared_kernel: the waves share each
+// chunk, a wave scores 16 positions and 16 pairs and then takes a quarter of DC for all pairs, with the
+// weights exchanged through LDS: small registers, short steps, two barriers a chunk. Many pairs (64 or
+// 128), latent_own_kernel: a wave owns 32 pairs whole, q and O filling its 512 registers, and P goes
+// from the scores to P.V without leaving them; 64 pairs take two waves on one chunk and two on the
+// next, joined at the end, because LDS reads (each wave reads whole chunks) are the limit there.
+//
+// Work is split without the host: the chunks of all tiles, and tile_cost(NC) for each tile's own start and
+// end, form one line, and of G workgroups the g-th takes [g T / G, (g + 1) T / G). The lengths are read
+// on the device, so eager steps and replays of a captured one run the same code. A workgroup that
+// begins or ends inside a tile leaves a partial (m, l, O), at most two of them, and
+// latent_merge_kernel joins each cut tile.
 //
 // Visible and masked: a masked position's weight is an exact 0, and what it multiplies must be
 // finite. Slots behind the context are never read (the last position stands in for them). Rows of one
-// request see different ends; if a raw score in their last chunks is not finite, the chunk's
-// non-finite elements are taken out of the values before P.V: rows that see that position get NaN
-// from its score, the others must not notice.
+// request see different ends; if a raw score in their last chunks is not finite, the non-finite
+// elements are taken out of the values there: rows that see that position get NaN from its score, the
+// others must not notice.
+#include <type_traits>
+
 #include "attention_common.h"
 
 namespace ayk {
@@ -46,13 +53,16 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 namespace {
 
 constexpr int kRope = 64;
-constexpr int kChunk = 32;       // positions
-constexpr int kStages = 4;       // chunks in LDS
-constexpr int kLatentWaves = 4;
-constexpr int kTableWindow = 1024;  // block-table entries in LDS
+constexpr int kChunk = 32;   // positions
+constexpr int kStages = 4;   // chunks in LDS
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kTableWindow = 1024;      // block-table entries in LDS
 constexpr int kPlaceWords = 8;
-// Fewest chunks of one workgroup: a partial's write and merge cost about as much as two chunks.
-constexpr int kLeastChunks = 4;
+// What a tile of NC pairs costs beside its chunks (queries, first loads, output), in chunks.
+constexpr int tile_cost(int nc) { return nc == 64 ? 8 : 5; }
+// Fewest chunks, beside a tile's cost, for one workgroup: as many as a partial's write and merge are worth.
+constexpr int kLeastChunks = 2;
 
 template <bool BF16>
 __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 acc) {
@@ -72,7 +82,7 @@ __device__ __forceinline__ float product(float a, float b) {
   return a * b;
 }
 
-// 16 bytes a lane from base + offset to LDS at `to` + 16 * lane (`to` uniform).
+// 16 bytes a lane from base + offset (or from `at`) to LDS at `to` + 16 * lane (`to` uniform).
 __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, uint32_t offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
@@ -84,76 +94,132 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// Where in a row's 128-byte groups of 8 pieces piece c of position t is: c ^ swizzle(t). Any 8
-// consecutive positions differ, and 4 consecutive ones differ in pairs of pieces.
-__host__ __device__ constexpr int swizzle(int t) { return ((t & 3) << 1) | ((t >> 2) & 1); }
+// Where 16-byte pieces stand in LDS. Its 64 banks serve 16 pieces a cycle, in a 16-byte read those of
+// lanes 0-7 and 24-31, 8-15 and 16-23, and so on (measured: 4.0 cycles a read where these 16 differ
+// modulo 256 bytes, 8.0 where two meet). Piece c of a latent of position t is at c ^ (t % 16) of its
+// row, piece c of a rotary part (rows of 128 bytes) at c ^ (t / 2 % 8), piece c of a pair's weights
+// (rows of 64 bytes) at c ^ (pair / 4 % 4).
+__host__ __device__ constexpr int latent_swizzle(int t) { return t & 15; }
+__host__ __device__ constexpr int rope_swizzle(int t) { return (t >> 1) & 7; }
+__host__ __device__ constexpr int weight_swizzle(int pair) { return (pair >> 2) & 3; }
+
+template <int DC>
+struct Stage {
+  uint16_t latent[kChunk * DC];
+  uint16_t rope[kChunk * kRope];
+};
 
 template <int DC, int NT>
 struct __align__(16) LatentShared {
-  struct Stage {
-    uint16_t latent[kChunk * DC];
-    uint16_t rope[kChunk * kRope];
-  };
-  Stage stage[kStages];
-  // weights [pair][position], 8 bytes of padding a row against bank conflicts
-  uint16_t weight[2][NT * 16 * (kChunk + 8)];
+  Stage<DC> stage[kStages];
+  uint16_t weight[2][NT * 16 * kChunk];  // [pair][position]
   int32_t table[kTableWindow];
   float exchange[2][NT * 16];
   int32_t flag[2];
-  int32_t sums[kLatentWaves][2];
-  int32_t place[kPlaceWords];
+  int32_t sums[kWaves][2];
+  int32_t place[8];
 };
 
-// A workgroup's place in the line of chunks.
-struct Place {
-  int request, tile, chunk, first_row, chunks, rows, total, active;
+__device__ __forceinline__ int length_of(const LatentParams& p, int request) {
+  return max(0, min(p.kv_lengths[request], p.max_len));
+}
+__device__ __forceinline__ int chunks_of(int length) { return max(1, (length + kChunk - 1) / kChunk); }
+
+// Chunks [from, to) of a tile, to be worked on by one workgroup.
+struct Piece {
+  int request, tile, first_row, rows, length;
+  int from, to;
+  bool whole;
 };
 
-// Chunks of the whole step and where workgroup `group` of `groups` begins. Every thread takes a run
-// of requests; two sums over the workgroup's threads find the request that holds the beginning.
-template <int NC, class Shared>
-__device__ __forceinline__ Place find_place(const LatentParams& p, Shared& lds, int group, int groups) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int threads = kLatentWaves * kWave;
-  const int each = (p.n_requests + threads - 1) / threads;
-  const int from = min(p.n_requests, tid * each), to = min(p.n_requests, from + each);
-  auto chunks_of = [&](int b) { return max(1, (max(0, min(p.kv_lengths[b], p.max_len)) + kChunk - 1) / kChunk); };
-  auto items_of = [&](int b, int rows) { return (rows * p.heads + NC - 1) / NC * chunks_of(b); };
-  int items = 0, rows = 0;
-  for (int b = from; b < to; ++b) {
-    const int r = max(0, p.rows[b]);
-    rows += r;
-    items += items_of(b, r);
+// A workgroup's walk along the line of tiles.
+template <int NC>
+struct Walk {
+  int request, tile, unit, first_row, chunks, rows, length;  // the next tile, from its `unit` on
+  int left;                                                   // units
+
+  __device__ __forceinline__ bool next(const LatentParams& p, Piece& piece) {
+    while (left > 0) {
+      const int take = min(chunks + tile_cost(NC) - unit, left);
+      piece.request = request;
+      piece.tile = tile;
+      piece.first_row = first_row;
+      piece.rows = rows;
+      piece.length = length;
+      piece.from = max(0, unit - tile_cost(NC));
+      piece.to = unit + take - tile_cost(NC);
+      piece.whole = piece.from == 0 && piece.to == chunks;
+      left -= take;
+      unit = 0;
+      ++tile;
+      if (left > 0 && tile * NC >= rows * p.heads) {
+        tile = 0;
+        do {
+          first_row += rows;
+          if (++request >= p.n_requests) {  // (the step's numbers changed under the launch)
+            left = 0;
+            break;
+          }
+          rows = max(0, p.rows[request]);
+        } while (rows == 0);
+        if (left > 0) {
+          length = length_of(p, request);
+          chunks = chunks_of(length);
+        }
+      }
+      if (piece.to > piece.from) return true;
+    }
+    return false;
   }
-  int items_upto = items, rows_upto = rows;
+};
+
+// Where workgroup `group` of `groups` begins. Every thread takes a run of requests; two sums over the
+// workgroup's threads find the request that holds the beginning. False: no work.
+template <int NC, class Shared>
+__device__ __forceinline__ bool find_place(const LatentParams& p, Shared& lds, int group, int groups, Walk<NC>& walk) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (p.n_requests + kThreads - 1) / kThreads;
+  const int from = min(p.n_requests, tid * each), to = min(p.n_requests, from + each);
+  auto units_of = [&](int length, int rows) { return (rows * p.heads + NC - 1) / NC * (chunks_of(length) + tile_cost(NC)); };
+  int units = 0, rows = 0, first_rows = 0, first_length = 0;
+  for (int b = from; b < to; ++b) {
+    const int r = max(0, p.rows[b]), length = length_of(p, b);
+    if (b == from) first_rows = r, first_length = length;
+    rows += r;
+    units += units_of(length, r);
+  }
+  int units_upto = units, rows_upto = rows;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int a = __shfl_up(items_upto, d), c = __shfl_up(rows_upto, d);
-    if (lane >= d) items_upto += a, rows_upto += c;
+    const int a = __shfl_up(units_upto, d), c = __shfl_up(rows_upto, d);
+    if (lane >= d) units_upto += a, rows_upto += c;
   }
-  if (lane == 63) lds.sums[wave][0] = items_upto, lds.sums[wave][1] = rows_upto;
+  if (lane == 63) lds.sums[wave][0] = units_upto, lds.sums[wave][1] = rows_upto;
   __syncthreads();
   int total = 0;
 #pragma unroll
-  for (int w = 0; w < kLatentWaves; ++w) {
-    if (w < wave) items_upto += lds.sums[w][0], rows_upto += lds.sums[w][1];
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) units_upto += lds.sums[w][0], rows_upto += lds.sums[w][1];
     total += lds.sums[w][0];
   }
-  const int active = max(1, min(groups, total / kLeastChunks));
-  const int begin = (int)((int64_t)min(group, active) * total / active);
-  int before = items_upto - items;
-  if (begin >= before && begin < items_upto) {
+  const int active = max(1, min(groups, total / (tile_cost(NC) + kLeastChunks)));
+  auto begin_of = [&](int i) { return (int)((int64_t)i * total / active); };
+  const int begin = begin_of(min(group, active));
+  int before = units_upto - units;
+  if (begin >= before && begin < units_upto) {
     int row = rows_upto - rows;
     for (int b = from; b < to; ++b) {
-      const int r = max(0, p.rows[b]), n = items_of(b, r);
+      const int r = b == from ? first_rows : max(0, p.rows[b]);
+      const int length = b == from ? first_length : length_of(p, b);
+      const int n = units_of(length, r), tile = chunks_of(length) + tile_cost(NC);
       if (begin < before + n) {
-        const int c = chunks_of(b);
         lds.place[0] = b;
-        lds.place[1] = (begin - before) / c;
-        lds.place[2] = (begin - before) % c;
+        lds.place[1] = (begin - before) / tile;
+        lds.place[2] = (begin - before) % tile;
         lds.place[3] = row;
-        lds.place[4] = c;
+        lds.place[4] = chunks_of(length);
         lds.place[5] = r;
+        lds.place[6] = length;
         break;
       }
       before += n;
@@ -162,328 +228,387 @@ __device__ __forceinline__ Place find_place(const LatentParams& p, Shared& lds, 
   }
   __syncthreads();
   auto uniform = [&](int i) { return __builtin_amdgcn_readfirstlane(lds.place[i]); };
-  return Place{uniform(0), uniform(1), uniform(2), uniform(3), uniform(4), uniform(5), total, active};
+  walk.request = uniform(0);
+  walk.tile = uniform(1);
+  walk.unit = uniform(2);
+  walk.first_row = uniform(3);
+  walk.chunks = uniform(4);
+  walk.rows = uniform(5);
+  walk.length = uniform(6);
+  walk.left = begin_of(group + 1) - begin;
+  const bool some = group < active && total > 0;
+  if (group < active && tid == 0) {  // for the merge
+    int32_t* place = p.places + group * kPlaceWords;
+    place[0] = walk.tile;
+    place[1] = max(0, walk.unit - tile_cost(NC));
+    place[2] = walk.first_row;
+    place[3] = walk.chunks;
+    place[4] = walk.rows;
+    place[5] = total;
+    place[6] = active;
+  }
+  return some;
+}
+
+// A piece's geometry.
+struct Tile {
+  int first_pos;   // of the request's first row
+  int context;     // positions that some pair sees
+  int least_pos;   // what every pair sees: up to and with this position
+  int to;          // chunks from piece.from to here hold any of them
+  int pairs;       // of this tile, as far as there are rows
+  int64_t pair0;
+};
+
+template <int NC>
+__device__ __forceinline__ Tile tile_of(const LatentParams& p, const Piece& piece) {
+  Tile t;
+  const int pair = piece.tile * NC;
+  t.first_pos = piece.length - piece.rows;
+  t.pair0 = (int64_t)piece.first_row * p.heads + pair;
+  const int pairs = min(piece.rows * p.heads - pair, NC);
+  t.pairs = (int)max((int64_t)0, min((int64_t)pairs, (int64_t)p.n_rows * p.heads - t.pair0));
+  t.context = piece.length == 0 ? 0 : max(0, min(piece.length, t.first_pos + (pair + pairs - 1) / p.heads + 1));
+  t.least_pos = t.first_pos + pair / p.heads;
+  t.to = min(piece.to, (t.context + kChunk - 1) / kChunk);
+  return t;
+}
+
+// The chunks [w0, w1) whose blocks fit the table window, and the first of those blocks.
+struct Window {
+  int b0, blocks, w1;
+};
+__device__ __forceinline__ Window window_of(const LatentParams& p, const Tile& t, int w0) {
+  Window w;
+  w.b0 = (int)quotient((uint32_t)(w0 * kChunk), p.by_block);
+  const int last = (int)quotient((uint32_t)(min(t.to * kChunk, t.context) - 1), p.by_block);
+  w.blocks = min(kTableWindow, last - w.b0 + 1);
+  w.w1 = w.b0 + w.blocks > last ? t.to : (w.b0 + w.blocks) * p.block_size / kChunk;
+  return w;
+}
+
+__device__ __forceinline__ void stage_table(const LatentParams& p, int request, const Window& w, int32_t* s_table) {
+  const int32_t* table = p.block_table + request * p.table_stride + w.b0;
+  for (int i = threadIdx.x; i < w.blocks; i += kThreads) {
+    const uint32_t id = (uint32_t)table[i];
+    s_table[i] = id < (uint32_t)p.num_blocks ? (int)id : 0;
+  }
+}
+
+// The slot of position first + lane % MINE; positions past `last` are replaced by it.
+template <int MINE>
+__device__ __forceinline__ uint32_t slot_of(const LatentParams& p, const int32_t* s_table, int b0, int first, int last) {
+  const int pos = min(first + (int)(threadIdx.x & (MINE - 1)), last);
+  const uint32_t block = quotient((uint32_t)pos, p.by_block);
+  return (uint32_t)s_table[block - b0] * (uint32_t)p.block_size + ((uint32_t)pos - block * (uint32_t)p.block_size);
+}
+
+// Ask for a share of a chunk (of several waves `wave`): MINE rows of latents, 1024 bytes a load, and one load of their
+// rotary parts, 8 lanes a position.
+template <int DC, int MINE>
+__device__ __forceinline__ void fetch(const LatentParams& p, uint32_t slot, int wave, uint32_t stage) {
+  static_assert(MINE <= 8, "a load of rotary parts covers 8 positions");
+  constexpr int ROW = (DC + kRope) * 2;
+  constexpr int PER_LOAD = 1024 / (DC * 2);
+  const int lane = threadIdx.x & 63, first = wave * MINE;
+  const uint8_t* cache = reinterpret_cast<const uint8_t*>(p.cache);
+#pragma unroll
+  for (int j = 0; j < MINE / PER_LOAD; ++j) {
+    const uint32_t to = stage + (uint32_t)((first + j * PER_LOAD) * DC * 2);
+    if constexpr (PER_LOAD == 1) {
+      const uint32_t s = __builtin_amdgcn_readlane(slot, j);
+      load_to_lds(to, cache + (uint64_t)s * ROW, (uint32_t)((lane ^ latent_swizzle(first + j)) * 16));
+    } else {
+      const uint32_t s0 = __builtin_amdgcn_readlane(slot, 2 * j), s1 = __builtin_amdgcn_readlane(slot, 2 * j + 1);
+      const int piece = (lane & 31) ^ latent_swizzle(first + 2 * j + (lane >> 5));
+      load_to_lds(to, cache + (uint64_t)(lane < 32 ? s0 : s1) * ROW + piece * 16);
+    }
+  }
+  const uint32_t s = (uint32_t)__shfl((int)slot, lane >> 3);
+  if (MINE == 8 || lane < MINE * 8)
+    load_to_lds(stage + (uint32_t)(kChunk * DC * 2 + first * kRope * 2),
+                cache + (uint64_t)s * ROW + (DC * 2 + ((lane & 7) ^ rope_swizzle(first + (lane >> 3))) * 16));
+}
+
+// The queries of pair `pair` of a tile as MFMA operands (zeros where there is none): 8 elements of
+// each 32 for every lane of the pair's column.
+template <int DC, int N>
+__device__ __forceinline__ void load_query(const LatentParams& p, const Tile& t, int pair, u32x4 (&q)[N]) {
+  const int mq = (threadIdx.x >> 4) & 3;
+  const u32x4* from = reinterpret_cast<const u32x4*>(p.q + (pair < t.pairs ? t.pair0 + pair : 0) * (DC + kRope)) + mq;
+#pragma unroll
+  for (int s = 0; s < N; ++s) q[s] = from[4 * s];
+}
+template <int N>
+__device__ __forceinline__ void drop_query(bool real, u32x4 (&q)[N]) {
+  if (!real) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) q[s] = u32x4{0, 0, 0, 0};
+  }
+}
+// Said to the compiler, not only to the hardware: it would otherwise wait for the queries, and with
+// them for every chunk on its way, at each of their uses.
+__device__ __forceinline__ void queries_are_here() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt 0
+
+// N operands from LDS, each used by products: read in groups of G, one group ahead of the products.
+// (Left alone, the compiler reads one operand, waits for it and multiplies, and with one wave on a
+// SIMD nothing else fills the wait: a chunk of 32 positions and 16 pairs took 1.5 us so.)
+template <int N, int G, class Read, class Use>
+__device__ __forceinline__ void read_ahead(Read read, Use use) {
+  static_assert(N % G == 0, "whole groups");
+  u32x4 a[2][G];
+#pragma unroll
+  for (int i = 0; i < G; ++i) a[0][i] = read(i);
+#pragma unroll
+  for (int g = 0; g < N / G; ++g) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      if ((g + 1) * G + i < N) a[(g + 1) & 1][i] = read((g + 1) * G + i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < G; ++i) use(g * G + i, a[g & 1][i]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Non-finite elements of a word of two, replaced by zeros.
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite_word(uint32_t w) {
+  constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+  if ((w & EXP) == EXP) w &= 0xffff0000u;
+  if (((w >> 16) & EXP) == EXP) w &= 0xffffu;
+  return w;
+}
+
+// Four elements of an output, or of a partial output.
+template <bool BF16>
+__device__ __forceinline__ void put_output(uint16_t* out, f32x4 o, float by) {
+  u32x2 two;
+  two.x = Elem<BF16>::round(o[0] * by) | Elem<BF16>::round(o[1] * by) << 16;
+  two.y = Elem<BF16>::round(o[2] * by) | Elem<BF16>::round(o[3] * by) << 16;
+  *reinterpret_cast<u32x2*>(out) = two;
 }
 
 template <int DC, bool BF16, int NT>
-__global__ __launch_bounds__(kLatentWaves* kWave, 1) void latent_attention_kernel(const LatentParams p) {
+__global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const LatentParams p) {
   constexpr int NC = NT * 16;
-  constexpr int ROW = DC + kRope;
-  constexpr int KS = DC / 32;          // steps of q.k over the latent; two more over the rotary part
-  constexpr int NQ = NT == 4 ? 2 : 1;  // 16-pair tiles of a wave's q.k
-  constexpr int DT = DC / kLatentWaves / 16;  // 16-element slices of a wave's P.V
-  constexpr int ROWS_PER_LOAD = 1024 / (DC * 2);
-  constexpr int LOADS = 8 / ROWS_PER_LOAD + 1;  // a wave's per chunk
+  constexpr int KS = DC / 32;       // steps of q.k over the latent; two more over the rotary part
+  constexpr int SLICE = DC / kWaves;     // elements of a wave's P.V
+  constexpr int DT = SLICE / 16;
+  // Waves that score (2 for each 16 pairs) and waves that fetch: the last four, which have no scores
+  // up to 32 pairs, or all.
+  constexpr int SCORING = 2 * NT;
+  constexpr int FETCHING = NT == 4 ? kWaves : 4;
+  constexpr int MINE = kChunk / FETCHING;  // positions of a chunk that a wave fetches
+  constexpr int LOADS = MINE * DC * 2 / 1024 + 1;
   typedef LatentShared<DC, NT> Shared;
   __shared__ Shared lds;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int mt = lane & 15, mq = lane >> 4;
-  const int kg = wave & 1, half = wave >> 1;  // q.k: positions 16 kg .., tiles NQ half ..
-  const bool scores = NT > 1 || half == 0;
-  const int groups = gridDim.x, group = blockIdx.x;
+  const int kg = wave & 1, ct = wave >> 1;  // scores: positions 16 kg .. of the chunk, pairs 16 ct ..
+  const bool scores = wave < SCORING;
+  const int fetching = wave - (kWaves - FETCHING);  // which of those waves, below 0: none
 
-  Place at = find_place<NC>(p, lds, group, groups);
-  if (group < at.active && tid < kPlaceWords) {
-    const int words[kPlaceWords] = {at.request, at.tile, at.chunk, at.first_row, at.chunks, at.rows, at.total, at.active};
-    int w = words[0];
-#pragma unroll
-    for (int i = 1; i < kPlaceWords; ++i) w = tid == i ? words[i] : w;
-    p.places[group * kPlaceWords + tid] = w;
-  }
-  if (group >= at.active || at.total == 0) return;
-  const int begin = (int)((int64_t)group * at.total / at.active);
-  int left = (int)((int64_t)(group + 1) * at.total / at.active) - begin;
+  Walk<NC> walk;
+  if (!find_place<NC>(p, lds, blockIdx.x, gridDim.x, walk)) return;
 
   const uint32_t lds_base = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) Shared*)&lds);
   // a lane's offsets into a stage (bytes)
   const int key = kg * 16 + mt;
-  int k_at[2], v_at[4];
+  int k_at[4], r_at[2], v_at[DT];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) k_at[i] = ((4 * i + mq) ^ swizzle(key)) * 16;
+  for (int i = 0; i < 4; ++i) k_at[i] = key * DC * 2 + ((4 * i + mq) ^ latent_swizzle(key)) * 16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = 4 * mq + (mt >> 2);
-    v_at[i] = t * DC * 2 + wave * (DC / kLatentWaves) * 2 + ((2 * i + ((mt & 3) >> 1)) ^ swizzle(t)) * 16 + (mt & 1) * 8;
+  for (int i = 0; i < 2; ++i) r_at[i] = kChunk * DC * 2 + key * kRope * 2 + ((4 * i + mq) ^ rope_swizzle(key)) * 16;
+#pragma unroll
+  for (int i = 0; i < DT; ++i) {
+    const int t = 4 * mq + (mt >> 2), piece = wave * (SLICE / 8) + 2 * i + ((mt & 3) >> 1);
+    v_at[i] = t * DC * 2 + (piece >> 4) * 256 + ((piece & 15) ^ latent_swizzle(t)) * 16 + (mt & 1) * 8;
   }
-  // what this wave fetches: positions 8 wave .. 8 wave + 7 of each chunk
-  const uint32_t rope_from = DC * 2 + ((lane & 7) ^ swizzle(lane >> 3)) * 16;
 
-  while (left > 0) {
-    // --- one tile, chunks [at.chunk, end) of it
-    const int end = min(at.chunks, at.chunk + left);
-    const bool whole = at.chunk == 0 && end == at.chunks;
-    const int pairs = min(at.rows * p.heads - at.tile * NC, NC);
-    const int length = max(0, min(p.kv_lengths[at.request], p.max_len));
-    const int first_pos = length - at.rows;
-    // the last row of the tile sees the most
-    const int context = length == 0 ? 0 : max(0, min(length, first_pos + (at.tile * NC + pairs - 1) / p.heads + 1));
-    const int from = at.chunk, to = min(end, (context + kChunk - 1) / kChunk);
-    // rows from here on are not seen by every pair
-    const int least_pos = first_pos + at.tile * NC / p.heads;
-    const int64_t pair0 = (int64_t)at.first_row * p.heads + at.tile * NC;
-    const int64_t pairs_left = (int64_t)p.n_rows * p.heads - pair0;  // (row counts that disagree stay in bounds)
-
-    int my_pos[NQ];
-    u32x4 q[NQ][KS + 2];
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      const int c = (half * NQ + j) * 16 + mt;
-      const bool real = scores && c < pairs && c < pairs_left;
-      my_pos[j] = real ? first_pos + (at.tile * NC + c) / p.heads : -1;
-      const u32x4* from_q = reinterpret_cast<const u32x4*>(p.q + (pair0 + (real ? c : 0)) * ROW) + mq;
-#pragma unroll
-      for (int s = 0; s < KS + 2; ++s) q[j][s] = real ? from_q[4 * s] : u32x4{0, 0, 0, 0};
-    }
+  Piece piece;
+  while (walk.next(p, piece)) {
+    const Tile tile = tile_of<NC>(p, piece);
+    const int my_pair = ct * 16 + mt;
+    const bool real = scores && my_pair < tile.pairs;
+    const int my_pos = real ? tile.first_pos + (piece.tile * NC + my_pair) / p.heads : -1;
+    u32x4 q[KS + 2];
     f32x4 o[DT][NT];
-    float m[NT], l[NQ];
+    float m[NT], my_m = -INFINITY, l = 0.f;  // of every pair; of my_pair, with its sum over this wave's positions
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       m[c] = -INFINITY;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) l[j] = 0.f;
 
-    const int32_t* table = p.block_table + at.request * p.table_stride;
-    for (int w0 = from; w0 < to;) {
-      // --- a window of the block table
-      const int b0 = (int)quotient((uint32_t)(w0 * kChunk), p.by_block);
-      const int last_block = (int)quotient((uint32_t)(min(to * kChunk, context) - 1), p.by_block);
-      const int blocks = min(kTableWindow, last_block - b0 + 1);
-      // whole chunks that its blocks cover
-      const int w1 = b0 + blocks > last_block ? to : (b0 + blocks) * p.block_size / kChunk;
+    for (int w0 = piece.from; w0 < tile.to;) {
+      const Window win = window_of(p, tile, w0);
       __syncthreads();
-      for (int i = tid; i < blocks; i += kLatentWaves * kWave) {
-        const uint32_t id = (uint32_t)table[b0 + i];
-        lds.table[i] = id < (uint32_t)p.num_blocks ? (int)id : 0;
-      }
+      stage_table(p, piece.request, win, lds.table);
       if (tid < 2) lds.flag[tid] = 0;
       __syncthreads();
-
-      auto fetch = [&](int chunk) {
-        const int pos = min(chunk * kChunk + wave * 8 + (lane & 7), context - 1);
-        const uint32_t block = quotient((uint32_t)pos, p.by_block);
-        const uint32_t slot = (uint32_t)lds.table[block - b0] * (uint32_t)p.block_size + ((uint32_t)pos - block * (uint32_t)p.block_size);
-        const uint32_t stage = lds_base + (uint32_t)((chunk & (kStages - 1)) * sizeof(typename Shared::Stage));
-        const uint8_t* cache = reinterpret_cast<const uint8_t*>(p.cache);
-#pragma unroll
-        for (int j = 0; j < 8 / ROWS_PER_LOAD; ++j) {
-          const uint32_t lds_to = stage + (uint32_t)((wave * 8 + j * ROWS_PER_LOAD) * DC * 2);
-          if constexpr (ROWS_PER_LOAD == 1) {
-            const uint32_t s = __builtin_amdgcn_readlane(slot, j);
-            load_to_lds(lds_to, cache + (uint64_t)s * (ROW * 2), (uint32_t)((lane ^ swizzle(j)) * 16));
-          } else {
-            const uint32_t s0 = __builtin_amdgcn_readlane(slot, 2 * j), s1 = __builtin_amdgcn_readlane(slot, 2 * j + 1);
-            const uint32_t s = lane < 32 ? s0 : s1;
-            const int piece = (lane & 31) ^ (lane < 32 ? swizzle(2 * j) : swizzle(2 * j + 1));
-            load_to_lds(lds_to, cache + (uint64_t)s * (ROW * 2) + piece * 16);
-          }
-        }
-        const uint32_t s = (uint32_t)__shfl((int)slot, lane >> 3);
-        load_to_lds(stage + (uint32_t)(kChunk * DC * 2 + wave * 8 * kRope * 2), cache + (uint64_t)s * (ROW * 2) + rope_from);
+      uint32_t slot = 0;  // of the next chunk to ask for, looked up ahead
+      auto look_up = [&](int chunk) {
+        if (chunk < win.w1)
+          slot = slot_of<MINE>(p, lds.table, win.b0, chunk * kChunk + fetching * MINE, tile.context - 1);
       };
-
+      auto get = [&](int chunk) {
+        fetch<DC, MINE>(p, slot, fetching, lds_base + (uint32_t)((chunk & (kStages - 1)) * sizeof(Stage<DC>)));
+        look_up(chunk + 1);
+      };
+      if (fetching >= 0) {
+        look_up(w0);
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i)
-        if (w0 + i < w1) fetch(w0 + i);
+        for (int i = 0; i < kStages - 1; ++i)
+          if (w0 + i < win.w1) get(w0 + i);
+      }
+      if (scores && w0 == piece.from) load_query<DC>(p, tile, real ? my_pair : NC, q);
+      if (scores) queries_are_here();
+      drop_query(real, q);
 
-      for (int chunk = w0; chunk < w1; ++chunk) {
-        const uint8_t* stage = reinterpret_cast<const uint8_t*>(&lds.stage[chunk & (kStages - 1)]);
-        if (chunk + 2 < w1) wait_loads<2 * LOADS>();
-        else if (chunk + 1 < w1) wait_loads<LOADS>();
-        else wait_loads<0>();
+      for (int chunk = w0; chunk < win.w1; ++chunk) {
+        uint8_t* stage = reinterpret_cast<uint8_t*>(&lds.stage[chunk & (kStages - 1)]);
+        if (fetching >= 0) {
+          if (chunk + 2 < win.w1) wait_loads<2 * LOADS>();
+          else if (chunk + 1 < win.w1) wait_loads<LOADS>();
+          else wait_loads<0>();
+        }
         lds_barrier();  // the chunk is here, and nobody works on the one before it
-        if (chunk + kStages - 1 < w1) fetch(chunk + kStages - 1);
+        // Of two waves of a SIMD that both fetch, one does so before its scores and one after them.
+        const bool more = fetching >= 0 && chunk + kStages - 1 < win.w1;
+        const bool early = more && (NT < 4 || wave < 4), late = more && !early;
+        if (early) get(chunk + kStages - 1);
         if (tid == 0) lds.flag[(chunk + 1) & 1] = 0;
 
         const int t0 = chunk * kChunk;
-        const bool masked = t0 + kChunk > context || t0 + kChunk - 1 > least_pos;
-        f32x4 s[NQ];
-        float before[NQ];  // the sums without this chunk
-        // weights of this wave's scores under the maximum m
-        auto put_weights = [&] {
+        const bool masked = t0 + kChunk > tile.context || t0 + kChunk - 1 > tile.least_pos;
+        f32x4 s{0.f, 0.f, 0.f, 0.f};
+        const float before = l;  // the sum without this chunk
+        // weights of this wave's scores under the maximum my_m, on top of the sum `so_far`
+        auto put_weights = [&](float so_far) {
+          const float base = my_m == -INFINITY ? 0.f : my_m;
+          float w[4];
 #pragma unroll
-          for (int j = 0; j < NQ; ++j) {
-            const float mj = NT == 4 ? (half ? m[(NT == 4 ? 2 : 0) + j] : m[j]) : NT == 2 ? (half ? m[NT - 1] : m[0]) : m[0];
-            const float base = mj == -INFINITY ? 0.f : mj;
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[j][i] - base);
-            l[j] = before[j] + ((w[0] + w[1]) + (w[2] + w[3]));
-            u32x2 hi, lo;
-            split_weights4<BF16>(w, hi, lo);
-            const int row = ((half * NQ + j) * 16 + mt) * (kChunk + 8) + 8 * mq + 4 * kg;
-            *reinterpret_cast<u32x2*>(&lds.weight[0][row]) = hi;
-            if constexpr (split_p(BF16)) *reinterpret_cast<u32x2*>(&lds.weight[1][row]) = lo;
-          }
+          for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[i] - base);
+          l = so_far + ((w[0] + w[1]) + (w[2] + w[3]));
+          u32x2 hi, lo;
+          split_weights4<BF16>(w, hi, lo);
+          const int row = my_pair * kChunk + (mq ^ weight_swizzle(my_pair)) * 8 + 4 * kg;
+          *reinterpret_cast<u32x2*>(&lds.weight[0][row]) = hi;
+          if constexpr (split_p(BF16)) *reinterpret_cast<u32x2*>(&lds.weight[1][row]) = lo;
         };
         if (scores) {
-#pragma unroll
-          for (int j = 0; j < NQ; ++j) {
-            s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            before[j] = l[j];
-          }
-          const uint8_t* row = stage + key * DC * 2;
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(row + (k >> 1) * 128 + k_at[k & 1]);
-#pragma unroll
-            for (int j = 0; j < NQ; ++j) s[j] = mfma32<BF16>(a, q[j][k], s[j]);
-          }
-          const uint8_t* tail = stage + kChunk * DC * 2 + key * kRope * 2;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(tail + k_at[k]);
-#pragma unroll
-            for (int j = 0; j < NQ; ++j) s[j] = mfma32<BF16>(a, q[j][KS + k], s[j]);
-          }
+          f32x4 t{0.f, 0.f, 0.f, 0.f};  // (two sums: one would be a chain of products that wait for each other)
+          read_ahead<KS + 2, KS != 16 ? 5 : NT == 4 ? 2 : 6>(
+              [&](int k) {
+                return *reinterpret_cast<const u32x4*>(stage + (k < KS ? k_at[k & 3] + (k >> 2) * 256 : r_at[k & 1]));
+              },
+              [&](int k, u32x4 a) {
+                if (k & 1) t = mfma32<BF16>(a, q[k], t);
+                else s = mfma32<BF16>(a, q[k], s);
+              });
+          s += t;
           bool passes = false, odd = false;
+          const int seen = min(my_pos, tile.context - 1) - t0 - kg * 16 - 4 * mq;  // of the lane's 4 positions: i <= seen
 #pragma unroll
-          for (int j = 0; j < NQ; ++j) {
-            const float mj = NT == 4 ? (half ? m[(NT == 4 ? 2 : 0) + j] : m[j]) : NT == 2 ? (half ? m[NT - 1] : m[0]) : m[0];
-            const int seen = min(my_pos[j], context - 1) - t0 - kg * 16 - 4 * mq;  // position i of the lane's 4: i <= seen
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (masked) odd |= !(__builtin_fabsf(s[j][i]) < INFINITY);
-              const float t = product(s[j][i], p.scale_log2);
-              s[j][i] = !masked || i <= seen ? t : -INFINITY;
-              passes |= s[j][i] > mj + kRescaleSlack;
-            }
+          for (int i = 0; i < 4; ++i) {
+            if (masked) odd |= !(__builtin_fabsf(s[i]) < INFINITY);
+            const float t = product(s[i], p.scale_log2);
+            s[i] = !masked || i <= seen ? t : -INFINITY;
+            passes |= s[i] > my_m + kRescaleSlack;
           }
           const int word = (__builtin_amdgcn_ballot_w64(passes) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(odd) ? 2 : 0);
           if (word && lane == 0) atomicOr(&lds.flag[chunk & 1], word);
-          put_weights();
+          put_weights(before);
         }
+        if (late) get(chunk + kStages - 1);
+        // this wave's values, on their way while it waits for the weights
+        u32x4 v[DT];
+        auto read_values = [&] {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const uint16_t* at = reinterpret_cast<const uint16_t*>(stage + v_at[d]);
+            const u32x2 a = lds_read_transposed(at), b = lds_read_transposed(at + 16 * DC);
+            v[d] = u32x4{a.x, a.y, b.x, b.y};
+          }
+        };
+        read_values();
         lds_barrier();
         const int word = __builtin_amdgcn_readfirstlane(lds.flag[chunk & 1]);
         if (word) {
           if (word & 2) {
-            // this wave's slice of the values: 32 positions x DC / 4 elements, in 16-byte pieces
-            uint8_t* mine = const_cast<uint8_t*>(stage) + wave * (DC / kLatentWaves) * 2;
-            constexpr int PIECES = DC / kLatentWaves / 8;
-            for (int i = lane; i < kChunk * PIECES; i += kWave) {
-              uint32_t* x = reinterpret_cast<uint32_t*>(mine + (i / PIECES) * DC * 2 + (i % PIECES) * 16);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-                uint32_t w = x[e];
-                if ((w & EXP) == EXP) w &= 0xffff0000u;
-                if (((w >> 16) & EXP) == EXP) w &= 0xffffu;
-                x[e] = w;
-              }
-            }
+            // a share of the chunk's values (all of them are clean behind the next barrier)
+            uint32_t* mine = reinterpret_cast<uint32_t*>(stage) + wave * (kChunk / kWaves) * DC / 2;
+            for (int i = lane; i < kChunk / kWaves * DC / 2; i += kWave) mine[i] = finite_word<BF16>(mine[i]);
           }
           // every pair's maximum over the chunk, then the state and the weights under the new one
           if (scores) {
-#pragma unroll
-            for (int j = 0; j < NQ; ++j) {
-              const float top = column_max(fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
-              if (mq == 0) lds.exchange[kg][(half * NQ + j) * 16 + mt] = top;
-            }
+            const float top = column_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+            if (mq == 0) lds.exchange[kg][my_pair] = top;
           }
           lds_barrier();
-          float by[NT];
+          float by = 1.f;  // of my_pair
 #pragma unroll
           for (int c = 0; c < NT; ++c) {
             const float top = fmaxf(m[c], fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]));
-            by[c] = top == m[c] ? 1.f : fast_exp2(m[c] - top);
+            const float b = top == m[c] ? 1.f : fast_exp2(m[c] - top);
             m[c] = top;
+            if (c == ct) my_m = top, by = b;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][c] *= by[c];
+            for (int d = 0; d < DT; ++d) o[d][c] *= b;
           }
-          if (scores) {
-#pragma unroll
-            for (int j = 0; j < NQ; ++j) {
-              const float b = NT == 4 ? (half ? by[(NT == 4 ? 2 : 0) + j] : by[j]) : NT == 2 ? (half ? by[NT - 1] : by[0]) : by[0];
-              before[j] *= b;
-            }
-            put_weights();
-          }
+          if (scores) put_weights(before * by);
           lds_barrier();
+          if (word & 2) read_values();
         }
         // O^T += V^T P^T
-        u32x4 w[2][NT];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-          const int row = (c * 16 + mt) * (kChunk + 8) + 8 * mq;
-          w[0][c] = *reinterpret_cast<const u32x4*>(&lds.weight[0][row]);
-          if constexpr (split_p(BF16)) w[1][c] = *reinterpret_cast<const u32x4*>(&lds.weight[1][row]);
-        }
+          const int row = (c * 16 + mt) * kChunk + (mq ^ weight_swizzle(mt)) * 8;
+          const u32x4 hi = *reinterpret_cast<const u32x4*>(&lds.weight[0][row]);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const uint16_t* v = reinterpret_cast<const uint16_t*>(stage + v_at[d & 3] + (d >> 2) * 128);
-          const u32x2 a = lds_read_transposed(v), b = lds_read_transposed(v + 16 * DC);
-          const u32x4 va = u32x4{a.x, a.y, b.x, b.y};
+          for (int d = 0; d < DT; ++d) o[d][c] = mfma32<BF16>(v[d], hi, o[d][c]);
+          if constexpr (split_p(BF16)) {
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(&lds.weight[1][row]);
 #pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            o[d][c] = mfma32<BF16>(va, w[0][c], o[d][c]);
-            if constexpr (split_p(BF16)) o[d][c] = mfma32<BF16>(va, w[1][c], o[d][c]);
+            for (int d = 0; d < DT; ++d) o[d][c] = mfma32<BF16>(v[d], lo, o[d][c]);
           }
         }
       }
-      w0 = w1;
+      w0 = win.w1;
     }
 
     // --- the tile's sums, and its output or this workgroup's part of it
-    if (scores) {
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        float sum = l[j];
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        l[j] = sum;
-      }
-    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
     lds_barrier();  // the exchange may still be read
-    if (scores && mq == 0) {
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) lds.exchange[kg][(half * NQ + j) * 16 + mt] = l[j];
-    }
+    if (scores && mq == 0) lds.exchange[kg][my_pair] = l;
     lds_barrier();
-    const int slot = 2 * group + (at.chunk == 0 ? 1 : 0);
+    const int slot = 2 * blockIdx.x + (piece.from == 0 ? 1 : 0);
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       const int pair = c * 16 + mt;
       const float sum = lds.exchange[0][pair] + lds.exchange[1][pair];
-      if (pair < pairs && pair < pairs_left) {
-        const int e0 = wave * (DC / kLatentWaves) + 4 * mq;
-        if (whole) {
-          const float by = sum == 0.f ? 0.f : 1.f / sum;
-          uint16_t* out = static_cast<uint16_t*>(p.out) + (pair0 + pair) * DC + e0;
+      if (pair >= tile.pairs) continue;
+      const int e0 = wave * SLICE + 4 * mq;
+      if (piece.whole) {
+        const float by = sum == 0.f ? 0.f : 1.f / sum;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + (tile.pair0 + pair) * DC + e0;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            u32x2 two;
-            two.x = Elem<BF16>::round(o[d][c][0] * by) | Elem<BF16>::round(o[d][c][1] * by) << 16;
-            two.y = Elem<BF16>::round(o[d][c][2] * by) | Elem<BF16>::round(o[d][c][3] * by) << 16;
-            *reinterpret_cast<u32x2*>(out + d * 16) = two;
-          }
-        } else {
-          if (wave == 0 && mq == 0) {
-            p.part_ml[(slot * NC + pair) * 2] = m[c];
-            p.part_ml[(slot * NC + pair) * 2 + 1] = sum;
-          }
-          float* out = p.part_o + ((int64_t)slot * NC + pair) * DC + e0;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(out + d * 16) = o[d][c];
+        for (int d = 0; d < DT; ++d) put_output<BF16>(out + d * 16, o[d][c], by);
+      } else {
+        if (wave == 0 && mq == 0) {
+          p.part_ml[(slot * NC + pair) * 2] = m[c];
+          p.part_ml[(slot * NC + pair) * 2 + 1] = sum;
         }
+        float* out = p.part_o + ((int64_t)slot * NC + pair) * DC + e0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(out + d * 16) = o[d][c];
       }
     }
-
-    // --- on to the next tile
-    left -= end - at.chunk;
-    at.chunk = 0;
-    if (left > 0 && (at.tile + 1) * NC >= at.rows * p.heads) {
-      at.tile = -1;
-      do {
-        at.first_row += at.rows;
-        if (++at.request >= p.n_requests) return;  // (lengths changed under the launch)
-        at.rows = max(0, p.rows[at.request]);
-      } while (at.rows == 0);
-      at.chunks = max(1, (max(0, min(p.kv_lengths[at.request], p.max_len)) + kChunk - 1) / kChunk);
-    }
-    ++at.tile;
   }
 }
 
@@ -494,18 +619,18 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p,
   constexpr int EPL = DC / 64;
   const int g = blockIdx.x + 1, lane = threadIdx.x & 63;
   const int32_t* place = p.places + g * kPlaceWords;
-  const int total = p.places[6], active = p.places[7];
+  const int total = p.places[5], active = p.places[6];
   if (g >= active) return;
-  const int chunk = place[2], chunks = place[4];
+  const int chunk = place[1], chunks = place[3];
   if (chunk == 0) return;
   auto begin_of = [&](int i) { return (int)((int64_t)i * total / active); };
-  const int start = begin_of(g) - chunk;  // of the tile
+  const int start = begin_of(g) - chunk;  // of the tile's chunks
   if (begin_of(g - 1) > start) return;
   int last = g;  // the last workgroup with chunks of this tile
   while (last + 1 < active && begin_of(last + 1) < start + chunks) ++last;
   const int pair = blockIdx.y * 4 + (threadIdx.x >> 6);
-  const int tile = place[1], rows = place[5];
-  const int64_t at = (int64_t)place[3] * p.heads + tile * NC + pair;
+  const int tile = place[0], rows = place[4];
+  const int64_t at = (int64_t)place[2] * p.heads + tile * NC + pair;
   if (tile * NC + pair >= rows * p.heads || at >= (int64_t)p.n_rows * p.heads) return;
   // part i of the tile: workgroup g - 1's began the tile, the others' continued it
   auto slot_of = [&](int i) { return (int64_t)(2 * i + (i == g - 1 ? 1 : 0)) * NC + pair; };
@@ -535,33 +660,26 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p,
   const float by = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* out = static_cast<uint16_t*>(p.out) + at * DC + lane * 4;
 #pragma unroll
-  for (int e = 0; e < EPL; e += 4) {
-    u32x2 two;
-    two.x = Elem<BF16>::round(o[e] * by) | Elem<BF16>::round(o[e + 1] * by) << 16;
-    two.y = Elem<BF16>::round(o[e + 2] * by) | Elem<BF16>::round(o[e + 3] * by) << 16;
-    *reinterpret_cast<u32x2*>(out + e * 64) = two;
-  }
-}
-
-template <int DC, bool BF16, int NT>
-hipError_t launch_pairs(const LatentParams& p, int compute_units, hipStream_t stream) {
-  hipLaunchKernelGGL((latent_attention_kernel<DC, BF16, NT>), dim3(compute_units), dim3(kLatentWaves * kWave), 0, stream, p);
-  const hipError_t err = hipGetLastError();
-  if (err != hipSuccess || compute_units < 2) return err;
-  hipLaunchKernelGGL((latent_merge_kernel<DC, BF16, NT * 16>), dim3(compute_units - 1, NT * 4), dim3(256), 0, stream, p,
-                     compute_units);
-  return hipGetLastError();
+  for (int e = 0; e < EPL; e += 4) put_output<BF16>(out + e * 64, f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]}, by);
 }
 
 template <int DC, bool BF16>
 hipError_t launch_type(const LatentParams& p, int pairs, int compute_units, hipStream_t stream) {
-  if (pairs == 16) return launch_pairs<DC, BF16, 1>(p, compute_units, stream);
-  if (pairs == 32) return launch_pairs<DC, BF16, 2>(p, compute_units, stream);
-  return launch_pairs<DC, BF16, 4>(p, compute_units, stream);
+  const dim3 grid(compute_units), merge_grid(compute_units - 1, pairs / 4);
+  if (pairs == 16) hipLaunchKernelGGL((latent_attention_kernel<DC, BF16, 1>), grid, dim3(kThreads), 0, stream, p);
+  else if (pairs == 32) hipLaunchKernelGGL((latent_attention_kernel<DC, BF16, 2>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((latent_attention_kernel<DC, BF16, 4>), grid, dim3(kThreads), 0, stream, p);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess || compute_units < 2) return err;
+  if (pairs == 16) hipLaunchKernelGGL((latent_merge_kernel<DC, BF16, 16>), merge_grid, dim3(256), 0, stream, p, compute_units);
+  else if (pairs == 32) hipLaunchKernelGGL((latent_merge_kernel<DC, BF16, 32>), merge_grid, dim3(256), 0, stream, p, compute_units);
+  else hipLaunchKernelGGL((latent_merge_kernel<DC, BF16, 64>), merge_grid, dim3(256), 0, stream, p, compute_units);
+  return hipGetLastError();
 }
 
 }  // namespace
 
+// A tile holds the pairs of an average request, up to 64.
 int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads) {
   const int64_t each = n_requests > 0 ? n_rows * heads / n_requests : 0;
   return each <= 16 ? 16 : each <= 32 ? 32 : 64;
