@@ -235,4 +235,67 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
                   op);
 }
 
+size_t ayk_latent_chunks_workspace_bytes(int64_t ws_rows, int32_t heads_at_once) {
+  if (ws_rows < 0 || ws_rows % ayk::kLatentChunkTokens != 0 || ws_rows > INT32_MAX || heads_at_once < 1) return 0;
+  // rotary parts, then keys, values and exponents of each head
+  return (size_t)ws_rows * 128 + (size_t)heads_at_once * ((size_t)ws_rows * 512 + (size_t)ws_rows / ayk::kLatentChunkTokens * 8);
+}
+
+int ayk_latent_chunks(void* out, const void* q, const void* cache, const void* keys, const void* values,
+                      const int32_t* block_table, int64_t table_stride, const int32_t* token_tiles,
+                      int32_t n_token_tiles, const int32_t* row_tiles, int32_t n_row_tiles, int64_t ws_rows,
+                      int32_t heads_at_once, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                      int32_t num_blocks, int32_t block_size, int32_t dtype, float scale, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const char* op = "ayk_latent_chunks";
+  if (latent_dim != 256 && latent_dim != 512)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: latent_dim %d is not 256 or 512", op, latent_dim);
+  if (rope_dim != 64) return fail(AYK_ERR_UNSUPPORTED, "%s: rope_dim %d is not 64", op, rope_dim);
+  if (dtype != AYK_DTYPE_FP16 && dtype != AYK_DTYPE_BF16)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: dtype %d is not fp16 (0) or bf16 (1)", op, dtype);
+  if (num_heads < 1 || heads_at_once < 1)
+    return fail(AYK_ERR_ARGUMENT, "%s: num_heads %d, heads_at_once %d", op, num_heads, heads_at_once);
+  const int rc = check_pool(op, num_blocks, block_size);
+  if (rc != AYK_OK) return rc;
+  if (n_token_tiles < 0 || n_row_tiles < 0 || ws_rows < 0 || ws_rows % ayk::kLatentChunkTokens != 0 || ws_rows > INT32_MAX)
+    return fail(AYK_ERR_ARGUMENT, "%s: %d token tiles, %d row tiles, ws_rows %lld (a multiple of 128)", op, n_token_tiles,
+                n_row_tiles, (long long)ws_rows);
+  if (n_row_tiles == 0) return ok();
+  if (!out || !q || !cache || !keys || !values || !block_table || !row_tiles || (n_token_tiles > 0 && !token_tiles))
+    return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
+  if (misaligned(16, {out, q, cache, keys, values, workspace}))
+    return fail(AYK_ERR_ARGUMENT, "%s: out, q, cache, keys, values and workspace must be 16-byte aligned", op);
+  if (heads_at_once > num_heads) heads_at_once = num_heads;
+  const size_t need = ayk_latent_chunks_workspace_bytes(ws_rows, heads_at_once);
+  if (need > workspace_bytes || (need > 0 && !workspace))
+    return fail(AYK_ERR_WORKSPACE, "%s: the workspace holds %zu bytes, %zu are needed", op, workspace_bytes, need);
+  if ((int64_t)(n_token_tiles > n_row_tiles ? n_token_tiles : n_row_tiles) * heads_at_once > INT32_MAX)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: %d and %d tiles of %d heads exceed one launch", op, n_token_tiles, n_row_tiles,
+                heads_at_once);
+  ayk::LatentChunkParams p{};
+  p.out = out;
+  p.q = static_cast<const uint16_t*>(q);
+  p.cache = static_cast<const uint16_t*>(cache);
+  p.keys = static_cast<const uint16_t*>(keys);
+  p.values = static_cast<const uint16_t*>(values);
+  p.block_table = block_table;
+  p.token_tiles = token_tiles;
+  p.row_tiles = row_tiles;
+  p.table_stride = table_stride;
+  p.ws_rows = ws_rows;
+  p.n_token_tiles = n_token_tiles;
+  p.n_row_tiles = n_row_tiles;
+  p.heads = num_heads;
+  p.num_blocks = num_blocks;
+  p.block_size = block_size;
+  p.by_block = ayk::divisor_of(block_size);
+  p.scale_log2 = scale * kLog2e;
+  p.group_heads = heads_at_once;
+  p.ws_rope = static_cast<uint16_t*>(workspace);
+  p.ws_keys = p.ws_rope + ws_rows * 64;
+  p.ws_values = p.ws_keys + heads_at_once * ws_rows * 128;
+  p.ws_exponents = reinterpret_cast<int32_t*>(p.ws_values + heads_at_once * ws_rows * 128);
+  return launched(ayk::launch_latent_chunks(p, latent_dim, dtype == AYK_DTYPE_BF16, static_cast<hipStream_t>(stream)), op);
+}
+
 }  // extern "C"

@@ -203,6 +203,33 @@ size_t latent_workspace_bytes(int32_t latent_dim, int pairs, int compute_units);
 hipError_t launch_latent_attention(const LatentParams& p, int32_t latent_dim, bool bf16, int pairs, int compute_units,
                                    hipStream_t stream);
 
+// Chunks over a latent cache with expanded keys and values (latent_chunks.hip). Tiles are int32
+// quadruples: of tokens (request, first position, the request's length, workspace row), of rows (first
+// row, rows, workspace row of the request, first row's position).
+constexpr int kLatentChunkTokens = 128;
+constexpr int kLatentChunkRows = 128;
+struct LatentChunkParams {
+  void* out;
+  const uint16_t* q;
+  const uint16_t* cache;
+  const uint16_t* keys;
+  const uint16_t* values;
+  const int32_t* block_table;
+  const int32_t* token_tiles;
+  const int32_t* row_tiles;
+  int64_t table_stride;
+  int64_t ws_rows;  // a multiple of kLatentChunkTokens
+  int32_t n_token_tiles, n_row_tiles, heads, num_blocks, block_size;
+  Divisor by_block;
+  float scale_log2;
+  int32_t group_heads, first_head;  // heads expanded at a time; the launch's own
+  uint16_t* ws_rope;                // [ws_rows, 64]
+  uint16_t* ws_keys;                // [group_heads, ws_rows, 128]
+  uint16_t* ws_values;
+  int32_t* ws_exponents;            // [group_heads, ws_rows / 128, 2]
+};
+hipError_t launch_latent_chunks(const LatentChunkParams& p, int32_t latent_dim, bool bf16, hipStream_t stream);
+
 // mode: 0 = gather (dst index i), 1 = copy (dst ids), 2 = zero (no source)
 hipError_t launch_block_op(int mode, const void* src_k, const void* src_v, void* dst_k, void* dst_v,
                            const void* src_ids, const void* dst_ids, bool ids64, int64_t n,

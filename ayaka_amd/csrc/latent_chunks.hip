@@ -1,0 +1,547 @@
+// Attention of chunks of new tokens over a latent cache, expanded form (gfx950).
+//
+//   k[h, t] = [keys[h] latent_t | rotary part_t],  v[h, t] = values[h] latent_t,
+//   out[row, h] = softmax(scale * q[row, h] . k[h, .]) v[h, .]   over positions 0 .. position(row).
+// A (row, head, position) takes 2 (192 + 128) operations so, against 2 (2 DC + 64) on the latents
+// themselves (a third at DC 512); expanding takes 2 * 256 * DC per (head, position), once for all rows.
+//
+// Two kernels, for as many heads at a time as the workspace holds:
+//
+// latent_expand_kernel: a product of 128 tokens by one head's 256 outputs (its keys, then its values),
+// 8 waves of 64 x 64 on v_mfma_f32_16x16x32, operands through LDS in steps of 64 of DC, three steps in
+// flight (global_load_lds). Tokens are gathered from their pages here; what follows reads straight lines.
+//
+// Keys and values are kept as fp16 whatever the model's type, with a power of two for every 128 tokens,
+// head and of both kinds, chosen from the largest finite value there, so nothing overflows and each
+// element is within 2^-12 of itself (or 2^-39 of its tile's largest): bf16 keys and values would each
+// cost the outputs as much as their own rounding does. The scales are uniform in the attention's
+// loop: the key's joins the factor that scores take anyway, the value's the exponent.
+//
+// latent_chunk_kernel: a workgroup (8 waves) per 128 rows of a request and head. Four waves of 32 rows
+// work on every other 32 positions and four on those between (two waves to a SIMD, one's softmax under
+// the other's products); joined at the end in LDS. S^T = K Q^T, weights stay in the lane that scored
+// them, O^T += V^T P^T with values read transposed, as the other attention kernels. Rounds of 64
+// positions (40 KB) in a ring of three.
+#include <type_traits>
+
+#include "attention_common.h"
+
+namespace ayk {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+namespace {
+
+constexpr int kRope = 64;
+constexpr int kNope = 128;
+constexpr int kValue = 128;
+constexpr int kTokens = kLatentChunkTokens;  // of an expanded tile, with one scale
+constexpr int kRows = kLatentChunkRows;      // of a workgroup
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * kWave;
+
+template <bool BF16>
+__device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 acc) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t quotient(uint32_t n, Divisor d) {
+  return (uint32_t)(((uint64_t)__umulhi(n, d.magic) + n) >> d.shift);
+}
+
+// 16 bytes a lane to LDS at `to` + 16 * lane (`to` uniform).
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+template <class T>
+__device__ __forceinline__ uint32_t lds_offset(T* p) {
+  return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) T*)p);
+}
+
+// Where piece c (16 bytes) of row r stands in LDS, for rows of 128 and of 256 bytes: any 16 rows that
+// one cycle's reads touch are spread over all 64 banks.
+__device__ __forceinline__ int swizzle128(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int swizzle256(int r) { return r & 15; }
+
+// The power of two that brings a largest magnitude into [2^13, 2^14).
+__device__ __forceinline__ int exponent_for(float largest) {
+  if (largest == 0.f) return -100;
+  return max(-100, min(114, (int)((__float_as_uint(largest) >> 23) & 255) - 126 - 14));
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ float finite_magnitude(float x) {
+  const float a = __builtin_fabsf(x);
+  return a < INFINITY ? a : 0.f;  // (also where it is NaN)
+}
+__device__ __forceinline__ uint32_t two_halves(float a, float b) {
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+}
+
+// --- expansion
+
+constexpr int kStep = 64;        // of DC in LDS at a time
+constexpr int kSteps = 3;        // in flight
+constexpr int kOutputs = kNope + kValue;
+
+template <int DC, bool BF16>
+__global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const LatentChunkParams p) {
+  struct Shared {
+    uint16_t token[kSteps][kTokens * kStep];
+    uint16_t weight[kSteps][kOutputs * kStep];
+    float largest[kWaves];
+  };
+  __shared__ __align__(16) Shared lds;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int mt = lane & 15, mq = lane >> 4;
+  const int head = blockIdx.x % p.group_heads, tile = blockIdx.x / p.group_heads;
+  const int request = p.token_tiles[4 * tile], first = p.token_tiles[4 * tile + 1], length = p.token_tiles[4 * tile + 2];
+  const int64_t ws_row = p.token_tiles[4 * tile + 3];
+  const int real_head = p.first_head + head;
+
+  // What this wave fetches of each step, 8 rows a load: 16 tokens and 32 outputs.
+  const uint8_t* from[6];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = wave * 16 + i * 8 + (lane >> 3);
+    const uint32_t pos = (uint32_t)min(first + row, length - 1);
+    const uint32_t block = quotient(pos, p.by_block);
+    const uint32_t id = (uint32_t)p.block_table[request * p.table_stride + block];
+    const uint64_t slot = (uint64_t)(id < (uint32_t)p.num_blocks ? id : 0u) * (uint32_t)p.block_size + (pos - block * (uint32_t)p.block_size);
+    from[i] = reinterpret_cast<const uint8_t*>(p.cache) + slot * ((DC + kRope) * 2) + ((lane & 7) ^ swizzle128(row)) * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = wave * 32 + i * 8 + (lane >> 3);
+    const uint16_t* w = row < kNope ? p.keys + ((int64_t)real_head * kNope + row) * DC
+                                    : p.values + ((int64_t)real_head * kValue + row - kNope) * DC;
+    from[2 + i] = reinterpret_cast<const uint8_t*>(w) + ((lane & 7) ^ swizzle128(row)) * 16;
+  }
+  const uint32_t token_lds = lds_offset(&lds.token[0][0]), weight_lds = lds_offset(&lds.weight[0][0]);
+  auto get = [&](int step) {
+    const uint32_t s = (uint32_t)(step % kSteps);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      load_to_lds(token_lds + s * (kTokens * kStep * 2) + (wave * 16 + i * 8) * (kStep * 2), from[i] + step * (kStep * 2));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      load_to_lds(weight_lds + s * (kOutputs * kStep * 2) + (wave * 32 + i * 8) * (kStep * 2), from[2 + i] + step * (kStep * 2));
+  };
+  // the rotary parts go along once, from the first head's workgroups
+  if (real_head == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = wave * 16 + i * 8 + (lane >> 3);
+      const uint8_t* rope = from[i] - ((lane & 7) ^ swizzle128(row)) * 16 + DC * 2 + (lane & 7) * 16;
+      *reinterpret_cast<u32x4*>(p.ws_rope + (ws_row + row) * kRope + (lane & 7) * 8) = *reinterpret_cast<const u32x4*>(rope);
+    }
+  }
+
+  // Outputs are the product's rows and tokens its columns, so that a lane holds 4 outputs of a token.
+  const int m = wave & 1, n = wave >> 1;  // 64 tokens, 64 outputs
+  f32x4 acc[4][4];  // [outputs][tokens]
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int STEPS = DC / kStep;
+  get(0);
+  get(1);
+#pragma unroll
+  for (int step = 0; step < STEPS; ++step) {
+    if (step + 1 < STEPS) wait_loads<6>();
+    else wait_loads<0>();
+    lds_barrier();
+    if (step + 2 < STEPS) get(step + 2);
+    const uint8_t* token = reinterpret_cast<const uint8_t*>(lds.token[step % kSteps]) + m * 64 * kStep * 2;
+    const uint8_t* weight = reinterpret_cast<const uint8_t*>(lds.weight[step % kSteps]) + n * 64 * kStep * 2;
+    u32x4 a[2][4], b[2][4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = i * 16 + mt, piece = (4 * k + mq) ^ swizzle128(row);
+        a[k][i] = *reinterpret_cast<const u32x4*>(weight + row * (kStep * 2) + piece * 16);
+        b[k][i] = *reinterpret_cast<const u32x4*>(token + row * (kStep * 2) + piece * 16);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mfma32<BF16>(a[k][i], b[k][j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // The scale of the tile's keys (waves 0-3) and of its values (4-7).
+  float largest = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) largest = fmaxf(largest, finite_magnitude(acc[i][j][e]));
+  largest = column_max(largest);
+#pragma unroll
+  for (int d = 8; d >= 1; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+  if (lane == 0) lds.largest[wave] = largest;
+  lds_barrier();
+  const int half = n >> 1;  // keys, values
+  largest = fmaxf(fmaxf(lds.largest[4 * half], lds.largest[4 * half + 1]), fmaxf(lds.largest[4 * half + 2], lds.largest[4 * half + 3]));
+  const int exponent = exponent_for(largest);
+  const float by = power(-exponent);
+  // Through LDS (rows of 512 bytes, as tokens; every wave is past its last read), then whole rows out.
+  uint8_t* rows = reinterpret_cast<uint8_t*>(&lds.token[0][0]);
+  static_assert(offsetof(Shared, largest) >= kTokens * kOutputs * 2, "the tile fits where the operands were");
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int token = m * 64 + j * 16 + mt, output = n * 64 + i * 16 + 4 * mq;
+      const u32x2 x = {two_halves(acc[i][j][0] * by, acc[i][j][1] * by), two_halves(acc[i][j][2] * by, acc[i][j][3] * by)};
+      *reinterpret_cast<u32x2*>(rows + token * (kOutputs * 2) + (((output >> 3) ^ swizzle256(token)) * 16) + (output & 4) * 2) = x;
+    }
+  lds_barrier();
+  const int64_t ws = (int64_t)head * p.ws_rows + ws_row;
+#pragma unroll
+  for (int i = 0; i < kTokens * kOutputs / 8 / kThreads; ++i) {
+    const int at = i * kThreads + tid, token = at >> 5, piece = at & 31;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(rows + token * (kOutputs * 2) + ((piece ^ swizzle256(token)) * 16));
+    uint16_t* to = piece < 16 ? p.ws_keys : p.ws_values;
+    *reinterpret_cast<u32x4*>(to + (ws + token) * kNope + (piece & 15) * 8) = x;
+  }
+  if (tid == 0 || tid == 4 * kWave) p.ws_exponents[(head * (p.ws_rows / kTokens) + ws_row / kTokens) * 2 + half] = exponent;
+}
+
+// --- attention
+
+constexpr int kPositions = 32;            // of a wave's step
+constexpr int kRound = 2 * kPositions;    // of both halves of the workgroup
+constexpr int kRing = 3;
+
+struct Round {
+  uint16_t keys[kRound * kNope];
+  uint16_t values[kRound * kValue];
+  uint16_t rope[kRound * kRope];
+};
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentChunkParams p) {
+  struct Shared {
+    Round round[kRing];
+    float state[4][2][3][16];  // (m, l, exponent) of the later half's rows
+  };
+  __shared__ __align__(16) Shared lds;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int mt = lane & 15, mq = lane >> 4;
+  const int rg = wave & 3, kg = wave >> 2;  // 32 rows, every other 32 positions
+  const int head = blockIdx.x % p.group_heads, tile = blockIdx.x / p.group_heads;
+  const int first_row = p.row_tiles[4 * tile], n_rows = p.row_tiles[4 * tile + 1], first_pos = p.row_tiles[4 * tile + 3];
+  const int64_t ws_row = p.row_tiles[4 * tile + 2];
+  const int real_head = p.first_head + head;
+  const int context = first_pos + n_rows;  // positions that the last row sees
+  const int rounds = (context + kRound - 1) / kRound;
+
+  const uint8_t* keys = reinterpret_cast<const uint8_t*>(p.ws_keys + ((int64_t)head * p.ws_rows + ws_row) * kNope);
+  const uint8_t* values = reinterpret_cast<const uint8_t*>(p.ws_values + ((int64_t)head * p.ws_rows + ws_row) * kValue);
+  const uint8_t* rope = reinterpret_cast<const uint8_t*>(p.ws_rope + ws_row * kRope);
+  const int32_t* exponents = p.ws_exponents + (head * (p.ws_rows / kTokens) + ws_row / kTokens) * 2;
+  const uint32_t ring = lds_offset(&lds.round[0]);
+  // a wave's loads of a round: 8 rows of keys, of values (4 a load) and of rotary parts (8 a load)
+  uint32_t at[3];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = wave * 8 + i * 4 + (lane >> 4);
+    at[i] = row * 256 + ((lane & 15) ^ swizzle256(row)) * 16;
+  }
+  at[2] = (wave * 8 + (lane >> 3)) * 128 + ((lane & 7) ^ swizzle128(wave * 8 + (lane >> 3))) * 16;
+  auto get = [&](int round) {
+    const uint32_t to = ring + (uint32_t)(round % kRing) * sizeof(Round) + wave * 8 * 256;
+    const int64_t from = (int64_t)round * kRound * 256;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load_to_lds(to + i * 1024, keys + from, at[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load_to_lds(to + kRound * 256 + i * 1024, values + from, at[i]);
+    load_to_lds(ring + (uint32_t)(round % kRing) * sizeof(Round) + 2 * kRound * 256 + wave * 8 * 128, rope + from / 2, at[2]);
+  };
+  constexpr int LOADS = 5;
+
+  // The queries: 16 rows a tile, their first part as fp16 under a power of two of each row's own.
+  u32x4 q[2][4], qr[2][2];
+  int unit[2];  // the power of two that a raw score of the first part is worth, but for the keys'
+  int my_pos[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = rg * 32 + j * 16 + mt;
+    my_pos[j] = row < n_rows ? first_pos + row : -1;
+    const u32x4* from =
+        reinterpret_cast<const u32x4*>(p.q + ((int64_t)(first_row + (row < n_rows ? row : 0)) * p.heads + real_head) * (kNope + kRope)) + mq;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[j][k] = from[4 * k];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) qr[j][k] = from[16 + 4 * k];
+  }
+  if (rounds > 0) get(0);
+  if (rounds > 1) get(1);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float largest = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        largest = fmaxf(largest, fmaxf(finite_magnitude(Elem<BF16>::lo(q[j][k][e])), finite_magnitude(Elem<BF16>::hi(q[j][k][e]))));
+    const int exponent = exponent_for(column_max(largest));
+    const float by = power(-exponent);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[j][k][e] = two_halves(Elem<BF16>::lo(q[j][k][e]) * by, Elem<BF16>::hi(q[j][k][e]) * by);
+    unit[j] = exponent;
+  }
+  f32x4 o[8][2];
+  float m[2], l[2];
+  int value_exponent = -100;  // of O
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    m[j] = -INFINITY;
+    l[j] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[d][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  int k_at[4], r_at[2], v_at[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k_at[i] = mt * 256 + ((4 * i + mq) ^ swizzle256(mt)) * 16;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r_at[i] = 2 * kRound * 256 + mt * 128 + ((4 * i + mq) ^ swizzle128(mt)) * 16;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int t = 4 * mq + (mt >> 2);
+    v_at[i] = kRound * 256 + t * 256 + ((2 * i + ((mt & 3) >> 1)) ^ swizzle256(t)) * 16 + (mt & 1) * 8;
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt 0, said to the compiler: its waits for the queries end here
+
+  const int first_masked = first_pos + rg * 32;  // rows of this wave see up to there, all of them
+  for (int round = 0; round < rounds; ++round) {
+    if (round + 1 < rounds) wait_loads<LOADS>();
+    else wait_loads<0>();
+    lds_barrier();
+    if (round + 2 < rounds) get(round + 2);
+    const int t0 = round * kRound + kg * kPositions;
+    if (t0 >= context || t0 > first_masked + 31) continue;  // nothing for these rows
+    uint8_t* here = reinterpret_cast<uint8_t*>(&lds.round[round % kRing]);
+    const uint8_t* k_here = here + kg * kPositions * 256;
+    const uint8_t* r_here = here + kg * kPositions * 128;
+    const int key_exponent = exponents[(t0 / kTokens) * 2], new_exponent = exponents[(t0 / kTokens) * 2 + 1];
+
+    f32x4 s[2][2], r[2][2];  // [16 positions][16 rows], of the first part and of the rotary part
+    u32x4 a[2][6];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[h][k] = *reinterpret_cast<const u32x4*>(k_here + h * 16 * 256 + k_at[k]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) a[h][4 + k] = *reinterpret_cast<const u32x4*>(r_here + h * 16 * 128 + r_at[k]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 v[8];
+    auto read_values = [&] {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(k_here + v_at[d]);
+        const u32x2 x = lds_read_transposed(from), y = lds_read_transposed(from + 16 * kValue);
+        v[d] = u32x4{x.x, x.y, y.x, y.y};
+      }
+    };
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        r[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s[h][j] = mfma32<false>(a[h][k], q[j][k], s[h][j]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) r[h][j] = mfma32<BF16>(a[h][4 + k], qr[j][k], r[h][j]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_values();
+    __builtin_amdgcn_sched_barrier(0);
+
+    const bool masked = t0 + kPositions - 1 > first_masked;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float by = __builtin_ldexpf(p.scale_log2, unit[j] + key_exponent);
+      const int seen = my_pos[j] - t0 - 4 * mq;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float t = __builtin_fmaf(s[h][j][i], by, r[h][j][i] * p.scale_log2);
+          if (masked) {
+            odd |= !(__builtin_fabsf(t) < INFINITY);
+            s[h][j][i] = 16 * h + i <= seen ? t : -INFINITY;
+          } else {
+            s[h][j][i] = t;
+          }
+        }
+    }
+    if (masked && __builtin_amdgcn_ballot_w64(odd)) {
+      // Values that are not finite leave this wave's positions (others that read them here see such a
+      // position's score, or do the same).
+      uint32_t* words = reinterpret_cast<uint32_t*>(here + kRound * 256 + kg * kPositions * 256);
+      for (int i = lane; i < kPositions * kValue / 2; i += kWave) {
+        uint32_t w = words[i];
+        if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+        if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
+        words[i] = w;
+      }
+      read_values();
+    }
+    if (new_exponent > value_exponent) {
+      const float by = power(max(-126, value_exponent - new_exponent));
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d][j] *= by;
+      value_exponent = new_exponent;
+    }
+    float top[2];
+    bool passes = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      top[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])),
+                     fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
+      passes |= top[j] > m[j] + kRescaleSlack;
+    }
+    if (__builtin_amdgcn_ballot_w64(passes)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float now = fmaxf(m[j], column_max(top[j]));
+        const float by = now == m[j] ? 1.f : fast_exp2(m[j] - now);
+        m[j] = now;
+        l[j] *= by;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d][j] *= by;
+      }
+    }
+    // the values' scale: weights carry 2^lower, the sum takes it back
+    const int below = max(-126, new_exponent - value_exponent);
+    const float lower = (float)below, raise = power(-below);
+    u32x4 w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float base = m[j] == -INFINITY ? 0.f : m[j];
+      float e[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[4 * h + i] = fast_exp2((s[h][j][i] - base) + lower);
+      l[j] = __builtin_fmaf(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])), raise, l[j]);
+      w[j] = u32x4{two_halves(e[0], e[1]), two_halves(e[2], e[3]), two_halves(e[4], e[5]), two_halves(e[6], e[7])};
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) o[d][j] = mfma32<false>(v[d], w[j], o[d][j]);
+    __builtin_amdgcn_s_setprio(0);
+  }
+
+  // --- the two halves joined: the later one's state through LDS
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    l[j] += __shfl_xor(l[j], 16);
+    l[j] += __shfl_xor(l[j], 32);
+  }
+  lds_barrier();
+  f32x4* hand = reinterpret_cast<f32x4*>(&lds.round[0]);
+  static_assert(sizeof(lds.round) >= 4 * 16 * kWave * 16, "four waves' O");
+  if (kg == 1) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (mq == 0) {
+        lds.state[rg][j][0][mt] = m[j];
+        lds.state[rg][j][1][mt] = l[j];
+        lds.state[rg][j][2][mt] = (float)value_exponent;
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) hand[((rg * 2 + j) * 8 + d) * kWave + lane] = o[d][j];
+    }
+  }
+  lds_barrier();
+  if (kg == 1) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float pm = lds.state[rg][j][0][mt], pl = lds.state[rg][j][1][mt];
+    const int pe = (int)lds.state[rg][j][2][mt], high = max(value_exponent, pe);
+    const float now = fmaxf(m[j], pm);
+    const float mine = now == m[j] ? 1.f : fast_exp2(m[j] - now), other = now == pm ? 1.f : fast_exp2(pm - now);
+    const float sum = l[j] * mine + pl * other;
+    const float total = sum == 0.f ? 0.f : 1.f / sum;
+    const float a = mine * power(max(-126, value_exponent - high)), b = other * power(max(-126, pe - high));
+    const int row = rg * 32 + j * 16 + mt;
+    if (row >= n_rows) continue;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + ((int64_t)(first_row + row) * p.heads + real_head) * kValue + 4 * mq;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const f32x4 x = hand[((rg * 2 + j) * 8 + d) * kWave + lane];
+      uint32_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = Elem<BF16>::round(__builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, high));
+      *reinterpret_cast<u32x2*>(out + d * 16) = u32x2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+    }
+  }
+}
+
+template <bool BF16>
+hipError_t launch_type(LatentChunkParams p, int32_t latent_dim, hipStream_t stream) {
+  const int group = p.group_heads;
+  for (p.first_head = 0; p.first_head < p.heads; p.first_head += group) {
+    p.group_heads = p.heads - p.first_head < group ? p.heads - p.first_head : group;
+    const dim3 expand((unsigned)(p.n_token_tiles * p.group_heads)), attend((unsigned)(p.n_row_tiles * p.group_heads));
+    if (p.n_token_tiles == 0) {
+      // nothing but rows without a context
+    } else if (latent_dim == 512) hipLaunchKernelGGL((latent_expand_kernel<512, BF16>), expand, dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((latent_expand_kernel<256, BF16>), expand, dim3(kThreads), 0, stream, p);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    hipLaunchKernelGGL((latent_chunk_kernel<BF16>), attend, dim3(kThreads), 0, stream, p);
+    err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_latent_chunks(const LatentChunkParams& p, int32_t latent_dim, bool bf16, hipStream_t stream) {
+  if (p.n_row_tiles == 0) return hipSuccess;
+  return bf16 ? launch_type<true>(p, latent_dim, stream) : launch_type<false>(p, latent_dim, stream);
+}
+
+}  // namespace ayk

@@ -67,6 +67,7 @@ __all__ = [
     "advance_graph_metadata",
     "attend",
     "attend_latent",
+    "attend_latent_chunks",
     "attend_with",
     "choose_partitions",
     "choose_split",
@@ -1622,4 +1623,4 @@ def _stage_split(staging: HipGraphPlan, lengths: np.ndarray, block_size: int) ->
 
 
 # the family's ops over latent caches, which share this module's plans and scratch
-from ayaka_amd.hip.latent import attend_latent  # noqa: E402
+from ayaka_amd.hip.latent import attend_latent, attend_latent_chunks  # noqa: E402

@@ -1,12 +1,15 @@
-"""Attention over latent caches: the host side of ``attention.attend_latent``.
+"""Attention over latent caches: the host side of ``attention.attend_latent`` and
+``attention.attend_latent_chunks`` (``include/ayaka_hip_latent.h``).
 
-The launch (``include/ayaka_hip_latent.h``) reads lengths, rows and tables on the device and splits the
-step's contexts there, so an eagerly planned step, a verify window and a captured bucket are the same
-call; the workspace is the one the device's split launches share.
+The first's launch reads lengths, rows and tables on the device and splits the step's contexts there,
+so an eagerly planned step, a verify window and a captured bucket are the same call. The second's takes
+tile lists of a planned step, made on its first call and kept in the plan, as the multi-row launch's.
+The workspace of both is the one the device's split launches share.
 """
 
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from ayaka_amd.attention import AttentionMetadata
@@ -14,13 +17,19 @@ from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import _fastpath, _lib
 from ayaka_amd.hip import attention as _attention
 from ayaka_amd.hip._checks import capturing, dtype_name, require_device, require_latent_buffers, require_like, stream_handle
-from ayaka_amd.kvcache import LatentBuffers
+from ayaka_amd.kvcache import LatentBuffers, LatentWeights
 
-__all__ = ["LATENT_DIMS", "ROPE_DIM", "attend_latent"]
+__all__ = ["LATENT_DIMS", "ROPE_DIM", "attend_latent", "attend_latent_chunks"]
 
 #: Widths of the latent, and of the rotary part, the kernels are built for.
 LATENT_DIMS = frozenset({256, 512})
 ROPE_DIM = 64
+#: Widths of the expanded keys (without their rotary part) and values.
+NOPE_DIM = VALUE_DIM = 128
+#: Tokens of an expanded tile and rows of an attending one (the C library's).
+TILE_TOKENS = TILE_ROWS = 128
+#: Most bytes of expanded keys and values; a step that needs more expands some heads at a time.
+EXPANDED_BYTES = 512 << 20
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
 
 
@@ -115,4 +124,82 @@ def _attend_latent(op: str, q: torch.Tensor, buffers: LatentBuffers, meta: Atten
         meta.rows_per_request.data_ptr(), requests, n_rows, heads, buffers.latent_dim, buffers.rope_dim,
         buffers.num_blocks, buffers.block_size, table.shape[1], _DTYPE_CODES[cache.dtype], float(scale),
         scratch.data_ptr(), scratch.numel(),
+    ), stream, device, True, record)
+
+
+def _chunk_tiles(op: str, step: "_attention.HipAttentionPlan", device: torch.device,
+                 capture: bool) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """The step's token tiles and row tiles (heaviest first) on the device, and its workspace rows."""
+    found = step.work.get("latent-chunks")
+    if found is not None:
+        return found
+    if capture:
+        raise BackendError(f"{op}: the tile lists of this step are built on its first call; run the step once "
+                           "eagerly before capturing it", context={"op": op})
+    tokens, rows, ws_rows, first_row = [], [], 0, 0
+    for request, (count, length) in enumerate(zip(step.rows, step.kv_lengths)):
+        base = first_row + np.arange(0, count, TILE_ROWS)
+        size = np.minimum(TILE_ROWS, first_row + count - base)
+        if count and length:
+            at = np.arange(0, length, TILE_TOKENS)
+            tokens.append(np.stack((np.full_like(at, request), at, np.full_like(at, length), ws_rows + at), axis=1))
+            rows.append(np.stack((base, size, np.full_like(base, ws_rows), length - count + base - first_row), axis=1))
+            ws_rows += at.size * TILE_TOKENS
+        elif count:
+            rows.append(np.stack((base, size, np.zeros_like(base), -size), axis=1))
+        first_row += count
+    if ws_rows > np.iinfo(np.int32).max:
+        raise BackendError(f"{op}: contexts of {ws_rows} positions in all exceed one launch", context={"op": op})
+    row_list = np.concatenate(rows)
+    row_list = row_list[np.argsort(-(row_list[:, 1] + row_list[:, 3]), kind="stable")]
+    token_list = np.concatenate(tokens) if tokens else np.zeros((0, 4), dtype=np.int64)
+    found = (*(torch.from_numpy(x.astype(np.int32).reshape(-1)).to(device) for x in (token_list, row_list)), ws_rows)
+    step.work["latent-chunks"] = found
+    return found
+
+
+def attend_latent_chunks(q: torch.Tensor, weights: LatentWeights, buffers: LatentBuffers, meta: AttentionMetadata,
+                         out: torch.Tensor, *, scale: float) -> None:
+    """Attention of chunks of rows over their requests' latent contexts, keys and values expanded.
+
+    Head h's key of a position is ``weights.keys[h] @ latent`` with the position's rotary part behind it,
+    its value ``weights.values[h] @ latent``; ``q`` [N, heads, 128 + 64] are the queries as projected, with
+    their rotary part rotated, and ``out`` [N, heads, 128] are the heads' outputs. The context's keys and
+    values are expanded once for all rows, into scratch, so this is for steps of many rows per request
+    (some hundred; ``attend_latent`` serves the others without expanding). For steps made by ``plan``;
+    captured after one eager call. Expanded keys and values are held in fp16 with scales of
+    their own (2^-12 relative, any magnitude).
+    """
+    op = "attention.attend_latent_chunks"
+    key = ("attend_latent_chunks", id(buffers), id(meta), scale,
+           _fastpath.signature((q, out, buffers.k, weights.keys, weights.values)))
+    _replayed(meta, key, (buffers, meta), q,
+              lambda record: _attend_latent_chunks(op, q, weights, buffers, meta, out, scale, record))
+
+
+def _attend_latent_chunks(op: str, q: torch.Tensor, weights: LatentWeights, buffers: LatentBuffers,
+                          meta: AttentionMetadata, out: torch.Tensor, scale: float,
+                          record: "_fastpath.Recorder | None") -> None:
+    heads = _require_latent_step(op, q, buffers, meta, out, NOPE_DIM + ROPE_DIM, VALUE_DIM)
+    cache, table, step = buffers.cache, meta.block_table, meta.plan
+    for name, tensor, width in (("weights.keys", weights.keys, NOPE_DIM), ("weights.values", weights.values, VALUE_DIM)):
+        require_like(op, name, tensor, (heads, width, buffers.latent_dim), cache.dtype)
+        require_device(op, name, tensor, cache.device)
+    if not isinstance(step, _attention.HipAttentionPlan):
+        raise BackendError(f"{op}: needs a step made by plan; a decode bucket's rows take attend_latent",
+                           context={"op": op, "argument": "meta"})
+    if q.shape[0] == 0:
+        return
+    device, lib, capture = cache.device, _lib.lib(), capturing(q)
+    tokens, rows, ws_rows = _chunk_tiles(op, step, device, capture)
+    at_once = heads if ws_rows == 0 else max(1, min(heads, EXPANDED_BYTES // (ws_rows * 512)))
+    if at_once >= 8:
+        at_once -= at_once % 8 if at_once < heads else 0  # (a head's workgroups then share an XCD)
+    stream = stream_handle(device)
+    scratch = _attention._workspace(op, device, lib.ayk_latent_chunks_workspace_bytes(ws_rows, at_once), capture, stream)
+    _attention._call(op, lib.ayk_latent_chunks, (
+        out.data_ptr(), q.data_ptr(), cache.data_ptr(), weights.keys.data_ptr(), weights.values.data_ptr(),
+        table.data_ptr(), table.stride(0), tokens.data_ptr(), tokens.numel() // 4, rows.data_ptr(), rows.numel() // 4,
+        ws_rows, at_once, heads, buffers.latent_dim, buffers.rope_dim, buffers.num_blocks, buffers.block_size,
+        _DTYPE_CODES[cache.dtype], float(scale), scratch.data_ptr(), scratch.numel(),
     ), stream, device, True, record)

@@ -79,6 +79,31 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
                          int32_t block_size, int32_t max_blocks, int32_t dtype, float scale, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/*
+ * The same cache with keys and values expanded from the latents, for chunks of many rows:
+ *   key(h, t) = [keys[h] . latent(t) | rotary part(t)],  value(h, t) = values[h] . latent(t)
+ *   out[row, h] = sum over t of softmax(scale * q[row, h] . key(h, .))(t) * value(h, t)
+ * q [n_rows, num_heads, 128 + 64], out [n_rows, num_heads, 128], keys and values [num_heads, 128,
+ * latent_dim], contiguous and 16-byte aligned, as the cache; dtype fp16 or bf16; latent_dim 256 or 512.
+ * Expanded keys and values are fp16 under a power of two for every 128 tokens, head and kind (within 2^-12
+ * of themselves down to 2^-27 of the largest there, then within 2^-39 of it).
+ * The step comes as two device lists of int32 quadruples, made on the host:
+ *   token_tiles (request, first position, the request's length, workspace row): every 128 positions of each
+ *     request with rows, its workspace rows following each other and starting at a multiple of 128;
+ *   row_tiles (first row, rows, workspace row of the request's position 0, position of the first row): up to
+ *     128 consecutive rows of a request, whose positions follow each other; rows without a context have the
+ *     position -rows (and get zeros). Rows in no tile are not written.
+ * ws_rows: workspace rows, a multiple of 128. heads_at_once heads are expanded, then attended to, at a time.
+ * workspace: ayk_latent_chunks_workspace_bytes(ws_rows, heads_at_once), 16-byte aligned.
+ */
+size_t ayk_latent_chunks_workspace_bytes(int64_t ws_rows, int32_t heads_at_once);
+int ayk_latent_chunks(void* out, const void* q, const void* cache, const void* keys, const void* values,
+                      const int32_t* block_table, int64_t table_stride, const int32_t* token_tiles,
+                      int32_t n_token_tiles, const int32_t* row_tiles, int32_t n_row_tiles, int64_t ws_rows,
+                      int32_t heads_at_once, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                      int32_t num_blocks, int32_t block_size, int32_t dtype, float scale, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
