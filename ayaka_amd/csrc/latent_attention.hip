@@ -19,7 +19,7 @@
 //  * S^T = K Q^T, then O^T += V^T P^T, v_mfma_f32_16x16x32 with q and O in registers; the values are the
 //    latents already in LDS, read transposed (ds_read_b64_tr_b16). A bf16 P is taken in two parts (high
 //    and remainder by truncation: one bf16 would lose 2^-9 of each weight, as much as the output's own
-//    rounding), an fp16 P rounded to nearest (2^-12).
+//    rounding), an fp16 P rounded to nearest (2^-11).
 //  * The running maximum moves only when a score passes it by kRescaleSlack; until then weights up to
 //    2^kRescaleSlack keep their accuracy and nothing is rescaled.
 //
@@ -39,7 +39,7 @@
 // Visible and masked: a masked position's weight is an exact 0, and what it multiplies must be
 // finite. Slots behind the context are never read (the last position stands in for them). Rows of one
 // request see different ends; if a raw score in their last chunks is not finite, the non-finite
-// elements are taken out of the values there: rows that see that position get NaN from its score, the
+// elements are taken out of the values there, and rows that see them get NaN in their place: the
 // others must not notice.
 #include <type_traits>
 
@@ -372,12 +372,16 @@ __device__ __forceinline__ void read_ahead(Read read, Use use) {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+template <bool BF16>
+__device__ __forceinline__ bool is_finite(uint32_t bits) {
+  constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+  return (bits & EXP) != EXP;
+}
 // Non-finite elements of a word of two, replaced by zeros.
 template <bool BF16>
 __device__ __forceinline__ uint32_t finite_word(uint32_t w) {
-  constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-  if ((w & EXP) == EXP) w &= 0xffff0000u;
-  if (((w >> 16) & EXP) == EXP) w &= 0xffffu;
+  if (!is_finite<BF16>(w)) w &= 0xffff0000u;
+  if (!is_finite<BF16>(w >> 16)) w &= 0xffffu;
   return w;
 }
 
@@ -434,6 +438,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
     const int my_pair = ct * 16 + mt;
     const bool real = scores && my_pair < tile.pairs;
     const int my_pos = real ? tile.first_pos + (piece.tile * NC + my_pair) / p.heads : -1;
+    bool emptied = false;  // values lost non-finite elements
     u32x4 q[KS + 2];
     f32x4 o[DT][NT];
     float m[NT], my_m = -INFINITY, l = 0.f;  // of every pair; of my_pair, with its sum over this wave's positions
@@ -525,7 +530,9 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
           put_weights(before);
         }
         if (late) get(chunk + kStages - 1);
-        // this wave's values, on their way while it waits for the weights
+        // this wave's values, on their way while it waits for the weights (of 64 pairs, only afterwards: the
+        // registers hold no more)
+        constexpr bool EARLY = NT < 4;
         u32x4 v[DT];
         auto read_values = [&] {
 #pragma unroll
@@ -535,14 +542,19 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
             v[d] = u32x4{a.x, a.y, b.x, b.y};
           }
         };
-        read_values();
+        if (EARLY) read_values();
         lds_barrier();
         const int word = __builtin_amdgcn_readfirstlane(lds.flag[chunk & 1]);
         if (word) {
-          if (word & 2) {
-            // a share of the chunk's values (all of them are clean behind the next barrier)
-            uint32_t* mine = reinterpret_cast<uint32_t*>(stage) + wave * (kChunk / kWaves) * DC / 2;
-            for (int i = lane; i < kChunk / kWaves * DC / 2; i += kWave) mine[i] = finite_word<BF16>(mine[i]);
+          if (word & 2) {  // (what they stand for comes after the loop)
+            emptied = true;
+            constexpr int PIECES = SLICE / 8;  // of this wave's values, which it alone reads from here on
+            for (int i = lane; i < kChunk * PIECES; i += kWave) {
+              const int t = i / PIECES, piece = wave * PIECES + i % PIECES;
+              uint32_t* x = reinterpret_cast<uint32_t*>(stage + t * DC * 2 + (piece ^ latent_swizzle(t)) * 16);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = finite_word<BF16>(x[e]);
+            }
           }
           // every pair's maximum over the chunk, then the state and the weights under the new one
           if (scores) {
@@ -553,17 +565,20 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
           float by = 1.f;  // of my_pair
 #pragma unroll
           for (int c = 0; c < NT; ++c) {
-            const float top = fmaxf(m[c], fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]));
-            const float b = top == m[c] ? 1.f : fast_exp2(m[c] - top);
-            m[c] = top;
-            if (c == ct) my_m = top, by = b;
+            const float top = fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]);
+            // (a pair by its own scores alone: what others see must not change its roundings)
+            const float now = top > m[c] + kRescaleSlack ? top : m[c];
+            const float b = now == m[c] ? 1.f : fast_exp2(m[c] - now);
+            m[c] = now;
+            if (c == ct) my_m = now, by = b;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d][c] *= b;
           }
           if (scores) put_weights(before * by);
           lds_barrier();
-          if (word & 2) read_values();
+          if (EARLY && (word & 2)) read_values();
         }
+        if (!EARLY) read_values();
         // O^T += V^T P^T
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
@@ -579,6 +594,30 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
         }
       }
       w0 = win.w1;
+    }
+
+    if (emptied) {
+      // NaN for the pairs that see such an element (0 times infinity where its score is -inf, and what the
+      // score made of it elsewhere), in the chunks that some pair does not see whole
+      const int first_chunk = max(piece.from, max(0, tile.least_pos + 1) / kChunk);
+#pragma unroll 1
+      for (int t = first_chunk * kChunk; t < min(tile.to * kChunk, tile.context); ++t) {
+        const uint32_t block = quotient((uint32_t)t, p.by_block);
+        const uint32_t id = (uint32_t)p.block_table[piece.request * p.table_stride + block];
+        const uint64_t slot = (uint64_t)(id < (uint32_t)p.num_blocks ? id : 0u) * (uint32_t)p.block_size + ((uint32_t)t - block * (uint32_t)p.block_size);
+        const uint16_t* from = p.cache + slot * (DC + kRope) + wave * SLICE + 4 * mq;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(from + d * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool off = !is_finite<BF16>((i & 2 ? x.y : x.x) >> (16 * (i & 1)) & 0xffffu);
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+              if (off && tile.first_pos + (piece.tile * NC + c * 16 + mt) / p.heads >= t) o[d][c][i] = NAN;
+          }
+        }
+      }
     }
 
     // --- the tile's sums, and its output or this workgroup's part of it

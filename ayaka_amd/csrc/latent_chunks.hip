@@ -13,7 +13,7 @@
 //
 // Keys and values are kept as fp16 whatever the model's type, with a power of two for every 128 tokens,
 // head and of both kinds, chosen from the largest finite value there, so nothing overflows and each
-// element is within 2^-12 of itself (or 2^-39 of its tile's largest): bf16 keys and values would each
+// element is within 2^-11 of itself (or 2^-38 of its tile's largest): bf16 keys and values would each
 // cost the outputs as much as their own rounding does. The scales are uniform in the attention's
 // loop: the key's joins the factor that scores take anyway, the value's the exponent.
 //
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     if (round + 2 < rounds) get(round + 2);
     const int t0 = round * kRound + kg * kPositions;
     if (t0 >= context || t0 > first_masked + 31) continue;  // nothing for these rows
-    uint8_t* here = reinterpret_cast<uint8_t*>(&lds.round[round % kRing]);
+    const uint8_t* here = reinterpret_cast<const uint8_t*>(&lds.round[round % kRing]);
     const uint8_t* k_here = here + kg * kPositions * 256;
     const uint8_t* r_here = here + kg * kPositions * 128;
     const int key_exponent = exponents[(t0 / kTokens) * 2], new_exponent = exponents[(t0 / kTokens) * 2 + 1];
@@ -358,14 +358,6 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     }
     __builtin_amdgcn_sched_barrier(0);
     u32x4 v[8];
-    auto read_values = [&] {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const uint16_t* from = reinterpret_cast<const uint16_t*>(k_here + v_at[d]);
-        const u32x2 x = lds_read_transposed(from), y = lds_read_transposed(from + 16 * kValue);
-        v[d] = u32x4{x.x, x.y, y.x, y.y};
-      }
-    };
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -388,7 +380,12 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
         for (int j = 0; j < 2; ++j) r[h][j] = mfma32<BF16>(a[h][4 + k], qr[j][k], r[h][j]);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
-    read_values();
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(k_here + v_at[d]);
+      const u32x2 x = lds_read_transposed(from), y = lds_read_transposed(from + 16 * kValue);
+      v[d] = u32x4{x.x, x.y, y.x, y.y};
+    }
     __builtin_amdgcn_sched_barrier(0);
 
     const bool masked = t0 + kPositions - 1 > first_masked;
@@ -411,16 +408,29 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
         }
     }
     if (masked && __builtin_amdgcn_ballot_w64(odd)) {
-      // Values that are not finite leave this wave's positions (others that read them here see such a
-      // position's score, or do the same).
-      uint32_t* words = reinterpret_cast<uint32_t*>(here + kRound * 256 + kg * kPositions * 256);
-      for (int i = lane; i < kPositions * kValue / 2; i += kWave) {
-        uint32_t w = words[i];
-        if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
-        if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
-        words[i] = w;
+      // Values that are not finite become zeros, behind NaN for the rows that see them.
+      const uint8_t* mine = here + kRound * 256 + kg * kPositions * 256;
+#pragma unroll 1
+      for (int t = 0; t < kPositions; ++t) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(mine + t * 256 + ((2 * d + (mq >> 1)) ^ swizzle256(t)) * 16 + (mq & 1) * 8);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool off = ((i & 2 ? x.y : x.x) >> (16 * (i & 1)) & 0x7c00u) == 0x7c00u;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (off && t0 + t <= my_pos[j]) o[d][j][i] = NAN;
+          }
+        }
       }
-      read_values();
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((v[d][i] & 0x7c00u) == 0x7c00u) v[d][i] &= 0xffff0000u;
+          if ((v[d][i] & 0x7c000000u) == 0x7c000000u) v[d][i] &= 0xffffu;
+        }
     }
     if (new_exponent > value_exponent) {
       const float by = power(max(-126, value_exponent - new_exponent));
@@ -441,7 +451,9 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     if (__builtin_amdgcn_ballot_w64(passes)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float now = fmaxf(m[j], column_max(top[j]));
+        const float highest = column_max(top[j]);
+        // (a row by its own scores alone: what others see must not change its roundings)
+        const float now = highest > m[j] + kRescaleSlack ? highest : m[j];
         const float by = now == m[j] ? 1.f : fast_exp2(m[j] - now);
         m[j] = now;
         l[j] *= by;

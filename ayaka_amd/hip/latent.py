@@ -15,7 +15,6 @@ import torch
 from ayaka_amd.attention import AttentionMetadata
 from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import _fastpath, _lib
-from ayaka_amd.hip import attention as _attention
 from ayaka_amd.hip._checks import capturing, dtype_name, require_device, require_latent_buffers, require_like, stream_handle
 from ayaka_amd.kvcache import LatentBuffers, LatentWeights
 
@@ -168,7 +167,7 @@ def attend_latent_chunks(q: torch.Tensor, weights: LatentWeights, buffers: Laten
     values are expanded once for all rows, into scratch, so this is for steps of many rows per request
     (some hundred; ``attend_latent`` serves the others without expanding). For steps made by ``plan``;
     captured after one eager call. Expanded keys and values are held in fp16 with scales of
-    their own (2^-12 relative, any magnitude).
+    their own (2^-11 relative, any magnitude).
     """
     op = "attention.attend_latent_chunks"
     key = ("attend_latent_chunks", id(buffers), id(meta), scale,
@@ -203,3 +202,7 @@ def _attend_latent_chunks(op: str, q: torch.Tensor, weights: LatentWeights, buff
         ws_rows, at_once, heads, buffers.latent_dim, buffers.rope_dim, buffers.num_blocks, buffers.block_size,
         _DTYPE_CODES[cache.dtype], float(scale), scratch.data_ptr(), scratch.numel(),
     ), stream, device, True, record)
+
+
+# last: attention takes this module's ops into its family, and this module its plans and scratch
+from ayaka_amd.hip import attention as _attention  # noqa: E402

@@ -85,8 +85,8 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
  *   out[row, h] = sum over t of softmax(scale * q[row, h] . key(h, .))(t) * value(h, t)
  * q [n_rows, num_heads, 128 + 64], out [n_rows, num_heads, 128], keys and values [num_heads, 128,
  * latent_dim], contiguous and 16-byte aligned, as the cache; dtype fp16 or bf16; latent_dim 256 or 512.
- * Expanded keys and values are fp16 under a power of two for every 128 tokens, head and kind (within 2^-12
- * of themselves down to 2^-27 of the largest there, then within 2^-39 of it).
+ * Expanded keys and values are fp16 under a power of two for every 128 tokens, head and kind (within 2^-11
+ * of themselves down to 2^-27 of the largest there, then within 2^-38 of it).
  * The step comes as two device lists of int32 quadruples, made on the host:
  *   token_tiles (request, first position, the request's length, workspace row): every 128 positions of each
  *     request with rows, its workspace rows following each other and starting at a multiple of 128;
