@@ -53,6 +53,12 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, Divisor d) {
   return (uint32_t)(((uint64_t)__umulhi(n, d.magic) + n) >> d.shift);
 }
 
+// Rounded by itself, never part of an fma.
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // 16 bytes a lane to LDS at `to` + 16 * lane (`to` uniform).
 __device__ __forceinline__ void load_to_lds(uint32_t to, const uint8_t* base, uint32_t offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
@@ -230,6 +236,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
 constexpr int kPositions = 32;            // of a wave's step
 constexpr int kRound = 2 * kPositions;    // of both halves of the workgroup
 constexpr int kRing = 3;
+constexpr int kWindow = 256;  // tiles whose exponents wait in LDS
 
 struct Round {
   uint16_t keys[kRound * kNope];
@@ -242,6 +249,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
   struct Shared {
     Round round[kRing];
     float state[4][2][3][16];  // (m, l, exponent) of the later half's rows
+    int32_t exponent[kWindow][2];  // of the tiles being read
   };
   __shared__ __align__(16) Shared lds;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -333,19 +341,32 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     v_at[i] = kRound * 256 + t * 256 + ((2 * i + ((mt & 3) >> 1)) ^ swizzle256(t)) * 16 + (mt & 1) * 8;
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt 0, said to the compiler: its waits for the queries end here
+  // Scores stay as the products give them, to be scaled inside the exponent, but for rows whose maximum
+  // is so large that one scaled and rounded by itself and one scaled in an fma could be whole powers of
+  // two apart, and for a negative scale.
+  bool far[2] = {p.scale_log2 < 0.f, p.scale_log2 < 0.f};
+  bool any_far = p.scale_log2 < 0.f;
 
   const int first_masked = first_pos + rg * 32;  // rows of this wave see up to there, all of them
   for (int round = 0; round < rounds; ++round) {
     if (round + 1 < rounds) wait_loads<LOADS>();
     else wait_loads<0>();
     lds_barrier();
+    if (round % (kWindow * kTokens / kRound) == 0) {
+      // The exponents come by way of LDS: a load of the compiler's own in every round would make it wait
+      // there for all the loads to LDS that are on their way.
+      const int first = round / (kTokens / kRound), n = min(kWindow, (context + kTokens - 1) / kTokens - first);
+      for (int i = tid; i < 2 * n; i += kThreads) lds.exponent[i >> 1][i & 1] = exponents[2 * first + i];
+      lds_barrier();
+    }
     if (round + 2 < rounds) get(round + 2);
     const int t0 = round * kRound + kg * kPositions;
     if (t0 >= context || t0 > first_masked + 31) continue;  // nothing for these rows
     const uint8_t* here = reinterpret_cast<const uint8_t*>(&lds.round[round % kRing]);
     const uint8_t* k_here = here + kg * kPositions * 256;
     const uint8_t* r_here = here + kg * kPositions * 128;
-    const int key_exponent = exponents[(t0 / kTokens) * 2], new_exponent = exponents[(t0 / kTokens) * 2 + 1];
+    const int key_exponent = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][0]);
+    const int new_exponent = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][1]);
 
     f32x4 s[2][2], r[2][2];  // [16 positions][16 rows], of the first part and of the rotary part
     u32x4 a[2][6];
@@ -390,22 +411,29 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
 
     const bool masked = t0 + kPositions - 1 > first_masked;
     bool odd = false;
+    float by[2] = {p.scale_log2, p.scale_log2};  // of what s holds from here on
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float by = __builtin_ldexpf(p.scale_log2, unit[j] + key_exponent);
-      const int seen = my_pos[j] - t0 - 4 * mq;
+      const float ratio = __builtin_ldexpf(1.f, unit[j] + key_exponent);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float t = __builtin_fmaf(s[h][j][i], by, r[h][j][i] * p.scale_log2);
-          if (masked) {
-            odd |= !(__builtin_fabsf(t) < INFINITY);
-            s[h][j][i] = 16 * h + i <= seen ? t : -INFINITY;
-          } else {
-            s[h][j][i] = t;
+        for (int i = 0; i < 4; ++i) s[h][j][i] = __builtin_fmaf(s[h][j][i], ratio, r[h][j][i]);
+    }
+    if (masked || any_far) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int seen = my_pos[j] - t0 - 4 * mq;
+        const bool whole = masked || far[j];
+        by[j] = whole ? 1.f : p.scale_log2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            odd |= !(__builtin_fabsf(s[h][j][i]) < INFINITY);
+            s[h][j][i] = 16 * h + i <= seen ? (whole ? product(s[h][j][i], p.scale_log2) : s[h][j][i]) : -INFINITY;
           }
-        }
+      }
     }
     if (masked && __builtin_amdgcn_ballot_w64(odd)) {
       // Values that are not finite become zeros, behind NaN for the rows that see them.
@@ -433,11 +461,11 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
         }
     }
     if (new_exponent > value_exponent) {
-      const float by = power(max(-126, value_exponent - new_exponent));
+      const float down = power(max(-126, value_exponent - new_exponent));
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d][j] *= by;
+        for (int d = 0; d < 8; ++d) o[d][j] *= down;
       value_exponent = new_exponent;
     }
     float top[2];
@@ -445,7 +473,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       top[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])),
-                     fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
+                     fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3]))) * by[j];
       passes |= top[j] > m[j] + kRescaleSlack;
     }
     if (__builtin_amdgcn_ballot_w64(passes)) {
@@ -454,12 +482,21 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
         const float highest = column_max(top[j]);
         // (a row by its own scores alone: what others see must not change its roundings)
         const float now = highest > m[j] + kRescaleSlack ? highest : m[j];
-        const float by = now == m[j] ? 1.f : fast_exp2(m[j] - now);
+        const float down = now == m[j] ? 1.f : fast_exp2(m[j] - now);
         m[j] = now;
-        l[j] *= by;
+        l[j] *= down;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d][j] *= by;
+        for (int d = 0; d < 8; ++d) o[d][j] *= down;
+        far[j] |= __builtin_fabsf(now) > 16777216.f && now != -INFINITY;
+        if (far[j] && by[j] != 1.f) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[h][j][i] = product(s[h][j][i], p.scale_log2);
+          by[j] = 1.f;
+        }
       }
+      any_far = __builtin_amdgcn_ballot_w64(far[0] | far[1]) != 0;
     }
     // the values' scale: weights carry 2^lower, the sum takes it back
     const int below = max(-126, new_exponent - value_exponent);
@@ -467,12 +504,12 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     u32x4 w[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float base = m[j] == -INFINITY ? 0.f : m[j];
+      const float from = lower - (m[j] == -INFINITY ? 0.f : m[j]);
       float e[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[4 * h + i] = fast_exp2((s[h][j][i] - base) + lower);
+        for (int i = 0; i < 4; ++i) e[4 * h + i] = fast_exp2(__builtin_fmaf(s[h][j][i], by[j], from));
       l[j] = __builtin_fmaf(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])), raise, l[j]);
       w[j] = u32x4{two_halves(e[0], e[1]), two_halves(e[2], e[3]), two_halves(e[4], e[5]), two_halves(e[6], e[7])};
     }
