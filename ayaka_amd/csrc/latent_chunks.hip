@@ -75,8 +75,9 @@ __device__ __forceinline__ uint32_t lds_offset(T* p) {
   return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) T*)p);
 }
 
-// Where piece c (16 bytes) of row r stands in LDS, for rows of 128 and of 256 bytes: any 16 rows that
+// Where piece c (16 bytes) of row r stands in LDS, for rows of 64, 128 and 256 bytes: any 16 rows that
 // one cycle's reads touch are spread over all 64 banks.
+__device__ __forceinline__ int swizzle64(int r) { return (r >> 2) & 3; }
 __device__ __forceinline__ int swizzle128(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int swizzle256(int r) { return r & 15; }
 
@@ -96,12 +97,12 @@ __device__ __forceinline__ uint32_t two_halves(float a, float b) {
 
 // --- expansion
 
-constexpr int kStep = 64;        // of DC in LDS at a time
+constexpr int kStep = 32;        // of DC in LDS at a time
 constexpr int kSteps = 3;        // in flight
 constexpr int kOutputs = kNope + kValue;
 
 template <int DC, bool BF16>
-__global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const LatentChunkParams p) {
+__global__ __launch_bounds__(kThreads, 4) void latent_expand_kernel(const LatentChunkParams p) {
   struct Shared {
     uint16_t token[kSteps][kTokens * kStep];
     uint16_t weight[kSteps][kOutputs * kStep];
@@ -116,41 +117,39 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
   const int64_t ws_row = p.token_tiles[4 * tile + 3];
   const int real_head = p.first_head + head;
 
-  // What this wave fetches of each step, 8 rows a load: 16 tokens and 32 outputs.
-  const uint8_t* from[6];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = wave * 16 + i * 8 + (lane >> 3);
+  auto slot_of = [&](int row) {
     const uint32_t pos = (uint32_t)min(first + row, length - 1);
     const uint32_t block = quotient(pos, p.by_block);
     const uint32_t id = (uint32_t)p.block_table[request * p.table_stride + block];
-    const uint64_t slot = (uint64_t)(id < (uint32_t)p.num_blocks ? id : 0u) * (uint32_t)p.block_size + (pos - block * (uint32_t)p.block_size);
-    from[i] = reinterpret_cast<const uint8_t*>(p.cache) + slot * ((DC + kRope) * 2) + ((lane & 7) ^ swizzle128(row)) * 16;
-  }
+    return reinterpret_cast<const uint8_t*>(p.cache) +
+           ((uint64_t)(id < (uint32_t)p.num_blocks ? id : 0u) * (uint32_t)p.block_size + (pos - block * (uint32_t)p.block_size)) * ((DC + kRope) * 2);
+  };
+  // What this wave fetches of each step, 16 rows a load: 16 tokens and 32 outputs.
+  const uint8_t* from[3];
+  const int row16 = lane >> 2, piece16 = ((lane & 3) ^ swizzle64(row16)) * 16;
+  from[0] = slot_of(wave * 16 + row16) + piece16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = wave * 32 + i * 8 + (lane >> 3);
+  for (int i = 0; i < 2; ++i) {
+    const int row = wave * 32 + i * 16 + row16;
     const uint16_t* w = row < kNope ? p.keys + ((int64_t)real_head * kNope + row) * DC
                                     : p.values + ((int64_t)real_head * kValue + row - kNope) * DC;
-    from[2 + i] = reinterpret_cast<const uint8_t*>(w) + ((lane & 7) ^ swizzle128(row)) * 16;
+    from[1 + i] = reinterpret_cast<const uint8_t*>(w) + piece16;
   }
   const uint32_t token_lds = lds_offset(&lds.token[0][0]), weight_lds = lds_offset(&lds.weight[0][0]);
   auto get = [&](int step) {
     const uint32_t s = (uint32_t)(step % kSteps);
+    load_to_lds(token_lds + s * (kTokens * kStep * 2) + wave * 16 * (kStep * 2), from[0] + step * (kStep * 2));
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      load_to_lds(token_lds + s * (kTokens * kStep * 2) + (wave * 16 + i * 8) * (kStep * 2), from[i] + step * (kStep * 2));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      load_to_lds(weight_lds + s * (kOutputs * kStep * 2) + (wave * 32 + i * 8) * (kStep * 2), from[2 + i] + step * (kStep * 2));
+      load_to_lds(weight_lds + s * (kOutputs * kStep * 2) + (wave * 32 + i * 16) * (kStep * 2), from[1 + i] + step * (kStep * 2));
   };
   // the rotary parts go along once, from the first head's workgroups
   if (real_head == 0) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = wave * 16 + i * 8 + (lane >> 3);
-      const uint8_t* rope = from[i] - ((lane & 7) ^ swizzle128(row)) * 16 + DC * 2 + (lane & 7) * 16;
-      *reinterpret_cast<u32x4*>(p.ws_rope + (ws_row + row) * kRope + (lane & 7) * 8) = *reinterpret_cast<const u32x4*>(rope);
+      *reinterpret_cast<u32x4*>(p.ws_rope + (ws_row + row) * kRope + (lane & 7) * 8) =
+          *reinterpret_cast<const u32x4*>(slot_of(row) + DC * 2 + (lane & 7) * 16);
     }
   }
 
@@ -166,28 +165,24 @@ __global__ __launch_bounds__(kThreads, 1) void latent_expand_kernel(const Latent
   get(1);
 #pragma unroll
   for (int step = 0; step < STEPS; ++step) {
-    if (step + 1 < STEPS) wait_loads<6>();
+    if (step + 1 < STEPS) wait_loads<3>();
     else wait_loads<0>();
     lds_barrier();
     if (step + 2 < STEPS) get(step + 2);
     const uint8_t* token = reinterpret_cast<const uint8_t*>(lds.token[step % kSteps]) + m * 64 * kStep * 2;
     const uint8_t* weight = reinterpret_cast<const uint8_t*>(lds.weight[step % kSteps]) + n * 64 * kStep * 2;
-    u32x4 a[2][4], b[2][4];
+    u32x4 a[4], b[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = i * 16 + mt, piece = (4 * k + mq) ^ swizzle128(row);
-        a[k][i] = *reinterpret_cast<const u32x4*>(weight + row * (kStep * 2) + piece * 16);
-        b[k][i] = *reinterpret_cast<const u32x4*>(token + row * (kStep * 2) + piece * 16);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int at = (i * 16 + mt) * (kStep * 2) + (mq ^ swizzle64(mt)) * 16;
+      a[i] = *reinterpret_cast<const u32x4*>(weight + at);
+      b[i] = *reinterpret_cast<const u32x4*>(token + at);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma32<BF16>(a[k][i], b[k][j], acc[i][j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma32<BF16>(a[i], b[j], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
   }
 
