@@ -57,7 +57,7 @@ constexpr int kChunk = 32;   // positions
 constexpr int kStages = 4;   // chunks in LDS
 constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kTableWindow = 1024;      // block-table entries in LDS
+constexpr int kTableWindow = 768;       // block-table entries in LDS
 constexpr int kPlaceWords = 8;
 // What a tile of NC pairs costs beside its chunks (queries, first loads, output), in chunks.
 constexpr int tile_cost(int nc) { return nc == 64 ? 8 : 5; }
@@ -103,19 +103,17 @@ __host__ __device__ constexpr int latent_swizzle(int t) { return t & 15; }
 __host__ __device__ constexpr int rope_swizzle(int t) { return (t >> 1) & 7; }
 __host__ __device__ constexpr int weight_swizzle(int pair) { return (pair >> 2) & 3; }
 
-template <int DC>
-struct Stage {
-  uint16_t latent[kChunk * DC];
-  uint16_t rope[kChunk * kRope];
-};
+// Tiles of 64 pairs score a chunk while they weigh the one before it.
+constexpr bool ahead(int nt) { return nt == 4; }
 
 template <int DC, int NT>
 struct __align__(16) LatentShared {
-  Stage<DC> stage[kStages];
-  uint16_t weight[2][NT * 16 * kChunk];  // [pair][position]
+  uint16_t latent[kStages][kChunk * DC];
+  uint16_t rope[ahead(NT) ? 3 : kStages][kChunk * kRope];
+  uint16_t weight[ahead(NT) ? 2 : 1][2][NT * 16 * kChunk];  // [chunk][high, low][pair][position]
   int32_t table[kTableWindow];
   float exchange[2][NT * 16];
-  int32_t flag[2];
+  int32_t flag[3];
   int32_t sums[kWaves][2];
   int32_t place[8];
 };
@@ -306,7 +304,7 @@ __device__ __forceinline__ uint32_t slot_of(const LatentParams& p, const int32_t
 // Ask for a share of a chunk (of several waves `wave`): MINE rows of latents, 1024 bytes a load, and one load of their
 // rotary parts, 8 lanes a position.
 template <int DC, int MINE>
-__device__ __forceinline__ void fetch(const LatentParams& p, uint32_t slot, int wave, uint32_t stage) {
+__device__ __forceinline__ void fetch(const LatentParams& p, uint32_t slot, int wave, uint32_t latent, uint32_t rope) {
   static_assert(MINE <= 8, "a load of rotary parts covers 8 positions");
   constexpr int ROW = (DC + kRope) * 2;
   constexpr int PER_LOAD = 1024 / (DC * 2);
@@ -314,7 +312,7 @@ __device__ __forceinline__ void fetch(const LatentParams& p, uint32_t slot, int 
   const uint8_t* cache = reinterpret_cast<const uint8_t*>(p.cache);
 #pragma unroll
   for (int j = 0; j < MINE / PER_LOAD; ++j) {
-    const uint32_t to = stage + (uint32_t)((first + j * PER_LOAD) * DC * 2);
+    const uint32_t to = latent + (uint32_t)((first + j * PER_LOAD) * DC * 2);
     if constexpr (PER_LOAD == 1) {
       const uint32_t s = __builtin_amdgcn_readlane(slot, j);
       load_to_lds(to, cache + (uint64_t)s * ROW, (uint32_t)((lane ^ latent_swizzle(first + j)) * 16));
@@ -326,7 +324,7 @@ __device__ __forceinline__ void fetch(const LatentParams& p, uint32_t slot, int 
   }
   const uint32_t s = (uint32_t)__shfl((int)slot, lane >> 3);
   if (MINE == 8 || lane < MINE * 8)
-    load_to_lds(stage + (uint32_t)(kChunk * DC * 2 + first * kRope * 2),
+    load_to_lds(rope + (uint32_t)(first * kRope * 2),
                 cache + (uint64_t)s * ROW + (DC * 2 + ((lane & 7) ^ rope_swizzle(first + (lane >> 3))) * 16));
 }
 
@@ -403,6 +401,8 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
   // Waves that score (2 for each 16 pairs) and waves that fetch: the last four, which have no scores
   // up to 32 pairs, or all.
   constexpr int SCORING = 2 * NT;
+  constexpr bool AHEAD = ahead(NT);
+  constexpr int DEPTH = AHEAD ? 2 : kStages - 1;  // chunks on their way or here, beside those worked on
   constexpr int FETCHING = NT == 4 ? kWaves : 4;
   constexpr int MINE = kChunk / FETCHING;  // positions of a chunk that a wave fetches
   constexpr int LOADS = MINE * DC * 2 / 1024 + 1;
@@ -419,13 +419,14 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
   if (!find_place<NC>(p, lds, blockIdx.x, gridDim.x, walk)) return;
 
   const uint32_t lds_base = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) Shared*)&lds);
+  auto rope_of = [](int chunk) { return AHEAD ? chunk % 3 : chunk & (kStages - 1); };
   // a lane's offsets into a stage (bytes)
   const int key = kg * 16 + mt;
   int k_at[4], r_at[2], v_at[DT];
 #pragma unroll
   for (int i = 0; i < 4; ++i) k_at[i] = key * DC * 2 + ((4 * i + mq) ^ latent_swizzle(key)) * 16;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) r_at[i] = kChunk * DC * 2 + key * kRope * 2 + ((4 * i + mq) ^ rope_swizzle(key)) * 16;
+  for (int i = 0; i < 2; ++i) r_at[i] = key * kRope * 2 + ((4 * i + mq) ^ rope_swizzle(key)) * 16;
 #pragma unroll
   for (int i = 0; i < DT; ++i) {
     const int t = 4 * mq + (mt >> 2), piece = wave * (SLICE / 8) + 2 * i + ((mt & 3) >> 1);
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
       const Window win = window_of(p, tile, w0);
       __syncthreads();
       stage_table(p, piece.request, win, lds.table);
-      if (tid < 2) lds.flag[tid] = 0;
+      if (tid < 3) lds.flag[tid] = 0;
       __syncthreads();
       uint32_t slot = 0;  // of the next chunk to ask for, looked up ahead
       auto look_up = [&](int chunk) {
@@ -461,136 +462,173 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
           slot = slot_of<MINE>(p, lds.table, win.b0, chunk * kChunk + fetching * MINE, tile.context - 1);
       };
       auto get = [&](int chunk) {
-        fetch<DC, MINE>(p, slot, fetching, lds_base + (uint32_t)((chunk & (kStages - 1)) * sizeof(Stage<DC>)));
+        fetch<DC, MINE>(p, slot, fetching, lds_base + (uint32_t)((chunk & (kStages - 1)) * sizeof(lds.latent[0])),
+                        lds_base + (uint32_t)(offsetof(Shared, rope) + rope_of(chunk) * sizeof(lds.rope[0])));
         look_up(chunk + 1);
       };
       if (fetching >= 0) {
         look_up(w0);
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i)
+        for (int i = 0; i < DEPTH; ++i)
           if (w0 + i < win.w1) get(w0 + i);
       }
       if (scores && w0 == piece.from) load_query<DC>(p, tile, real ? my_pair : NC, q);
       if (scores) queries_are_here();
       drop_query(real, q);
 
-      for (int chunk = w0; chunk < win.w1; ++chunk) {
-        uint8_t* stage = reinterpret_cast<uint8_t*>(&lds.stage[chunk & (kStages - 1)]);
-        if (fetching >= 0) {
-          if (chunk + 2 < win.w1) wait_loads<2 * LOADS>();
-          else if (chunk + 1 < win.w1) wait_loads<LOADS>();
-          else wait_loads<0>();
-        }
-        lds_barrier();  // the chunk is here, and nobody works on the one before it
-        // Of two waves of a SIMD that both fetch, one does so before its scores and one after them.
-        const bool more = fetching >= 0 && chunk + kStages - 1 < win.w1;
-        const bool early = more && (NT < 4 || wave < 4), late = more && !early;
-        if (early) get(chunk + kStages - 1);
-        if (tid == 0) lds.flag[(chunk + 1) & 1] = 0;
-
+      f32x4 s;       // the scores of a chunk
+      float before;  // and the sum without it
+      bool masked;
+      auto flag_of = [&](int chunk) -> int32_t& { return lds.flag[AHEAD ? chunk % 3 : chunk & 1]; };
+      // weights of this wave's scores under the maximum my_m, on top of the sum `so_far`
+      auto put_weights = [&](int chunk, float so_far) {
+        const float base = my_m == -INFINITY ? 0.f : my_m;
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[i] - base);
+        l = so_far + ((w[0] + w[1]) + (w[2] + w[3]));
+        u32x2 hi, lo;
+        split_weights4<BF16>(w, hi, lo);
+        const int row = my_pair * kChunk + (mq ^ weight_swizzle(my_pair)) * 8 + 4 * kg;
+        auto& weight = lds.weight[AHEAD ? chunk & 1 : 0];
+        *reinterpret_cast<u32x2*>(&weight[0][row]) = hi;
+        if constexpr (split_p(BF16)) *reinterpret_cast<u32x2*>(&weight[1][row]) = lo;
+      };
+      auto score = [&](int chunk) {
         const int t0 = chunk * kChunk;
-        const bool masked = t0 + kChunk > tile.context || t0 + kChunk - 1 > tile.least_pos;
-        f32x4 s{0.f, 0.f, 0.f, 0.f};
-        const float before = l;  // the sum without this chunk
-        // weights of this wave's scores under the maximum my_m, on top of the sum `so_far`
-        auto put_weights = [&](float so_far) {
-          const float base = my_m == -INFINITY ? 0.f : my_m;
-          float w[4];
+        const uint8_t* latent = reinterpret_cast<const uint8_t*>(lds.latent[chunk & (kStages - 1)]);
+        const uint8_t* rope = reinterpret_cast<const uint8_t*>(lds.rope[rope_of(chunk)]);
+        before = l;
+        masked = t0 + kChunk > tile.context || t0 + kChunk - 1 > tile.least_pos;
+        s = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 t{0.f, 0.f, 0.f, 0.f};  // (two sums: one would be a chain of products that wait for each other)
+        read_ahead<KS + 2, KS != 16 ? 5 : NT == 4 ? 2 : 6>(
+            [&](int k) { return *reinterpret_cast<const u32x4*>(k < KS ? latent + k_at[k & 3] + (k >> 2) * 256 : rope + r_at[k & 1]); },
+            [&](int k, u32x4 a) {
+              if (k & 1) t = mfma32<BF16>(a, q[k], t);
+              else s = mfma32<BF16>(a, q[k], s);
+            });
+        s += t;
+        bool passes = false, odd = false;
+        const int seen = min(my_pos, tile.context - 1) - t0 - kg * 16 - 4 * mq;  // of the lane's 4 positions: i <= seen
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[i] - base);
-          l = so_far + ((w[0] + w[1]) + (w[2] + w[3]));
-          u32x2 hi, lo;
-          split_weights4<BF16>(w, hi, lo);
-          const int row = my_pair * kChunk + (mq ^ weight_swizzle(my_pair)) * 8 + 4 * kg;
-          *reinterpret_cast<u32x2*>(&lds.weight[0][row]) = hi;
-          if constexpr (split_p(BF16)) *reinterpret_cast<u32x2*>(&lds.weight[1][row]) = lo;
-        };
+        for (int i = 0; i < 4; ++i) {
+          if (masked) odd |= !(__builtin_fabsf(s[i]) < INFINITY);
+          const float t = product(s[i], p.scale_log2);
+          s[i] = !masked || i <= seen ? t : -INFINITY;
+          passes |= s[i] > my_m + kRescaleSlack;
+        }
+        const int word = (__builtin_amdgcn_ballot_w64(passes) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(odd) ? 2 : 0);
+        if (word && lane == 0) atomicOr(&flag_of(chunk), word);
+        put_weights(chunk, before);
+      };
+      u32x4 v[DT];  // this wave's values of a chunk
+      auto read_values = [&](int chunk) {
+        const uint8_t* latent = reinterpret_cast<const uint8_t*>(lds.latent[chunk & (kStages - 1)]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const uint16_t* at = reinterpret_cast<const uint16_t*>(latent + v_at[d]);
+          const u32x2 a = lds_read_transposed(at), b = lds_read_transposed(at + 16 * DC);
+          v[d] = u32x4{a.x, a.y, b.x, b.y};
+        }
+      };
+      // Where a score passed its pair's maximum, or one is not finite; true: values changed.
+      auto settle = [&](int chunk) {
+        const int word = __builtin_amdgcn_readfirstlane(flag_of(chunk));
+        if (!word) return false;
+        if (word & 2) {  // (what they stand for comes after the loop)
+          emptied = true;
+          constexpr int PIECES = SLICE / 8;  // of this wave's values, which it alone reads from here on
+          for (int i = lane; i < kChunk * PIECES; i += kWave) {
+            const int t = i / PIECES, piece = wave * PIECES + i % PIECES;
+            uint32_t* x = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(lds.latent[chunk & (kStages - 1)]) + t * DC * 2 +
+                                                      (piece ^ latent_swizzle(t)) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = finite_word<BF16>(x[e]);
+          }
+        }
+        // every pair's maximum over the chunk, then the state and the weights under the new one
         if (scores) {
-          f32x4 t{0.f, 0.f, 0.f, 0.f};  // (two sums: one would be a chain of products that wait for each other)
-          read_ahead<KS + 2, KS != 16 ? 5 : NT == 4 ? 2 : 6>(
-              [&](int k) {
-                return *reinterpret_cast<const u32x4*>(stage + (k < KS ? k_at[k & 3] + (k >> 2) * 256 : r_at[k & 1]));
-              },
-              [&](int k, u32x4 a) {
-                if (k & 1) t = mfma32<BF16>(a, q[k], t);
-                else s = mfma32<BF16>(a, q[k], s);
-              });
-          s += t;
-          bool passes = false, odd = false;
-          const int seen = min(my_pos, tile.context - 1) - t0 - kg * 16 - 4 * mq;  // of the lane's 4 positions: i <= seen
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (masked) odd |= !(__builtin_fabsf(s[i]) < INFINITY);
-            const float t = product(s[i], p.scale_log2);
-            s[i] = !masked || i <= seen ? t : -INFINITY;
-            passes |= s[i] > my_m + kRescaleSlack;
-          }
-          const int word = (__builtin_amdgcn_ballot_w64(passes) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(odd) ? 2 : 0);
-          if (word && lane == 0) atomicOr(&lds.flag[chunk & 1], word);
-          put_weights(before);
+          const float top = column_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+          if (mq == 0) lds.exchange[kg][my_pair] = top;
         }
-        if (late) get(chunk + kStages - 1);
-        // this wave's values, on their way while it waits for the weights (of 64 pairs, only afterwards: the
-        // registers hold no more)
-        constexpr bool EARLY = NT < 4;
-        u32x4 v[DT];
-        auto read_values = [&] {
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const uint16_t* at = reinterpret_cast<const uint16_t*>(stage + v_at[d]);
-            const u32x2 a = lds_read_transposed(at), b = lds_read_transposed(at + 16 * DC);
-            v[d] = u32x4{a.x, a.y, b.x, b.y};
-          }
-        };
-        if (EARLY) read_values();
         lds_barrier();
-        const int word = __builtin_amdgcn_readfirstlane(lds.flag[chunk & 1]);
-        if (word) {
-          if (word & 2) {  // (what they stand for comes after the loop)
-            emptied = true;
-            constexpr int PIECES = SLICE / 8;  // of this wave's values, which it alone reads from here on
-            for (int i = lane; i < kChunk * PIECES; i += kWave) {
-              const int t = i / PIECES, piece = wave * PIECES + i % PIECES;
-              uint32_t* x = reinterpret_cast<uint32_t*>(stage + t * DC * 2 + (piece ^ latent_swizzle(t)) * 16);
+        float by = 1.f;  // of my_pair
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = finite_word<BF16>(x[e]);
-            }
-          }
-          // every pair's maximum over the chunk, then the state and the weights under the new one
-          if (scores) {
-            const float top = column_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-            if (mq == 0) lds.exchange[kg][my_pair] = top;
-          }
-          lds_barrier();
-          float by = 1.f;  // of my_pair
+        for (int c = 0; c < NT; ++c) {
+          const float top = fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]);
+          // (a pair by its own scores alone: what others see must not change its roundings)
+          const float now = top > m[c] + kRescaleSlack ? top : m[c];
+          const float b = now == m[c] ? 1.f : fast_exp2(m[c] - now);
+          m[c] = now;
+          if (c == ct) my_m = now, by = b;
 #pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            const float top = fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]);
-            // (a pair by its own scores alone: what others see must not change its roundings)
-            const float now = top > m[c] + kRescaleSlack ? top : m[c];
-            const float b = now == m[c] ? 1.f : fast_exp2(m[c] - now);
-            m[c] = now;
-            if (c == ct) my_m = now, by = b;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][c] *= b;
-          }
-          if (scores) put_weights(before * by);
-          lds_barrier();
-          if (EARLY && (word & 2)) read_values();
+          for (int d = 0; d < DT; ++d) o[d][c] *= b;
         }
-        if (!EARLY) read_values();
-        // O^T += V^T P^T
+        if (scores) put_weights(chunk, before * by);
+        lds_barrier();
+        return (word & 2) != 0;
+      };
+      auto weigh = [&](int chunk) {  // O^T += V^T P^T
+        const auto& weight = lds.weight[AHEAD ? chunk & 1 : 0];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
           const int row = (c * 16 + mt) * kChunk + (mq ^ weight_swizzle(mt)) * 8;
-          const u32x4 hi = *reinterpret_cast<const u32x4*>(&lds.weight[0][row]);
+          const u32x4 hi = *reinterpret_cast<const u32x4*>(&weight[0][row]);
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[d][c] = mfma32<BF16>(v[d], hi, o[d][c]);
           if constexpr (split_p(BF16)) {
-            const u32x4 lo = *reinterpret_cast<const u32x4*>(&lds.weight[1][row]);
+            const u32x4 lo = *reinterpret_cast<const u32x4*>(&weight[1][row]);
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d][c] = mfma32<BF16>(v[d], lo, o[d][c]);
           }
+        }
+      };
+
+      if constexpr (AHEAD) {
+        // One barrier a chunk. Of the two waves of a SIMD one weighs the last chunk and then scores this
+        // one, the other the other way round: the products of one run beside the exponentials of the other.
+        if (w0 + 1 < win.w1) wait_loads<LOADS>();
+        else wait_loads<0>();
+        lds_barrier();
+        for (int chunk = w0; chunk <= win.w1; ++chunk) {
+          if (tid == 0) lds.flag[(chunk + 1) % 3] = 0;
+          const bool more = chunk + 2 < win.w1;
+          if (wave < 4) {
+            if (more) get(chunk + 2);
+            if (chunk > w0) {
+              read_values(chunk - 1);
+              weigh(chunk - 1);
+            }
+          }
+          if (chunk < win.w1) score(chunk);
+          if (wave >= 4) {
+            if (more) get(chunk + 2);
+            if (chunk > w0) {
+              read_values(chunk - 1);
+              weigh(chunk - 1);
+            }
+          }
+          if (more) wait_loads<LOADS>();
+          else wait_loads<0>();
+          lds_barrier();  // the next chunk is here, and this one's weights
+          if (chunk < win.w1) settle(chunk);
+        }
+      } else {
+        for (int chunk = w0; chunk < win.w1; ++chunk) {
+          if (fetching >= 0) {
+            if (chunk + 2 < win.w1) wait_loads<2 * LOADS>();
+            else if (chunk + 1 < win.w1) wait_loads<LOADS>();
+            else wait_loads<0>();
+          }
+          lds_barrier();  // the chunk is here, and nobody works on the one before it
+          if (fetching >= 0 && chunk + DEPTH < win.w1) get(chunk + DEPTH);
+          if (tid == 0) lds.flag[(chunk + 1) & 1] = 0;
+          if (scores) score(chunk);
+          read_values(chunk);  // on their way while the wave waits for the weights
+          lds_barrier();
+          if (settle(chunk)) read_values(chunk);
+          weigh(chunk);
         }
       }
       w0 = win.w1;

@@ -235,11 +235,11 @@ hipError_t launch_rotate_store(RotateParams p, int type, bool side_by_side, int 
   p.tasks_per_row = tasks;
   if (tasks == 0) return hipSuccess;
   p.by_tasks = divisor_of(tasks);
-  // Rows per workgroup and workgroups per row: rows share a workgroup (up to 4 tasks a lane) once
+  // Rows per workgroup and workgroups per row: rows share a workgroup (up to 2 tasks a lane; with 4 a prefill step of 16 heads took 44 us, with 2 43) once
   // there are two workgroups for every compute unit, and a row of many heads is dealt to several
   // while there are fewer.
   const int wanted = 2 * compute_units;
-  int rows = std::min({std::max(1, p.n_rows / wanted), std::max(1, 4 * kThreads / tasks), kMostAngles / std::max(1, p.pairs)});
+  int rows = std::min({std::max(1, p.n_rows / wanted), std::max(1, 2 * kThreads / tasks), kMostAngles / std::max(1, p.pairs)});
   rows = std::max(1, rows);
   const int groups = (p.n_rows + rows - 1) / rows;
   const int split = std::max(1, std::min((rows * tasks + kThreads - 1) / kThreads, wanted / groups));
