@@ -422,11 +422,10 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
   auto rope_of = [](int chunk) { return AHEAD ? chunk % 3 : chunk & (kStages - 1); };
   // a lane's offsets into a stage (bytes)
   const int key = kg * 16 + mt;
-  int k_at[4], r_at[2], v_at[DT];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) k_at[i] = key * DC * 2 + ((4 * i + mq) ^ latent_swizzle(key)) * 16;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) r_at[i] = key * kRope * 2 + ((4 * i + mq) ^ rope_swizzle(key)) * 16;
+  // (the others of its places differ from the first in a few bits, which costs an instruction each and no register)
+  int k_first = key * DC * 2 + (mq ^ latent_swizzle(key)) * 16;
+  int r_first = key * kRope * 2 + (mq ^ rope_swizzle(key)) * 16;
+  int v_at[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) {
     const int t = 4 * mq + (mt >> 2), piece = wave * (SLICE / 8) + 2 * i + ((mt & 3) >> 1);
@@ -499,11 +498,12 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
         const uint8_t* latent = reinterpret_cast<const uint8_t*>(lds.latent[chunk & (kStages - 1)]);
         const uint8_t* rope = reinterpret_cast<const uint8_t*>(lds.rope[rope_of(chunk)]);
         before = l;
+        asm volatile("" : "+v"(k_first), "+v"(r_first));
         masked = t0 + kChunk > tile.context || t0 + kChunk - 1 > tile.least_pos;
         s = f32x4{0.f, 0.f, 0.f, 0.f};
         f32x4 t{0.f, 0.f, 0.f, 0.f};  // (two sums: one would be a chain of products that wait for each other)
         read_ahead<KS + 2, KS != 16 ? 5 : NT == 4 ? 2 : 6>(
-            [&](int k) { return *reinterpret_cast<const u32x4*>(k < KS ? latent + k_at[k & 3] + (k >> 2) * 256 : rope + r_at[k & 1]); },
+            [&](int k) { return *reinterpret_cast<const u32x4*>(k < KS ? latent + (k_first ^ (k & 3) << 6) + (k >> 2) * 256 : rope + (r_first ^ (k & 1) << 6)); },
             [&](int k, u32x4 a) {
               if (k & 1) t = mfma32<BF16>(a, q[k], t);
               else s = mfma32<BF16>(a, q[k], s);
