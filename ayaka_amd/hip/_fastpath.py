@@ -66,8 +66,7 @@ def signature(tensors: tuple) -> tuple:
         return (a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), a.shape, b.shape, c.shape,
                 d.shape, a.stride(), b.stride(), c.stride(), d.stride(), a.dtype, b.dtype, c.dtype,
                 d.dtype)
-    return (tuple(t.data_ptr() for t in tensors) + tuple(t.shape for t in tensors)
-            + tuple(t.stride() for t in tensors) + tuple(t.dtype for t in tensors))
+    return tuple([x for t in tensors for x in (t.data_ptr(), t.shape, t.stride(), t.dtype)])
 
 
 def convert(types: list, args: tuple) -> tuple:

@@ -186,6 +186,16 @@ def _turned(op: str, name: str, rows: torch.Tensor, out: torch.Tensor | None, n_
 _NO_ROWS = (0, 0, 0, 0, 0, 0)
 
 
+def _given(*tensors: torch.Tensor | None) -> tuple[tuple, int]:
+    """Those of a call's tensors that are not ``None``, and which are, as bits. (A rotation's own tensor
+    is not among them: it goes by the rotation's identity, which is frozen and kept.)"""
+    absent = 0
+    for i, t in enumerate(tensors):
+        if t is None:
+            absent |= 1 << i
+    return tuple([t for t in tensors if t is not None]) if absent else tensors, absent
+
+
 def _replayed(meta: AttentionMetadata, key: tuple, keep: tuple, call) -> None:
     """``call(record)``, or the launch it recorded in the step's plan when it ran with this ``key``."""
     cache = getattr(meta.plan, "launches", None)
@@ -213,12 +223,10 @@ def rotate(q: torch.Tensor | None, k: torch.Tensor | None, meta: AttentionMetada
     write: ``store`` takes the rotated keys.
     """
     op = "kvcache.rotate"
-    given = [t for t in (q, k) if t is not None]
-    if not given:
+    if q is None and k is None:
         raise BackendError(f"{op}: neither q nor k is given", context={"op": op})
-    tensors = (*given, q if q_out is None else q_out, k if k_out is None else k_out, rotary.turns)
-    key = ("rotate", id(meta), id(rotary), q is None, k is None,
-           _fastpath.signature(tuple(t for t in tensors if t is not None)))
+    tensors, absent = _given(q, k, q_out, k_out)
+    key = ("rotate", id(meta), id(rotary), absent, _fastpath.signature(tensors))
     _replayed(meta, key, (meta, rotary), lambda record: _rotate(op, q, k, meta, rotary, q_out, k_out, record))
 
 
@@ -255,10 +263,8 @@ def store_rotated(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, buff
     of the rows. Rows of padding requests are not stored.
     """
     op = "kvcache.store_rotated"
-    tensors = (k, v, buffers.k, buffers.v, rotary.turns)
-    if q is not None:
-        tensors += (q, q if q_out is None else q_out)
-    key = ("store_rotated", id(buffers), id(meta), id(rotary), _fastpath.signature(tensors))
+    tensors, absent = _given(k, v, buffers.k, buffers.v, q, q_out)
+    key = ("store_rotated", id(buffers), id(meta), id(rotary), absent, _fastpath.signature(tensors))
     _replayed(meta, key, (buffers, meta, rotary),
               lambda record: _store_rotated(op, q, k, v, buffers, meta, rotary, q_out, record))
 
@@ -296,12 +302,8 @@ def store_latent(latent: torch.Tensor, k_rope: torch.Tensor, buffers: LatentBuff
     Rows of padding requests are not stored.
     """
     op = "kvcache.store_latent"
-    tensors = (latent, k_rope, buffers.k)
-    if rotary is not None:
-        tensors += (rotary.turns,)
-    if q is not None:
-        tensors += (q, q if q_out is None else q_out)
-    key = ("store_latent", id(buffers), id(meta), id(rotary), _fastpath.signature(tensors))
+    tensors, absent = _given(latent, k_rope, buffers.k, q, q_out)
+    key = ("store_latent", id(buffers), id(meta), id(rotary), absent, _fastpath.signature(tensors))
     _replayed(meta, key, (buffers, meta, rotary),
               lambda record: _store_latent(op, latent, k_rope, buffers, meta, rotary, q, q_out, record))
 
