@@ -9,32 +9,38 @@
 // of rows and heads is cut into tiles of NC consecutive (row, head) pairs; every pair of a tile reads
 // the same context, which a workgroup streams once for all of them. With NC pairs a position of
 // 2 (DC + 64) bytes takes 2 NC (2 DC + 64) operations: at DC 512 memory and matrix cores take the
-// same time at about 190 pairs (255 with P.V's two products for bf16 counted once).
+// same time at about 140 pairs, at the rates that a copy and a library product reach (5.0 TB/s and 1.25
+// PFLOP/s); a bf16 P doubles the operations of its product.
 //
-//  * A workgroup (4 waves, one workgroup per compute unit) holds 4 chunks of 32 positions in LDS
+//  * A workgroup (8 waves, one workgroup per compute unit) holds 4 chunks of 32 positions in LDS
 //    (147 KB), fetched straight into it (global_load_lds_dwordx4, no registers), up to three on their
 //    way while one is worked on: 110 KB in flight per compute unit cover the latency at the full rate.
 //  * 16-byte pieces of a row are stored in an order that depends on the position (swizzle), which
 //    keeps both the row-wise reads (q.k) and the transposing ones (P.V) spread over the banks.
-//  * S^T = K Q^T, then O^T += V^T P^T, v_mfma_f32_16x16x32 with q and O in registers; the values are the
-//    latents already in LDS, read transposed (ds_read_b64_tr_b16). A bf16 P is taken in two parts (high
-//    and remainder by truncation: one bf16 would lose 2^-9 of each weight, as much as the output's own
-//    rounding), an fp16 P rounded to nearest (2^-11).
+//  * S^T = K Q^T: two waves for each 16 pairs, 16 positions each, q in registers. The weights go through
+//    LDS, and O^T += V^T P^T by all 8 waves, an eighth of DC each for all pairs (so a wave's q and O fit
+//    its 256 registers); the values are the latents already in LDS, read transposed
+//    (ds_read_b64_tr_b16). v_mfma_f32_16x16x32. A bf16 P is taken in two parts (high and remainder by
+//    truncation: one bf16 would lose 2^-9 of each weight, as much as the output's own rounding), an fp16
+//    P rounded to nearest (2^-11).
 //  * The running maximum moves only when a score passes it by kRescaleSlack; until then weights up to
 //    2^kRescaleSlack keep their accuracy and nothing is rescaled.
-//
-// Two kernels, by what bounds them. Few pairs (16 or 32), latent_shared_kernel: the waves share each
-// chunk, a wave scores 16 positions and 16 pairs and then takes a quarter of DC for all pairs, with the
-// weights exchanged through LDS: small registers, short steps, two barriers a chunk. Many pairs (64 or
-// 128), latent_own_kernel: a wave owns 32 pairs whole, q and O filling its 512 registers, and P goes
-// from the scores to P.V without leaving them; 64 pairs take two waves on one chunk and two on the
-// next, joined at the end, because LDS reads (each wave reads whole chunks) are the limit there.
+//  * Up to 32 pairs memory is the bound: two barriers a chunk, and the four waves without scores fetch.
+//    With 64 pairs the products are, so a chunk is scored while the last one is weighed, one barrier a
+//    chunk: of the two waves of a SIMD one weighs first and one scores first.
 //
 // Work is split without the host: the chunks of all tiles, and tile_cost(NC) for each tile's own start and
 // end, form one line, and of G workgroups the g-th takes [g T / G, (g + 1) T / G). The lengths are read
 // on the device, so eager steps and replays of a captured one run the same code. A workgroup that
 // begins or ends inside a tile leaves a partial (m, l, O), at most two of them, and
 // latent_merge_kernel joins each cut tile.
+//
+// Measured at DC 512 (this kernel + the merge): 64 requests of 4096 positions, 16 heads, bf16: 54 + 5 us,
+// 302 MB at 5.6 TB/s in the first; 61 requests of 16 to 16384 positions, 128 heads, bf16: 79 + 10 us; 32
+// requests of 4096 with 4 rows each, 32 heads, fp16: 69 + 9 us, 530 TFLOP/s in the first, where 3000 cycles a
+// chunk of 64 pairs go to 1150 of matrix instructions (1600 for bf16) and the reads of LDS and exponentials
+// that they do not cover; 4 requests of 128 to 1000, 16 heads: 15 + 4 us, which is the chain of
+// lengths, table, first rows (8 us) and a few chunks.
 //
 // Visible and masked: a masked position's weight is an exact 0, and what it multiplies must be
 // finite. Slots behind the context are never read (the last position stands in for them). Rows of one
@@ -59,9 +65,12 @@ constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kTableWindow = 768;       // block-table entries in LDS
 constexpr int kPlaceWords = 8;
-// What a tile of NC pairs costs beside its chunks (queries, first loads, output), in chunks.
+// What a tile of NC pairs costs beside its chunks (queries, first loads, output), in chunks. Measured with
+// 3, 5, 8 and 12: 64 pairs of the uneven requests above 102, 85, 80, 80 us, of the rows of four 68, 70, 69, 72;
+// 16 pairs of the 4 short requests 14, 15, 18, 21, of the 64 long ones 53, 55, 55, 55.
 constexpr int tile_cost(int nc) { return nc == 64 ? 8 : 5; }
-// Fewest chunks, beside a tile's cost, for one workgroup: as many as a partial's write and merge are worth.
+// Fewest chunks, beside a tile's cost, for one workgroup: as many as a partial's write and merge are worth
+// (the 4 short requests: 15 us with 2, 20 with 6; the others do not care).
 constexpr int kLeastChunks = 2;
 
 template <bool BF16>
@@ -756,7 +765,10 @@ hipError_t launch_type(const LatentParams& p, int pairs, int compute_units, hipS
 
 }  // namespace
 
-// A tile holds the pairs of an average request, up to 64.
+// A tile holds the pairs of an average request, up to 64: larger ones read a context less often, and cost
+// matrix time for pairs that are not there. Measured with 16, 32 and 64 pairs: 16 heads over 64 requests of
+// 4096 positions 54, 55, 74 us, over 4 short ones 15, 17, 27; 128 heads over uneven requests 158, 95, 79, four
+// rows of 32 heads 175, 100, 69.
 int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads) {
   const int64_t each = n_requests > 0 ? n_rows * heads / n_requests : 0;
   return each <= 16 ? 16 : each <= 32 ? 32 : 64;

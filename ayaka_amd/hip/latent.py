@@ -166,8 +166,9 @@ def attend_latent_chunks(q: torch.Tensor, weights: LatentWeights, buffers: Laten
     their rotary part rotated, and ``out`` [N, heads, 128] are the heads' outputs. The context's keys and
     values are expanded once for all rows, into scratch, so this is for steps of many rows per request
     (some hundred; ``attend_latent`` serves the others without expanding). For steps made by ``plan``;
-    captured after one eager call. Expanded keys and values are held in fp16 with scales of
-    their own (2^-11 relative, any magnitude).
+    captured after one eager call. Expanded keys and values are held in fp16 with a scale for every 128
+    positions of a head: each element is within 2^-11 of itself, whatever its magnitude, or within 2^-38 of
+    the largest finite one of those positions.
     """
     op = "attention.attend_latent_chunks"
     key = ("attend_latent_chunks", id(buffers), id(meta), scale,

@@ -163,6 +163,7 @@ def test_wide_tables_are_read_in_windows(ops) -> None:
     """More blocks than the table's window in LDS holds, whose ends fall inside chunks."""
     Scene(ops, [(1, 2500), (3, 1999)], heads=2, latent=256, block=1).check()
     Scene(ops, [(1, 5000)], heads=2, latent=256, block=3).check()
+    Scene(ops, [(2, 2500), (1, 30), (3, 1700)], heads=40, latent=256, block=1).check()
 
 
 @pytest.mark.parametrize("form", ["absorbed", "chunks"])
@@ -171,6 +172,45 @@ def test_large_scores(ops, form, dtype) -> None:
     """Scores of hundreds, where one position takes nearly all weight, and all equal ones."""
     Scene(ops, [(1, 300), (6, 150)], form=form, dtype=dtype, heads=3, q_scale=200.0, seed=3).check()
     Scene(ops, [(1, 300), (6, 150)], form=form, dtype=dtype, heads=3, q_scale=0.0, seed=3).check()
+
+
+@pytest.mark.parametrize("form", ["absorbed", "chunks"])
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 1e-30])
+def test_scales_of_any_sign(ops, form, scale) -> None:
+    s = Scene(ops, [(1, 300), (6, 150), (70, 70)], form=form, heads=3, seed=31)
+    s.scale = scale
+    s.check()
+
+
+@pytest.mark.parametrize("form", ["absorbed", "chunks"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+@pytest.mark.parametrize("size", [16.0, 2.0 ** 14])
+def test_scores_far_apart(ops, form, dtype, order, size) -> None:
+    """Scores thousands apart, up to 2^30: each row is the value of one position it sees. Every number that the
+    scores are made of is exact, so the position that wins is, and its weight is 1."""
+    length, rows, heads = 250, 130, 3
+    s = Scene(ops, [(1, 40), (rows, length)], form=form, dtype=dtype, heads=heads, seed=32)
+    key = {"up": np.arange(length), "down": -np.arange(length), "mixed": (np.arange(length) * 89) % 251 - 125}[order]
+    t = np.arange(length)
+    at = torch.as_tensor(s.table[1, t // 16]), torch.as_tensor(t % 16)
+    s.cache[(*at, 0)] = torch.tensor(key).to(s.dtype).to(DEV)
+    s.q.zero_()
+    s.q[..., 0] = size
+    if form == "chunks":  # the key's first element is the latent's
+        s.weights.keys.zero_()
+        s.weights.keys[:, 0, 0] = 1
+    s.scale = 1024.0
+    got, want = s.run().double().cpu().numpy()[1:], s.want()[0][1:]
+    winner = np.array([np.argmax(key[:length - rows + i + 1]) for i in range(rows)])
+    values = s.cache[at].double().cpu().numpy()[winner][:, None, :s.latent].repeat(heads, 1)
+    if form == "chunks":
+        values = np.einsum("rhc,hvc->rhv", values, s.weights.values.double().cpu().numpy())
+    assert np.allclose(want, values, rtol=1e-12, atol=1e-12)
+    bound = torch.finfo(s.dtype).eps / 2 * np.abs(values) + (2.0 ** -11 + 2.0 ** -20) * (np.abs(values) + 2.0 ** -26)
+    if form == "chunks":  # three half steps of fp16, and a value's sum: 18 roundings of 2^-24 of up to 40
+        bound = bound * 2 + 2.0 ** -14
+    assert np.all(np.abs(got - values) <= bound)
 
 
 def test_a_maximum_that_grows_all_the_way(ops) -> None:
@@ -213,13 +253,18 @@ def test_rows_do_not_notice_what_they_do_not_see(ops, form, dtype, value, where)
             assert np.isnan(want[row, h]).all() == bool(got[row, h].isnan().all())
 
 
-@pytest.mark.parametrize("form", ["absorbed", "chunks"])
-def test_types_lowest_and_highest_values(ops, form) -> None:
-    s = Scene(ops, [(2, 70)], form=form, heads=2, seed=6)
-    lowest = torch.finfo(torch.bfloat16).min
-    s.cache[int(s.table[0, 1]), 3] = lowest  # position 19: every product with it overflows
+def test_types_lowest_and_highest_values(ops) -> None:
+    s = Scene(ops, [(2, 70)], heads=2, seed=6)
+    s.cache[int(s.table[0, 4]), 5] = torch.finfo(torch.bfloat16).min  # position 69: every product with it overflows
     got = s.run()
-    assert np.array_equal(np.isnan(got.float().cpu().numpy()).all(-1) | True, np.ones((2, 2), bool))
+    assert torch.equal(got[0], Scene(ops, [(2, 70)], heads=2, seed=6).run()[0])  # the row before it
+    # scores that overflowed make NaN or, at -inf, no weight: what is a number is the definition's
+    got, want = got.double().cpu().numpy(), s.want()[0]
+    assert np.all(np.isnan(got) | (np.abs(got - want) <= 2 ** -6 * (1 + np.abs(want))))
+
+
+@pytest.mark.parametrize("form", ["absorbed", "chunks"])
+def test_values_of_all_that_the_type_holds(ops, form) -> None:
     s = Scene(ops, [(2, 70)], form=form, heads=2, seed=6, q_scale=0.0)
     s.cache[int(s.table[0, 1]), 3] = torch.where(s.cache[int(s.table[0, 1]), 3] > 0, 1e30, -1e30)
     s.check()
@@ -237,6 +282,16 @@ def test_chunks_beside_louder_and_quieter_ones(ops) -> None:
     t = np.arange(900)
     sizes = torch.tensor([1.0, 64.0, 2.0 ** -8, 2.0 ** 9, 1.0, 2.0 ** -20, 32.0, 0.0])[t // 128].to(DEV)
     at = torch.as_tensor(s.table[0, t // 16]), torch.as_tensor(t % 16)
+    s.cache[at] = (s.cache[at].float() * sizes[:, None]).to(s.dtype)
+    s.check()
+
+
+def test_chunks_over_a_long_context(ops) -> None:
+    """More tiles than the window of their scales holds, each of another magnitude."""
+    s = Scene(ops, [(3, 33100), (130, 140)], form="chunks", heads=1, block=64, seed=33, q_scale=0.3)
+    t = np.arange(33100)
+    sizes = torch.tensor(2.0 ** ((t // 128 * 5) % 7 - 3), dtype=torch.float32).to(DEV)
+    at = torch.as_tensor(s.table[0, t // 64]), torch.as_tensor(t % 64)
     s.cache[at] = (s.cache[at].float() * sizes[:, None]).to(s.dtype)
     s.check()
 
