@@ -60,6 +60,15 @@ struct Elem<false> {
   }
 };
 
+// Two floats rounded to nearest as a word of two elements, in one instruction (v_cvt_pk_bf16_f32,
+// v_cvt_pk_f16_f32): Elem::round's values, without its branch on NaN.
+template <bool BF16>
+__device__ __forceinline__ uint32_t round_two(float a, float b) {
+  typedef __bf16 two_bf16 __attribute__((ext_vector_type(2)));
+  if constexpr (BF16) return __builtin_bit_cast(uint32_t, two_bf16{(__bf16)a, (__bf16)b});
+  else return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __builtin_bit_cast(

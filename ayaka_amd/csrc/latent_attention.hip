@@ -395,10 +395,7 @@ __device__ __forceinline__ uint32_t finite_word(uint32_t w) {
 // Four elements of an output, or of a partial output.
 template <bool BF16>
 __device__ __forceinline__ void put_output(uint16_t* out, f32x4 o, float by) {
-  u32x2 two;
-  two.x = Elem<BF16>::round(o[0] * by) | Elem<BF16>::round(o[1] * by) << 16;
-  two.y = Elem<BF16>::round(o[2] * by) | Elem<BF16>::round(o[3] * by) << 16;
-  *reinterpret_cast<u32x2*>(out) = two;
+  *reinterpret_cast<u32x2*>(out) = u32x2{round_two<BF16>(o[0] * by, o[1] * by), round_two<BF16>(o[2] * by, o[3] * by)};
 }
 
 template <int DC, bool BF16, int NT>

@@ -562,10 +562,10 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
       const f32x4 x = hand[((rg * 2 + j) * 8 + d) * kWave + lane];
-      uint32_t y[4];
+      float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = Elem<BF16>::round(__builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, high));
-      *reinterpret_cast<u32x2*>(out + d * 16) = u32x2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+      for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, high);
+      *reinterpret_cast<u32x2*>(out + d * 16) = u32x2{round_two<BF16>(y[0], y[1]), round_two<BF16>(y[2], y[3])};
     }
   }
 }
