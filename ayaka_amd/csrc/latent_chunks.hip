@@ -11,7 +11,7 @@
 // 8 waves of 64 x 64 on v_mfma_f32_16x16x32, operands through LDS in steps of 32 of DC, three steps in
 // flight (global_load_lds, 74 KB). Two workgroups share a compute unit, so that one's first loads and
 // stores run beside the other's products: with one of twice the step 16384 tokens for 16 heads at DC 512
-// took 95 us, so 83 (0.83 PFLOP/s, and 134 MB written). Tokens are gathered from their pages here; what
+// took 95 us, so 82 (0.84 PFLOP/s, and 134 MB written). Tokens are gathered from their pages here; what
 // follows reads straight lines.
 //
 // Keys and values are kept as fp16 whatever the model's type, with a power of two for every 128 tokens,
@@ -85,7 +85,7 @@ __device__ __forceinline__ uint32_t lds_offset(T* p) {
 
 // Where piece c (16 bytes) of row r stands in LDS, for rows of 64, 128 and 256 bytes: any 16 rows that
 // one cycle's reads touch are spread over all 64 banks.
-__device__ __forceinline__ int swizzle64(int r) { return (r >> 2) & 3; }
+__device__ __forceinline__ int swizzle64(int r) { return (r >> 1) & 3; }
 __device__ __forceinline__ int swizzle128(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int swizzle256(int r) { return r & 15; }
 
