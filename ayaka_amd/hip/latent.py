@@ -98,7 +98,8 @@ def attend_latent(q: torch.Tensor, buffers: LatentBuffers, meta: AttentionMetada
     ``q`` [N, heads, latent_dim + 64] holds each head's query taken through the keys' matrix, and behind
     it its rotated part (what ``store_latent`` rotates); the score of a cached row is their product
     times ``scale``, and ``out`` [N, heads, latent_dim] receives the weighted sum of the latents, for the
-    values' matrix to be applied to. Rows see positions up to their own; padding rows get zeros.
+    values' matrix to be applied to. Rows see positions up to their own; padding rows get zeros. ``out``
+    overlaps no input.
     Any step serves: decode, verify windows, chunks (``attend_latent_chunks`` does those of many rows
     with a third of the work per score), graph metadata. Captured after one eager call.
     """
@@ -163,7 +164,7 @@ def attend_latent_chunks(q: torch.Tensor, weights: LatentWeights, buffers: Laten
 
     Head h's key of a position is ``weights.keys[h] @ latent`` with the position's rotary part behind it,
     its value ``weights.values[h] @ latent``; ``q`` [N, heads, 128 + 64] are the queries as projected, with
-    their rotary part rotated, and ``out`` [N, heads, 128] are the heads' outputs. The context's keys and
+    their rotary part rotated, and ``out`` [N, heads, 128], which overlaps no input, are the heads' outputs. The context's keys and
     values are expanded once for all rows, into scratch, so this is for steps of many rows per request
     (some hundred; ``attend_latent`` serves the others without expanding). For steps made by ``plan``;
     captured after one eager call. Expanded keys and values are held in fp16 with a scale for every 128

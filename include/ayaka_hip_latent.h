@@ -69,7 +69,7 @@ int ayk_store_latent(const void* latent, int64_t latent_row, const void* k_rope,
  * requests of rows[b] rows each, in order (n_rows in all), which are the last of kv_lengths[b] tokens; a
  * row attends to the positions up to its own; requests of length 0 give zeros. rows, kv_lengths and the
  * table are read on the device only: the call can be captured and replayed with others. Rows past the sum
- * of rows[] are not written.
+ * of rows[] are not written. out overlaps no input.
  * workspace: ayk_latent_attention_workspace_bytes, 16-byte aligned, the call's own while it runs.
  */
 size_t ayk_latent_attention_workspace_bytes(int32_t n_rows, int32_t n_requests, int32_t num_heads, int32_t latent_dim);

@@ -26,7 +26,7 @@ from ayaka_amd.backend import load_backend
 from ayaka_amd.enums import DType, ForwardMode
 from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import latent as hip_latent
-from ayaka_amd.kvcache import LatentBuffers, LatentWeights
+from ayaka_amd.kvcache import BlockPool, LatentBuffers, LatentWeights
 from ayaka_amd.rotary import rotary
 from oracle import latent as oracle
 
@@ -553,3 +553,59 @@ def test_a_model_layer_from_prompt_to_decode(ops) -> None:
         # queries rounded to bf16 after the keys' matrix (a half step, 2^-9 at most, of scores about 1) and
         # the latents' sums before the values' (another)
         assert np.linalg.norm(final.double().cpu().numpy() - want) <= 3 * 2 ** -8 * np.linalg.norm(want), step
+
+
+def test_a_decode_loop_that_advances_itself(ops) -> None:
+    """One captured graph raises the lengths, hands out blocks, stores and attends: every replay against the
+    definition over what the cache then holds, with rows of padding and a request that the pool cannot serve."""
+    heads, latent, block, width = 20, 512, 8, 6
+    t = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(41)
+    start = [5, 0, 8, 30]
+    ids = torch.arange(1, 33, dtype=torch.int32)
+    table = torch.zeros(4, width, dtype=torch.int32)
+    taken = 0
+    for b, length in enumerate(start):
+        held = -(-length // block)
+        table[b, :held] = ids[taken:taken + held]
+        taken += held
+    pool = BlockPool.in_place(ids[taken:taken + 4].to(DEV))  # 4 more blocks, and then none
+    cache = torch.randn(34, block, latent + 64, generator=g, device=DEV).to(t)
+    buffers = LatentBuffers(cache, latent)
+    turn, scale = rotary(64, device=DEV), 192 ** -0.5
+    bucket = ops.attention.graph_metadata(4, width, block, DEV)
+    ops.attention.update_graph_metadata(bucket, torch.tensor(start, dtype=torch.int32), table)
+    lengths = bucket.kv_lengths
+    new = torch.randn(4, latent + 64, generator=g, device=DEV).to(t)
+    q = torch.randn(4, heads, latent + 64, generator=g, device=DEV).to(t) * 0.4
+    turned, out = q.clone(), torch.empty(4, heads, latent, dtype=t, device=DEV)
+
+    def step():
+        lengths.add_(lengths > 0)
+        ops.attention.advance_graph_metadata(bucket, lengths, pool)
+        ops.kvcache.store_latent(new[:, :latent], new[:, latent:], buffers, bucket, turn, q[:, :, latent:], turned[:, :, latent:])
+        ops.attention.attend_latent(turned, buffers, bucket, out, scale=scale)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    served = set()
+    for i in range(14):
+        new.copy_(torch.randn(4, latent + 64, generator=g, device=DEV).to(t))
+        before = lengths.tolist()
+        graph.replay()
+        torch.cuda.synchronize()
+        now, held = lengths.tolist(), bucket.block_table.cpu().numpy()
+        for b in range(4):
+            assert now[b] in (0, before[b] + 1) and (before[b] or not now[b])
+            if now[b]:
+                slot = cache[int(held[b, (now[b] - 1) // block]), (now[b] - 1) % block]
+                assert torch.equal(slot[:latent], new[b, :latent])
+            served.add((b, bool(now[b])))
+        want = oracle.attention(turned.double().cpu().numpy(), cache.double().cpu().numpy(), held, [1] * 4, now, scale, latent)[0]
+        got = out.double().cpu().numpy()
+        assert np.linalg.norm(got - want) <= 1.5 * 2 ** -8 * np.linalg.norm(want)  # a half step of the output, weights 2^-14
+        assert not got[[b for b in range(4) if not now[b]]].any()
+    assert (1, True) not in served and any((b, False) in served and (b, True) in served for b in (0, 2, 3))
