@@ -492,9 +492,13 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = fast_exp2(s[i] - base);
-        l = so_far + ((w[0] + w[1]) + (w[2] + w[3]));
         u32x2 hi, lo;
         split_weights4<BF16>(w, hi, lo);
+        if constexpr (!BF16) {  // the sum of the weights as rounded: where one outweighs the others its rounding cancels
+          w[0] = Elem<false>::lo(hi.x), w[1] = Elem<false>::hi(hi.x);
+          w[2] = Elem<false>::lo(hi.y), w[3] = Elem<false>::hi(hi.y);
+        }
+        l = so_far + ((w[0] + w[1]) + (w[2] + w[3]));
         const int row = my_pair * kChunk + (mq ^ weight_swizzle(my_pair)) * 8 + 4 * kg;
         auto& weight = lds.weight[AHEAD ? chunk & 1 : 0];
         *reinterpret_cast<u32x2*>(&weight[0][row]) = hi;
