@@ -173,7 +173,8 @@ int ayk_store_latent(const void* latent, int64_t latent_row, const void* k_rope,
 
 size_t ayk_latent_attention_workspace_bytes(int32_t n_rows, int32_t n_requests, int32_t num_heads, int32_t latent_dim) {
   if (n_rows < 1 || n_requests < 1 || num_heads < 1 || (latent_dim != 256 && latent_dim != 512)) return 0;
-  return ayk::latent_workspace_bytes(latent_dim, ayk::latent_tile_pairs(n_rows, n_requests, num_heads), compute_units());
+  const int units = compute_units();
+  return ayk::latent_workspace_bytes(latent_dim, ayk::latent_tile_pairs(n_rows, n_requests, num_heads, units), units);
 }
 
 int ayk_latent_attention(void* out, const void* q, const void* cache, const int32_t* block_table, int64_t table_stride,
@@ -181,7 +182,32 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
                          int32_t num_heads, int32_t latent_dim, int32_t rope_dim, int32_t num_blocks,
                          int32_t block_size, int32_t max_blocks, int32_t dtype, float scale, void* workspace,
                          size_t workspace_bytes, void* stream) {
+  const int pairs = n_rows < 1 || n_requests < 1 || num_heads < 1
+                        ? 16 : ayk::latent_tile_pairs(n_rows, n_requests, num_heads, compute_units());
+  return ayk_latent_attention_tiles(out, q, cache, block_table, table_stride, kv_lengths, rows, n_requests, n_rows, num_heads,
+                                    latent_dim, rope_dim, num_blocks, block_size, max_blocks, dtype, scale, pairs, workspace,
+                                    workspace_bytes, stream);
+}
+
+int32_t ayk_latent_tile_pairs(const int32_t* rows, const int32_t* kv_lengths, int32_t n_requests, int32_t num_heads) {
+  if (!rows || !kv_lengths || n_requests < 1 || num_heads < 1) return 16;
+  return ayk::latent_tile_pairs(rows, kv_lengths, n_requests, num_heads, compute_units());
+}
+
+size_t ayk_latent_tiles_workspace_bytes(int32_t latent_dim, int32_t tile_pairs) {
+  if ((latent_dim != 256 && latent_dim != 512) || (tile_pairs != 16 && tile_pairs != 32 && tile_pairs != 64)) return 0;
+  return ayk::latent_workspace_bytes(latent_dim, tile_pairs, compute_units());
+}
+
+int ayk_latent_attention_tiles(void* out, const void* q, const void* cache, const int32_t* block_table,
+                               int64_t table_stride, const int32_t* kv_lengths, const int32_t* rows,
+                               int32_t n_requests, int32_t n_rows, int32_t num_heads, int32_t latent_dim,
+                               int32_t rope_dim, int32_t num_blocks, int32_t block_size, int32_t max_blocks,
+                               int32_t dtype, float scale, int32_t tile_pairs, void* workspace,
+                               size_t workspace_bytes, void* stream) {
   const char* op = "ayk_latent_attention";
+  if (tile_pairs != 16 && tile_pairs != 32 && tile_pairs != 64)
+    return fail(AYK_ERR_ARGUMENT, "%s: tile_pairs %d is not 16, 32 or 64", op, tile_pairs);
   if (n_rows < 0 || n_requests < 0)
     return fail(AYK_ERR_ARGUMENT, "%s: n_rows %d, n_requests %d", op, n_rows, n_requests);
   if (latent_dim != 256 && latent_dim != 512)
@@ -200,11 +226,11 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
     return fail(AYK_ERR_ARGUMENT, "%s: a required pointer is null", op);
   if (misaligned(16, {out, q, cache, workspace}))
     return fail(AYK_ERR_ARGUMENT, "%s: out, q, cache and workspace must be 16-byte aligned", op);
-  const size_t need = ayk_latent_attention_workspace_bytes(n_rows, n_requests, num_heads, latent_dim);
+  const size_t need = ayk_latent_tiles_workspace_bytes(latent_dim, tile_pairs);
   if (!workspace || workspace_bytes < need)
     return fail(AYK_ERR_WORKSPACE, "%s: the workspace holds %zu bytes, %zu are needed", op, workspace_bytes, need);
   // the kernel counts (row, head) pairs and the chunks of all tiles in 31 bits
-  const int pairs = ayk::latent_tile_pairs(n_rows, n_requests, num_heads);
+  const int pairs = tile_pairs;
   const int64_t positions = (int64_t)max_blocks * block_size;
   const int64_t tiles = (int64_t)n_rows * num_heads / pairs + n_requests;
   if ((int64_t)n_rows * num_heads > INT32_MAX || positions > INT32_MAX - 64 || tiles * (positions / 32 + 8) > INT32_MAX)

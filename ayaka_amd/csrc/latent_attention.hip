@@ -767,13 +767,45 @@ hipError_t launch_type(const LatentParams& p, int pairs, int compute_units, hipS
 
 }  // namespace
 
-// A tile holds the pairs of an average request, up to 64: larger ones read a context less often, and cost
-// matrix time for pairs that are not there. Measured with 16, 32 and 64 pairs: 16 heads over 64 requests of
-// 4096 positions 54, 55, 74 us, over 4 short ones 15, 17, 27; 128 heads over uneven requests 158, 95, 79, four
-// rows of 32 heads 175, 100, 69.
-int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads) {
-  const int64_t each = n_requests > 0 ? n_rows * heads / n_requests : 0;
-  return each <= 16 ? 16 : each <= 32 ? 32 : 64;
+// Pairs of a tile. Larger tiles read a context less often and take fewer products of few rows; smaller ones
+// make more work to share while there is not enough for every compute unit, and start and end sooner. With u
+// units a workgroup (as they are dealt out above) a launch takes about 13 + 1.15 u us with 16 pairs, 14 + 1.45 u
+// with 32 and 20 + 1.7 u with 64, fitted to 40 drawn steps and these (measured with 16, 32 and 64 pairs, main
+// kernel): 16 heads over 64 requests of 4096 positions 54, 55, 74 us, over 4 short ones 15, 17, 27; 128 heads over
+// 61 uneven requests 158, 95, 79; 4 rows of 32 heads over 4096 positions 175, 100, 69. Whole calls: 8 rows of 16
+// heads for 2 requests of 321 at most 17, 21, 32; 40 to 64 rows of 32 heads for 4 of 918 38, 35, 39.
+struct TileChoice {
+  int64_t units[3] = {0, 0, 0};
+  void add(int64_t requests, int64_t pairs, int64_t length) {
+    const int64_t chunks = length < kChunk ? 1 : (length + kChunk - 1) / kChunk;
+    for (int i = 0; i < 3; ++i) units[i] += requests * ((pairs + (16 << i) - 1) / (16 << i)) * (chunks + tile_cost(16 << i));
+  }
+  int best(int compute_units) const {
+    constexpr double START[3] = {13, 14, 20}, EACH[3] = {1.15, 1.45, 1.7};
+    int found = 16;
+    double least = 0;
+    for (int i = 0; i < 3; ++i) {
+      const int64_t most = units[i] / (tile_cost(16 << i) + kLeastChunks);
+      const int64_t workgroups = most < 1 ? 1 : most < compute_units ? most : compute_units;
+      const double us = START[i] + EACH[i] * (double)units[i] / (double)workgroups;
+      if (i == 0 || us < least) found = 16 << i, least = us;
+    }
+    return found;
+  }
+};
+
+int latent_tile_pairs(const int32_t* rows, const int32_t* kv_lengths, int32_t n_requests, int32_t heads, int compute_units) {
+  TileChoice choice;
+  for (int32_t b = 0; b < n_requests; ++b)
+    if (rows[b] > 0) choice.add(1, (int64_t)rows[b] * heads, kv_lengths[b]);
+  return choice.best(compute_units);
+}
+
+// Where the lengths are not known: requests of as many rows each, over 2048 positions.
+int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads, int compute_units) {
+  TileChoice choice;
+  if (n_requests > 0) choice.add(n_requests, (n_rows + n_requests - 1) / n_requests * heads, 2048);
+  return choice.best(compute_units);
 }
 
 size_t latent_workspace_bytes(int32_t latent_dim, int pairs, int compute_units) {

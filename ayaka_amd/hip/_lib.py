@@ -136,6 +136,12 @@ LATENT_EXPORTS: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_P, _P, _P, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P, _SZ, _P],
     ),
+    "ayk_latent_tile_pairs": (_I32, [_P, _P, _I32, _I32]),
+    "ayk_latent_tiles_workspace_bytes": (_SZ, [_I32, _I32]),
+    "ayk_latent_attention_tiles": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P, _SZ, _P],
+    ),
     "ayk_latent_chunks_workspace_bytes": (_SZ, [_I64, _I32]),
     "ayk_latent_chunks": (
         ctypes.c_int,

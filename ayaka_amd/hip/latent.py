@@ -117,14 +117,28 @@ def _attend_latent(op: str, q: torch.Tensor, buffers: LatentBuffers, meta: Atten
         return
     device, lib = cache.device, _lib.lib()
     stream, requests = stream_handle(device), table.shape[0]
-    nbytes = lib.ayk_latent_attention_workspace_bytes(n_rows, requests, heads, buffers.latent_dim)
+    pairs = _tile_pairs(meta.plan, n_rows, requests, heads)
+    nbytes = lib.ayk_latent_tiles_workspace_bytes(buffers.latent_dim, pairs)
     scratch = _attention._workspace(op, device, nbytes, capturing(q), stream)
-    _attention._call(op, lib.ayk_latent_attention, (
+    _attention._call(op, lib.ayk_latent_attention_tiles, (
         out.data_ptr(), q.data_ptr(), cache.data_ptr(), table.data_ptr(), table.stride(0), meta.kv_lengths.data_ptr(),
         meta.rows_per_request.data_ptr(), requests, n_rows, heads, buffers.latent_dim, buffers.rope_dim,
-        buffers.num_blocks, buffers.block_size, table.shape[1], _DTYPE_CODES[cache.dtype], float(scale),
+        buffers.num_blocks, buffers.block_size, table.shape[1], _DTYPE_CODES[cache.dtype], float(scale), pairs,
         scratch.data_ptr(), scratch.numel(),
     ), stream, device, True, record)
+
+
+def _tile_pairs(plan: "_attention.HipAttentionPlan | _attention.HipGraphPlan", n_rows: int, requests: int, heads: int) -> int:
+    """(Row, head) pairs of a tile: for the step's lengths, or for a bucket's 2048 positions a request."""
+    known = isinstance(plan, _attention.HipAttentionPlan)
+    found = plan.splits.get(("latent", heads)) if known else None
+    if found is None:
+        rows, lengths = (plan.rows, plan.kv_lengths) if known else ((-(-n_rows // requests),) * requests, (2048,) * requests)
+        rows, lengths = np.array(rows, dtype=np.int32), np.array(lengths, dtype=np.int32)
+        found = _lib.lib().ayk_latent_tile_pairs(rows.ctypes.data, lengths.ctypes.data, len(rows), heads)
+        if known:
+            plan.splits["latent", heads] = found
+    return found
 
 
 def _chunk_tiles(op: str, step: "_attention.HipAttentionPlan", device: torch.device,

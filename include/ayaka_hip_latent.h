@@ -80,6 +80,20 @@ int ayk_latent_attention(void* out, const void* q, const void* cache, const int3
                          size_t workspace_bytes, void* stream);
 
 /*
+ * The same with tiles of tile_pairs (row, head) pairs, 16, 32 or 64, which read a context together.
+ * ayk_latent_attention takes what is best for contexts of 2048 positions; where a caller knows a step's lengths,
+ * ayk_latent_tile_pairs says what is best for them (rows and kv_lengths in host memory).
+ */
+int32_t ayk_latent_tile_pairs(const int32_t* rows, const int32_t* kv_lengths, int32_t n_requests, int32_t num_heads);
+size_t ayk_latent_tiles_workspace_bytes(int32_t latent_dim, int32_t tile_pairs);
+int ayk_latent_attention_tiles(void* out, const void* q, const void* cache, const int32_t* block_table,
+                               int64_t table_stride, const int32_t* kv_lengths, const int32_t* rows,
+                               int32_t n_requests, int32_t n_rows, int32_t num_heads, int32_t latent_dim,
+                               int32_t rope_dim, int32_t num_blocks, int32_t block_size, int32_t max_blocks,
+                               int32_t dtype, float scale, int32_t tile_pairs, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
  * The same cache with keys and values expanded from the latents, for chunks of many rows:
  *   key(h, t) = [keys[h] . latent(t) | rotary part(t)],  value(h, t) = values[h] . latent(t)
  *   out[row, h] = sum over t of softmax(scale * q[row, h] . key(h, .))(t) * value(h, t)

@@ -344,6 +344,40 @@ def test_both_forms_agree(ops) -> None:
     assert float((got - want).norm() / want.norm()) < 8 * 2 ** -11
 
 
+@pytest.fixture(params=[16, 32, 64])
+def tiles(request, monkeypatch) -> int:
+    """The (row, head) pairs of a tile, whatever a step's lengths would have."""
+    monkeypatch.setattr(hip_latent, "_tile_pairs", lambda *_: request.param)
+    return request.param
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("latent", [256, 512])
+@pytest.mark.parametrize("heads", [1, 5, 16, 40, 128])
+def test_tiles_of_every_size(ops, tiles, dtype, latent, heads) -> None:
+    steps = [(1, 1), (1, 0), (2, 33), (1, 700), (5, 64), (0, 20), (17, 130), (1, 300)]
+    Scene(ops, steps, dtype=dtype, latent=latent, heads=heads, seed=tiles).check()
+
+
+def test_tiles_over_cut_contexts_and_windows(ops, tiles) -> None:
+    Scene(ops, [(1, 9000), (3, 4001)], heads=24, block=64, seed=42).check()
+    Scene(ops, [(2, 2500), (1, 30), (3, 1700)], heads=40, latent=256, block=1, dtype="fp16", seed=43).check()
+    Scene(ops, [(1, 300), (6, 150)], heads=30, q_scale=200.0, seed=44).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_tiles_do_not_show_what_a_row_does_not_see(ops, tiles, dtype, value) -> None:
+    steps = [(5, 300), (1, 64), (40, 40)]
+    s, clean = (Scene(ops, steps, dtype=dtype, heads=9, seed=45) for _ in range(2))
+    for b, t in ((0, 298), (2, 20)):
+        s.cache[int(s.table[b, t // 16]), t % 16, 7] = value
+    got, ref = s.run(), clean.run()
+    blind, seeing = [0, 1, 2, 5, *range(6, 26)], [3, 4, *range(26, 46)]
+    assert torch.equal(got[blind], ref[blind])
+    assert np.array_equal(got[seeing].isnan().cpu().numpy(), np.isnan(s.want()[0][seeing]))
+
+
 @pytest.mark.parametrize("form", ["absorbed", "chunks"])
 def test_same_bits_every_time(ops, form) -> None:
     s = Scene(ops, [(2, 3000), (1, 77), (30, 600)], form=form, heads=9, seed=12)

@@ -348,3 +348,31 @@ def test_weights_record() -> None:
     w = LatentWeights(torch.zeros(2, 128, 512), torch.zeros(2, 128, 512))
     assert w.keys.shape == w.values.shape
     assert isinstance(rotary(8, device="cpu"), Rotary)
+
+
+def test_tile_pairs_for_known_lengths() -> None:
+    """Small tiles while there is little to share, larger ones for many pairs over long contexts, never more
+    than the requests hold."""
+    import numpy as np
+
+    lib = _lib.lib()
+
+    def pairs(rows, lengths, heads):
+        rows, lengths = np.array(rows, dtype=np.int32), np.array(lengths, dtype=np.int32)
+        return lib.ayk_latent_tile_pairs(rows.ctypes.data, lengths.ctypes.data, len(rows), heads)
+
+    assert pairs([1] * 64, [4096] * 64, 16) == 16
+    assert pairs([4] * 32, [4096] * 32, 32) == 64
+    assert pairs([1] * 256, [2048] * 256, 128) == 64
+    assert pairs([8, 8], [26, 321], 16) == 16
+    assert pairs([1], [0], 1) == pairs([0, 0], [5, 5], 128) == 16
+    assert lib.ayk_latent_tile_pairs(None, None, 3, 16) == lib.ayk_latent_tile_pairs(16, 16, 0, 16) == 16
+    for tile in (16, 32, 64):  # a place, and two partials of (m, l) and the sums, a compute unit
+        assert lib.ayk_latent_tiles_workspace_bytes(512, tile) % (32 + 2 * tile * (2 + 512) * 4) == 0
+    assert lib.ayk_latent_tiles_workspace_bytes(512, 48) == lib.ayk_latent_tiles_workspace_bytes(500, 16) == 0
+    args = dict(out=16, q=16, cache=16, table=16, stride=4, lengths=16, rows=16, n_requests=2, n_rows=2, heads=8,
+                latent_dim=512, rope_dim=64, num_blocks=4, block_size=16, max_blocks=4, dtype=1, scale=1.0, tile_pairs=48,
+                workspace=16, workspace_bytes=1 << 40, stream=None)
+    assert lib.ayk_latent_attention_tiles(*args.values()) == 1 and b"tile_pairs 48" in lib.ayk_last_error()
+    args.update(tile_pairs=64, workspace_bytes=lib.ayk_latent_tiles_workspace_bytes(512, 64) - 1)
+    assert lib.ayk_latent_attention_tiles(*args.values()) == 4 and b"workspace" in lib.ayk_last_error()
