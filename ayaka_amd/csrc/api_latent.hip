@@ -273,7 +273,24 @@ int ayk_latent_chunks(void* out, const void* q, const void* cache, const void* k
                       int32_t heads_at_once, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
                       int32_t num_blocks, int32_t block_size, int32_t dtype, float scale, void* workspace,
                       size_t workspace_bytes, void* stream) {
+  return ayk_latent_chunks_split(out, q, cache, keys, values, block_table, table_stride, token_tiles, n_token_tiles, row_tiles,
+                                 n_row_tiles, ws_rows, heads_at_once, num_heads, latent_dim, rope_dim, num_blocks,
+                                 block_size, dtype, scale, 1, workspace, workspace_bytes, stream);
+}
+
+size_t ayk_latent_chunks_parts_bytes(int32_t n_row_tiles, int32_t heads_at_once, int32_t splits) {
+  if (n_row_tiles < 1 || heads_at_once < 1 || splits < 2 || splits > 64) return 0;
+  return (size_t)n_row_tiles * heads_at_once * splits * ayk::kLatentChunkRows * (128 + 2) * 4;
+}
+
+int ayk_latent_chunks_split(void* out, const void* q, const void* cache, const void* keys, const void* values,
+                            const int32_t* block_table, int64_t table_stride, const int32_t* token_tiles,
+                            int32_t n_token_tiles, const int32_t* row_tiles, int32_t n_row_tiles, int64_t ws_rows,
+                            int32_t heads_at_once, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                            int32_t num_blocks, int32_t block_size, int32_t dtype, float scale, int32_t splits,
+                            void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "ayk_latent_chunks";
+  if (splits < 1 || splits > 64) return fail(AYK_ERR_ARGUMENT, "%s: splits %d is not in [1, 64]", op, splits);
   if (latent_dim != 256 && latent_dim != 512)
     return fail(AYK_ERR_UNSUPPORTED, "%s: latent_dim %d is not 256 or 512", op, latent_dim);
   if (rope_dim != 64) return fail(AYK_ERR_UNSUPPORTED, "%s: rope_dim %d is not 64", op, rope_dim);
@@ -292,10 +309,12 @@ int ayk_latent_chunks(void* out, const void* q, const void* cache, const void* k
   if (misaligned(16, {out, q, cache, keys, values, workspace}))
     return fail(AYK_ERR_ARGUMENT, "%s: out, q, cache, keys, values and workspace must be 16-byte aligned", op);
   if (heads_at_once > num_heads) heads_at_once = num_heads;
-  const size_t need = ayk_latent_chunks_workspace_bytes(ws_rows, heads_at_once);
+  const size_t expanded = (ayk_latent_chunks_workspace_bytes(ws_rows, heads_at_once) + 15) & ~(size_t)15;
+  const size_t need = expanded + ayk_latent_chunks_parts_bytes(n_row_tiles, heads_at_once, splits);
   if (need > workspace_bytes || (need > 0 && !workspace))
     return fail(AYK_ERR_WORKSPACE, "%s: the workspace holds %zu bytes, %zu are needed", op, workspace_bytes, need);
-  if ((int64_t)(n_token_tiles > n_row_tiles ? n_token_tiles : n_row_tiles) * heads_at_once > INT32_MAX)
+  const int64_t cut_tiles = (int64_t)n_row_tiles * splits;
+  if ((n_token_tiles > cut_tiles ? n_token_tiles : cut_tiles) * heads_at_once > INT32_MAX)
     return fail(AYK_ERR_UNSUPPORTED, "%s: %d and %d tiles of %d heads exceed one launch", op, n_token_tiles, n_row_tiles,
                 heads_at_once);
   ayk::LatentChunkParams p{};
@@ -317,6 +336,9 @@ int ayk_latent_chunks(void* out, const void* q, const void* cache, const void* k
   p.by_block = ayk::divisor_of(block_size);
   p.scale_log2 = scale * kLog2e;
   p.group_heads = heads_at_once;
+  p.splits = splits;
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + expanded);
+  p.part_ml = p.part_o + cut_tiles * heads_at_once * ayk::kLatentChunkRows * 128;
   p.ws_rope = static_cast<uint16_t*>(workspace);
   p.ws_keys = p.ws_rope + ws_rows * 64;
   p.ws_values = p.ws_keys + heads_at_once * ws_rows * 128;

@@ -211,6 +211,8 @@ constexpr int kLatentChunkTokens = 128;
 constexpr int kLatentChunkRows = 128;
 struct LatentChunkParams {
   void* out;
+  float* part_ml;  // of a context's parts, where splits > 1: (m, l) of every row, and its output
+  float* part_o;
   const uint16_t* q;
   const uint16_t* cache;
   const uint16_t* keys;
@@ -224,6 +226,7 @@ struct LatentChunkParams {
   Divisor by_block;
   float scale_log2;
   int32_t group_heads, first_head;  // heads expanded at a time; the launch's own
+  int32_t splits;                   // parts that each row tile's context is cut into
   uint16_t* ws_rope;                // [ws_rows, 64]
   uint16_t* ws_keys;                // [group_heads, ws_rows, 128]
   uint16_t* ws_values;

@@ -24,6 +24,9 @@
 // work on every other 32 positions and four on those between (two waves to a SIMD); joined at the end in
 // LDS. S^T = K Q^T, weights stay in the lane that scored them, O^T += V^T P^T with values read
 // transposed, as the other attention kernels. Rounds of 64 positions (40 KB) in a ring of three.
+// Where row tiles and heads are fewer than the compute units the caller has each tile's context cut into parts,
+// a workgroup each, which latent_join_kernel joins: chunks of 600 rows of 4 heads over 3.6K positions take 42 us
+// so, 85 whole.
 // Bound by issue, not by memory: the loads alone take 34 us where 4 requests of 512 rows over 4096
 // positions, 16 heads, take 112 to 124 (0.65 PFLOP/s in the causal part). Of about 3100 cycles a round
 // 1280 are matrix instructions and as many vector ones, and exponentials do not run beside matrix
@@ -264,7 +267,10 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
   const int64_t ws_row = p.row_tiles[4 * tile + 2];
   const int real_head = p.first_head + head;
   const int context = first_pos + n_rows;  // positions that the last row sees
-  const int rounds = (context + kRound - 1) / kRound;
+  // this workgroup's part of the context
+  const int all_rounds = (context + kRound - 1) / kRound;
+  const int first_round = (int)((int64_t)blockIdx.y * all_rounds / p.splits);
+  const int rounds = (int)((int64_t)(blockIdx.y + 1) * all_rounds / p.splits);
 
   const uint8_t* keys = reinterpret_cast<const uint8_t*>(p.ws_keys + ((int64_t)head * p.ws_rows + ws_row) * kNope);
   const uint8_t* values = reinterpret_cast<const uint8_t*>(p.ws_values + ((int64_t)head * p.ws_rows + ws_row) * kValue);
@@ -305,8 +311,8 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
 #pragma unroll
     for (int k = 0; k < 2; ++k) qr[j][k] = from[16 + 4 * k];
   }
-  if (rounds > 0) get(0);
-  if (rounds > 1) get(1);
+  if (first_round < rounds) get(first_round);
+  if (first_round + 1 < rounds) get(first_round + 1);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     float largest = 0.f;
@@ -351,14 +357,14 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
   bool any_far = p.scale_log2 < 0.f;
 
   const int first_masked = first_pos + rg * 32;  // rows of this wave see up to there, all of them
-  for (int round = 0; round < rounds; ++round) {
+  for (int round = first_round; round < rounds; ++round) {
     if (round + 1 < rounds) wait_loads<LOADS>();
     else wait_loads<0>();
     lds_barrier();
-    if (round % (kWindow * kTokens / kRound) == 0) {
+    if (round == first_round || round % (kWindow * kTokens / kRound) == 0) {
       // The exponents come by way of LDS: a load of the compiler's own in every round would make it wait
       // there for all the loads to LDS that are on their way.
-      const int first = round / (kTokens / kRound), n = min(kWindow, (context + kTokens - 1) / kTokens - first);
+      const int first = round / (kTokens / kRound) / kWindow * kWindow, n = min(kWindow, (context + kTokens - 1) / kTokens - first);
       for (int i = tid; i < 2 * n; i += kThreads) lds.exponent[i >> 1][i & 1] = exponents[2 * first + i];
       lds_barrier();
     }
@@ -562,6 +568,22 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     const float a = mine * power(max(-126, value_exponent - high)), b = other * power(max(-126, pe - high));
     const int row = rg * 32 + j * 16 + mt;
     if (row >= n_rows) continue;
+    if (p.splits > 1) {  // a part's output and what it weighs, for the merge
+      const int64_t at = ((int64_t)blockIdx.x * p.splits + blockIdx.y) * kRows + row;
+      if (mq == 0) {
+        p.part_ml[at * 2] = now;
+        p.part_ml[at * 2 + 1] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const f32x4 x = hand[((rg * 2 + j) * 8 + d) * kWave + lane];
+        f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, high);
+        *reinterpret_cast<f32x4*>(p.part_o + at * kValue + d * 16 + 4 * mq) = y;
+      }
+      continue;
+    }
     uint16_t* out = static_cast<uint16_t*>(p.out) + ((int64_t)(first_row + row) * p.heads + real_head) * kValue + 4 * mq;
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
@@ -574,12 +596,38 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
   }
 }
 
+// Joins the parts of a context: block (tile and head, y) takes 8 rows, a lane 4 elements.
+template <bool BF16>
+__global__ __launch_bounds__(256) void latent_join_kernel(const LatentChunkParams p) {
+  const int head = blockIdx.x % p.group_heads, tile = blockIdx.x / p.group_heads;
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), e0 = (threadIdx.x & 31) * 4;
+  if (row >= p.row_tiles[4 * tile + 1]) return;
+  const int64_t first = (int64_t)blockIdx.x * p.splits * kRows + row;
+  float top = -INFINITY;
+  for (int i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_ml[(first + i * kRows) * 2]);
+  float sum = 0.f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < p.splits; ++i) {
+    const int64_t at = first + i * kRows;
+    const float m = p.part_ml[at * 2];
+    const float weight = p.part_ml[at * 2 + 1] * (m == top ? 1.f : fast_exp2(m - top));
+    sum += weight;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at * kValue + e0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] += x[k] * weight;
+  }
+  const float by = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + ((int64_t)(p.row_tiles[4 * tile] + row) * p.heads + p.first_head + head) * kValue + e0;
+  *reinterpret_cast<u32x2*>(out) = u32x2{round_two<BF16>(o[0] * by, o[1] * by), round_two<BF16>(o[2] * by, o[3] * by)};
+}
+
 template <bool BF16>
 hipError_t launch_type(LatentChunkParams p, int32_t latent_dim, hipStream_t stream) {
   const int group = p.group_heads;
   for (p.first_head = 0; p.first_head < p.heads; p.first_head += group) {
     p.group_heads = p.heads - p.first_head < group ? p.heads - p.first_head : group;
-    const dim3 expand((unsigned)(p.n_token_tiles * p.group_heads)), attend((unsigned)(p.n_row_tiles * p.group_heads));
+    const dim3 expand((unsigned)(p.n_token_tiles * p.group_heads)), attend((unsigned)(p.n_row_tiles * p.group_heads), (unsigned)p.splits);
     if (p.n_token_tiles == 0) {
       // nothing but rows without a context
     } else if (latent_dim == 512) hipLaunchKernelGGL((latent_expand_kernel<512, BF16>), expand, dim3(kThreads), 0, stream, p);
@@ -589,6 +637,11 @@ hipError_t launch_type(LatentChunkParams p, int32_t latent_dim, hipStream_t stre
     hipLaunchKernelGGL((latent_chunk_kernel<BF16>), attend, dim3(kThreads), 0, stream, p);
     err = hipGetLastError();
     if (err != hipSuccess) return err;
+    if (p.splits > 1) {
+      hipLaunchKernelGGL((latent_join_kernel<BF16>), dim3(attend.x, kRows / 8), dim3(256), 0, stream, p);
+      err = hipGetLastError();
+      if (err != hipSuccess) return err;
+    }
   }
   return hipSuccess;
 }

@@ -148,6 +148,12 @@ LATENT_EXPORTS: dict[str, tuple[object, list[object]]] = {
         [_P, _P, _P, _P, _P, _P, _I64, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _P,
          _SZ, _P],
     ),
+    "ayk_latent_chunks_parts_bytes": (_SZ, [_I32, _I32, _I32]),
+    "ayk_latent_chunks_split": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _P, _I64, _P, _I32, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32,
+         _P, _SZ, _P],
+    ),
 }
 
 _lock = threading.Lock()

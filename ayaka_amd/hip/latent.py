@@ -172,6 +172,33 @@ def _chunk_tiles(op: str, step: "_attention.HipAttentionPlan", device: torch.dev
     return found
 
 
+def _chunk_splits(step: "_attention.HipAttentionPlan", n_tiles: int, heads: int) -> int:
+    """Parts to cut each row tile's context into. A workgroup takes about 1.55 us a round of 64 positions and 8 us
+    to start and end, and parts cost about 6 us for their joining; the rounds of all are dealt to the compute
+    units, none of which is done before the longest tile. Cut where that saves 15% (of the whole call: chunks of 600
+    rows of 4 and 8 heads over 3.6K positions 85 and 96 us whole, 42 and 49 cut; of 20 heads over 1.6K, where the
+    model saves 7%, 70 whole and 85 cut)."""
+    found = step.splits.get(("latent-chunks", n_tiles, heads))
+    if found is None:
+        longest, total = 0, 0
+        for count, length in zip(step.rows, step.kv_lengths):
+            if count and length:
+                ends = np.minimum(length, length - count + np.arange(TILE_ROWS, count + TILE_ROWS, TILE_ROWS))
+                rounds = -(-ends // 64)
+                longest, total = max(longest, int(rounds.max())), total + int(rounds.sum())
+
+        def us(parts: int) -> float:
+            waves = -(-n_tiles * heads * parts // _attention.COMPUTE_UNITS)
+            return (max(-(-longest // parts), total * heads / _attention.COMPUTE_UNITS) * 1.55 + 8 * waves
+                    + (6 if parts > 1 else 0))
+
+        found = min((p for p in (1, 2, 3, 4, 6, 8, 12, 16) if p == 1 or 2 * p <= longest), key=us)
+        if us(found) > 0.85 * us(1):
+            found = 1
+        step.splits["latent-chunks", n_tiles, heads] = found
+    return found
+
+
 def attend_latent_chunks(q: torch.Tensor, weights: LatentWeights, buffers: LatentBuffers, meta: AttentionMetadata,
                          out: torch.Tensor, *, scale: float) -> None:
     """Attention of chunks of rows over their requests' latent contexts, keys and values expanded.
@@ -210,13 +237,16 @@ def _attend_latent_chunks(op: str, q: torch.Tensor, weights: LatentWeights, buff
     at_once = heads if ws_rows == 0 else max(1, min(heads, EXPANDED_BYTES // (ws_rows * 512)))
     if at_once >= 8:
         at_once -= at_once % 8 if at_once < heads else 0  # (a head's workgroups then share an XCD)
-    stream = stream_handle(device)
-    scratch = _attention._workspace(op, device, lib.ayk_latent_chunks_workspace_bytes(ws_rows, at_once), capture, stream)
-    _attention._call(op, lib.ayk_latent_chunks, (
+    stream, n_tiles = stream_handle(device), rows.numel() // 4
+    splits = _chunk_splits(step, n_tiles, at_once)
+    nbytes = (-(-lib.ayk_latent_chunks_workspace_bytes(ws_rows, at_once) // 16) * 16
+              + lib.ayk_latent_chunks_parts_bytes(n_tiles, at_once, splits))
+    scratch = _attention._workspace(op, device, nbytes, capture, stream)
+    _attention._call(op, lib.ayk_latent_chunks_split, (
         out.data_ptr(), q.data_ptr(), cache.data_ptr(), weights.keys.data_ptr(), weights.values.data_ptr(),
-        table.data_ptr(), table.stride(0), tokens.data_ptr(), tokens.numel() // 4, rows.data_ptr(), rows.numel() // 4,
+        table.data_ptr(), table.stride(0), tokens.data_ptr(), tokens.numel() // 4, rows.data_ptr(), n_tiles,
         ws_rows, at_once, heads, buffers.latent_dim, buffers.rope_dim, buffers.num_blocks, buffers.block_size,
-        _DTYPE_CODES[cache.dtype], float(scale), scratch.data_ptr(), scratch.numel(),
+        _DTYPE_CODES[cache.dtype], float(scale), splits, scratch.data_ptr(), scratch.numel(),
     ), stream, device, True, record)
 
 

@@ -118,6 +118,19 @@ int ayk_latent_chunks(void* out, const void* q, const void* cache, const void* k
                       int32_t num_blocks, int32_t block_size, int32_t dtype, float scale, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/*
+ * The same with the context of each row tile cut into `splits` parts, 1 to 64, for steps whose row tiles and
+ * heads are fewer than the compute units. workspace: ayk_latent_chunks_workspace_bytes rounded up to 16, and
+ * ayk_latent_chunks_parts_bytes more.
+ */
+size_t ayk_latent_chunks_parts_bytes(int32_t n_row_tiles, int32_t heads_at_once, int32_t splits);
+int ayk_latent_chunks_split(void* out, const void* q, const void* cache, const void* keys, const void* values,
+                            const int32_t* block_table, int64_t table_stride, const int32_t* token_tiles,
+                            int32_t n_token_tiles, const int32_t* row_tiles, int32_t n_row_tiles, int64_t ws_rows,
+                            int32_t heads_at_once, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                            int32_t num_blocks, int32_t block_size, int32_t dtype, float scale, int32_t splits,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

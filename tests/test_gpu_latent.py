@@ -378,6 +378,43 @@ def test_tiles_do_not_show_what_a_row_does_not_see(ops, tiles, dtype, value) -> 
     assert np.array_equal(got[seeing].isnan().cpu().numpy(), np.isnan(s.want()[0][seeing]))
 
 
+@pytest.fixture(params=[1, 2, 3, 7])
+def parts(request, monkeypatch) -> int:
+    """The parts that contexts are cut into, whatever a step's lengths would have."""
+    monkeypatch.setattr(hip_latent, "_chunk_splits", lambda *_: request.param)
+    return request.param
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", [1, 5])
+def test_chunks_over_cut_contexts(ops, parts, dtype, heads) -> None:
+    """Parts of many rounds and of none, of which a row sees some."""
+    Scene(ops, CHUNKS, form="chunks", dtype=dtype, heads=heads, seed=46).check()
+    Scene(ops, [(300, 1500), (2, 900)], form="chunks", dtype=dtype, heads=heads, q_scale=20.0, seed=47).check()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_cut_contexts_do_not_show_what_a_row_does_not_see(ops, parts, value) -> None:
+    s, clean = (Scene(ops, [(150, 400), (1, 64)], form="chunks", heads=3, seed=48) for _ in range(2))
+    s.cache[int(s.table[0, 330 // 16]), 330 % 16, 5] = value
+    got, ref = s.run(), clean.run()
+    assert torch.equal(got[:80], ref[:80]) and torch.equal(got[150], ref[150])
+    want = s.want()[0]
+    for row in range(80, 150):
+        for h in range(3):
+            assert np.isnan(want[row, h]).all() == bool(got[row, h].isnan().all())
+
+
+def test_long_contexts_cut_inside_their_scales_window(ops, monkeypatch) -> None:
+    monkeypatch.setattr(hip_latent, "_chunk_splits", lambda *_: 5)
+    s = Scene(ops, [(3, 40100)], form="chunks", heads=1, block=64, seed=49, q_scale=0.3)
+    t = np.arange(40100)
+    sizes = torch.tensor(2.0 ** ((t // 128 * 5) % 7 - 3), dtype=torch.float32).to(DEV)
+    at = torch.as_tensor(s.table[0, t // 64]), torch.as_tensor(t % 64)
+    s.cache[at] = (s.cache[at].float() * sizes[:, None]).to(s.dtype)
+    s.check()
+
+
 @pytest.mark.parametrize("form", ["absorbed", "chunks"])
 def test_same_bits_every_time(ops, form) -> None:
     s = Scene(ops, [(2, 3000), (1, 77), (30, 600)], form=form, heads=9, seed=12)

@@ -376,3 +376,28 @@ def test_tile_pairs_for_known_lengths() -> None:
     assert lib.ayk_latent_attention_tiles(*args.values()) == 1 and b"tile_pairs 48" in lib.ayk_last_error()
     args.update(tile_pairs=64, workspace_bytes=lib.ayk_latent_tiles_workspace_bytes(512, 64) - 1)
     assert lib.ayk_latent_attention_tiles(*args.values()) == 4 and b"workspace" in lib.ayk_last_error()
+
+
+def test_parts_of_chunk_contexts() -> None:
+    """Cut while workgroups are fewer than the compute units and contexts long; room for the parts."""
+    from ayaka_amd.hip import latent
+
+    def splits(rows, lengths, heads):
+        table = torch.arange(1, 1 + len(rows) * 300).view(len(rows), 300)
+        meta = hip_attention.plan(ForwardMode.MIXED, torch.tensor(rows), torch.tensor(lengths), table, 16)
+        return latent._chunk_splits(meta.plan, sum(-(-r // 128) for r in rows), heads)
+
+    assert splits([512] * 4, [4096] * 4, 16) == 1
+    assert splits([300], [300], 16) == 1
+    assert 2 <= splits([600], [4096], 4) <= 16
+    assert splits([5, 0], [0, 7], 4) == 1
+    lib = _lib.lib()
+    assert lib.ayk_latent_chunks_parts_bytes(3, 4, 1) == lib.ayk_latent_chunks_parts_bytes(0, 4, 2) == 0
+    assert lib.ayk_latent_chunks_parts_bytes(3, 4, 5) == 3 * 4 * 5 * 128 * 130 * 4
+    args = dict(out=16, q=16, cache=16, keys=16, values=16, table=16, stride=4, token_tiles=16, n_token_tiles=1, row_tiles=16,
+                n_row_tiles=1, ws_rows=128, at_once=8, heads=8, latent_dim=512, rope_dim=64, num_blocks=4, block_size=16,
+                dtype=1, scale=1.0, splits=65, workspace=16, workspace_bytes=1 << 40, stream=None)
+    assert lib.ayk_latent_chunks_split(*args.values()) == 1 and b"splits 65" in lib.ayk_last_error()
+    room = -(-lib.ayk_latent_chunks_workspace_bytes(128, 8) // 16) * 16 + lib.ayk_latent_chunks_parts_bytes(1, 8, 3)
+    args.update(splits=3, workspace_bytes=room - 1)
+    assert lib.ayk_latent_chunks_split(*args.values()) == 4 and b"workspace" in lib.ayk_last_error()
