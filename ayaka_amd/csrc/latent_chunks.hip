@@ -520,9 +520,13 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[4 * h + i] = fast_exp2(__builtin_fmaf(s[h][j][i], by[j], from));
       w[j] = u32x4{two_halves(e[0], e[1]), two_halves(e[2], e[3]), two_halves(e[4], e[5]), two_halves(e[6], e[7])};
-      if constexpr (!BF16) {  // the sum of the weights as rounded: where one outweighs the others its rounding cancels
+      if constexpr (!BF16) {
+        // The sum of the weights as rounded: where one outweighs the others its rounding cancels. Not below a louder
+        // tile, where what they carry of the scale may leave nothing of them.
+        if (below == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[2 * i] = Elem<false>::lo(w[j][i]), e[2 * i + 1] = Elem<false>::hi(w[j][i]);
+          for (int i = 0; i < 4; ++i) e[2 * i] = Elem<false>::lo(w[j][i]), e[2 * i + 1] = Elem<false>::hi(w[j][i]);
+        }
       }
       l[j] = __builtin_fmaf(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])), raise, l[j]);
     }
