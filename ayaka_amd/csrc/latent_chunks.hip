@@ -17,8 +17,13 @@
 // Keys and values are kept as fp16 whatever the model's type, with a power of two for every 128 tokens,
 // head and of both kinds, chosen from the largest finite value there, so nothing overflows and each
 // element is within 2^-11 of itself (or 2^-38 of its tile's largest): bf16 keys and values would each
-// cost the outputs as much as their own rounding does. The scales are uniform in the attention's
-// loop: the key's joins the factor that scores take anyway, the value's the exponent.
+// cost the outputs as much as their own rounding does. The key's scale joins the factor that scores take
+// anyway. The value's, 2^e of a tile, meets a reference of each row's own: beside the running maximum m of its scores a
+// row keeps a level E, about the largest score - m + e so far, and
+//   O = sum_t 2^(score_t - m + e_t - E) code_t,   l = sum_t 2^(score_t - m),   out = 2^E O / l.
+// Weights are at most 2^kRescaleSlack with the scale and without it, tiles that weigh nothing cost nothing however
+// loud they are, and the sum never sees a scale. E and e are whole, so where they agree, as they do for most
+// tiles, a weight is one exponential, and elsewhere it is multiplied by a power of two.
 //
 // latent_chunk_kernel: a workgroup (8 waves) per 128 rows of a request and head. Four waves of 32 rows
 // work on every other 32 positions and four on those between (two waves to a SIMD); joined at the end in
@@ -98,6 +103,15 @@ __device__ __forceinline__ int exponent_for(float largest) {
   return max(-100, min(114, (int)((__float_as_uint(largest) >> 23) & 255) - 126 - 14));
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// 2^x for x up to 0 as part * 2^whole: past fp32's least too, and times another power of two as exact as by itself.
+struct Power {
+  float part;
+  int whole;
+};
+__device__ __forceinline__ Power power_of(float x) {
+  const float whole = __builtin_rintf(fmaxf(x, -1000.f));
+  return Power{fast_exp2(x - whole), (int)whole};
+}
 __device__ __forceinline__ float finite_magnitude(float x) {
   const float a = __builtin_fabsf(x);
   return a < INFINITY ? a : 0.f;  // (also where it is NaN)
@@ -254,7 +268,7 @@ template <bool BF16>
 __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentChunkParams p) {
   struct Shared {
     Round round[kRing];
-    float state[4][2][3][16];  // (m, l, exponent) of the later half's rows
+    float state[4][2][3][16];  // (m, l, level) of the later half's rows
     int32_t exponent[kWindow][2];  // of the tiles being read
   };
   __shared__ __align__(16) Shared lds;
@@ -330,12 +344,12 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     unit[j] = exponent;
   }
   f32x4 o[8][2];
-  float m[2], l[2];
-  int value_exponent = -100;  // of O
+  float m[2], l[2], level[2];  // (level: whole; of O, where m is a number)
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     m[j] = -INFINITY;
     l[j] = 0.f;
+    level[j] = 0.f;
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[d][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -375,7 +389,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     const uint8_t* k_here = here + kg * kPositions * 256;
     const uint8_t* r_here = here + kg * kPositions * 128;
     const int key_exponent = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][0]);
-    const int new_exponent = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][1]);
+    const float exponent = (float)__builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][1]);
 
     f32x4 s[2][2], r[2][2];  // [16 positions][16 rows], of the first part and of the rotary part
     u32x4 a[2][6];
@@ -469,33 +483,32 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
           if ((v[d][i] & 0x7c000000u) == 0x7c000000u) v[d][i] &= 0xffffu;
         }
     }
-    if (new_exponent > value_exponent) {
-      const float down = power(max(-126, value_exponent - new_exponent));
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int d = 0; d < 8; ++d) o[d][j] *= down;
-      value_exponent = new_exponent;
-    }
     float top[2];
     bool passes = false;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       top[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])),
                      fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3]))) * by[j];
-      passes |= top[j] > m[j] + kRescaleSlack;
+      // (a difference: beside a maximum whose neighbours are 16 away a sum could round up to what passes it)
+      passes |= top[j] - m[j] + fmaxf(exponent - level[j], 0.f) > kRescaleSlack;
     }
     if (__builtin_amdgcn_ballot_w64(passes)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float highest = column_max(top[j]);
-        // (a row by its own scores alone: what others see must not change its roundings)
-        const float now = highest > m[j] + kRescaleSlack ? highest : m[j];
-        const float down = now == m[j] ? 1.f : fast_exp2(m[j] - now);
+        // (a row by its own scores alone, and by scales only in whole powers of two: what others see must not change
+        // its roundings)
+        const bool moves = highest - m[j] > kRescaleSlack;
+        const float now = moves ? highest : m[j];
+        const float kept = moves ? ceilf(level[j] + (m[j] - now)) : level[j];
+        const float next = moves || highest - now + (exponent - kept) > kRescaleSlack ? fmaxf(kept, exponent + ceilf(highest - now)) : kept;
+        const Power down = moves ? power_of(m[j] - now) : Power{1.f, 0};
+        const float by_o = __builtin_ldexpf(down.part, down.whole + (int)fmaxf(level[j] - next, -2000.f));
         m[j] = now;
-        l[j] *= down;
+        level[j] = next;
+        l[j] *= __builtin_ldexpf(down.part, down.whole);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d][j] *= down;
+        for (int d = 0; d < 8; ++d) o[d][j] *= by_o;
         far[j] |= __builtin_fabsf(now) > 16777216.f && now != -INFINITY;
         if (far[j] && by[j] != 1.f) {
 #pragma unroll
@@ -507,28 +520,36 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
       }
       any_far = __builtin_amdgcn_ballot_w64(far[0] | far[1]) != 0;
     }
-    // the values' scale: weights carry 2^lower, the sum takes it back
-    const int below = max(-126, new_exponent - value_exponent);
-    const float lower = (float)below, raise = power(-below);
     u32x4 w[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float from = lower - (m[j] == -INFINITY ? 0.f : m[j]);
+      const float from = m[j] == -INFINITY ? 0.f : -m[j];
       float e[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[4 * h + i] = fast_exp2(__builtin_fmaf(s[h][j][i], by[j], from));
       w[j] = u32x4{two_halves(e[0], e[1]), two_halves(e[2], e[3]), two_halves(e[4], e[5]), two_halves(e[6], e[7])};
-      if constexpr (!BF16) {
-        // The sum of the weights as rounded: where one outweighs the others its rounding cancels. Not below a louder
-        // tile, where what they carry of the scale may leave nothing of them.
-        if (below == 0) {
+      float sum;
+      if constexpr (BF16) sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      else  // the sum of the weights as rounded: where one outweighs the others its rounding cancels
+        sum = ((Elem<false>::lo(w[j][0]) + Elem<false>::hi(w[j][0])) + (Elem<false>::lo(w[j][1]) + Elem<false>::hi(w[j][1]))) +
+              ((Elem<false>::lo(w[j][2]) + Elem<false>::hi(w[j][2])) + (Elem<false>::lo(w[j][3]) + Elem<false>::hi(w[j][3])));
+      l[j] += sum;
+      const float scale = m[j] == -INFINITY ? 0.f : exponent - level[j];
+      if (__builtin_amdgcn_ballot_w64(scale != 0.f)) {
+        // (a scale past 2^100: its weights may be below fp32's least while it is not in them)
+        if (__builtin_amdgcn_ballot_w64(scale > 100.f)) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[2 * i] = Elem<false>::lo(w[j][i]), e[2 * i + 1] = Elem<false>::hi(w[j][i]);
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (scale > 100.f) e[4 * h + i] = fast_exp2(__builtin_fmaf(s[h][j][i], by[j], from) + (scale - 100.f));
         }
+        const float times = power((int)fminf(fmaxf(scale, -126.f), 100.f));
+        w[j] = u32x4{two_halves(e[0] * times, e[1] * times), two_halves(e[2] * times, e[3] * times),
+                     two_halves(e[4] * times, e[5] * times), two_halves(e[6] * times, e[7] * times)};
       }
-      l[j] = __builtin_fmaf(((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7])), raise, l[j]);
     }
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -553,7 +574,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
       if (mq == 0) {
         lds.state[rg][j][0][mt] = m[j];
         lds.state[rg][j][1][mt] = l[j];
-        lds.state[rg][j][2][mt] = (float)value_exponent;
+        lds.state[rg][j][2][mt] = level[j];
       }
 #pragma unroll
       for (int d = 0; d < 8; ++d) hand[((rg * 2 + j) * 8 + d) * kWave + lane] = o[d][j];
@@ -563,13 +584,16 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
   if (kg == 1) return;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const float pm = lds.state[rg][j][0][mt], pl = lds.state[rg][j][1][mt];
-    const int pe = (int)lds.state[rg][j][2][mt], high = max(value_exponent, pe);
+    const float pm = lds.state[rg][j][0][mt], pl = lds.state[rg][j][1][mt], p_level = lds.state[rg][j][2][mt];
     const float now = fmaxf(m[j], pm);
-    const float mine = now == m[j] ? 1.f : fast_exp2(m[j] - now), other = now == pm ? 1.f : fast_exp2(pm - now);
-    const float sum = l[j] * mine + pl * other;
+    const float mine = now == m[j] ? 0.f : m[j] - now, other = now == pm ? 0.f : pm - now;
+    const Power by_mine = power_of(mine), by_other = power_of(other);
+    const float sum = __builtin_ldexpf(l[j] * by_mine.part, by_mine.whole) + __builtin_ldexpf(pl * by_other.part, by_other.whole);
     const float total = sum == 0.f ? 0.f : 1.f / sum;
-    const float a = mine * power(max(-126, value_exponent - high)), b = other * power(max(-126, pe - high));
+    // a half without scores has no level
+    const float high = fmaxf(fmaxf(ceilf(level[j] + mine), ceilf(p_level + other)), -200.f);
+    const float a = __builtin_ldexpf(by_mine.part, by_mine.whole + (int)fmaxf(level[j] - high, -2000.f));
+    const float b = __builtin_ldexpf(by_other.part, by_other.whole + (int)fmaxf(p_level - high, -2000.f));
     const int row = rg * 32 + j * 16 + mt;
     if (row >= n_rows) continue;
     if (p.splits > 1) {  // a part's output and what it weighs, for the merge
@@ -583,7 +607,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
         const f32x4 x = hand[((rg * 2 + j) * 8 + d) * kWave + lane];
         f32x4 y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, high);
+        for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, (int)high);
         *reinterpret_cast<f32x4*>(p.part_o + at * kValue + d * 16 + 4 * mq) = y;
       }
       continue;
@@ -594,7 +618,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
       const f32x4 x = hand[((rg * 2 + j) * 8 + d) * kWave + lane];
       float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, high);
+      for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf((o[d][j][i] * a + x[i] * b) * total, (int)high);
       *reinterpret_cast<u32x2*>(out + d * 16) = u32x2{round_two<BF16>(y[0], y[1]), round_two<BF16>(y[2], y[3])};
     }
   }
@@ -610,20 +634,25 @@ __global__ __launch_bounds__(256) void latent_join_kernel(const LatentChunkParam
   float top = -INFINITY;
   for (int i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_ml[(first + i * kRows) * 2]);
   float sum = 0.f;
+  for (int i = 0; i < p.splits; ++i) {
+    const float m = p.part_ml[(first + i * kRows) * 2];
+    const Power by = power_of(m == top ? 0.f : m - top);
+    sum += __builtin_ldexpf(p.part_ml[(first + i * kRows) * 2 + 1] * by.part, by.whole);
+  }
+  const float total = sum == 0.f ? 0.f : 1.f / sum;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int i = 0; i < p.splits; ++i) {
     const int64_t at = first + i * kRows;
     const float m = p.part_ml[at * 2];
-    const float weight = p.part_ml[at * 2 + 1] * (m == top ? 1.f : fast_exp2(m - top));
-    sum += weight;
+    const Power by = power_of(m == top ? 0.f : m - top);
+    const float weight = p.part_ml[at * 2 + 1] * by.part * total;
     const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at * kValue + e0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] += x[k] * weight;
+    for (int k = 0; k < 4; ++k) o[k] += __builtin_ldexpf(x[k] * weight, by.whole);
   }
-  const float by = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* out = static_cast<uint16_t*>(p.out) + ((int64_t)(p.row_tiles[4 * tile] + row) * p.heads + p.first_head + head) * kValue + e0;
-  *reinterpret_cast<u32x2*>(out) = u32x2{round_two<BF16>(o[0] * by, o[1] * by), round_two<BF16>(o[2] * by, o[3] * by)};
+  *reinterpret_cast<u32x2*>(out) = u32x2{round_two<BF16>(o[0], o[1]), round_two<BF16>(o[2], o[3])};
 }
 
 template <bool BF16>

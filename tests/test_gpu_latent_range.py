@@ -52,3 +52,34 @@ def test_every_position_counts_in_the_sum_of_weights(ops, parts, dtype, sizes) -
     s = Scene(ops, [(3, 900)], form="chunks", heads=2, dtype=dtype, seed=51, q_scale=0.05)
     resize(s, 0, sizes)
     s.check()
+
+
+def score(s: Scene, request: int, bits) -> None:
+    """Scores of one request by its rotary parts alone: position t's weight is 2 ** bits[t] of the one of a
+    position of 0 bits (as near as the element type holds it)."""
+    s.scale = 1 / 64
+    s.q[..., 128 if s.form == "chunks" else s.latent:] = 0
+    s.q[..., 128 if s.form == "chunks" else s.latent] = 1
+    if s.form == "chunks":
+        s.weights.keys.zero_()
+    else:
+        s.q[..., :s.latent] = 0
+    t = np.arange(s.lengths[request])
+    at = torch.as_tensor(s.table[request, t // s.block]), torch.as_tensor(t % s.block)
+    s.cache[(*at, s.latent)] = torch.tensor(np.asarray(bits, dtype=np.float64) * math.log(2) * 64).to(s.dtype).to(DEV)
+
+
+@pytest.mark.parametrize("loud_at", [0, 3, 6])
+@pytest.mark.parametrize("share", ["none", "as much"])
+@pytest.mark.parametrize("dtype,quiet,loud", [("fp16", -6, 13), ("bf16", -12, 12), ("bf16", -20, 20), ("bf16", -60, 70)])
+def test_values_that_weigh_nothing_cost_others_nothing(ops, parts, dtype, quiet, loud, share, loud_at) -> None:
+    """A tile far louder than the others, whose scores leave it no share of the output, or one like theirs."""
+    s = Scene(ops, [(3, 900), (140, 700)], form="chunks", heads=2, dtype=dtype, seed=52)
+    rng = np.random.default_rng(53)
+    for request, length in enumerate(s.lengths):
+        tile = np.arange(length) // 128
+        sizes = np.where(np.arange(tile[-1] + 1) == loud_at % (tile[-1] + 1), 2.0 ** loud, 2.0 ** quiet)
+        resize(s, request, sizes)
+        bits = rng.uniform(-12, 0, length)
+        score(s, request, np.where(sizes[tile] == 2.0 ** loud, bits + (-300 if share == "none" else quiet - loud), bits))
+    s.check()
