@@ -113,6 +113,13 @@ __host__ __device__ constexpr int latent_swizzle(int t) { return t & 15; }
 __host__ __device__ constexpr int rope_swizzle(int t) { return (t >> 1) & 7; }
 __host__ __device__ constexpr int weight_swizzle(int pair) { return (pair >> 2) & 3; }
 
+// The largest score that does not move a pair's maximum m, or one under it. (Where m's neighbours are 16 away the sum may
+// round up to m + 16, whose weight an fp16 P cannot hold.)
+__device__ __forceinline__ float limit_of(float m) {
+  const float limit = m + kRescaleSlack;
+  return limit - m > kRescaleSlack ? m : limit;
+}
+
 // Tiles of 64 pairs score a chunk while they weigh the one before it.
 constexpr bool ahead(int nt) { return nt == 4; }
 
@@ -521,13 +528,14 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
             });
         s += t;
         bool passes = false, odd = false;
+        const float limit = limit_of(my_m);
         const int seen = min(my_pos, tile.context - 1) - t0 - kg * 16 - 4 * mq;  // of the lane's 4 positions: i <= seen
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (masked) odd |= !(__builtin_fabsf(s[i]) < INFINITY);
           const float t = product(s[i], p.scale_log2);
           s[i] = !masked || i <= seen ? t : -INFINITY;
-          passes |= s[i] > my_m + kRescaleSlack;
+          passes |= s[i] > limit;
         }
         const int word = (__builtin_amdgcn_ballot_w64(passes) ? 1 : 0) | (__builtin_amdgcn_ballot_w64(odd) ? 2 : 0);
         if (word && lane == 0) atomicOr(&flag_of(chunk), word);
@@ -569,7 +577,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
         for (int c = 0; c < NT; ++c) {
           const float top = fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]);
           // (a pair by its own scores alone: what others see must not change its roundings)
-          const float now = top > m[c] + kRescaleSlack ? top : m[c];
+          const float now = top - m[c] > kRescaleSlack ? top : m[c];
           const float b = now == m[c] ? 1.f : fast_exp2(m[c] - now);
           m[c] = now;
           if (c == ct) my_m = now, by = b;

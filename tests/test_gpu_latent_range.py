@@ -83,3 +83,32 @@ def test_values_that_weigh_nothing_cost_others_nothing(ops, parts, dtype, quiet,
         bits = rng.uniform(-12, 0, length)
         score(s, request, np.where(sizes[tile] == 2.0 ** loud, bits + (-300 if share == "none" else quiet - loud), bits))
     s.check()
+
+
+@pytest.mark.parametrize("form", ["absorbed", "chunks"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("step", [16, 32])
+def test_scores_a_few_steps_of_their_own_apart(ops, form, dtype, step) -> None:
+    """Scores of 2^27, whose neighbours in fp32 are 16 apart: what a score passes by is compared as it is.
+    The rows are the last position's values, to 97 weights of 2^-16 (values within 8)."""
+    s = Scene(ops, [(1, 98)], form=form, dtype=dtype, heads=2, seed=56)
+    at = torch.as_tensor(s.table[0, np.arange(98) // 16]), torch.as_tensor(np.arange(98) % 16)
+    if form == "chunks":
+        s.weights.keys.zero_()
+    s.q.zero_()
+    rope = s.latent if form == "absorbed" else 128
+    s.q[..., rope], s.q[..., rope + 1] = 2.0 ** 14, 1.0
+    s.cache[(*at, s.latent)] = 2.0 ** 13
+    s.cache[(*at, s.latent + 1)] = torch.where(torch.arange(98) == 97, 16.0 + step, 16.0).to(s.dtype).to(DEV)
+    s.scale = float(np.float32(math.log(2)))  # a power of two a unit of score
+    assert np.float32(s.scale) * np.float32(1.4426950408889634) in (np.float32(1), np.nextafter(np.float32(1), np.float32(0)))
+    values = s.cache[(*at, slice(0, s.latent))].double().cpu().numpy()
+    if form == "chunks":
+        values = np.einsum("tc,hvc->htv", values, s.weights.values.double().cpu().numpy())
+    else:
+        values = np.broadcast_to(values, (2, 98, s.latent))
+    got, want = s.run().double().cpu().numpy()[0], values[:, 97]
+    assert np.abs(values).max() <= 8
+    # the other weights, and half steps: of the output, the value, the weight and its sum
+    bound = 97 * 2.0 ** -16 * 16 * (step == 16) + (torch.finfo(s.dtype).eps / 2 + 3 * 2.0 ** -11) * (np.abs(want) + 2.0 ** -14)
+    assert np.all(np.abs(got - want) <= bound)
