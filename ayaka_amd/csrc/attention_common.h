@@ -355,6 +355,11 @@ constexpr float kNoScore = -__FLT_MAX__;
 // How far (log2 units) the running max may trail a chunk's max before the
 // accumulators are rescaled: weights stay below 2^8, far inside fp32.
 constexpr float kRescaleSlack = 8.0f;
+// Where weights enter a product as one fp16 value each, a row's reference lies this far under the maximum it is
+// set at: weights from 2^7 there to 2^15 before the next one fill the type's range (65504), and one of 2^-x of that
+// maximum is held to 2^-11 of itself down to x = 21, then to 2^-32 of it, so that a long tail of little weight each keeps
+// its share. The factor is in the weights and in their sum alike.
+constexpr float kWeightLift = 7.0f;
 
 // Index of the first partial (partition 0) of (row, head), which has np partitions.
 // By default the partials are [n_rows, num_heads, max_partitions]; with staged

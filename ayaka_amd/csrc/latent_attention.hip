@@ -22,9 +22,9 @@
 //    its 256 registers); the values are the latents already in LDS, read transposed
 //    (ds_read_b64_tr_b16). v_mfma_f32_16x16x32. A bf16 P is taken in two parts (high and remainder by
 //    truncation: one bf16 would lose 2^-9 of each weight, as much as the output's own rounding), an fp16
-//    P rounded to nearest (2^-11).
+//    P rounded to nearest (2^-11, from 2^-21 of the maximum on 2^-32 of it: kWeightLift).
 //  * The running maximum moves only when a score passes it by kRescaleSlack; until then weights up to
-//    2^kRescaleSlack keep their accuracy and nothing is rescaled.
+//    2^kRescaleSlack times what they were keep their accuracy and nothing is rescaled.
 //  * Up to 32 pairs memory is the bound: two barriers a chunk, and the four waves without scores fetch.
 //    With 64 pairs the products are, so a chunk is scored while the last one is weighed, one barrier a
 //    chunk: of the two waves of a SIMD one weighs first and one scores first.
@@ -113,11 +113,16 @@ __host__ __device__ constexpr int latent_swizzle(int t) { return t & 15; }
 __host__ __device__ constexpr int rope_swizzle(int t) { return (t >> 1) & 7; }
 __host__ __device__ constexpr int weight_swizzle(int pair) { return (pair >> 2) & 3; }
 
-// The largest score that does not move a pair's maximum m, or one under it. (Where m's neighbours are 16 away the sum may
-// round up to m + 16, whose weight an fp16 P cannot hold.)
+// How far a pair's reference lies under the maximum that set it, and from there to where a score moves it. (A bf16 P
+// has fp32's range.)
+constexpr float lift(bool bf16) { return bf16 ? 0.f : kWeightLift; }
+constexpr float reach(bool bf16) { return lift(bf16) + kRescaleSlack; }
+// The largest score that does not move a reference m. Where m's neighbours are far apart the sum may round up to a score
+// whose weight an fp16 P cannot hold: past half a unit over (2^15.5 of 65504) it is m itself.
+template <bool BF16>
 __device__ __forceinline__ float limit_of(float m) {
-  const float limit = m + kRescaleSlack;
-  return limit - m > kRescaleSlack ? m : limit;
+  const float limit = m + reach(BF16);
+  return limit - m > reach(BF16) + 0.5f ? m : limit;
 }
 
 // Tiles of 64 pairs score a chunk while they weigh the one before it.
@@ -455,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
     bool emptied = false;  // values lost non-finite elements
     u32x4 q[KS + 2];
     f32x4 o[DT][NT];
-    float m[NT], my_m = -INFINITY, l = 0.f;  // of every pair; of my_pair, with its sum over this wave's positions
+    float m[NT], my_m = -INFINITY, l = 0.f;  // references of every pair; of my_pair, with its sum over this wave's positions
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
       m[c] = -INFINITY;
@@ -493,7 +498,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
       float before;  // and the sum without it
       bool masked;
       auto flag_of = [&](int chunk) -> int32_t& { return lds.flag[AHEAD ? chunk % 3 : chunk & 1]; };
-      // weights of this wave's scores under the maximum my_m, on top of the sum `so_far`
+      // weights of this wave's scores under the reference my_m, on top of the sum `so_far`
       auto put_weights = [&](int chunk, float so_far) {
         const float base = my_m == -INFINITY ? 0.f : my_m;
         float w[4];
@@ -528,7 +533,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
             });
         s += t;
         bool passes = false, odd = false;
-        const float limit = limit_of(my_m);
+        const float limit = limit_of<BF16>(my_m);
         const int seen = min(my_pos, tile.context - 1) - t0 - kg * 16 - 4 * mq;  // of the lane's 4 positions: i <= seen
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -551,7 +556,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
           v[d] = u32x4{a.x, a.y, b.x, b.y};
         }
       };
-      // Where a score passed its pair's maximum, or one is not finite; true: values changed.
+      // Where a score passed what its pair's reference reaches, or one is not finite; true: values changed.
       auto settle = [&](int chunk) {
         const int word = __builtin_amdgcn_readfirstlane(flag_of(chunk));
         if (!word) return false;
@@ -577,7 +582,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
         for (int c = 0; c < NT; ++c) {
           const float top = fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]);
           // (a pair by its own scores alone: what others see must not change its roundings)
-          const float now = top - m[c] > kRescaleSlack ? top : m[c];
+          const float now = top > limit_of<BF16>(m[c]) ? top - lift(BF16) : m[c];
           const float b = now == m[c] ? 1.f : fast_exp2(m[c] - now);
           m[c] = now;
           if (c == ct) my_m = now, by = b;

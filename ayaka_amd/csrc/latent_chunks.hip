@@ -18,10 +18,10 @@
 // head and of both kinds, chosen from the largest finite value there, so nothing overflows and each
 // element is within 2^-11 of itself (or 2^-38 of its tile's largest): bf16 keys and values would each
 // cost the outputs as much as their own rounding does. The key's scale joins the factor that scores take
-// anyway. The value's, 2^e of a tile, meets a reference of each row's own: beside the running maximum m of its scores a
-// row keeps a level E, about the largest score - m + e so far, and
+// anyway. The value's, 2^e of a tile, meets a reference of each row's own: beside a reference m for its scores
+// (kWeightLift under a running maximum) a row keeps a level E, about the largest score + e so far less that maximum, and
 //   O = sum_t 2^(score_t - m + e_t - E) code_t,   l = sum_t 2^(score_t - m),   out = 2^E O / l.
-// Weights are at most 2^kRescaleSlack with the scale and without it, tiles that weigh nothing cost nothing however
+// Weights are at most 2^15 with the scale and without it, tiles that weigh nothing cost nothing however
 // loud they are, and the sum never sees a scale. E and e are whole, so where they agree, as they do for most
 // tiles, a weight is one exponential, and elsewhere it is multiplied by a power of two.
 //
@@ -257,6 +257,7 @@ constexpr int kPositions = 32;            // of a wave's step
 constexpr int kRound = 2 * kPositions;    // of both halves of the workgroup
 constexpr int kRing = 3;
 constexpr int kWindow = 256;  // tiles whose exponents wait in LDS
+constexpr float kPasses = kWeightLift + kRescaleSlack;  // from a row's reference to where a score moves it
 
 struct Round {
   uint16_t keys[kRound * kNope];
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
       top[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])),
                      fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3]))) * by[j];
       // (a difference: beside a maximum whose neighbours are 16 away a sum could round up to what passes it)
-      passes |= top[j] - m[j] + fmaxf(exponent - level[j], 0.f) > kRescaleSlack;
+      passes |= top[j] - m[j] + fmaxf(exponent - level[j], 0.f) > kPasses;
     }
     if (__builtin_amdgcn_ballot_w64(passes)) {
 #pragma unroll
@@ -498,10 +499,10 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
         const float highest = column_max(top[j]);
         // (a row by its own scores alone, and by scales only in whole powers of two: what others see must not change
         // its roundings)
-        const bool moves = highest - m[j] > kRescaleSlack;
-        const float now = moves ? highest : m[j];
+        const bool moves = highest - m[j] > kPasses;
+        const float now = moves ? highest - kWeightLift : m[j];
         const float kept = moves ? ceilf(level[j] + (m[j] - now)) : level[j];
-        const float next = moves || highest - now + (exponent - kept) > kRescaleSlack ? fmaxf(kept, exponent + ceilf(highest - now)) : kept;
+        const float next = moves || highest - now + (exponent - kept) > kPasses ? fmaxf(kept, exponent + ceilf(highest - now - kWeightLift)) : kept;
         const Power down = moves ? power_of(m[j] - now) : Power{1.f, 0};
         const float by_o = __builtin_ldexpf(down.part, down.whole + (int)fmaxf(level[j] - next, -2000.f));
         m[j] = now;

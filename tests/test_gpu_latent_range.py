@@ -85,6 +85,43 @@ def test_values_that_weigh_nothing_cost_others_nothing(ops, parts, dtype, quiet,
     s.check()
 
 
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("form,dtype", [("absorbed", "fp16"), ("chunks", "fp16"), ("chunks", "bf16")])
+def test_a_long_flat_tail(ops, monkeypatch, form, dtype, first) -> None:
+    """One position of nearly all the weight, and 131071 of 2^-26 of it each, which make a share of 2^-9. Contexts
+    are not cut: a workgroup has the whole of one (in absorbed form one of as many requests as there are compute
+    units, over the same blocks).
+
+    A weight is held to 2^-11 of itself, or 2^-32 of the position's that set the running maximum, which is no more
+    than the largest, numerator and denominator alike: 2 n (2^-26 2^-11 + 2^-32) = 2^-13 (1 + 2^-5) of the values' size 1
+    (the tail's values are 1 and the other's 0). Beside it the output's rounding, a half step of 2^-9, and (n / 32 + 40) 2^-24 of
+    the sums."""
+    n, block = 1 << 17, 64
+    monkeypatch.setattr(hip_latent, "_chunk_splits", lambda *_: 1)
+    requests = 256 if form == "absorbed" else 1
+    s = Scene(ops, [(1, 5)] * requests, form=form, dtype=dtype, heads=1, latent=256, block=block, seed=54)
+    s.lengths, s.rows = [n] * requests, [1] * requests
+    s.table = np.tile(1 + np.arange(n // block), (requests, 1))
+    s.cache = torch.zeros(1 + n // block, block, 320, dtype=s.dtype, device=DEV)
+    s.cache[..., :256] = 1
+    s.meta = ops.attention.plan(ForwardMode.DECODE, torch.tensor(s.rows, device=DEV), torch.tensor(s.lengths, device=DEV),
+                                torch.tensor(s.table, device=DEV), block)
+    bits = np.random.default_rng(55).uniform(-26.5, -25.5, n)
+    most = 0 if first else n - 1
+    bits[most] = 0
+    score(s, 0, bits)
+    s.cache[int(s.table[0, most // block]), most % block, :256] = 0
+    if form == "chunks":
+        s.weights.values.zero_()
+        s.weights.values[..., 0] = 1
+    p = np.exp(s.cache[1:][..., 256].reshape(-1).double().cpu().numpy() / 64)
+    p[most] = 1
+    want = 1 - 1 / p.sum()
+    bound = 2.0 ** -13 * (1 + 2.0 ** -5) + want * torch.finfo(s.dtype).eps / 2 + (n / 32 + 40) * 2.0 ** -24 * want
+    assert abs(want - 2.0 ** -9) < 2.0 ** -13
+    assert float((s.run().double() - want).abs().max()) <= bound
+
+
 @pytest.mark.parametrize("form", ["absorbed", "chunks"])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("step", [16, 32])
