@@ -230,7 +230,7 @@ struct LatentChunkParams {
   uint16_t* ws_rope;                // [ws_rows, 64]
   uint16_t* ws_keys;                // [group_heads, ws_rows, 128]
   uint16_t* ws_values;
-  int32_t* ws_exponents;            // [group_heads, ws_rows / 128, 2]
+  int32_t* ws_exponents;            // [group_heads, ws_rows / 128, 2]: twice the exponent, and 1 where an element is not finite
 };
 hipError_t launch_latent_chunks(const LatentChunkParams& p, int32_t latent_dim, bool bf16, hipStream_t stream);
 

@@ -132,6 +132,7 @@ __global__ __launch_bounds__(kThreads, 4) void latent_expand_kernel(const Latent
     uint16_t token[kSteps][kTokens * kStep];
     uint16_t weight[kSteps][kOutputs * kStep];
     float largest[kWaves];
+    int32_t infinite[kWaves];  // not 0: among a wave's elements is one that is not finite
   };
   __shared__ __align__(16) Shared lds;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -213,20 +214,26 @@ __global__ __launch_bounds__(kThreads, 4) void latent_expand_kernel(const Latent
 
   // The scale of the tile's keys (waves 0-3) and of its values (4-7).
   float largest = 0.f;
+  bool infinite = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) largest = fmaxf(largest, finite_magnitude(acc[i][j][e]));
+      for (int e = 0; e < 4; ++e) {
+        largest = fmaxf(largest, finite_magnitude(acc[i][j][e]));
+        infinite |= !(__builtin_fabsf(acc[i][j][e]) < INFINITY);
+      }
+  infinite = __builtin_amdgcn_ballot_w64(infinite) != 0;
   largest = column_max(largest);
 #pragma unroll
   for (int d = 8; d >= 1; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
-  if (lane == 0) lds.largest[wave] = largest;
+  if (lane == 0) lds.largest[wave] = largest, lds.infinite[wave] = infinite;
   lds_barrier();
   const int half = n >> 1;  // keys, values
   largest = fmaxf(fmaxf(lds.largest[4 * half], lds.largest[4 * half + 1]), fmaxf(lds.largest[4 * half + 2], lds.largest[4 * half + 3]));
   const int exponent = exponent_for(largest);
+  infinite = lds.infinite[4 * half] | lds.infinite[4 * half + 1] | lds.infinite[4 * half + 2] | lds.infinite[4 * half + 3];
   const float by = power(-exponent);
   // Through LDS (rows of 512 bytes, as tokens; every wave is past its last read), then whole rows out.
   uint8_t* rows = reinterpret_cast<uint8_t*>(&lds.token[0][0]);
@@ -248,7 +255,7 @@ __global__ __launch_bounds__(kThreads, 4) void latent_expand_kernel(const Latent
     uint16_t* to = piece < 16 ? p.ws_keys : p.ws_values;
     *reinterpret_cast<u32x4*>(to + (ws + token) * kNope + (piece & 15) * 8) = x;
   }
-  if (tid == 0 || tid == 4 * kWave) p.ws_exponents[(head * (p.ws_rows / kTokens) + ws_row / kTokens) * 2 + half] = exponent;
+  if (tid == 0 || tid == 4 * kWave) p.ws_exponents[(head * (p.ws_rows / kTokens) + ws_row / kTokens) * 2 + half] = 2 * exponent + infinite;
 }
 
 // --- attention
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
   struct Shared {
     Round round[kRing];
     float state[4][2][3][16];  // (m, l, level) of the later half's rows
-    int32_t exponent[kWindow][2];  // of the tiles being read
+    int32_t exponent[kWindow][2];  // of the tiles being read: twice that, and 1 where an element is not finite
   };
   __shared__ __align__(16) Shared lds;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -389,8 +396,9 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     const uint8_t* here = reinterpret_cast<const uint8_t*>(&lds.round[round % kRing]);
     const uint8_t* k_here = here + kg * kPositions * 256;
     const uint8_t* r_here = here + kg * kPositions * 128;
-    const int key_exponent = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][0]);
-    const float exponent = (float)__builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][1]);
+    const int key_exponent = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][0]) >> 1;
+    const int value_word = __builtin_amdgcn_readfirstlane(lds.exponent[t0 / kTokens % kWindow][1]);
+    const float exponent = (float)(value_word >> 1);
 
     f32x4 s[2][2], r[2][2];  // [16 positions][16 rows], of the first part and of the rotary part
     u32x4 a[2][6];
@@ -434,7 +442,6 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     __builtin_amdgcn_sched_barrier(0);
 
     const bool masked = t0 + kPositions - 1 > first_masked;
-    bool odd = false;
     float by[2] = {p.scale_log2, p.scale_log2};  // of what s holds from here on
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -453,14 +460,13 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            odd |= !(__builtin_fabsf(s[h][j][i]) < INFINITY);
+          for (int i = 0; i < 4; ++i)
             s[h][j][i] = 16 * h + i <= seen ? (whole ? product(s[h][j][i], p.scale_log2) : s[h][j][i]) : -INFINITY;
-          }
       }
     }
-    if (masked && __builtin_amdgcn_ballot_w64(odd)) {
-      // Values that are not finite become zeros, behind NaN for the rows that see them.
+    if (masked && (value_word & 1)) {
+      // Values that are not finite become zeros, behind NaN for the rows that see them. (What says so are the values
+      // themselves: a finite latent may take one past the range of fp32 and leave its key and every score alone.)
       const uint8_t* mine = here + kRound * 256 + kg * kPositions * 256;
 #pragma unroll 1
       for (int t = 0; t < kPositions; ++t) {

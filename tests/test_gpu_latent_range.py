@@ -149,3 +149,22 @@ def test_scores_a_few_steps_of_their_own_apart(ops, form, dtype, step) -> None:
     # the other weights, and half steps: of the output, the value, the weight and its sum
     bound = 97 * 2.0 ** -16 * 16 * (step == 16) + (torch.finfo(s.dtype).eps / 2 + 3 * 2.0 ** -11) * (np.abs(want) + 2.0 ** -14)
     assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("at", [17, 300, 391])
+def test_values_past_the_range_of_fp32_stay_with_the_rows_that_see_them(ops, parts, at) -> None:
+    """Latents that the keys' matrix passes over and the values' takes past the largest fp32."""
+    steps = [(400, 400), (1, 64)]
+    s, clean = (Scene(ops, steps, form="chunks", heads=3, seed=57) for _ in range(2))
+    for x in (s, clean):
+        x.cache[..., 3] = 0
+        x.weights.keys[..., 3] = 0
+        x.weights.values[..., 3] = 0
+        x.weights.values[:, ::5, 3] = 1e30
+    s.cache[int(s.table[0, at // 16]), at % 16, 3] = 1e20
+    got, ref = s.run(), clean.run()
+    assert bool(ref.isfinite().all())
+    blind = [*range(at), 400]
+    assert torch.equal(got[blind], ref[blind])
+    assert not bool(got[at:400, :, ::5].isfinite().any())
+    assert torch.equal(got[at:400, :, 1::5], got[at:400, :, 1::5].nan_to_num(7.0, 7.0, 7.0))
