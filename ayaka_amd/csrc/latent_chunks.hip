@@ -351,6 +351,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
       for (int e = 0; e < 4; ++e) q[j][k][e] = two_halves(Elem<BF16>::lo(q[j][k][e]) * by, Elem<BF16>::hi(q[j][k][e]) * by);
     unit[j] = exponent;
   }
+  const bool loud = __builtin_amdgcn_ballot_w64(unit[0] > 127 - 114 || unit[1] > 127 - 114) != 0;  // (keys: up to 114)
   f32x4 o[8][2];
   float m[2], l[2], level[2];  // (level: whole; of O, where m is a number)
 #pragma unroll
@@ -445,7 +446,16 @@ __global__ __launch_bounds__(kThreads, 1) void latent_chunk_kernel(const LatentC
     float by[2] = {p.scale_log2, p.scale_log2};  // of what s holds from here on
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float ratio = __builtin_ldexpf(1.f, unit[j] + key_exponent);
+      int up = unit[j] + key_exponent;
+      if (loud) {  // past the largest power of two the factor comes in two, so that products of 0 stay 0
+        const int first = max(0, up - 127);
+        up -= first;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][j][i] = __builtin_ldexpf(s[h][j][i], first);
+      }
+      const float ratio = __builtin_ldexpf(1.f, up);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -168,3 +168,16 @@ def test_values_past_the_range_of_fp32_stay_with_the_rows_that_see_them(ops, par
     assert torch.equal(got[blind], ref[blind])
     assert not bool(got[at:400, :, ::5].isfinite().any())
     assert torch.equal(got[at:400, :, 1::5], got[at:400, :, 1::5].nan_to_num(7.0, 7.0, 7.0))
+
+
+def test_loud_queries_across_loud_keys(ops, parts) -> None:
+    """Queries and keys of 2^80 whose products are zeros: every position weighs the same."""
+    s = Scene(ops, [(3, 300), (130, 200)], form="chunks", heads=2, seed=58)
+    s.weights.keys.zero_()
+    s.weights.keys[:, 1, 1] = 1
+    s.weights.values[..., 1] = 0
+    s.cache[..., 1] = 2.0 ** 80
+    s.cache[..., s.latent:] = 0
+    s.q.zero_()
+    s.q[..., 0] = 2.0 ** 80
+    s.check()
