@@ -309,7 +309,8 @@ int ayk_latent_chunks_split(void* out, const void* q, const void* cache, const v
   if (misaligned(16, {out, q, cache, keys, values, workspace}))
     return fail(AYK_ERR_ARGUMENT, "%s: out, q, cache, keys, values and workspace must be 16-byte aligned", op);
   if (heads_at_once > num_heads) heads_at_once = num_heads;
-  const size_t expanded = (ayk_latent_chunks_workspace_bytes(ws_rows, heads_at_once) + 15) & ~(size_t)15;
+  size_t expanded = ayk_latent_chunks_workspace_bytes(ws_rows, heads_at_once);
+  if (splits > 1) expanded = (expanded + 15) & ~(size_t)15;  // (where the parts follow)
   const size_t need = expanded + ayk_latent_chunks_parts_bytes(n_row_tiles, heads_at_once, splits);
   if (need > workspace_bytes || (need > 0 && !workspace))
     return fail(AYK_ERR_WORKSPACE, "%s: the workspace holds %zu bytes, %zu are needed", op, workspace_bytes, need);
