@@ -229,11 +229,12 @@ int ayk_latent_attention_tiles(void* out, const void* q, const void* cache, cons
   const size_t need = ayk_latent_tiles_workspace_bytes(latent_dim, tile_pairs);
   if (!workspace || workspace_bytes < need)
     return fail(AYK_ERR_WORKSPACE, "%s: the workspace holds %zu bytes, %zu are needed", op, workspace_bytes, need);
-  // the kernel counts (row, head) pairs and the chunks of all tiles in 31 bits
+  // the kernel counts (row, head) pairs and the units of all tiles in 31 bits
   const int pairs = tile_pairs;
   const int64_t positions = (int64_t)max_blocks * block_size;
   const int64_t tiles = (int64_t)n_rows * num_heads / pairs + n_requests;
-  if ((int64_t)n_rows * num_heads > INT32_MAX || positions > INT32_MAX - 64 || tiles * (positions / 32 + 8) > INT32_MAX)
+  if ((int64_t)n_rows * num_heads > INT32_MAX || positions > INT32_MAX - 64 ||
+      tiles * ayk::latent_tile_units(pairs, positions) > INT32_MAX)
     return fail(AYK_ERR_UNSUPPORTED, "%s: %d rows of %d heads over tables of %lld positions exceed one launch", op, n_rows,
                 num_heads, (long long)positions);
   ayk::LatentParams p{};

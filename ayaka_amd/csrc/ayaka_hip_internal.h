@@ -200,6 +200,8 @@ struct LatentParams {
 // (row, head) pairs of one tile for rows of `heads` heads, `rows` of them to a request on average
 int latent_tile_pairs(const int32_t* rows, const int32_t* kv_lengths, int32_t n_requests, int32_t heads, int compute_units);
 int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads, int compute_units);
+// What one tile of that many pairs over a context of that length counts as in the line of work that is split
+int64_t latent_tile_units(int pairs, int64_t length);
 size_t latent_workspace_bytes(int32_t latent_dim, int pairs, int compute_units);
 hipError_t launch_latent_attention(const LatentParams& p, int32_t latent_dim, bool bf16, int pairs, int compute_units,
                                    hipStream_t stream);

@@ -780,6 +780,10 @@ hipError_t launch_type(const LatentParams& p, int pairs, int compute_units, hipS
 
 }  // namespace
 
+int64_t latent_tile_units(int pairs, int64_t length) {
+  return (length < kChunk ? 1 : (length + kChunk - 1) / kChunk) + tile_cost(pairs);
+}
+
 // Pairs of a tile. Larger tiles read a context less often and take fewer products of few rows; smaller ones
 // make more work to share while there is not enough for every compute unit, and start and end sooner. With u
 // units a workgroup (as they are dealt out above) a launch takes about 13 + 1.15 u us with 16 pairs, 14 + 1.45 u
@@ -790,8 +794,7 @@ hipError_t launch_type(const LatentParams& p, int pairs, int compute_units, hipS
 struct TileChoice {
   int64_t units[3] = {0, 0, 0};
   void add(int64_t requests, int64_t pairs, int64_t length) {
-    const int64_t chunks = length < kChunk ? 1 : (length + kChunk - 1) / kChunk;
-    for (int i = 0; i < 3; ++i) units[i] += requests * ((pairs + (16 << i) - 1) / (16 << i)) * (chunks + tile_cost(16 << i));
+    for (int i = 0; i < 3; ++i) units[i] += requests * ((pairs + (16 << i) - 1) / (16 << i)) * latent_tile_units(16 << i, length);
   }
   int best(int compute_units) const {
     constexpr double START[3] = {13, 14, 20}, EACH[3] = {1.15, 1.45, 1.7};

@@ -25,3 +25,30 @@ def test_the_documented_workspace_of_chunks_is_enough() -> None:
         args["workspace_bytes"] -= 1
         assert lib.ayk_latent_chunks(*args.values()) == 4
         assert f"{size} are needed".encode() in lib.ayk_last_error()
+
+
+def _attention_args(**kw) -> dict:
+    args = dict(out=16, q=16, cache=16, table=16, stride=0, lengths=16, rows=16, n_requests=0, n_rows=0, heads=1,
+                latent_dim=512, rope_dim=64, num_blocks=4, block_size=7, max_blocks=0, dtype=1, scale=1.0, tile_pairs=64,
+                workspace=16, workspace_bytes=1 << 40, stream=None)
+    assert not set(kw) - set(args)
+    return {**args, **kw}
+
+
+def test_the_units_of_a_launch_stay_below_2_to_31() -> None:
+    """What the kernel counts in 32 bits: every tile's chunks of 32 positions, the last one begun, and the tile's own
+    cost (8 chunks with 64 pairs, 5 with fewer), for as many tiles as rows and requests can make."""
+    lib = _lib.lib()
+    for pairs, cost in ((16, 5), (32, 5), (64, 8)):
+        for blocks in (1, 9, 147):  # 7, 63, 1029 positions: 1, 2, 33 chunks, of which the last holds 7, 31, 5
+            chunks = -(-blocks * 7 // 32) + cost
+            tiles = (1 << 31) // chunks  # the first number of tiles whose units may reach 2^31
+            while tiles * chunks < 1 << 31:
+                tiles += 1
+            requests = tiles - tiles // 2
+            rows = (tiles - requests) * pairs  # of one head: that many tiles, and one begun for every request
+            args = _attention_args(n_requests=requests, n_rows=rows, max_blocks=blocks, stride=blocks, tile_pairs=pairs)
+            if rows > (1 << 31) - 1:
+                continue
+            assert lib.ayk_latent_attention_tiles(*args.values()) == 2, (pairs, blocks)
+            assert b"exceed one launch" in lib.ayk_last_error()
