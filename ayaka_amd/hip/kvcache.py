@@ -27,6 +27,7 @@ from ayaka_amd.hip import _fastpath, _lib
 from ayaka_amd.hip._checks import (
     block_scales,
     compute_dtype,
+    dtype_name,
     require_buffers,
     require_device,
     require_index_tensor,
@@ -137,7 +138,7 @@ def _store(k: torch.Tensor, v: torch.Tensor, buffers: KVBuffers, meta: Attention
 
 
 def _rotation(op: str, meta: AttentionMetadata, rotary: Rotary | None, device: torch.device,
-              width: int) -> tuple:
+              width: int, n_rows: int) -> tuple:
     """The entry points' positions, and turns, pairs, order and magnitude of a rotation of rows of
     ``width`` elements (``None``: nothing turns)."""
     if rotary is None:
@@ -147,8 +148,9 @@ def _rotation(op: str, meta: AttentionMetadata, rotary: Rotary | None, device: t
         raise BackendError(f"{op}: the rotation turns {2 * pairs} elements of heads of {width}",
                            context={"op": op, "argument": "rotary"})
     positions = meta.positions
-    if positions.dtype != _I32 or not positions.is_contiguous():
-        raise BackendError(f"{op}: meta.positions must be a contiguous int32 tensor", context={"op": op})
+    if positions.dtype != _I32 or not positions.is_contiguous() or tuple(positions.shape) != (n_rows,):
+        raise BackendError(f"{op}: meta.positions must be a contiguous int32 [{n_rows}] tensor, got "
+                           f"{dtype_name(positions.dtype)} {list(positions.shape)}", context={"op": op, "argument": "meta"})
     require_device(op, "meta.positions", positions, device)
     return positions.data_ptr(), (rotary.turns.data_ptr(), pairs, int(rotary.interleaved), float(rotary.magnitude))
 
@@ -239,7 +241,7 @@ def _rotate(op: str, q, k, meta: AttentionMetadata, rotary: Rotary, q_out, k_out
     n_rows, width, dtype, device = meta.positions.shape[0], first.shape[2], first.dtype, first.device
     heads, q_args = _turned(op, "q", q, q_out, n_rows, width, dtype, device) if q is not None else (0, _NO_ROWS)
     kv_heads, k_args = _turned(op, "k", k, k_out, n_rows, width, dtype, device) if k is not None else (0, _NO_ROWS)
-    positions, turn = _rotation(op, meta, rotary, device, width)
+    positions, turn = _rotation(op, meta, rotary, device, width, n_rows)
     if n_rows == 0:
         return
     _launch(op, _lib.lib().ayk_rotate_and_cache, (
@@ -282,7 +284,7 @@ def _store_rotated(op: str, q, k, v, buffers: KVBuffers, meta: AttentionMetadata
     for name, rows in (("k", k), ("v", v)):
         require_rows(op, name, rows, (n_rows, kv_heads, width), dtype, device)
     heads, q_args = _turned(op, "q", q, q_out, n_rows, width, dtype, device) if q is not None else (0, _NO_ROWS)
-    positions, turn = _rotation(op, meta, rotary, device, width)
+    positions, turn = _rotation(op, meta, rotary, device, width, n_rows)
     if n_rows == 0:
         return
     _launch(op, _lib.lib().ayk_rotate_and_cache, (
@@ -323,7 +325,7 @@ def _store_latent(op: str, latent, k_rope, buffers: LatentBuffers, meta: Attenti
     if rotary is None and q is not None:
         raise BackendError(f"{op}: q is given and nothing to rotate it by", context={"op": op, "argument": "q"})
     heads, q_args = _turned(op, "q", q, q_out, n_rows, rope_dim, dtype, device) if q is not None else (0, _NO_ROWS)
-    positions, turn = _rotation(op, meta, rotary, device, rope_dim)
+    positions, turn = _rotation(op, meta, rotary, device, rope_dim, n_rows)
     if n_rows == 0:
         return
     _launch(op, _lib.lib().ayk_store_latent, (

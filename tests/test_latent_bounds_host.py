@@ -2,7 +2,17 @@
 
 from __future__ import annotations
 
+import dataclasses
+
+import pytest
+import torch
+
+from ayaka_amd.enums import ForwardMode
+from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import _lib
+from ayaka_amd.hip import attention as hip_attention
+from ayaka_amd.hip import kvcache as hip_kvcache
+from ayaka_amd.rotary import rotary
 
 
 def _chunk_args(**kw) -> dict:
@@ -52,3 +62,16 @@ def test_the_units_of_a_launch_stay_below_2_to_31() -> None:
                 continue
             assert lib.ayk_latent_attention_tiles(*args.values()) == 2, (pairs, blocks)
             assert b"exceed one launch" in lib.ayk_last_error()
+
+
+def test_steps_with_fewer_positions_than_rows_are_refused() -> None:
+    """Metadata whose positions were replaced by others: a row without one would read past them."""
+    meta = hip_attention.plan(ForwardMode.DECODE, torch.ones(4, dtype=torch.int32), torch.full((4,), 3, dtype=torch.int32),
+                              torch.arange(1, 5, dtype=torch.int32)[:, None], 16)
+    turn, cpu = rotary(64, device="cpu"), torch.device("cpu")
+    assert hip_kvcache._rotation("op", meta, turn, cpu, 64, 4)[1][1:] == (32, 0, 1.0)
+    assert hip_kvcache._rotation("op", meta, None, cpu, 64, 4) == (0, (0, 0, 0, 1.0))
+    for positions in (meta.positions[:3], meta.positions[:0], torch.zeros(5, dtype=torch.int32), torch.zeros(4, 1, dtype=torch.int32)):
+        other = dataclasses.replace(meta, positions=positions)
+        with pytest.raises(BackendError, match=r"meta.positions must be a contiguous int32 \[4\]"):
+            hip_kvcache._rotation("op", other, turn, cpu, 64, 4)
