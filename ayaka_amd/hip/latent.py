@@ -74,6 +74,17 @@ def _require_latent_step(op: str, q: torch.Tensor, buffers: LatentBuffers, meta:
     return heads
 
 
+def _require_described(op: str, step: "_attention.HipAttentionPlan", table: torch.Tensor, block_size: int, n_rows: int) -> None:
+    """Refuse a plan whose lists, which the tiles are made of, are not of this table and these rows."""
+    longest = max((length for count, length in zip(step.rows, step.kv_lengths) if count), default=0)
+    if len(step.rows) != table.shape[0] or sum(step.rows) != n_rows or longest > table.shape[1] * block_size:
+        raise BackendError(
+            f"{op}: the step was planned for {len(step.rows)} requests of {sum(step.rows)} rows in all and up to {longest} "
+            f"positions, its metadata has {n_rows} rows and a table of {list(table.shape)} blocks of {block_size}",
+            context={"op": op, "argument": "meta"},
+        )
+
+
 def _replayed(meta: AttentionMetadata, key: tuple, keep: tuple, q: torch.Tensor, call) -> None:
     cache = getattr(meta.plan, "launches", None)
     if cache is None:
@@ -230,6 +241,7 @@ def _attend_latent_chunks(op: str, q: torch.Tensor, weights: LatentWeights, buff
     if not isinstance(step, _attention.HipAttentionPlan):
         raise BackendError(f"{op}: needs a step made by plan; a decode bucket's rows take attend_latent",
                            context={"op": op, "argument": "meta"})
+    _require_described(op, step, table, meta.block_size, q.shape[0])
     if q.shape[0] == 0:
         return
     device, lib, capture = cache.device, _lib.lib(), capturing(q)

@@ -12,6 +12,7 @@ from ayaka_amd.errors import BackendError
 from ayaka_amd.hip import _lib
 from ayaka_amd.hip import attention as hip_attention
 from ayaka_amd.hip import kvcache as hip_kvcache
+from ayaka_amd.hip import latent
 from ayaka_amd.rotary import rotary
 
 
@@ -75,3 +76,18 @@ def test_steps_with_fewer_positions_than_rows_are_refused() -> None:
         other = dataclasses.replace(meta, positions=positions)
         with pytest.raises(BackendError, match=r"meta.positions must be a contiguous int32 \[4\]"):
             hip_kvcache._rotation("op", other, turn, cpu, 64, 4)
+
+
+def test_chunks_refuse_a_plan_of_another_step() -> None:
+    """Tile lists come from the plan's lengths: a table, or rows, that they do not describe would be read past."""
+    rows, lengths = torch.tensor([3, 1, 0], dtype=torch.int32), torch.tensor([40, 17, 90], dtype=torch.int32)
+    table = torch.arange(1, 19, dtype=torch.int32).view(3, 6)
+    meta = hip_attention.plan(ForwardMode.MIXED, rows, lengths, table, 16)
+    latent._require_described("op", meta.plan, meta.block_table, 16, 4)
+    latent._require_described("op", meta.plan, meta.block_table[:, :3], 16, 4)  # no row attends to the third request
+    for block_table, block_size, n_rows in (
+        (meta.block_table[:, :2], 16, 4), (meta.block_table[:2], 16, 4), (meta.block_table, 6, 4), (meta.block_table, 16, 3),
+        (meta.block_table, 16, 5),
+    ):
+        with pytest.raises(BackendError, match="planned for 3 requests of 4 rows in all and up to 40 positions"):
+            latent._require_described("op", meta.plan, block_table, block_size, n_rows)
