@@ -25,8 +25,8 @@ int check_rotation(const char* op, int32_t n_rows, int32_t heads, int32_t width,
   if (dtype != AYK_DTYPE_FP16 && dtype != AYK_DTYPE_BF16 && dtype != AYK_DTYPE_FP32)
     return fail(AYK_ERR_UNSUPPORTED, "%s: dtype %d is not fp16 (0), bf16 (1) or fp32 (3)", op, dtype);
   if (heads < 0) return fail(AYK_ERR_ARGUMENT, "%s: num_heads is negative (%d)", op, heads);
-  if (width < 2 || width > 1024 || width % 2 != 0)
-    return fail(AYK_ERR_UNSUPPORTED, "%s: a width of %d is not even and in [2, 1024]", op, width);
+  if (width < 2 || width > ayk::kRotateMostWidth || width % 2 != 0)
+    return fail(AYK_ERR_UNSUPPORTED, "%s: a width of %d is not even and in [2, %d]", op, width, ayk::kRotateMostWidth);
   if (pairs < 0 || 2 * pairs > width)
     return fail(AYK_ERR_ARGUMENT, "%s: %d pairs do not fit a width of %d", op, pairs, width);
   if (!std::isfinite(magnitude)) return fail(AYK_ERR_ARGUMENT, "%s: magnitude must be finite", op);

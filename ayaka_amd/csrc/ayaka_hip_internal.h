@@ -176,7 +176,7 @@ struct RotateParams {
   int32_t tasks_per_row, rows_per_workgroup;
   Divisor by_tasks;
 };
-int rotate_most_pairs();
+constexpr int kRotateMostWidth = 1024;  // elements of a head
 // type: AYK_DTYPE_* of every stream's elements
 hipError_t launch_rotate_store(RotateParams p, int type, bool side_by_side, int compute_units, hipStream_t stream);
 
@@ -197,7 +197,8 @@ struct LatentParams {
   float* part_ml;
   float* part_o;
 };
-// (row, head) pairs of one tile for rows of `heads` heads, `rows` of them to a request on average
+// (row, head) pairs of one tile: for requests of rows[b] rows and kv_lengths[b] positions (host memory), or of n_rows rows in
+// all where the lengths are not known
 int latent_tile_pairs(const int32_t* rows, const int32_t* kv_lengths, int32_t n_requests, int32_t heads, int compute_units);
 int latent_tile_pairs(int64_t n_rows, int32_t n_requests, int32_t heads, int compute_units);
 // What one tile of that many pairs over a context of that length counts as in the line of work that is split

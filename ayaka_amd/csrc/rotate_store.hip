@@ -34,6 +34,7 @@ namespace {
 constexpr int kThreads = 256;
 // (row, pair) cosines and sines of one workgroup
 constexpr int kMostAngles = 2048;
+static_assert(kMostAngles >= kRotateMostWidth / 2, "one row's pairs");
 
 // n / d for 0 <= n < 2^31 (as block_of in attention_common.h).
 __device__ __forceinline__ uint32_t quotient(uint32_t n, Divisor d) {
@@ -206,8 +207,6 @@ hipError_t launch_vector(const RotateParams& p, dim3 grid, bool side_by_side, hi
 }
 
 }  // namespace
-
-int rotate_most_pairs() { return kMostAngles / 4; }
 
 // Elements per vector that every address, stride and half of the streams is a multiple of.
 static int vector_elements(const RotateParams& p, int size, bool side_by_side) {

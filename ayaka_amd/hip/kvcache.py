@@ -401,7 +401,7 @@ def gather(
 def _move_scales(op: str, name: str, tensors: tuple[torch.Tensor, ...], ids: tuple[torch.Tensor, ...],
                  scales: torch.Tensor, device: torch.device) -> None:
     """The block op ``name`` on a block-scaled cache's scales, one block of them a row (the op
-    takes two caches of one shape: both are the scales, so each word is written twice alike)."""
+    takes two caches of one shape: both are the scales, moved once)."""
     _lib.check(
         op,
         getattr(_lib.lib(), name)(
