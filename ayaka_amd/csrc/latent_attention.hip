@@ -117,12 +117,12 @@ __host__ __device__ constexpr int weight_swizzle(int pair) { return (pair >> 2) 
 // has fp32's range.)
 constexpr float lift(bool bf16) { return bf16 ? 0.f : kWeightLift; }
 constexpr float reach(bool bf16) { return lift(bf16) + kRescaleSlack; }
-// The largest score that does not move a reference m. Where m's neighbours are far apart the sum may round up to a score
-// whose weight an fp16 P cannot hold: past half a unit over (2^15.5 of 65504) it is m itself.
+// The largest score that does not move a reference m. Where m's neighbours are far apart (`far`: at least 2 at 2^24) the
+// sum may round up to a score whose weight an fp16 P cannot hold: past half a unit over (2^15.5 of 65504) it is m itself.
 template <bool BF16>
-__device__ __forceinline__ float limit_of(float m) {
+__device__ __forceinline__ float limit_of(float m, bool far) {
   const float limit = m + reach(BF16);
-  return limit - m > reach(BF16) + 0.5f ? m : limit;
+  return !BF16 && far && limit - m > reach(BF16) + 0.5f ? m : limit;
 }
 
 // Tiles of 64 pairs score a chunk while they weigh the one before it.
@@ -458,6 +458,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
     const bool real = scores && my_pair < tile.pairs;
     const int my_pos = real ? tile.first_pos + (piece.tile * NC + my_pair) / p.heads : -1;
     bool emptied = false;  // values lost non-finite elements
+    bool far = false;      // of some pair's reference
     u32x4 q[KS + 2];
     f32x4 o[DT][NT];
     float m[NT], my_m = -INFINITY, l = 0.f;  // references of every pair; of my_pair, with its sum over this wave's positions
@@ -533,7 +534,7 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
             });
         s += t;
         bool passes = false, odd = false;
-        const float limit = limit_of<BF16>(my_m);
+        const float limit = limit_of<BF16>(my_m, far);
         const int seen = min(my_pos, tile.context - 1) - t0 - kg * 16 - 4 * mq;  // of the lane's 4 positions: i <= seen
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -582,13 +583,14 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attention_kernel(const Lat
         for (int c = 0; c < NT; ++c) {
           const float top = fmaxf(lds.exchange[0][c * 16 + mt], lds.exchange[1][c * 16 + mt]);
           // (a pair by its own scores alone: what others see must not change its roundings)
-          const float now = top > limit_of<BF16>(m[c]) ? top - lift(BF16) : m[c];
+          const float now = top > limit_of<BF16>(m[c], true) ? top - lift(BF16) : m[c];
           const float b = now == m[c] ? 1.f : fast_exp2(m[c] - now);
           m[c] = now;
           if (c == ct) my_m = now, by = b;
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[d][c] *= b;
         }
+        if constexpr (!BF16) far |= __builtin_amdgcn_ballot_w64(__builtin_fabsf(my_m) >= 16777216.f && my_m != -INFINITY) != 0;
         if (scores) put_weights(chunk, before * by);
         lds_barrier();
         return (word & 2) != 0;
