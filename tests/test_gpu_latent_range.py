@@ -181,3 +181,21 @@ def test_loud_queries_across_loud_keys(ops, parts) -> None:
     s.q.zero_()
     s.q[..., 0] = 2.0 ** 80
     s.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("louder", [2.0 ** -6, 2.0, 64.0])
+def test_scales_of_positions_not_seen_change_no_bits(ops, parts, dtype, louder) -> None:
+    """A position that sets its tile's scales, seen by some rows: the others' outputs keep every bit. (Elements from 2^-27
+    of a tile's largest on are not rounded otherwise under another power of two.)"""
+    steps = [(150, 400), (1, 64)]
+    s, clean = (Scene(ops, steps, form="chunks", dtype=dtype, heads=3, seed=48) for _ in range(2))
+    at = (int(s.table[0, 330 // 16]), 330 % 16, slice(0, s.latent))
+    s.cache[at] *= louder
+    for x in (s, clean):
+        if louder < 1:  # there it is the clean one that is louder
+            x.cache[at] *= 8
+    got, ref = s.run(), clean.run()
+    assert torch.equal(got[:80], ref[:80]) and torch.equal(got[150], ref[150])
+    assert not torch.equal(got[80:150], ref[80:150])
+    s.check(got)
