@@ -37,7 +37,7 @@
 //
 // Measured at DC 512 (this kernel + the merge): 64 requests of 4096 positions, 16 heads, bf16: 54 + 5 us,
 // 302 MB at 5.6 TB/s in the first; 61 requests of 16 to 16384 positions, 128 heads, bf16: 79 + 10 us; 32
-// requests of 4096 with 4 rows each, 32 heads, fp16: 69 + 9 us, 530 TFLOP/s in the first, where 3000 cycles a
+// requests of 4096 with 4 rows each, 32 heads, fp16: 72 + 9 us, 510 TFLOP/s in the first, where 3000 cycles a
 // chunk of 64 pairs go to 1150 of matrix instructions (1600 for bf16) and the reads of LDS and exponentials
 // that they do not cover; 4 requests of 128 to 1000, 16 heads: 15 + 4 us, which is the chain of
 // lengths, table, first rows (8 us) and a few chunks.
@@ -107,8 +107,9 @@ __device__ __forceinline__ void wait_loads() {
 // lanes 0-3, 12-15 and 20-27, and so on (measured: 4.0 cycles a read where these 16 differ
 // modulo 256 bytes, 8.0 where two meet). Piece c of a latent of position t is at c ^ (t % 16) of its
 // row, piece c of a rotary part (rows of 128 bytes) at c ^ (t / 2 % 8), piece c of a pair's weights
-// (rows of 64 bytes) at c ^ (pair / 4 % 4): there two meet in a read, and yet an fp16 verify window takes
-// 69 us so and 73 with c ^ (pair / 2 % 4), where none do.
+// (rows of 64 bytes) at c ^ (pair / 4 % 4): there two meet in a read, and yet the fp16 verify windows above take
+// 71 us so and 73 with c ^ (pair / 2 % 4), where none do; steps of 128 bf16 heads 78 either way, and calls on inputs
+// that change the same within half a percent.
 __host__ __device__ constexpr int latent_swizzle(int t) { return t & 15; }
 __host__ __device__ constexpr int rope_swizzle(int t) { return (t >> 1) & 7; }
 __host__ __device__ constexpr int weight_swizzle(int pair) { return (pair >> 2) & 3; }

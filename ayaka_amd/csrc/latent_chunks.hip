@@ -11,8 +11,8 @@
 // 8 waves of 64 x 64 on v_mfma_f32_16x16x32, operands through LDS in steps of 32 of DC, three steps in
 // flight (global_load_lds, 74 KB). Two workgroups share a compute unit, so that one's first loads and
 // stores run beside the other's products: with one of twice the step 16384 tokens for 16 heads at DC 512
-// took 95 us, so 82 (0.84 PFLOP/s, and 134 MB written). Tokens are gathered from their pages here; what
-// follows reads straight lines.
+// took 95 us at their best, so 80 (0.86 PFLOP/s, and 134 MB written; 92 at the median of 20 launches from rest, as
+// the card lowers its clock). Tokens are gathered from their pages here; what follows reads straight lines.
 //
 // Keys and values are kept as fp16 whatever the model's type, with a power of two for every 128 tokens,
 // head and of both kinds, chosen from the largest finite value there, so nothing overflows and each
@@ -33,8 +33,8 @@
 // a workgroup each, which latent_join_kernel joins: chunks of 600 rows of 4 heads over 3.6K positions take 42 us
 // so, 85 whole.
 // Bound by issue, not by memory: the loads alone take 34 us where 4 requests of 512 rows over 4096
-// positions, 16 heads, take 112 to 124 (0.65 PFLOP/s in the causal part). Of about 3100 cycles a round
-// 1280 are matrix instructions and as many vector ones, and exponentials do not run beside matrix
+// positions, 16 heads, take 112 at their best and 131 at the median (0.72 and 0.61 PFLOP/s in the causal part). Of
+// about 3100 cycles a round 1280 are matrix instructions and as many vector ones, and exponentials do not run beside matrix
 // instructions of the same SIMD (alone 8.7 cycles each; beside a wave of products they wait for its
 // end). Measured and left: the waves of a SIMD half a round apart, keys read a round ahead, both
 // within 3% of this and longer.

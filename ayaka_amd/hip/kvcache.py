@@ -301,7 +301,8 @@ def store_latent(latent: torch.Tensor, k_rope: torch.Tensor, buffers: LatentBuff
     goes to its slot; ``q`` [N, heads, rope_dim], the queries' rotary parts, is rotated in place or
     into ``q_out`` (the tail of the absorbed queries, say) in the same launch. All may be views whose
     rows are contiguous. Without ``rotary`` the key parts are stored as they are, and there is no ``q``.
-    Rows of padding requests are not stored.
+    Rows of padding requests are not stored. The cache is float16, bfloat16 or float32; this backend's attention is
+    over float16 and bfloat16 ones (a float32 cache can be written and its blocks moved, for attention elsewhere).
     """
     op = "kvcache.store_latent"
     tensors, absent = _given(latent, k_rope, buffers.k, q, q_out)

@@ -112,7 +112,9 @@ def attend_latent(q: torch.Tensor, buffers: LatentBuffers, meta: AttentionMetada
     values' matrix to be applied to. Rows see positions up to their own; padding rows get zeros. ``out``
     overlaps no input.
     Any step serves: decode, verify windows, chunks (``attend_latent_chunks`` does those of many rows
-    with a third of the work per score), graph metadata. Captured after one eager call.
+    with a third of the work per score), graph metadata. Captured after one eager call. Caches are float16, with
+    weights in float16 (within 2^-11 of themselves, or 2^-32 of a row's largest), or bfloat16, with weights of 16 bits
+    or more; ``store_latent`` writes float32 ones too, which this backend does not attend to.
     """
     op = "attention.attend_latent"
     key = ("attend_latent", id(buffers), id(meta), scale, _fastpath.signature((q, out, buffers.k)))
@@ -221,7 +223,10 @@ def attend_latent_chunks(q: torch.Tensor, weights: LatentWeights, buffers: Laten
     (some hundred; ``attend_latent`` serves the others without expanding). For steps made by ``plan``;
     captured after one eager call. Expanded keys and values are held in fp16 with a scale for every 128
     positions of a head: each element is within 2^-11 of itself, whatever its magnitude, or within 2^-38 of
-    the largest finite one of those positions.
+    the largest finite one of those positions (for rows before that one too). Weights are fp16 as well: each weight
+    times value is within 2^-11 of itself, or within 2^-32 of the largest weight times largest value of its 128
+    positions that the row's sum has met; the sum of weights sees no value. Of queries the first 128 elements are fp16
+    under a scale of each row's own.
     """
     op = "attention.attend_latent_chunks"
     key = ("attend_latent_chunks", id(buffers), id(meta), scale,

@@ -197,7 +197,8 @@ except ImportError:
 
 class LatentBuffers(NamedTuple):
     """The latent cache of one layer: ``cache`` contiguous ``[num_blocks, block_size, latent_dim +
-    rope_dim]`` in the compute dtype, the latent first."""
+    rope_dim]`` in the compute dtype, the latent first. (The hip backend attends to float16 and bfloat16 ones; it writes
+    and moves float32 ones too.)"""
 
     cache: Tensor
     latent_dim: int

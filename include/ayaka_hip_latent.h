@@ -65,7 +65,8 @@ int ayk_store_latent(const void* latent, int64_t latent_row, const void* k_rope,
  *   score(row, head, t) = scale * q[row, head] . cache_row(t)
  *   out[row, head]      = sum over t of softmax(score)(t) * latent(t)
  * q [n_rows, num_heads, latent_dim + 64], out [n_rows, num_heads, latent_dim], contiguous and 16-byte
- * aligned, as the cache; dtype fp16 or bf16; latent_dim 256 or 512, rope_dim 64. The step has n_requests
+ * aligned, as the cache; dtype fp16 (weights in fp16: within 2^-11 of themselves or 2^-32 of a row's largest) or bf16
+ * (16 bits of a weight or more); latent_dim 256 or 512, rope_dim 64. The step has n_requests
  * requests of rows[b] rows each, in order (n_rows in all), which are the last of kv_lengths[b] tokens; a
  * row attends to the positions up to its own; requests of length 0 give zeros. rows, kv_lengths and the
  * table are read on the device only: the call can be captured and replayed with others. Rows past the sum
@@ -100,7 +101,8 @@ int ayk_latent_attention_tiles(void* out, const void* q, const void* cache, cons
  * q [n_rows, num_heads, 128 + 64], out [n_rows, num_heads, 128], keys and values [num_heads, 128,
  * latent_dim], contiguous and 16-byte aligned, as the cache; dtype fp16 or bf16; latent_dim 256 or 512.
  * Expanded keys and values are fp16 under a power of two for every 128 tokens, head and kind (within 2^-11
- * of themselves down to 2^-27 of the largest there, then within 2^-38 of it).
+ * of themselves down to 2^-27 of the largest there, then within 2^-38 of it). Weights are fp16 too, within 2^-11 of
+ * themselves or, values' powers of two included, 2^-32 of a row's largest.
  * The step comes as two device lists of int32 quadruples, made on the host:
  *   token_tiles (request, first position, the request's length, workspace row): every 128 positions of each
  *     request with rows, its workspace rows following each other and starting at a multiple of 128;
